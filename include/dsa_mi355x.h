@@ -367,6 +367,58 @@ int dsa_sparse_attn_sink(int kind, const void* q, const void* kv, const int32_t*
 int dsa_act_quant(int in_kind, const void* x, int64_t rows, int64_t n, int out_kind, void* y, float* scales,
                   int round_scale, void* stream);
 
+/*
+ * 8-bit matrix product with a scale for each token and each output channel, over rows as dsa_act_quant
+ * writes them:
+ *   out[m, n] = (sum_k x[m, k] w[n, k]) * x_scale[m] * w_scale[n] + bias[n]
+ *  x [M, K] int8, w [N, K] int8 (a row for each output channel), x_scale [M], w_scale [N] and bias [N] (or NULL)
+ *  fp32; out [M, N] of out_kind (bf16, fp16 or fp32).  The sums are exact (int32); the rest is fp32, rounded
+ *  once to the output.  1 <= K <= 131071; no alignment is asked of the rows.
+ */
+size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K);
+
+int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_scale, const float* w_scale,
+                     const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * Root-mean-square norm of each query and key head with the rotation of its first R elements, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight;  (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)
+ * c, s = cos / sin[positions[t], pair] (fp32 [table_len, R / 2]); pair i is elements (i, i + R / 2), or
+ * (2i, 2i + 1) with `interleaved`.  Token t's heads are D-element rows at q + t * q_stride (elements; so q, k
+ * and v may be parts of one projection's output).  Weights [D] fp32 or of `kind`, or NULL (ones).
+ * slots NULL: k_out [T, G, D].  Else k_out and v_out are caches of cache_rows rows [G, D]: token t's keys and
+ * values (v unchanged) go to row slots[t]; slots outside [0, cache_rows) write nothing; slots in it must differ.
+ * A position outside [0, table_len) marks padding: q_out and k_out rows of zeros, nothing to a cache.
+ * bf16 or fp16; D a multiple of 8 up to 512, R a multiple of 16 up to D; rows start on 16 bytes.
+ */
+int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                     int64_t v_stride, const void* q_weight, const void* k_weight, int weight_kind,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t table_len, int64_t T,
+                     int64_t H, int64_t G, int64_t D, int64_t R, float eps, int interleaved, const int32_t* slots,
+                     int64_t cache_rows, void* q_out, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of new tokens over a paged cache (dense: every key a token sees), grouped heads of D = 64 or 128.
+ * Sequence b brings the last len_b of its kv_len[b] tokens; token i of them sits at position
+ * p = kv_len - len_b + i and sees key j iff 0 <= j < kv_len, j <= p (is_causal), j >= p - win_left (unless
+ * win_left is -1) and the key's page block_table[b, j / block_size] lies in [0, num_blocks).
+ *  q [T, H, D]: with cu_q [B] (inclusive prefix sums of the lengths) packed; without, T = B * S padded rows,
+ *  actual_q_len [B] or NULL (S each).  k_cache, v_cache [num_blocks, block_size, G, D]; block_table
+ *  [B, max_blocks]; query heads g*H/G .. read KV head g; sinks [H] fp32 (natural-log units) or NULL, added to
+ *  the denominator; out [T, H, D]; lse [T, H] fp32, natural log, sink included.  Rows that see nothing (padding
+ *  rows, rows behind cu_q[B - 1] too) get out = 0 and lse = -inf (or the sink).  What lies in pages behind a
+ *  sequence's last key is not read into a result; within a sequence K and V are finite.
+ *  max_keys of the workspace query is max_blocks * block_size.
+ */
+size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys);
+
+int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                      const int32_t* cu_q, const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T,
+                      int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
+                      int64_t max_blocks, int is_causal, int64_t win_left, const float* sinks, float sm_scale,
+                      void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -48,6 +48,22 @@ hipError_t launch_sparse_attn_sink(int is_fp16, const void* q, const void* kv, c
                                    void* out, float* lse, void* workspace, hipStream_t stream);
 hipError_t launch_act_quant(int in_kind, const void* x, int64_t rows, int64_t n, int out_kind, void* y,
                             float* scales, int round_scale, hipStream_t stream);
+hipError_t launch_quant_matmul(int out_kind, const void* x, const void* w, const float* sx, const float* sw,
+                               const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
+                               hipStream_t stream);
+size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+hipError_t launch_qk_norm_rope(int is_fp16, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                               const void* v, int64_t v_stride, const void* qw, const void* kw, int w_f32,
+                               const int32_t* positions, const float* cos, const float* sin, int64_t table,
+                               int64_t T, int64_t H, int64_t G, int64_t D, int64_t R, float eps, int interleaved,
+                               const int32_t* slots, int64_t rows, void* q_out, void* k_out, void* v_out,
+                               hipStream_t stream);
+size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most);
+hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
+                            const int32_t* cu_q, const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B,
+                            int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
+                            int64_t max_blocks, int causal, int64_t win_left, const float* sinks, float sm_scale,
+                            void* out, float* lse, void* workspace, hipStream_t stream);
 hipError_t launch_sparse_flash_mla(int is_fp16, const void* q, int64_t T, int64_t H, int64_t B,
                                    const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len,
                                    const void* ori_kv, int64_t ori_blocks, int64_t ori_bs, const int32_t* ori_bt,
@@ -532,6 +548,106 @@ int dsa_sparse_attn_sink(int kind, const void* q, const void* kv, const int32_t*
   if (need > 0 && !workspace) return reject("sparse_attn: null workspace");
   return ok(dsa::launch_sparse_attn_sink(kind == DSA_KIND_FP16, q, kv, topk_idxs, B, M, H, N, topk, sinks,
                                          softmax_scale, out, lse, workspace, static_cast<hipStream_t>(stream)));
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int check_quant_matmul(int64_t M, int64_t N, int64_t K) {
+  // A grid dimension of 128-row tiles; int32 sums of products of at most 2^14.
+  if (M < 0 || N < 0 || M > 8388480 || N > kMaxInt - 4096) return reject("quant_matmul: bad M / N");
+  if (K < 1 || K > 131071) return reject("quant_matmul: K must be in [1, 131071]");
+  return 0;
+}
+
+size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || check_quant_matmul(M, N, K)) return 0;
+  return dsa::quant_matmul_workspace_bytes(M, N, K);
+}
+
+int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_scale, const float* w_scale,
+                     const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (out_kind != DSA_KIND_BF16 && out_kind != DSA_KIND_FP16 && out_kind != DSA_KIND_FP32)
+    return reject("quant_matmul: output kind must be bf16, fp16 or fp32");
+  if (const int rc = check_quant_matmul(M, N, K)) return rc;
+  if (M > 0 && N > 0 && (!x || !w || !x_scale || !w_scale || !out)) return reject("quant_matmul: null pointer");
+  const size_t need = dsa_quant_matmul_workspace_size(M, N, K);
+  if (workspace_bytes < need) return reject("quant_matmul: workspace too small");
+  if (need > 0 && (!workspace || !aligned16(workspace))) return reject("quant_matmul: null or unaligned workspace");
+  return ok(dsa::launch_quant_matmul(out_kind, x, w, x_scale, w_scale, bias, M, N, K, out, workspace,
+                                     static_cast<hipStream_t>(stream)));
+}
+
+int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                     int64_t v_stride, const void* q_weight, const void* k_weight, int weight_kind,
+                     const int32_t* positions, const float* cos, const float* sin, int64_t table_len, int64_t T,
+                     int64_t H, int64_t G, int64_t D, int64_t R, float eps, int interleaved, const int32_t* slots,
+                     int64_t cache_rows, void* q_out, void* k_out, void* v_out, void* stream) {
+  if (kind != DSA_KIND_BF16 && kind != DSA_KIND_FP16) return reject("qk_norm_rope: kind must be bf16 or fp16");
+  if (weight_kind != kind && weight_kind != DSA_KIND_FP32)
+    return reject("qk_norm_rope: weights must be fp32 or of the inputs' kind");
+  if (D < 8 || D > 512 || D % 8 != 0) return reject("qk_norm_rope: D must be a multiple of 8 in [8, 512]");
+  if (R < 0 || R > D || R % 16 != 0) return reject("qk_norm_rope: R must be a multiple of 16 in [0, D]");
+  if (T < 0 || H < 0 || G < 0 || H > 65536 || G > 65536 || table_len < 0 || table_len > kMaxInt || cache_rows < 0 ||
+      cache_rows > kMaxInt || T > kMaxInt || T * (H + 2 * G) > kMaxInt)
+    return reject("qk_norm_rope: bad sizes");
+  if (!(eps >= 0.f)) return reject("qk_norm_rope: eps must not be negative");
+  if (T * (H + G) == 0) return 0;
+  const bool paged = slots != nullptr;
+  if (!positions || (R > 0 && table_len > 0 && (!cos || !sin)) || (H > 0 && (!q || !q_out)) ||
+      (G > 0 && (!k || !k_out || (paged && (!v || !v_out)))))
+    return reject("qk_norm_rope: null pointer");
+  if (q_stride % 8 != 0 || k_stride % 8 != 0 || (paged && v_stride % 8 != 0) || q_stride < 0 || k_stride < 0 ||
+      (paged && v_stride < 0))
+    return reject("qk_norm_rope: token strides must be multiples of 8 elements");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) ||
+      (paged && (!aligned16(v) || !aligned16(v_out))))
+    return reject("qk_norm_rope: rows must start on 16 bytes");
+  return ok(dsa::launch_qk_norm_rope(kind == DSA_KIND_FP16, q, q_stride, k, k_stride, v, v_stride, q_weight, k_weight,
+                                     weight_kind == DSA_KIND_FP32, positions, cos, sin, table_len, T, H, G, D, R, eps,
+                                     interleaved ? 1 : 0, slots, cache_rows, q_out, k_out, v_out,
+                                     static_cast<hipStream_t>(stream)));
+}
+
+// Sizes that both the workspace query and the call need in range.
+static bool paged_gqa_sizes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
+  return T >= 0 && B >= 1 && B <= 65535 && H >= 1 && G >= 1 && H % G == 0 && G <= 65535 && T <= kMaxInt &&
+         H <= 65535 && T * H <= kMaxInt - 65536 && (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096;
+}
+
+size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {
+  if (T <= 0 || !paged_gqa_sizes(T, B, H, G, D, max_keys)) return 0;
+  return dsa::paged_gqa_workspace_bytes(T, B, H, G, D, max_keys);
+}
+
+int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                      const int32_t* cu_q, const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T,
+                      int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
+                      int64_t max_blocks, int is_causal, int64_t win_left, const float* sinks, float sm_scale,
+                      void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  if (kind != DSA_KIND_BF16 && kind != DSA_KIND_FP16) return reject("paged_gqa: kind must be bf16 or fp16");
+  if (D != 64 && D != 128) return reject("paged_gqa: D must be 64 or 128");
+  if (G < 1 || H < 1 || H % G != 0) return reject("paged_gqa: H must be a multiple of kv_group");
+  if (block_size < 1 || max_blocks < 1 || num_blocks < 1 || block_size > kMaxInt || max_blocks > kMaxInt ||
+      num_blocks > kMaxInt / block_size)
+    return reject("paged_gqa: bad page sizes");
+  if (max_blocks > (kMaxInt - 4096) / block_size || !paged_gqa_sizes(T, B, H, G, D, max_blocks * block_size))
+    return reject("paged_gqa: sizes out of range");
+  if (!cu_q && (S < 0 || S > kMaxInt || B * S != T)) return reject("paged_gqa: T must be B * S without cu_q");
+  if (win_left < -1 || win_left > kMaxInt - 4096) return reject("paged_gqa: win_left must be -1 (none) or a key count");
+  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return reject("paged_gqa: sm_scale must be positive");
+  if (T == 0) return 0;
+  if (!q || !k_cache || !v_cache || !block_table || !actual_kv_len || !out || !lse)
+    return reject("paged_gqa: null pointer");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return reject("paged_gqa: rows must start on 16 bytes");
+  const size_t need = dsa_paged_gqa_workspace_size(T, B, H, G, D, max_blocks * block_size);
+  if (workspace_bytes < need) return reject("paged_gqa: workspace too small");
+  if (need > 0 && (!workspace || !aligned16(workspace))) return reject("paged_gqa: null or unaligned workspace");
+  return ok(dsa::launch_paged_gqa(kind == DSA_KIND_FP16, q, k_cache, v_cache, block_table, cu_q, actual_q_len,
+                                  actual_kv_len, T, B, S, H, G, D, num_blocks, block_size, max_blocks,
+                                  is_causal ? 1 : 0, win_left, sinks, sm_scale, out, lse, workspace,
+                                  static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

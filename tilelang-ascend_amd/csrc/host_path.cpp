@@ -18,6 +18,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -48,6 +49,11 @@ struct Entries {
   decltype(&dsa_lightning_indexer_tnd_fused) tndf;
   decltype(&dsa_sparse_flash_mla_workspace_size) v4_ws;
   decltype(&dsa_sparse_flash_mla) v4;
+  decltype(&dsa_quant_matmul_workspace_size) qmm_ws;
+  decltype(&dsa_quant_matmul) qmm;
+  decltype(&dsa_qk_norm_rope) rope;
+  decltype(&dsa_paged_gqa_workspace_size) pgqa_ws;
+  decltype(&dsa_paged_gqa_fwd) pgqa;
 } E;
 bool bound = false;
 
@@ -463,6 +469,151 @@ PyObject* flash_mla(PyObject*, PyObject* const* v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (x, weight, x_scale, weight_scale, bias, out kind)
+PyObject* quant_matmul(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t kind = 0;
+  DSA_PLAIN(bound && n == 6 && int_of(v[5], kind));
+  for (int i = 0; i < 4; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const at::Tensor &x = THPVariable_Unpack(v[0]), &w = THPVariable_Unpack(v[1]), &xs = THPVariable_Unpack(v[2]),
+                   &ws = THPVariable_Unpack(v[3]);
+  const Arg bias(v[4]);
+  DSA_PLAIN(x.is_cuda() && x.dim() >= 2 && w.dim() == 2 && x.numel() > 0 && w.numel() > 0 && !bias.other);
+  const c10::Device dev = x.device();
+  const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K;
+  DSA_PLAIN(plain(x, dev, at::kChar) && plain(w, dev, at::kChar) && plain(xs, dev, at::kFloat) &&
+            plain(ws, dev, at::kFloat) && w.size(1) == K && K <= 131071 && xs.numel() == M && ws.numel() == N);
+  if (bias) DSA_PLAIN(plain(*bias.t, dev, at::kFloat) && bias.t->dim() == 1 && bias.t->numel() == N);
+  DSA_PLAIN(kind == DSA_KIND_BF16 || kind == DSA_KIND_FP16 || kind == DSA_KIND_FP32);
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = N;
+  at::Tensor out, work;
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    out = make(sizes, kind == DSA_KIND_FP32 ? at::kFloat : kind == DSA_KIND_FP16 ? at::kHalf : at::kBFloat16, dev);
+    const size_t bytes = E.qmm_ws(M, N, K);
+    if (bytes) work = make({(int64_t)bytes}, at::kByte, dev);
+    rc = E.qmm((int)kind, x.data_ptr(), w.data_ptr(), xs.data_ptr<float>(), ws.data_ptr<float>(), bias.ptr<float>(), M,
+               N, K, out.data_ptr(), bytes ? work.data_ptr() : nullptr, bytes, stream(dev));
+  }
+  DSA_RC(rc);
+  return wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// [T, n, D] on `dev` whose tokens may lie apart, each with contiguous heads and on 16 bytes.
+bool heads_ok(const at::Tensor& t, c10::Device dev, at::ScalarType st, int64_t T, int64_t D, int64_t& stride) {
+  if (t.device() != dev || t.scalar_type() != st || t.dim() != 3 || t.size(0) != T || t.size(1) < 1 ||
+      t.size(2) != D || t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != D))
+    return false;
+  stride = T > 1 ? t.stride(0) : t.size(1) * D;
+  return stride % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+
+// (q, k, v, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slots, eps, interleaved): v, the caches and
+// the slots together, or none of them
+PyObject* qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  DSA_PLAIN(bound && n == 13 && THPVariable_CheckExact(v[0]) && THPVariable_CheckExact(v[1]) &&
+            THPVariable_CheckExact(v[5]) && THPVariable_CheckExact(v[6]) && THPVariable_CheckExact(v[7]) &&
+            PyFloat_CheckExact(v[11]) && PyBool_Check(v[12]));
+  const at::Tensor &q = THPVariable_Unpack(v[0]), &k = THPVariable_Unpack(v[1]), &pos = THPVariable_Unpack(v[5]),
+                   &cos = THPVariable_Unpack(v[6]), &sin = THPVariable_Unpack(v[7]);
+  const Arg val(v[2]), qw(v[3]), kw(v[4]), kc(v[8]), vc(v[9]), slots(v[10]);
+  DSA_PLAIN(q.is_cuda() && q.dim() == 3 && q.size(0) > 0 && !val.other && !qw.other && !kw.other && !kc.other &&
+            !vc.other && !slots.other);
+  const c10::Device dev = q.device();
+  const at::ScalarType st = q.scalar_type();
+  const int kind = kind16(st);
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
+  int64_t qs = 0, ks = 0, vs = 0;
+  DSA_PLAIN(kind >= 0 && D % 8 == 0 && D >= 8 && D <= 512 && heads_ok(q, dev, st, T, D, qs) &&
+            heads_ok(k, dev, st, T, D, ks));
+  const int64_t G = k.size(1);
+  int wkind = kind;
+  for (const Arg* w : {&qw, &kw})
+    if (*w) {
+      const at::ScalarType ws = w->t->scalar_type();
+      DSA_PLAIN((ws == st || ws == at::kFloat) && plain(*w->t, dev, ws) && w->t->dim() == 1 && w->t->numel() == D);
+      wkind = ws == at::kFloat ? DSA_KIND_FP32 : kind;
+    }
+  if (qw && kw) DSA_PLAIN(qw.t->scalar_type() == kw.t->scalar_type());
+  DSA_PLAIN(plain(cos, dev, at::kFloat) && plain(sin, dev, at::kFloat) && cos.dim() == 2 && cos.sizes() == sin.sizes());
+  const int64_t R = 2 * cos.size(1);
+  DSA_PLAIN(R % 16 == 0 && R <= D && plain(pos, dev, at::kInt) && pos.numel() == T);
+  const bool paged = (bool)kc;
+  DSA_PLAIN(paged == (bool)val && paged == (bool)vc && paged == (bool)slots);
+  if (paged)
+    DSA_PLAIN(heads_ok(*val.t, dev, st, T, D, vs) && val.t->size(1) == G && kc.t->dim() == 4 &&
+              plain(*kc.t, dev, st) && plain(*vc.t, dev, st) && kc.t->sizes() == vc.t->sizes() &&
+              kc.t->size(2) == G && kc.t->size(3) == D && plain(*slots.t, dev, at::kInt) && slots.t->numel() == T);
+  const double eps = PyFloat_AS_DOUBLE(v[11]);
+  DSA_PLAIN(eps >= 0);
+  const bool pairs = v[12] == Py_True;
+  at::Tensor qo, ko;
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    qo = make({T, H, D}, st, dev);
+    ko = paged ? *kc.t : make({T, G, D}, st, dev);
+    rc = E.rope(kind, q.data_ptr(), qs, k.data_ptr(), ks, val.ptr<void>(), vs, qw.ptr<void>(), kw.ptr<void>(), wkind,
+                pos.data_ptr<int32_t>(), cos.data_ptr<float>(), sin.data_ptr<float>(), cos.size(0), T, H, G, D, R,
+                (float)eps, pairs, slots.ptr<int32_t>(), paged ? kc.t->size(0) * kc.t->size(1) : 0, qo.data_ptr(),
+                ko.data_ptr(), paged ? vc.t->data_ptr() : nullptr, stream(dev));
+  }
+  DSA_RC(rc);
+  return pair(std::move(qo), std::move(ko));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, v_cache, block_table, sm_scale, q lengths, kv lengths, is_causal, win_left, sinks)
+PyObject* paged_gqa(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t win = -1;
+  DSA_PLAIN(bound && n == 10 && PyFloat_CheckExact(v[4]) && PyBool_Check(v[7]) && int_of(v[8], win));
+  for (int i = 0; i < 4; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const at::Tensor &q = THPVariable_Unpack(v[0]), &kc = THPVariable_Unpack(v[1]), &vc = THPVariable_Unpack(v[2]),
+                   &bt = THPVariable_Unpack(v[3]);
+  const Arg ql(v[5]), kl(v[6]), sinks(v[9]);
+  DSA_PLAIN(q.is_cuda() && (q.dim() == 3 || q.dim() == 4) && kc.dim() == 4 && bt.dim() == 2 && q.numel() > 0 && kl &&
+            !sinks.other && win >= -1 && win < 0x7fffffff - 4096);
+  const c10::Device dev = q.device();
+  const at::ScalarType st = q.scalar_type();
+  const int kind = kind16(st);
+  const bool packed = q.dim() == 3;
+  const int64_t B = bt.size(0), H = q.size(-2), D = q.size(-1), G = kc.size(2), blocks = kc.size(0), bs = kc.size(1),
+                mb = bt.size(1), S = packed ? 0 : q.size(1), T = packed ? q.size(0) : B * S;
+  DSA_PLAIN(kind >= 0 && plain(q, dev, st) && plain(kc, dev, st) && plain(vc, dev, st) && kc.sizes() == vc.sizes() &&
+            plain(bt, dev, at::kInt) && (D == 64 || D == 128) && kc.size(3) == D && G > 0 && H % G == 0 && B > 0 &&
+            mb > 0 && blocks > 0 && bs > 0 && lens_ok(ql, dev, B) && lens_ok(kl, dev, B) &&
+            (packed ? (bool)ql : q.size(0) == B));
+  if (sinks) DSA_PLAIN(plain(*sinks.t, dev, at::kFloat) && sinks.t->dim() == 1 && sinks.t->numel() == H);
+  for (const at::Tensor* t : {&q, &kc, &vc}) DSA_PLAIN((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0);
+  const double scale = PyFloat_AS_DOUBLE(v[4]);
+  DSA_PLAIN(scale > 0 && scale <= 1e30);
+  const bool causal = v[7] == Py_True;
+  at::Tensor out, lse, ws;
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    out = make(q.sizes(), st, dev);
+    lse = make(q.sizes().slice(0, q.dim() - 1), at::kFloat, dev);
+    const size_t bytes = E.pgqa_ws(T, B, H, G, D, mb * bs);
+    if (bytes) ws = make({(int64_t)bytes}, at::kByte, dev);
+    rc = E.pgqa(kind, q.data_ptr(), kc.data_ptr(), vc.data_ptr(), bt.data_ptr<int32_t>(),
+                packed ? ql.ptr<int32_t>() : nullptr, packed ? nullptr : ql.ptr<int32_t>(), kl.ptr<int32_t>(), T, B, S,
+                H, G, D, blocks, bs, mb, causal, win, sinks.ptr<float>(), (float)scale, out.data_ptr(),
+                lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr, bytes, stream(dev));
+  }
+  DSA_RC(rc);
+  return pair(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
 // ({entry name: address})
 PyObject* bind(PyObject*, PyObject* d) {
   struct Slot {
@@ -485,7 +636,12 @@ PyObject* bind(PyObject*, PyObject* d) {
                {"dsa_lightning_indexer_tnd_fused_workspace_size", &E.tndf_ws},
                {"dsa_lightning_indexer_tnd_fused", &E.tndf},
                {"dsa_sparse_flash_mla_workspace_size", &E.v4_ws},
-               {"dsa_sparse_flash_mla", &E.v4}};
+               {"dsa_sparse_flash_mla", &E.v4},
+               {"dsa_quant_matmul_workspace_size", &E.qmm_ws},
+               {"dsa_quant_matmul", &E.qmm},
+               {"dsa_qk_norm_rope", &E.rope},
+               {"dsa_paged_gqa_workspace_size", &E.pgqa_ws},
+               {"dsa_paged_gqa_fwd", &E.pgqa}};
   for (const Slot& s : slots) {
     PyObject* o = PyDict_Check(d) ? PyDict_GetItemString(d, s.name) : nullptr;
     void* p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -511,6 +667,9 @@ PyMethodDef methods[] = {fast<topk>("topk"),
                          fast<decode_parts>("decode_parts"),
                          fast<indexer>("indexer"),
                          fast<flash_mla>("flash_mla"),
+                         fast<quant_matmul>("quant_matmul"),
+                         fast<qk_norm_rope>("qk_norm_rope"),
+                         fast<paged_gqa>("paged_gqa"),
                          {"bind", bind, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsa_host_path", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -391,6 +391,183 @@ std::tuple<at::Tensor, at::Tensor> sparse_attn_meta(const at::Tensor& q, const a
           at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat))};
 }
 
+// x [..., K] int8, weight [N, K] int8, their row scales, bias [N] -> [..., N] in dtype (bf16 by default).
+at::Tensor quant_matmul(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& x_scale,
+                        const at::Tensor& weight_scale, const c10::optional<at::Tensor>& bias,
+                        c10::optional<at::ScalarType> dtype_opt) {
+  require(x, "x");
+  require(weight, "weight");
+  require_on(weight, x, "weight");
+  TORCH_CHECK(x.scalar_type() == at::kChar && weight.scalar_type() == at::kChar,
+              "dsa.quant_matmul: x and weight must be int8");
+  TORCH_CHECK(x.dim() >= 2 && weight.dim() == 2 && weight.size(1) == x.size(-1),
+              "dsa.quant_matmul: x must be [..., K] and weight [N, K] (got ", x.sizes(), ", ", weight.sizes(), ")");
+  const at::ScalarType dtype = dtype_opt.value_or(at::kBFloat16);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
+              "dsa.quant_matmul: dtype must be bfloat16, float16 or float32");
+  const int64_t K = x.size(-1), N = weight.size(0);
+  TORCH_CHECK(K >= 1 && K <= 131071, "dsa.quant_matmul: K must be in [1, 131071] (got ", K, ")");
+  const int64_t M = x.numel() / K;
+  c10::OptionalDeviceGuard guard(x.device());
+  auto xs = aux_f32(x_scale, x, M, "x_scale");
+  auto ws = aux_f32(weight_scale, x, N, "weight_scale");
+  auto b = aux_f32(bias, x, N, "bias");
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  auto out = at::empty(sizes, x.options().dtype(dtype));
+  if (M > 0 && N > 0) {
+    const size_t bytes = dsa_quant_matmul_workspace_size(M, N, K);
+    auto work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    check_rc(dsa_quant_matmul(kind_of(out), ptr(x), ptr(weight), static_cast<float*>(ptr(xs)),
+                              static_cast<float*>(ptr(ws)), ptr_or_null<float>(b), M, N, K, ptr(out),
+                              bytes ? ptr(work) : nullptr, bytes, stream_of(x)),
+             "quant_matmul");
+  }
+  return out;
+}
+
+at::Tensor quant_matmul_meta(const at::Tensor& x, const at::Tensor& weight, const at::Tensor&, const at::Tensor&,
+                             const c10::optional<at::Tensor>&, c10::optional<at::ScalarType> dtype_opt) {
+  auto sizes = x.sizes().vec();
+  sizes.back() = weight.size(0);
+  return at::empty(sizes, x.options().dtype(dtype_opt.value_or(at::kBFloat16)));
+}
+
+// Token stride of a [T, n, D] argument whose tokens may lie apart.
+int64_t heads_stride(const at::Tensor& t, const at::Tensor& q, const char* name) {
+  require_on(t, q, name);
+  TORCH_CHECK(t.scalar_type() == q.scalar_type() && t.dim() == 3 && t.size(0) == q.size(0) && t.size(2) == q.size(2) &&
+                  t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == t.size(2)),
+              "dsa.qk_norm_rope: ", name, " must be [T, heads, D] of one dtype with contiguous heads (got ", t.sizes(),
+              ", strides ", t.strides(), ")");
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+}
+
+void norm_rope(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& v,
+               const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+               const at::Tensor& positions, const at::Tensor& cos, const at::Tensor& sin,
+               const c10::optional<at::Tensor>& slots, double eps, bool interleaved, int64_t rows, at::Tensor& q_out,
+               const at::Tensor& k_out, const c10::optional<at::Tensor>& v_out) {
+  const int64_t T = q.size(0), H = q.size(1), D = q.size(2), G = k.size(1);
+  const int64_t qs = heads_stride(q, q, "q"), ks = heads_stride(k, q, "k"), vs = v ? heads_stride(*v, q, "v") : 0;
+  TORCH_CHECK(!v || v->size(1) == G, "dsa.qk_norm_rope: v must have k's heads");
+  require_on(cos, q, "cos");
+  require_on(sin, q, "sin");
+  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), "dsa.qk_norm_rope: cos and sin must be [positions, R / 2]");
+  auto c = aux_f32(cos, q, cos.numel(), "cos"), s = aux_f32(sin, q, sin.numel(), "sin");
+  auto qw = aux_f32(q_weight, q, D, "q_weight"), kw = aux_f32(k_weight, q, D, "k_weight");
+  // 64-bit values past 32 bits mark padding; cast as they are they would come back as small ones.
+  const auto fit = [](const at::Tensor& t) { return t.scalar_type() == at::kLong ? t.clamp(-1, 0x7fffffff) : t; };
+  auto pos = aux_i32(fit(positions), q, T, "positions");
+  auto at_rows = aux_i32(slots ? c10::make_optional(fit(*slots)) : slots, q, T, "slots");
+  if (T == 0) return;
+  check_rc(dsa_qk_norm_rope(kind_of(q), ptr(q), qs, ptr(k), ks, ptr_or_null<void>(v), vs, ptr_or_null<void>(qw),
+                            ptr_or_null<void>(kw), DSA_KIND_FP32, static_cast<int32_t*>(ptr(pos)),
+                            static_cast<float*>(ptr(c)), static_cast<float*>(ptr(s)), cos.size(0), T, H, G, D,
+                            2 * cos.size(1), (float)eps, interleaved ? 1 : 0, ptr_or_null<int32_t>(at_rows), rows,
+                            ptr(q_out), ptr(k_out), ptr_or_null<void>(v_out), stream_of(q)),
+           "qk_norm_rope");
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const at::Tensor& k,
+                                                const c10::optional<at::Tensor>& q_weight,
+                                                const c10::optional<at::Tensor>& k_weight, const at::Tensor& positions,
+                                                const at::Tensor& cos, const at::Tensor& sin, double eps,
+                                                bool interleaved) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "dsa.qk_norm_rope: q and k must be [T, heads, D] on a device");
+  c10::OptionalDeviceGuard guard(q.device());
+  auto qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), q.options());
+  norm_rope(q, k, c10::nullopt, q_weight, k_weight, positions, cos, sin, c10::nullopt, eps, interleaved, 0, qo, ko,
+            c10::nullopt);
+  return {qo, ko};
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_meta(const at::Tensor& q, const at::Tensor& k,
+                                                     const c10::optional<at::Tensor>&,
+                                                     const c10::optional<at::Tensor>&, const at::Tensor&,
+                                                     const at::Tensor&, const at::Tensor&, double, bool) {
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options())};
+}
+
+// Keys and values to rows slots[t] of the caches [blocks, block_size, G, D], in place.
+at::Tensor qk_norm_rope_paged(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                              const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+                              const at::Tensor& positions, const at::Tensor& cos, const at::Tensor& sin,
+                              at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots, double eps,
+                              bool interleaved) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "dsa.qk_norm_rope: q and k must be [T, heads, D] on a device");
+  for (const at::Tensor* c : {&k_cache, &v_cache}) {
+    require(*c, "cache");
+    require_on(*c, q, "cache");
+    TORCH_CHECK(c->dim() == 4 && c->size(2) == k.size(1) && c->size(3) == q.size(2) &&
+                    c->scalar_type() == q.scalar_type() && c->sizes() == k_cache.sizes(),
+                "dsa.qk_norm_rope_paged: caches must be [blocks, block_size, ", k.size(1), ", ", q.size(2), "] (got ",
+                c->sizes(), ")");
+  }
+  c10::OptionalDeviceGuard guard(q.device());
+  auto qo = at::empty(q.sizes(), q.options());
+  norm_rope(q, k, v, q_weight, k_weight, positions, cos, sin, slots, eps, interleaved,
+            k_cache.size(0) * k_cache.size(1), qo, k_cache, v_cache);
+  return qo;
+}
+
+at::Tensor qk_norm_rope_paged_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                   const c10::optional<at::Tensor>&, const c10::optional<at::Tensor>&,
+                                   const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor, at::Tensor,
+                                   const at::Tensor&, double, bool) {
+  return at::empty(q.sizes(), q.options());
+}
+
+// q [T, H, D] (actual_seq_lengths_query: inclusive prefix sums) or [B, S, H, D] (lengths, or none).
+std::tuple<at::Tensor, at::Tensor> paged_gqa_fwd(const at::Tensor& q, const at::Tensor& k_cache,
+                                                 const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                 const at::Tensor& actual_seq_lengths_kv, double sm_scale,
+                                                 const c10::optional<at::Tensor>& actual_seq_lengths_query,
+                                                 bool is_causal, int64_t win_left,
+                                                 const c10::optional<at::Tensor>& sinks) {
+  require(q, "q");
+  require(k_cache, "k_cache");
+  require(v_cache, "v_cache");
+  require_on(k_cache, q, "k_cache");
+  require_on(v_cache, q, "v_cache");
+  TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() &&
+                  k_cache.size(3) == q.size(-1) && block_table.dim() == 2,
+              "dsa.paged_gqa_fwd: q [T, H, D] or [B, S, H, D], caches [blocks, block_size, G, D], block_table [B, n]");
+  TORCH_CHECK(k_cache.scalar_type() == q.scalar_type() && v_cache.scalar_type() == q.scalar_type(),
+              "dsa.paged_gqa_fwd: cache dtypes must equal q dtype");
+  const bool packed = q.dim() == 3;
+  const int64_t B = block_table.size(0), mb = block_table.size(1), S = packed ? 0 : q.size(1),
+                T = packed ? q.size(0) : B * S;
+  TORCH_CHECK(packed ? actual_seq_lengths_query.has_value() : q.size(0) == B,
+              "dsa.paged_gqa_fwd: packed queries need prefix sums, padded ones one row of block_table per sequence");
+  c10::OptionalDeviceGuard guard(q.device());
+  auto bt = aux_i32(block_table, q, -1, "block_table");
+  auto kl = aux_i32(actual_seq_lengths_kv, q, B, "actual_seq_lengths_kv");
+  auto ql = aux_i32(actual_seq_lengths_query, q, B, "actual_seq_lengths_query");
+  const int64_t H = q.size(-2), D = q.size(-1), G = k_cache.size(2);
+  auto sk = aux_f32(sinks, q, H, "sinks");
+  auto out = at::empty(q.sizes(), q.options());
+  auto lse = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat));
+  const size_t bytes = dsa_paged_gqa_workspace_size(T, B, H, G, D, mb * k_cache.size(1));
+  auto ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  int32_t* qlp = ptr_or_null<int32_t>(ql);
+  check_rc(dsa_paged_gqa_fwd(kind_of(q), ptr(q), ptr(k_cache), ptr(v_cache), static_cast<int32_t*>(ptr(bt)),
+                             packed ? qlp : nullptr, packed ? nullptr : qlp, static_cast<int32_t*>(ptr(kl)), T, B, S, H,
+                             G, D, k_cache.size(0), k_cache.size(1), mb, is_causal ? 1 : 0, win_left,
+                             ptr_or_null<float>(sk), (float)sm_scale, ptr(out), static_cast<float*>(ptr(lse)),
+                             bytes ? ptr(ws) : nullptr, bytes, stream_of(q)),
+           "paged_gqa_fwd");
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_gqa_fwd_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                      const at::Tensor&, const at::Tensor&, double,
+                                                      const c10::optional<at::Tensor>&, bool, int64_t,
+                                                      const c10::optional<at::Tensor>&) {
+  return {at::empty(q.sizes(), q.options()),
+          at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat))};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(dsa, m) {
@@ -408,6 +585,20 @@ TORCH_LIBRARY(dsa, m) {
       "Tensor seqused_kv, Tensor? sinks, float softmax_scale, Tensor? cmp_kv=None, Tensor? cmp_block_table=None, "
       "Tensor? cmp_sparse_indices=None, int cmp_ratio=4, int ori_win_left=127, int max_cmp=-1) -> (Tensor, Tensor)");
   m.def("act_quant(Tensor x, bool round_scale=False, ScalarType? dtype=None) -> (Tensor, Tensor)");
+  m.def(
+      "quant_matmul(Tensor x, Tensor weight, Tensor x_scale, Tensor weight_scale, Tensor? bias=None, "
+      "ScalarType? dtype=None) -> Tensor");
+  m.def(
+      "qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor positions, Tensor cos, Tensor sin, "
+      "float eps=1e-6, bool interleaved=False) -> (Tensor, Tensor)");
+  m.def(
+      "qk_norm_rope_paged(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor positions, "
+      "Tensor cos, Tensor sin, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, float eps=1e-6, "
+      "bool interleaved=False) -> Tensor");
+  m.def(
+      "paged_gqa_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor actual_seq_lengths_kv, "
+      "float sm_scale, Tensor? actual_seq_lengths_query=None, bool is_causal=True, int win_left=-1, "
+      "Tensor? sinks=None) -> (Tensor, Tensor)");
   m.def("sparse_attn(Tensor q, Tensor kv, Tensor? attn_sink, Tensor topk_idxs, float softmax_scale) -> (Tensor, Tensor)");
 }
 
@@ -418,6 +609,10 @@ TORCH_LIBRARY_IMPL(dsa, CUDA, m) {
   m.impl("sparse_flash_mla", &sparse_flash_mla);
   m.impl("act_quant", &act_quant);
   m.impl("sparse_attn", &sparse_attn);
+  m.impl("quant_matmul", &quant_matmul);
+  m.impl("qk_norm_rope", &qk_norm_rope);
+  m.impl("qk_norm_rope_paged", &qk_norm_rope_paged);
+  m.impl("paged_gqa_fwd", &paged_gqa_fwd);
 }
 
 TORCH_LIBRARY_IMPL(dsa, Meta, m) {
@@ -427,4 +622,8 @@ TORCH_LIBRARY_IMPL(dsa, Meta, m) {
   m.impl("sparse_flash_mla", &sparse_flash_mla_meta);
   m.impl("act_quant", &act_quant_meta);
   m.impl("sparse_attn", &sparse_attn_meta);
+  m.impl("quant_matmul", &quant_matmul_meta);
+  m.impl("qk_norm_rope", &qk_norm_rope_meta);
+  m.impl("qk_norm_rope_paged", &qk_norm_rope_paged_meta);
+  m.impl("paged_gqa_fwd", &paged_gqa_fwd_meta);
 }
