@@ -374,8 +374,9 @@ int dsa_act_quant(int in_kind, const void* x, int64_t rows, int64_t n, int out_k
  *  x [M, K] int8, w [N, K] int8 (a row for each output channel), x_scale [M], w_scale [N] and bias [N] (or NULL)
  *  fp32; out [M, N] of out_kind (bf16, fp16 or fp32).  The sums are exact (int32); the rest is fp32, rounded
  *  once to the output.  1 <= K <= 131071; no alignment is asked of the rows.
+ * `aligned` of the workspace query: 1 when x and w start on 16 bytes; other operands are copied into it.
  */
-size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K);
+size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int aligned);
 
 int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_scale, const float* w_scale,
                      const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,

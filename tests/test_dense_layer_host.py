@@ -1,5 +1,5 @@
 """CPU checks of the dense layer's entries: argument checks of the C ABI (no kernel is launched), host tensors,
-workspace sizes, registered schemas, the static check of the attention kernels' LDS waits."""
+workspace sizes, registered schemas, the static check of the kernels' explicit LDS waits."""
 import pytest
 import torch
 
@@ -14,8 +14,8 @@ def test_quant_matmul_c_checks(dsa):
                     (dict(K=131072), b"K must"), (dict(x=None), b"null")]:
         assert call(**kw) == 1 and msg in lib.dsa_last_error_message()
     assert call(M=0) == 0 and call(N=0) == 0
-    assert lib.dsa_quant_matmul_workspace_size(-1, 4, 64) == 0
-    assert lib.dsa_quant_matmul_workspace_size(4, 4, 0) == 0
+    assert lib.dsa_quant_matmul_workspace_size(-1, 4, 64, 1) == 0
+    assert lib.dsa_quant_matmul_workspace_size(4, 4, 0, 1) == 0
 
 
 def test_norm_rope_c_checks(dsa):
@@ -84,7 +84,8 @@ def test_meta_shapes(dsa):
     assert o.shape == q.shape and l.shape == (7, 8) and l.dtype == torch.float32
 
 
-def test_attention_lds_waits_cover_their_reads(tmp_path_factory):
-    kernels, findings = asm_lds.check_asm(_asm(tmp_path_factory, "paged_gqa.hip"))
-    assert len(kernels) >= 8, kernels
+@pytest.mark.parametrize("name,nkernels", [("paged_gqa.hip", 8), ("quant_matmul.hip", 6)])
+def test_lds_waits_cover_their_reads(tmp_path_factory, name, nkernels):
+    kernels, findings = asm_lds.check_asm(_asm(tmp_path_factory, name))
+    assert len(kernels) >= nkernels, kernels
     assert not findings, "\n".join(map(str, findings[:20]))

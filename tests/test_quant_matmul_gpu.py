@@ -21,7 +21,8 @@ def _check(out, x, w, xs, ws, bias, dtype):
 SIZES = [
     (1, 1, 1), (1, 16, 64), (2, 33, 65), (7, 129, 127), (16, 256, 512), (17, 130, 1000), (33, 513, 4096),
     (64, 576, 7168), (65, 200, 2112), (100, 512, 16), (128, 128, 128), (129, 127, 63), (255, 257, 192),
-    (256, 256, 256), (300, 1000, 1024), (513, 640, 130), (1021, 2113, 515),
+    (256, 256, 256), (300, 1000, 1024), (513, 640, 130), (1021, 2113, 515), (24, 300, 4112), (48, 1000, 2064),
+    (200, 136, 4096), (2900, 3000, 200), (2817, 3001, 77),
 ]
 
 

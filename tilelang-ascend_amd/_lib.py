@@ -85,7 +85,7 @@ SIGNATURES = {
     "dsa_sparse_attention_fwd": (_c_int, [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
                                           _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_int,
                                           _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
-    "dsa_quant_matmul_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "dsa_quant_matmul_workspace_size": (_c_size, [_c_i64, _c_i64, _c_i64, _c_int]),
     "dsa_quant_matmul": (_c_int, [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp,
                                   _c_size, _c_vp]),
     "dsa_qk_norm_rope": (_c_int, [_c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_vp,

@@ -51,7 +51,7 @@ hipError_t launch_act_quant(int in_kind, const void* x, int64_t rows, int64_t n,
 hipError_t launch_quant_matmul(int out_kind, const void* x, const void* w, const float* sx, const float* sw,
                                const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
                                hipStream_t stream);
-size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, bool aligned);
 hipError_t launch_qk_norm_rope(int is_fp16, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                                const void* v, int64_t v_stride, const void* qw, const void* kw, int w_f32,
                                const int32_t* positions, const float* cos, const float* sin, int64_t table,
@@ -556,12 +556,14 @@ static int check_quant_matmul(int64_t M, int64_t N, int64_t K) {
   // A grid dimension of 128-row tiles; int32 sums of products of at most 2^14.
   if (M < 0 || N < 0 || M > 8388480 || N > kMaxInt - 4096) return reject("quant_matmul: bad M / N");
   if (K < 1 || K > 131071) return reject("quant_matmul: K must be in [1, 131071]");
+  if (((M + 127) / 128) * ((N + 127) / 128) > kMaxInt || (M + N) * K > ((int64_t)1 << 42))
+    return reject("quant_matmul: sizes out of range");
   return 0;
 }
 
-size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K) {
+size_t dsa_quant_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int aligned) {
   if (M <= 0 || N <= 0 || check_quant_matmul(M, N, K)) return 0;
-  return dsa::quant_matmul_workspace_bytes(M, N, K);
+  return dsa::quant_matmul_workspace_bytes(M, N, K, aligned != 0);
 }
 
 int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_scale, const float* w_scale,
@@ -571,7 +573,7 @@ int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_
     return reject("quant_matmul: output kind must be bf16, fp16 or fp32");
   if (const int rc = check_quant_matmul(M, N, K)) return rc;
   if (M > 0 && N > 0 && (!x || !w || !x_scale || !w_scale || !out)) return reject("quant_matmul: null pointer");
-  const size_t need = dsa_quant_matmul_workspace_size(M, N, K);
+  const size_t need = dsa_quant_matmul_workspace_size(M, N, K, aligned16(x) && aligned16(w));
   if (workspace_bytes < need) return reject("quant_matmul: workspace too small");
   if (need > 0 && (!workspace || !aligned16(workspace))) return reject("quant_matmul: null or unaligned workspace");
   return ok(dsa::launch_quant_matmul(out_kind, x, w, x_scale, w_scale, bias, M, N, K, out, workspace,

@@ -493,7 +493,8 @@ PyObject* quant_matmul(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const NoGil unlocked;
     const c10::OptionalDeviceGuard guard(dev);
     out = make(sizes, kind == DSA_KIND_FP32 ? at::kFloat : kind == DSA_KIND_FP16 ? at::kHalf : at::kBFloat16, dev);
-    const size_t bytes = E.qmm_ws(M, N, K);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(w.data_ptr());
+    const size_t bytes = E.qmm_ws(M, N, K, (at & 15) == 0);
     if (bytes) work = make({(int64_t)bytes}, at::kByte, dev);
     rc = E.qmm((int)kind, x.data_ptr(), w.data_ptr(), xs.data_ptr<float>(), ws.data_ptr<float>(), bias.ptr<float>(), M,
                N, K, out.data_ptr(), bytes ? work.data_ptr() : nullptr, bytes, stream(dev));

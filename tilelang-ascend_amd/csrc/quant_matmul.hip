@@ -18,7 +18,8 @@ struct QmmArgs {
   const float* sw;    // [N]
   const float* bias;  // [N] or null
   void* out;          // [M, N]
-  int M, N, K;
+  int* part;          // [splits, M, part_ld] sums of a split product
+  int M, N, K, part_ld;
 };
 
 // i32 16x16 += A 16x64 B 64x16: lane (r = lane & 15, g = lane >> 4) gives row r of A and column r of B,
@@ -49,12 +50,21 @@ __device__ __forceinline__ void qmm_store4(void* out, int64_t at, const float (&
   }
 }
 
-// Any sizes and any alignment: 128 x 128 of the output a workgroup, 64 x 64 a wave, k in steps of 64 through two
-// LDS stages.  A row's 16-byte chunks are read where they lie (byte aligned); the chunk that K ends in is
-// read by bytes.  LDS rows hold 4 chunks; chunk c of row r lies at c ^ 2 ((r >> 3) & 1), so that the 32 chunks a
-// half wave reads at once (16 rows, two chunks) fall on distinct banks.
-constexpr int kQmmTile = 128;
-constexpr int kQmmStep = 64;
+// The scaled, biased value of a sum.
+__device__ __forceinline__ float qmm_value(const QmmArgs& a, int sum, int n, float sx) {
+  float v = (float)sum * sx * a.sw[n];
+  if (a.bias) v += a.bias[n];
+  return v;
+}
+
+// Up to 16 tokens: bound by the weights' bytes.  A workgroup takes 16 output channels and all tokens; its eight
+// waves share the rows' bytes, 128 of each row at a time, and load straight into the product's operands, four such
+// units ahead (two: 16 tokens of 9216 x 7168 took 23.6 us instead of 21.6; eight: 24.1): nothing is shared between
+// waves but the sums, joined through LDS.  Rows may start at any byte; the unit that K ends in is read by chunks that
+// are cut there.  One token of 9216 x 7168: 15.6 us, 4.2 TB/s.
+constexpr int kQmmRowWaves = 8;
+constexpr int kQmmUnit = 128;
+constexpr int kQmmDeep = 4;
 
 __device__ __forceinline__ u32x4 qmm_chunk(const uint8_t* row, int k, int K) {
   u32x4 v = {0, 0, 0, 0};
@@ -67,111 +77,401 @@ __device__ __forceinline__ u32x4 qmm_chunk(const uint8_t* row, int k, int K) {
 }
 
 template <int kOut>
-__global__ __launch_bounds__(256, 2) void qmm_tile_kernel(QmmArgs a) {
-  __shared__ __align__(16) uint8_t lds[2][2][kQmmTile * kQmmStep];  // stage, operand (w, x)
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+__global__ __launch_bounds__(kQmmRowWaves * kWave) void qmm_rows_kernel(QmmArgs a) {
+  __shared__ __align__(16) int part[kQmmRowWaves][16 * 16];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, g = lane >> 4;
-  const int m0 = blockIdx.y * kQmmTile, n0 = blockIdx.x * kQmmTile;
-  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64;
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* wr = a.w + (int64_t)min(n0 + r, a.N - 1) * a.K;
+  const uint8_t* xr = a.x + (int64_t)min(r, a.M - 1) * a.K;
 
-  // Thread t stages chunks t & 3 of rows t / 4 and t / 4 + 64; rows past the edge repeat the last one.
-  const uint8_t* src[2][2];
-  int dst[2];
+  i32x4 acc = {0, 0, 0, 0};
+  u32x4 wv[kQmmDeep][2], xv[kQmmDeep][2];
+  auto load = [&](int d, int k) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int row = tid / 4 + 64 * j;
-    src[0][j] = a.w + (int64_t)min(n0 + row, a.N - 1) * a.K;
-    src[1][j] = a.x + (int64_t)min(m0 + row, a.M - 1) * a.K;
-    dst[j] = row * kQmmStep + 16 * ((tid & 3) ^ (2 * ((row >> 3) & 1)));
-  }
-  u32x4 reg[2][2];
-  auto load = [&](int k0) {
-    const int k = k0 + 16 * (tid & 3);
-    if (k0 + kQmmStep <= a.K) {
-#pragma unroll
-      for (int o = 0; o < 2; ++o)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) __builtin_memcpy(&reg[o][j], src[o][j] + k, 16);
-    } else {
-#pragma unroll
-      for (int o = 0; o < 2; ++o)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) reg[o][j] = qmm_chunk(src[o][j], k, a.K);
+    for (int h = 0; h < 2; ++h) {
+      __builtin_memcpy(&wv[d][h], wr + k + 64 * h + 16 * g, 16);
+      __builtin_memcpy(&xv[d][h], xr + k + 64 * h + 16 * g, 16);
     }
   };
-  auto put = [&](int st) {
+  auto mul = [&](int d) {
 #pragma unroll
-    for (int o = 0; o < 2; ++o)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) *reinterpret_cast<u32x4*>(&lds[st][o][dst[j]]) = reg[o][j];
+    for (int h = 0; h < 2; ++h) acc = qmm_mfma(wv[d][h], xv[d][h], acc);
   };
-  i32x4 acc[4][4];  // [n block][m block]
+  const int full = a.K / kQmmUnit;  // whole units; wave w takes units w, w + 8, ...
+  const int mine = full > wave ? (full - wave + kQmmRowWaves - 1) / kQmmRowWaves : 0;
+  const int step = kQmmRowWaves * kQmmUnit;
+  int k = wave * kQmmUnit;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int d = 0; d < kQmmDeep; ++d)
+    if (d < mine) load(d, k + d * step);
+  int e = 0;
+  for (; e + 2 * kQmmDeep <= mine; e += kQmmDeep) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-
-  const int off = r * kQmmStep + 16 * (g ^ (2 * ((r >> 3) & 1)));
-  const int steps = (a.K + kQmmStep - 1) / kQmmStep;
-  load(0);
-  put(0);
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();
-    if (s + 1 < steps) load((s + 1) * kQmmStep);
-    const uint8_t *lw = lds[s & 1][0] + wn * kQmmStep + off, *lx = lds[s & 1][1] + wm * kQmmStep + off;
-    u32x4 wv[4], xv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const u32x4*>(lw + i * 16 * kQmmStep);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xv[i] = *reinterpret_cast<const u32x4*>(lx + i * 16 * kQmmStep);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = qmm_mfma(wv[i], xv[j], acc[i][j]);
-    // The other stage's reads were done before the barrier above.
-    if (s + 1 < steps) put((s + 1) & 1);
+    for (int d = 0; d < kQmmDeep; ++d) {
+      mul(d);
+      load(d, k + (kQmmDeep + d) * step);
+    }
+    k += kQmmDeep * step;
   }
+  for (; e < mine; e += kQmmDeep) {  // at most twice
+#pragma unroll
+    for (int d = 0; d < kQmmDeep; ++d) {
+      if (e + d < mine) mul(d);
+      if (e + kQmmDeep + d < mine) load(d, k + (kQmmDeep + d) * step);
+    }
+    k += kQmmDeep * step;
+  }
+  if (full * kQmmUnit < a.K && full % kQmmRowWaves == wave) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int kk = full * kQmmUnit + 64 * h + 16 * g;
+      wv[0][h] = qmm_chunk(wr, kk, a.K);
+      xv[0][h] = qmm_chunk(xr, kk, a.K);
+    }
+    mul(0);
+  }
+  *reinterpret_cast<i32x4*>(&part[wave][r * 16 + 4 * g]) = acc;
+  __syncthreads();
+  const int m = tid / 16, n = n0 + tid % 16;
+  if (m >= a.M || n >= a.N) return;
+  int sum = 0;
+#pragma unroll
+  for (int v = 0; v < kQmmRowWaves; ++v) sum += part[v][tid];
+  qmm_store1<kOut>(a.out, (int64_t)m * a.N + n, qmm_value(a, sum, n, a.sx[m]));
+}
 
+// More tokens: kBM x kBN of the output a workgroup, bound by the matrix cores.  The operands' rows stream into
+// LDS by DMA, 128 bytes of each at a time, two stages; a wave multiplies kTM tokens by 64 channels (32x32x32
+// products, channels on the M axis).  Chunk c (16 bytes) of row r lies at c ^ ((r >> 2) & 7), so that the 32 rows
+// a half wave reads at one c fall on distinct banks; the DMA fetches the chunks in that order.  Rows start on 16
+// bytes and hold whole chunks (qmm_pack_kernel sees to it where they do not); chunks past K come from a row of zeros.
+// 16384 x 9216 x 7168: 1089 us, 1988 TOP/s; the DMA alone takes 836 us there, the LDS reads 495, and the matrix cores
+// reach 3200 to 3700 on random operands (clock), a library's 8192^3 2089.
+// With kSplit the steps are dealt to gridDim.z workgroups, which leave int32 sums for qmm_join_kernel.
+constexpr int kQmmStep = 128;                    // whole lines of a row: with 64 (four stages) 16384 x 9216 x 7168
+constexpr int kQmmStages = 2;                    // took 1120 us, 1089 with 128
+constexpr int kQmmLanes = kQmmStep / 16;         // of a row in a DMA instruction
+constexpr int kQmmRows = kWave / kQmmLanes;      // rows of a DMA instruction
+constexpr int kQmmParts = kQmmStep / 32;
+__host__ __device__ constexpr int qmm_swz(int row) { return (row / (512 / kQmmStep)) & (kQmmLanes - 1); }
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void qmm_lds_void;
+typedef const __attribute__((address_space(1))) void qmm_gbl_void;
+static __device__ __align__(128) uint8_t kQmmZeros[16];
+
+// LDS reads as inline asm: through plain loads the compiler would wait for every DMA in flight before each.
+template <int kOff>
+__device__ __forceinline__ void qmm_b128(u32x4& out, uint32_t addr) {
+  __asm__ __volatile__("ds_read_b128 %0, %1 offset:%2" : "=v"(out) : "v"(addr), "i"(kOff));
+}
+// All but the kLeft youngest LDS reads have returned; v passes through so that no use moves above the wait.
+template <int kLeft, int N>
+__device__ __forceinline__ void qmm_lds_wait(u32x4 (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) __asm__ __volatile__("" : "+v"(v[i]));
+  __asm__ __volatile__("s_waitcnt lgkmcnt(%0)" ::"i"(kLeft) : "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) __asm__ __volatile__("" : "+v"(v[i]));
+}
+
+template <int kBM, int kBN, int kWM, int kWN>
+struct QmmShape {
+  static constexpr int kWaves = kWM * kWN, kTM = kBM / kWM, kTN = kBN / kWN;
+  static constexpr int kFM = kTM / 32, kFN = kTN / 32;
+  static constexpr int kStage = (kBM + kBN) * kQmmStep;
+  static constexpr int kInstr = (kBM + kBN) / kQmmRows / kWaves;  // DMA instructions of a wave and step
+  static_assert((kBM + kBN) % (kQmmRows * kWaves) == 0 && kBN % 32 == 0, "whole DMA instructions");
+};
+
+template <int kOut, int kBM, int kBN, int kWM, int kWN, bool kSplit>
+__global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
+  typedef QmmShape<kBM, kBN, kWM, kWN> S;
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  // Consecutive workgroup ids go to the eight XCDs in turn: each XCD takes a run of tiles of its own, in groups of
+  // 8 rows of tiles walked column by column, so that the tiles in flight on it share operand rows in its L2.
+  const int tm = (a.M + kBM - 1) / kBM, tn = (a.N + kBN - 1) / kBN, tiles = tm * tn;
+  int id = blockIdx.x;
+  {
+    const int per = tiles / 8, rest = tiles % 8, x = id & 7, i = id >> 3;
+    id = x * per + min(x, rest) + i;
+  }
+  constexpr int kGroup = 8;
+  const int grp = id / (kGroup * tn), in = id - grp * kGroup * tn;
+  const int height = min(kGroup, tm - grp * kGroup);
+  const int m0 = (grp * kGroup + in % height) * kBM, n0 = in / height * kBN;
+  const int wn = (wave % kWN) * S::kTN, wm = (wave / kWN) * S::kTM;
+
+  const int all = (a.K + kQmmStep - 1) / kQmmStep;
+  int s0 = 0, s1 = all;
+  if constexpr (kSplit) {
+    s0 = (int)((int64_t)all * blockIdx.z / gridDim.z);
+    s1 = (int)((int64_t)all * (blockIdx.z + 1) / gridDim.z);
+  }
+  // The rows of instruction wave + kWaves * j of the stage (channels, then tokens); edge rows repeat the last.
+  const uint8_t* src[S::kInstr];
+  int chunks[S::kInstr];
+#pragma unroll
+  for (int j = 0; j < S::kInstr; ++j) {
+    const int row = kQmmRows * (wave + S::kWaves * j) + lane / kQmmLanes;
+    const bool is_w = row < kBN;
+    chunks[j] = 16 * ((lane & (kQmmLanes - 1)) ^ qmm_swz(row));  // kBN is a multiple of 32: the same in either operand
+    const int64_t at = is_w ? min(n0 + row, a.N - 1) : min(m0 + row - kBN, a.M - 1);
+    src[j] = (is_w ? a.w : a.x) + at * a.K + chunks[j] + (int64_t)s0 * kQmmStep;
+  }
+  auto dma = [&](int s) {
+    uint8_t* dst = lds + (s & 1) * S::kStage;
+    if ((s + 1) * kQmmStep <= a.K) {
+#pragma unroll
+      for (int j = 0; j < S::kInstr; ++j) {
+        __builtin_amdgcn_global_load_lds((qmm_gbl_void*)src[j], (qmm_lds_void*)(dst + (wave + S::kWaves * j) * 1024), 16,
+                                         0, 0);
+        src[j] += kQmmStep;
+      }
+    } else {  // the last step of a K off 128
+#pragma unroll
+      for (int j = 0; j < S::kInstr; ++j) {
+        const uint8_t* p = s * kQmmStep + chunks[j] < a.K ? src[j] : kQmmZeros;
+        __builtin_amdgcn_global_load_lds((qmm_gbl_void*)p, (qmm_lds_void*)(dst + (wave + S::kWaves * j) * 1024), 16, 0, 0);
+      }
+    }
+  };
+  i32x16 acc[S::kFN][S::kFM];
+#pragma unroll
+  for (int i = 0; i < S::kFN; ++i)
+#pragma unroll
+    for (int j = 0; j < S::kFM; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+  const int r = lane & 31, hi = lane >> 5;
+  uint32_t off[kQmmParts];
+#pragma unroll
+  for (int q = 0; q < kQmmParts; ++q) off[q] = r * kQmmStep + 16 * ((2 * q + hi) ^ qmm_swz(r));
+  const uint32_t lw = (uint32_t)(uintptr_t)(const qmm_lds_void*)(lds + wn * kQmmStep);
+  const uint32_t lx = (uint32_t)(uintptr_t)(const qmm_lds_void*)(lds + (kBN + wm) * kQmmStep);
+
+  // A step's parts (32 bytes of each row): the reads of the next part are in flight under a part's products, across
+  // the step's end too, where the barrier lies ahead of the last part's products.
+  constexpr int kR = S::kFN + S::kFM;
+  u32x4 v[2][kR];
+  auto read = [&](u32x4(&o)[kR], int s, int q) {
+    const uint32_t st = (s & 1) * S::kStage, w = lw + st + off[q], x = lx + st + off[q];
+    qmm_b128<0>(o[0], w);
+    qmm_b128<32 * kQmmStep>(o[1], w);
+    qmm_b128<0>(o[2], x);
+    if constexpr (S::kFM > 1) qmm_b128<32 * kQmmStep>(o[3], x);
+    if constexpr (S::kFM > 2) qmm_b128<64 * kQmmStep>(o[4], x);
+    if constexpr (S::kFM > 3) qmm_b128<96 * kQmmStep>(o[5], x);
+  };
+  static_assert(S::kFN == 2 && S::kFM <= 4, "the reads above");
+  auto mul = [&](const u32x4(&o)[kR]) {
+#pragma unroll
+    for (int j = 0; j < S::kFM; ++j)
+#pragma unroll
+      for (int i = 0; i < S::kFN; ++i)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, o[i]),
+                                                          __builtin_bit_cast(i32x4, o[S::kFN + j]), acc[i][j], 0, 0, 0);
+  };
+  // This wave's part of the youngest stage is in LDS; behind the barrier everyone's is, and all reads of the stage
+  // before it are done.
+  auto turn = [&] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __builtin_amdgcn_s_barrier();
+  };
+  dma(s0);
+  turn();
+  if (s0 + 1 < s1) dma(s0 + 1);
+  read(v[0], s0, 0);
+  auto parts = [&](int s) {  // all products of the stage but the last part's, whose operands are left in v[1]
+#pragma unroll
+    for (int q = 0; q < kQmmParts - 1; ++q) {
+      read(v[(q + 1) & 1], s, q + 1);
+      qmm_lds_wait<kR>(v[q & 1]);
+      mul(v[q & 1]);
+    }
+    qmm_lds_wait<0>(v[1]);
+  };
+  for (int s = s0; s + 1 < s1; ++s) {
+    parts(s);
+    turn();
+    if (s + 2 < s1) dma(s + 2);
+    read(v[0], s + 1, 0);
+    mul(v[1]);
+  }
+  parts(s1 - 1);
+  mul(v[1]);
+
+  // Lane (r, hi) holds channels 8 c + 4 hi + e (c = 0 .. 3, e = 0 .. 3) of token r of a 32 x 32 block.
   const bool vec = (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = m0 + wm + 16 * j + r;
+  for (int j = 0; j < S::kFM; ++j) {
+    const int m = m0 + wm + 32 * j + r;
     if (m >= a.M) continue;
     const float sx = a.sx[m];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + wn + 16 * i + 4 * g;
-      float v[4];
+    for (int i = 0; i < S::kFN; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int ne = min(n + e, a.N - 1);
-        v[e] = (float)acc[i][j][e] * sx * a.sw[ne];
-        if (a.bias) v[e] += a.bias[ne];
-      }
-      const int64_t at = (int64_t)m * a.N + n;
-      if (vec) {
-        if (n < a.N) qmm_store4<kOut>(a.out, at, v);
-      } else {
+      for (int c = 0; c < 4; ++c) {
+        const int n = n0 + wn + 32 * i + 8 * c + 4 * hi;
+        if constexpr (kSplit) {
+          // Rows of the sums are padded to a multiple of 4 channels.
+          if (n < a.N)
+            *reinterpret_cast<i32x4*>(a.part + ((int64_t)blockIdx.z * a.M + m) * a.part_ld + n) =
+                i32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
+        } else {
+          float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < a.N) qmm_store1<kOut>(a.out, at + e, v[e]);
+          for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, acc[i][j][4 * c + e], min(n + e, a.N - 1), sx);
+          const int64_t at = (int64_t)m * a.N + n;
+          if (vec) {
+            if (n < a.N) qmm_store4<kOut>(a.out, at, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.N) qmm_store1<kOut>(a.out, at + e, v[e]);
+          }
+        }
       }
-    }
   }
 }
 
+// Sums of the splits, scaled and biased: four channels a thread.
 template <int kOut>
-static hipError_t qmm_launch(const QmmArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.N + kQmmTile - 1) / kQmmTile), (unsigned)((a.M + kQmmTile - 1) / kQmmTile));
-  hipLaunchKernelGGL((qmm_tile_kernel<kOut>), grid, dim3(256), 0, stream, a);
+__global__ __launch_bounds__(256) void qmm_join_kernel(QmmArgs a, int splits) {
+  const int quads = a.part_ld / 4;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (int64_t)a.M * quads) return;
+  const int m = (int)(t / quads), n = 4 * (int)(t - (int64_t)m * quads);
+  i32x4 sum = {0, 0, 0, 0};
+  for (int z = 0; z < splits; ++z)
+    sum += *reinterpret_cast<const i32x4*>(a.part + ((int64_t)z * a.M + m) * a.part_ld + n);
+  const float sx = a.sx[m];
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, sum[e], min(n + e, a.N - 1), sx);
+  const int64_t at = (int64_t)m * a.N + n;
+  if ((a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+    qmm_store4<kOut>(a.out, at, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) qmm_store1<kOut>(a.out, at + e, v[e]);
+  }
+}
+
+// Rows of K bytes anywhere to rows of ld bytes (a multiple of 128) on 16 bytes, zeros behind K: a chunk a thread.
+__global__ __launch_bounds__(256) void qmm_pack_kernel(const uint8_t* x, int64_t M, const uint8_t* w, int64_t N, int K,
+                                                       int ld, uint8_t* to) {
+  const int chunks = ld / 16;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= (M + N) * chunks) return;
+  const int64_t row = t / chunks;
+  const int k = 16 * (int)(t - row * chunks);
+  *reinterpret_cast<u32x4*>(to + t * 16) = qmm_chunk(row < M ? x + row * K : w + (row - M) * K, k, K);
+}
+
+// The launch of a call: which kernel, and the workspace's parts.
+struct QmmPlan {
+  int tile;    // 16: the kernel for few tokens; 32, 64, 128: tokens of a tile of 128 channels; 256: of 256 channels
+  bool pack;   // operands copied to aligned rows first
+  int splits;  // workgroups that share a tile's K
+  size_t pack_bytes, part_bytes;
+};
+
+static int64_t qmm_ld(int64_t K) { return (K + 127) / 128 * 128; }
+
+// `odd`: rows do not start on 16 bytes or hold no whole number of chunks.
+static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
+  QmmPlan p = {16, false, 1, 0, 0};
+  // Up to 16 tokens every workgroup reads all of x beside its 16 rows of w: one token of 9216 x 7168 takes 15.6 us
+  // (19.7 with split tiles), 16 tokens 21.6 (20.5); 32 tokens 33 against 21.4, 64 (7168 x 8192) 28.8 against 20.7.
+  if (M <= 16) return p;
+  p.pack = odd;
+  if (odd) p.pack_bytes = (size_t)((M + N) * qmm_ld(K));
+  p.tile = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  const int64_t small = ((M + p.tile - 1) / p.tile) * ((N + 127) / 128);
+  const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+  // The larger tile multiplies 1.2 times as fast (8192^3: 1932 against 1595 TOP/s) where the rounds of 256
+  // workgroups it makes are as full as the rounds of 512 of the smaller one.
+  const double full_big = (double)big / (double)((big + 255) / 256 * 256);
+  const double full_small = (double)small / (double)((small + 511) / 512 * 512);
+  if (p.tile == 128 && full_big > 0.82 * full_small && big >= 128) {
+    p.tile = 256;
+    return p;
+  }
+  // Few tiles share their K, up to two workgroups a CU and eight steps each.
+  const int64_t steps = (K + kQmmStep - 1) / kQmmStep;
+  while (p.splits < 8 && small * p.splits * 2 <= 512 && steps >= 8 * p.splits) p.splits *= 2;
+  if (p.splits > 1) p.part_bytes = (size_t)(p.splits * M * ((N + 3) / 4 * 4) * 4);
+  return p;
+}
+
+static bool qmm_odd_rows(const void* x, const void* w, int64_t K) {
+  return K % 16 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) != 0;
+}
+
+// `aligned`: the operands start on 16 bytes.
+size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
+  const QmmPlan p = qmm_plan(M, N, K, !aligned || K % 16 != 0);
+  return p.pack_bytes + p.part_bytes;
+}
+
+template <int kOut, int kBM, int kBN, int kWM, int kWN, bool kSplit>
+static hipError_t qmm_launch_tile(const QmmArgs& a, int splits, hipStream_t stream) {
+  constexpr int lds = kQmmStages * QmmShape<kBM, kBN, kWM, kWN>::kStage;
+  static_assert(lds <= 160 * 1024, "LDS");
+  const hipError_t e = set_dynamic_lds_once<qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kSplit>>(lds);
+  if (e != hipSuccess) return e;
+  const dim3 grid((unsigned)(((a.M + kBM - 1) / kBM) * ((a.N + kBN - 1) / kBN)), 1, splits);
+  hipLaunchKernelGGL((qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kSplit>), grid, dim3(kWM * kWN * kWave), lds, stream, a);
   return hipGetLastError();
 }
 
-size_t quant_matmul_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+template <int kOut, int kBM, int kWM, int kWN>
+static hipError_t qmm_launch_shared(const QmmArgs& a, int splits, hipStream_t stream) {
+  if (splits == 1) return qmm_launch_tile<kOut, kBM, 128, kWM, kWN, false>(a, 1, stream);
+  const hipError_t e = qmm_launch_tile<kOut, kBM, 128, kWM, kWN, true>(a, splits, stream);
+  if (e != hipSuccess) return e;
+  const int64_t quads = (int64_t)a.M * (a.part_ld / 4);
+  hipLaunchKernelGGL((qmm_join_kernel<kOut>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
+  return hipGetLastError();
+}
 
-// Caller validated: 1 <= K <= 131071, M and N within the grid (M <= 65535 * 128), out_kind in {bf16, fp16, fp32}.
+template <int kOut>
+static hipError_t qmm_launch(QmmArgs a, void* workspace, hipStream_t stream) {
+  const QmmPlan p = qmm_plan(a.M, a.N, a.K, qmm_odd_rows(a.x, a.w, a.K));
+  if (p.tile == 16) {
+    hipLaunchKernelGGL((qmm_rows_kernel<kOut>), dim3((unsigned)((a.N + 15) / 16)), dim3(kQmmRowWaves * kWave), 0, stream,
+                       a);
+    return hipGetLastError();
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.part = reinterpret_cast<int*>(ws + p.pack_bytes);
+  a.part_ld = (a.N + 3) / 4 * 4;
+  if (p.pack) {
+    const int ld = (int)qmm_ld(a.K);
+    const int64_t chunks = ((int64_t)a.M + a.N) * (ld / 16);
+    hipLaunchKernelGGL(qmm_pack_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, stream, a.x, (int64_t)a.M,
+                       a.w, (int64_t)a.N, a.K, ld, ws);
+    a.x = ws;
+    a.w = ws + (int64_t)a.M * ld;
+    a.K = ld;
+  }
+  switch (p.tile) {
+    case 32: return qmm_launch_shared<kOut, 32, 1, 2>(a, p.splits, stream);
+    case 64: return qmm_launch_shared<kOut, 64, 2, 2>(a, p.splits, stream);
+    case 128: return qmm_launch_shared<kOut, 128, 2, 2>(a, p.splits, stream);
+    default: return qmm_launch_tile<kOut, 256, 256, 2, 4, false>(a, 1, stream);
+  }
+}
+
+// Caller validated: 1 <= K <= 131071, M and N within the grids, out_kind in {bf16, fp16, fp32}, a workspace of
+// quant_matmul_workspace_bytes.
 hipError_t launch_quant_matmul(int out_kind, const void* x, const void* w, const float* sx, const float* sw,
-                               const float* bias, int64_t M, int64_t N, int64_t K, void* out, void*,
+                               const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
                                hipStream_t stream) {
   if (M == 0 || N == 0) return hipSuccess;
   QmmArgs a;
@@ -184,10 +484,12 @@ hipError_t launch_quant_matmul(int out_kind, const void* x, const void* w, const
   a.M = (int)M;
   a.N = (int)N;
   a.K = (int)K;
+  a.part = nullptr;
+  a.part_ld = 0;
   switch (out_kind) {
-    case kQmmBf16: return qmm_launch<kQmmBf16>(a, stream);
-    case kQmmFp16: return qmm_launch<kQmmFp16>(a, stream);
-    default: return qmm_launch<kQmmFp32>(a, stream);
+    case kQmmBf16: return qmm_launch<kQmmBf16>(a, workspace, stream);
+    case kQmmFp16: return qmm_launch<kQmmFp16>(a, workspace, stream);
+    default: return qmm_launch<kQmmFp32>(a, workspace, stream);
   }
 }
 

@@ -416,7 +416,8 @@ at::Tensor quant_matmul(const at::Tensor& x, const at::Tensor& weight, const at:
   sizes.back() = N;
   auto out = at::empty(sizes, x.options().dtype(dtype));
   if (M > 0 && N > 0) {
-    const size_t bytes = dsa_quant_matmul_workspace_size(M, N, K);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(ptr(x)) | reinterpret_cast<uintptr_t>(ptr(weight));
+    const size_t bytes = dsa_quant_matmul_workspace_size(M, N, K, (at & 15) == 0);
     auto work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
     check_rc(dsa_quant_matmul(kind_of(out), ptr(x), ptr(weight), static_cast<float*>(ptr(xs)),
                               static_cast<float*>(ptr(ws)), ptr_or_null<float>(b), M, N, K, ptr(out),

@@ -54,7 +54,8 @@ def quant_matmul(x: torch.Tensor, weight: torch.Tensor, x_scale: torch.Tensor, w
         out = torch.empty(x.shape[:-1] + (N,), dtype=dtype, device=dev)
         if M and N:
             lib = _lib.load_library()
-            ws_bytes = lib.dsa_quant_matmul_workspace_size(M, N, K)
+            aligned = (x.data_ptr() | weight.data_ptr()) % 16 == 0
+            ws_bytes = lib.dsa_quant_matmul_workspace_size(M, N, K, 1 if aligned else 0)
             ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
             rc = lib.dsa_quant_matmul(_OUT[dtype], _lib.ptr(x), _lib.ptr(weight), _lib.ptr(x_scale),
                                       _lib.ptr(weight_scale), _lib.ptr(bias), M, N, K, _lib.ptr(out), _lib.ptr(ws),
