@@ -10,26 +10,37 @@
 // lse = -inf (or its sink).
 //
 // Rows.  The Hg heads of a group's tokens are rows of one product: row rho = i * Hg + h of sequence b and group g,
-// cut into tiles of 16 kHB rows, so that each key is read once for a tile whatever Hg.  Tile i of sequence b has
-// the slot floor(start_b * Hg / rows) + b + i: sequences get disjoint slots without a prefix sum, and a grid of
-// floor(T * Hg / rows) + B + 1 slots holds them all (b = B is the padding behind the last packed sequence).
+// cut into tiles of kR rows, so that each key is read once for a tile whatever Hg.  Tile i of sequence b has
+// the slot floor(start_b * Hg / kR) + b + i: sequences get disjoint slots without a prefix sum, and a grid of
+// floor(T * Hg / kR) + B + 1 slots holds them all (b = B is the padding behind the last packed sequence).
 //
-// Work split.  A workgroup's four waves take 32 keys each of a unit of 128, every wave with a ring of its own
-// in LDS (no workgroup barrier in the loop), an online softmax and a merge at the end.  Where there are tiles enough
-// a workgroup takes a tile and all its keys.  Otherwise the units of all tiles form one line that is cut into
-// equal parts, a workgroup each, so that batches of uneven lengths load the card evenly; a tile whose line is
-// cut leaves parts (unnormalised sums in fp32, with maximum and sum) that a second launch joins.
+// Two ways over a tile's keys, by rows per sequence (pg_plan):
+//  - pg_keys: 16 or 32 rows, for decode batches, bound by the caches' bytes.  Four waves hold the same rows and
+//    take 32 keys each of a unit of 128, every wave with a ring of its own in LDS and no barrier in the loop; the
+//    waves' sums are merged at the end.
+//  - pg_rows: 256 rows, 32 a wave, for chunks and prompts, bound by matrix cores, exponentials and LDS reads alike.
+//    Eight waves share tiles of 64 keys in LDS.  Waves w and w + 4 lie on one SIMD and take turns: one
+//    multiplies (scores of a tile and the products of the tile before with V) while the other takes exponentials.
 //
-// Per 32 keys and wave: S^T = K Q^T (keys on the M axis of 16x16x32 products), the softmax in base 2 (a lane holds
-// 8 scores of one row), O^T += V^T P^T with V^T through transposing LDS reads.
+// Work split.  Where there are tiles enough a workgroup takes a tile and all its keys.  Otherwise the units of all
+// tiles form one line that is cut into equal parts, a workgroup each, so that batches of uneven lengths load
+// the card evenly; a tile whose line is cut leaves parts (unnormalised sums in fp32, with maximum and sum) that a
+// second launch joins.
+//
+// S^T = K Q^T with keys on the M axis, so that a lane holds many scores of one row; softmax in base 2; O^T += V^T P^T
+// with V^T through transposing LDS reads.  Probabilities are rounded to the caches' 16 bits for that product, the sum
+// of them is taken before the rounding, in fp32, as maxima and all sums are.
+#include <type_traits>
+
 #include "gqa_common.hpp"
 
 namespace dsa {
 
-constexpr int kPgTile = 32;                 // keys a wave takes at once
+constexpr int kPgTile = 32;                 // keys a wave of pg_keys takes at once
 constexpr int kPgWaves = 4;
 constexpr int kPgThreads = kPgWaves * kWave;
 constexpr int kPgUnit = kPgWaves * kPgTile;  // 128 keys
+constexpr int kPgMaxSlots = 1024;            // of a call whose tiles share the line of units
 constexpr float kPgInf = __builtin_huge_valf();
 
 struct PgArgs {
@@ -45,6 +56,9 @@ struct PgArgs {
   float* lse;             // [T, H]
   float* part;            // parts: sums [16 kHB, D], then (maximum, sum) [16 kHB, 2]
   int T, B, S, H, G, Hg, block_size, max_blocks, num_blocks, causal, win, wgs;
+  int slots;              // of the call
+  uint32_t div_mul;       // j / block_size = umulhi(j, div_mul) >> div_shift for 0 <= j < 2^31; 0: block_size is 1
+  int div_shift;
   float scale_log2;  // sm_scale * log2(e)
 };
 
@@ -82,21 +96,25 @@ __host__ __device__ constexpr int pg_swz(int k) {
   return kD == 128 ? 4 * ((k >> 1) & 3) + 2 * ((k >> 3) & 1) : 2 * ((k >> 2) & 3);
 }
 
-template <int kHB, int kD>
-__host__ __device__ constexpr int pg_part_floats() { return 16 * kHB * (kD + 2); }
+// Floats of a part: the rows' sums, then their (maximum, sum).
+template <int kR, int kD>
+__host__ __device__ constexpr int pg_part_floats() { return kR * (kD + 2); }
 
-// Two stages of K and V of 32 keys a wave; the merge reuses a wave's ring, its (maximum, sum) lie behind.
-template <int kHB, int kD>
-__host__ __device__ constexpr int pg_lds_bytes() { return kPgWaves * 2 * 2 * kPgTile * kD * 2 + kPgWaves * 16 * kHB * 2 * 4; }
+// j / block_size for 0 <= j < 2^31.  With l = ceil(log2 d) and M = floor(2^(31 + l) / d) + 1, M d exceeds 2^(31 + l) by
+// at most 2^l, so j M / 2^(31 + l) exceeds j / d by less than 1 / d and has its whole part.
+__device__ __forceinline__ int pg_block(const PgArgs& a, int j) {
+  return a.div_mul ? (int)(__umulhi((uint32_t)j, a.div_mul) >> a.div_shift) : j;
+}
 
 // Keys behind a sequence's last one, and of pages outside the pool, load this row: 0 times what lies there need
 // not be 0.
 static __device__ __align__(128) uint8_t kPgZeroRow[256];
 
 // The keys [k0, k1) of tile `tile` of sequence s, group kvg; `whole`: these are all its keys (the result goes to
-// out and lse, otherwise to the part).
+// out and lse, otherwise to the part).  Two stages of K and V of 32 keys a wave; the merge reuses a wave's ring, its
+// (maximum, sum) lie behind.
 template <bool kF16, int kD, int kHB>
-__device__ __forceinline__ void pg_item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
+__device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
   constexpr int kRow = kD * 2;
   constexpr int kTileBytes = kPgTile * kRow;
@@ -146,7 +164,7 @@ __device__ __forceinline__ void pg_item(const PgArgs& a, const PgSeq& s, int b, 
   auto phys = [&](int j) {
     int row = -1;
     if (j < k1) {
-      const int blk = j / a.block_size, page = bt[blk];
+      const int blk = pg_block(a, j), page = bt[blk];
       if (page >= 0 && page < a.num_blocks) row = page * a.block_size + (j - blk * a.block_size);
     }
     return row;
@@ -351,210 +369,605 @@ __device__ __forceinline__ void pg_item(const PgArgs& a, const PgSeq& s, int b, 
   __syncthreads();  // the rings are free for the next item
 }
 
-// Slot of the first tile of sequence b, rows of one tile kR: strictly increasing in b.
+// LDS position of 16-byte chunk c of key k of pg_rows' tiles is c ^ pr_swz(k).  K operand reads (a half wave: 32 keys,
+// one chunk) meet each position of the 512 bytes of all banks once: bits 1 to 4 of the key (256-byte rows) or 2 to 4
+// (128-byte rows) go to different chunks.  Transposed V reads (8 keys, 64 bytes of each) do too: the upper chunk bits
+// come from the keys' low bits.
+template <int kD>
+__host__ __device__ constexpr int pr_swz(int k) {
+  return (kD == 128 ? 4 * ((k >> 1) & 3) : 4 * ((k >> 2) & 1)) + ((k >> 3) & 3);
+}
+
+template <bool kF16>
+__device__ __forceinline__ f32x16 pr_mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (kF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// All but the kLeft youngest LDS reads have returned; v passes through so that no use moves above the wait.
+template <int kLeft, int N, typename V>
+__device__ __forceinline__ void pr_lds_wait(V (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) __asm__ __volatile__("" : "+v"(v[i]));
+  __asm__ __volatile__("s_waitcnt lgkmcnt(%0)" ::"i"(kLeft) : "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) __asm__ __volatile__("" : "+v"(v[i]));
+}
+
+// The larger of x here and in the lane 32 away.
+__device__ __forceinline__ float pr_max32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pr_sum32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+constexpr int kPrWaves = 8;
+constexpr int kPrThreads = kPrWaves * kWave;
+constexpr int kPrRows = 32 * kPrWaves;  // 256
+constexpr int kPrTile = 64;             // keys
+
+// As pg_keys, for 256 rows.  Body t of a wave is C(t): scores of tile t and the products of tile t - 1 with V, a
+// barrier, X(t): exponentials of tile t, a barrier; waves 4 to 7 run one barrier behind, so that on each SIMD one
+// wave is in C while the other is in X.  Rings of four stages: X(t) starts the DMA of K of tile t + 3 and V of tile
+// t + 2, into the stages of K(t - 1) and V(t - 2), whose last reads (in C(t - 1) of the later waves) lie before the
+// barrier ahead of X(t) of the earlier ones; the wait at the end of C(t) leaves only what X(t - 1) started in flight,
+// so that behind the next barrier K(t + 1) and V(t) are whole.
+template <bool kF16, int kD>
+__device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
+                                        bool whole, float* part, uint8_t* lds) {
+  constexpr int kRow = kD * 2;
+  constexpr int kTileBytes = kPrTile * kRow;
+  constexpr int kChunks = kD / 8;
+  constexpr int kRpi = kWave / kChunks;               // rows a DMA instruction moves
+  constexpr int kI = kPrTile / kRpi / kPrWaves;       // DMA instructions of a wave and tile
+  constexpr int kSt = kD / 16;                        // steps of the score product
+  constexpr int kNb = kD / 32;                        // 32-column blocks of the output
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane & 31, hi = lane >> 5;
+
+  const int rows = s.span * a.Hg;
+  const int first = tile * kPrRows + 32 * wave;
+  const int rho = min(first + r, rows - 1);
+  const int tok = rho / a.Hg, head = kvg * a.Hg + rho - tok * a.Hg;
+  const int64_t qrow = (int64_t)(s.start + tok) * a.H + head;
+  // Q operand (B): row r, dims 16 st + 8 hi .. + 7.
+  u32x4 qb[kSt];
+#pragma unroll
+  for (int st = 0; st < kSt; ++st) qb[st] = *reinterpret_cast<const u32x4*>(a.q + qrow * kD + 16 * st + 8 * hi);
+  const int pos = s.n - s.len + tok;
+  const int lim = tok < s.len ? (a.causal ? min(pos, s.n - 1) : s.n - 1) : -1;  // the row sees keys low .. lim
+  const int low = a.win >= 0 ? max(pos, 0) - a.win : 0;
+  int lim_min = lim, lim_max = lim, low_min = low, low_max = low;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    lim_min = min(lim_min, __shfl_xor(lim_min, o, kWave));
+    lim_max = max(lim_max, __shfl_xor(lim_max, o, kWave));
+    low_min = min(low_min, __shfl_xor(low_min, o, kWave));
+    low_max = max(low_max, __shfl_xor(low_max, o, kWave));
+  }
+  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+  lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+  low_min = __builtin_amdgcn_readfirstlane(low_min);
+  low_max = __builtin_amdgcn_readfirstlane(low_max);
+  if (first >= rows) lim_max = -1;  // no rows: this wave only moves tiles
+
+  f32x16 o[kNb];
+#pragma unroll
+  for (int p = 0; p < kNb; ++p)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[p][i] = 0.f;
+  float m_run = -kPgInf, l_run = 0.f;
+
+  const int32_t* bt = a.table + (int64_t)b * a.max_blocks;
+  const int nt = k1 > k0 ? (k1 - k0 + kPrTile - 1) / kPrTile : 0;
+  if (nt > 0) {
+    // Pages outside the pool hide their keys: looked for once, the comparisons look again where there are any.
+    int outside = 0;
+    for (int blk = pg_block(a, k0) + tid; blk <= pg_block(a, k1 - 1); blk += kPrThreads)
+      outside |= (uint32_t)bt[blk] >= (uint32_t)a.num_blocks;
+    const bool holes = __syncthreads_or(outside) != 0;
+
+    const uint8_t *kb = reinterpret_cast<const uint8_t*>(a.kc), *vb = reinterpret_cast<const uint8_t*>(a.vc);
+    const int crow = lane / kChunks, cpos = lane % kChunks;
+    const uint8_t* zero = kPgZeroRow + 16 * (cpos & 15);
+    // Page of this lane's key in DMA instruction i of tile t (read without a condition: the waits below count
+    // instructions) and the key's place in it; -1: no key.
+    struct Look {
+      int page, rem;
+    };
+    auto look = [&](int t, int i) {
+      const int j = k0 + t * kPrTile + (wave + kPrWaves * i) * kRpi + crow;
+      const int jc = min(j, k1 - 1), blk = pg_block(a, jc);
+      return Look{bt[blk], j < k1 ? jc - blk * a.block_size : -1};
+    };
+    // Row of the caches, -1 where there is no key.
+    auto row_of = [&](const Look& l) {
+      const bool ok = l.rem >= 0 && (uint32_t)l.page < (uint32_t)a.num_blocks;
+      return ok ? l.page * a.block_size + l.rem : -1;
+    };
+    auto dma = [&](const uint8_t* cache, int row, int ring, int t, int i) {
+      const int n = wave + kPrWaves * i;
+      const int64_t at = ((int64_t)row * a.G + kvg) * kRow + 16 * (cpos ^ pr_swz<kD>(n * kRpi + crow));
+      const uint8_t* src = row >= 0 ? cache + at : zero;
+      __builtin_amdgcn_global_load_lds((gqa_gbl_void*)src,
+                                       (gqa_lds_void*)(lds + (4 * ring + (t & 3)) * kTileBytes + n * 1024), 16, 0, 0);
+    };
+    Look next[kI];  // of tile t + 3
+    int vnext[kI];  // of tile t + 2
+    {
+      int at0[kI], at1[kI];
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        at0[i] = row_of(look(0, i));
+        at1[i] = row_of(look(1, i));
+        vnext[i] = row_of(look(2, i));
+        next[i] = look(3, i);
+      }
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(kb, at0[i], 0, 0, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(vb, at0[i], 1, 0, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(kb, at1[i], 0, 1, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(vb, at1[i], 1, 1, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(kb, vnext[i], 0, 2, i);
+    }
+
+    const uint32_t lds0 = gqa_lds_u32(lds);
+    // K operand (A), step st, key block kb: key 32 kb + r, dims 16 st + 8 hi .. + 7.
+    const uint32_t k_at = lds0 + r * kRow + 16 * (hi ^ pr_swz<kD>(r));
+    // V^T operand (A), 16 keys from 16 u, columns 32 p ..: lane group (hi, h) of 16 lanes (q = lane & 15) addresses
+    // keys 4 hi + (q >> 2) (+ 8 for the second read), columns 16 h + 8 (q & 1) + 4 ((q >> 1) & 1) .. + 3, and receives
+    // those keys of one column each: operand row 16 h + 4 c + e is column 16 h + 8 (c & 1) + 4 (c >> 1) + e, so that
+    // a lane's results 8 x .. 8 x + 7 are columns 16 x + 8 hi .. + 7.
+    const int q = lane & 15, h = (lane >> 4) & 1, vk = 4 * hi + (q >> 2);
+    const uint32_t v_at =
+        lds0 + 4 * kTileBytes + vk * kRow + 16 * ((2 * h + (q & 1)) ^ pr_swz<kD>(vk)) + 8 * ((q >> 1) & 1);
+
+    u32x4 pb[4];
+    u32x4 kop[2][4];
+    u32x2 vop[2][2 * kNb];
+    // Scores: batch i holds the operands of steps 2 i, 2 i + 1 of both key blocks.
+    auto k_read = [&](int t, auto batch) {
+      constexpr int i = decltype(batch)::value;
+      const uint32_t at = k_at + (t & 3) * kTileBytes;
+      gqa_b128<0>(kop[i & 1][0], at ^ (64 * i));
+      gqa_b128<32 * kRow>(kop[i & 1][1], at ^ (64 * i));
+      gqa_b128<0>(kop[i & 1][2], at ^ (64 * i + 32));
+      gqa_b128<32 * kRow>(kop[i & 1][3], at ^ (64 * i + 32));
+    };
+    f32x16 none;  // no sums yet
+#pragma unroll
+    for (int i = 0; i < 16; ++i) none[i] = 0.f;
+    auto k_mul = [&](f32x16(&c)[2], auto batch) {
+      constexpr int i = decltype(batch)::value;
+      c[0] = pr_mfma<kF16>(kop[i & 1][0], qb[2 * i], i == 0 ? none : c[0]);
+      c[1] = pr_mfma<kF16>(kop[i & 1][1], qb[2 * i], i == 0 ? none : c[1]);
+      c[0] = pr_mfma<kF16>(kop[i & 1][2], qb[2 * i + 1], c[0]);
+      c[1] = pr_mfma<kF16>(kop[i & 1][3], qb[2 * i + 1], c[1]);
+    };
+    auto v_read = [&](int t, auto step) {
+      constexpr int u = decltype(step)::value;
+      const uint32_t at = v_at + (t & 3) * kTileBytes;
+#pragma unroll
+      for (int p = 0; p < kNb; ++p) {
+        gqa_tr<16 * u * kRow>(vop[u & 1][2 * p], at ^ (64 * p + 16 * ((2 * u) & 3)));
+        gqa_tr<(16 * u + 8) * kRow>(vop[u & 1][2 * p + 1], at ^ (64 * p + 16 * ((2 * u + 1) & 3)));
+      }
+    };
+    auto v_mul = [&](auto step) {
+      constexpr int u = decltype(step)::value;
+#pragma unroll
+      for (int p = 0; p < kNb; ++p) {
+        const u32x2 x = vop[u & 1][2 * p], y = vop[u & 1][2 * p + 1];
+        o[p] = pr_mfma<kF16>(u32x4{x.x, x.y, y.x, y.y}, pb[u], o[p]);
+      }
+    };
+    constexpr std::integral_constant<int, 0> c0{};
+    constexpr std::integral_constant<int, 1> c1{};
+    constexpr std::integral_constant<int, 2> c2{};
+    constexpr std::integral_constant<int, 3> c3{};
+    constexpr int kV = 2 * kNb;  // LDS reads of a step
+    // The scores of tile t; the reads of tile pv's first V step go out under its last products (pv < 0: none).
+    auto scores = [&](f32x16(&c)[2], int t, auto with_v) {
+      k_read(t, c0);
+      k_read(t, c1);
+      pr_lds_wait<4>(kop[0]);
+      k_mul(c, c0);
+      if constexpr (kD == 128) {
+        k_read(t, c2);
+        pr_lds_wait<4>(kop[1]);
+        k_mul(c, c1);
+        k_read(t, c3);
+        pr_lds_wait<4>(kop[0]);
+        k_mul(c, c2);
+      }
+      if constexpr (decltype(with_v)::value) {
+        v_read(t - 1, c0);
+        pr_lds_wait<kV>(kop[1]);
+      } else {
+        pr_lds_wait<0>(kop[1]);
+      }
+      if constexpr (kD == 128) k_mul(c, c3);
+      else k_mul(c, c1);
+    };
+    auto products = [&](int t, auto started) {
+      if constexpr (!decltype(started)::value) v_read(t, c0);
+      v_read(t, c1);
+      pr_lds_wait<kV>(vop[0]);
+      v_mul(c0);
+      v_read(t, c2);
+      pr_lds_wait<kV>(vop[1]);
+      v_mul(c1);
+      v_read(t, c3);
+      pr_lds_wait<kV>(vop[0]);
+      v_mul(c2);
+      pr_lds_wait<0>(vop[1]);
+      v_mul(c3);
+    };
+    auto softmax = [&](f32x16(&c)[2], int j0) {
+      if (holes || j0 + kPrTile - 1 > lim_min || j0 < low_max) {
+        uint64_t there = ~(uint64_t)0;  // keys in pages of the pool
+        if (holes) there = __ballot((uint32_t)bt[pg_block(a, min(j0 + lane, k1 - 1))] < (uint32_t)a.num_blocks);
+        const int up = lim - j0 - 4 * hi, down = low - j0 - 4 * hi;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t bits = (uint32_t)(there >> (32 * k)) >> (4 * hi);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 8 * (i >> 2) + (i & 3);
+            const bool see = 32 * k + j <= up && 32 * k + j >= down && ((bits >> j) & 1u);
+            c[k][i] = see ? c[k][i] : -kPgInf;
+          }
+        }
+      }
+      float mx = fmaxf(c[0][0], c[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(c[0][i], c[1][i]));
+      mx = pr_max32(mx) * a.scale_log2;  // sm_scale > 0
+      // The reference moves only when it falls 2^8 behind: a probability is at most 2^8 then, in the range of every
+      // type here, and most tiles leave the sums as they are.
+      if (__any(mx > m_run + 8.f)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = m_new == -kPgInf ? 1.f : fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int p = 0; p < kNb; ++p) o[p] *= alpha;
+      }
+      const float m_use = m_run == -kPgInf ? 0.f : m_run;
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          c[k][i] = fast_exp2(fmaf(c[k][i], a.scale_log2, -m_use));
+          sum += c[k][i];
+        }
+      l_run += sum;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int x = 8 * (u & 1);
+        const f32x16& e = c[u >> 1];
+        pb[u] = u32x4{gqa_pack<kF16>(e[x], e[x + 1]), gqa_pack<kF16>(e[x + 2], e[x + 3]),
+                      gqa_pack<kF16>(e[x + 4], e[x + 5]), gqa_pack<kF16>(e[x + 6], e[x + 7])};
+      }
+    };
+    // Tiles that no row of the wave sees take no part in its sums.
+    auto seen = [&](int t) {
+      const int j0 = k0 + t * kPrTile;
+      return j0 <= lim_max && j0 + kPrTile - 1 >= low_min;
+    };
+
+    gqa_wait_vmcnt<4 * kI>();
+    __builtin_amdgcn_s_barrier();
+    if (wave >= 4) __builtin_amdgcn_s_barrier();
+    bool before = false;  // tile t - 1 was seen
+    for (int t = 0; t < nt; ++t) {
+      const bool now = seen(t);
+      f32x16 c[2];
+      __builtin_amdgcn_s_setprio(1);
+      if (now && before) {
+        scores(c, t, std::true_type{});
+        products(t - 1, std::true_type{});
+      } else if (now) {
+        scores(c, t, std::false_type{});
+      } else if (before) {
+        products(t - 1, std::false_type{});
+      }
+      __builtin_amdgcn_s_setprio(0);
+      gqa_wait_vmcnt<2 * kI>();
+      __builtin_amdgcn_s_barrier();
+      {
+        int at[kI];
+#pragma unroll
+        for (int i = 0; i < kI; ++i) at[i] = row_of(next[i]);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) next[i] = look(t + 4, i);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) dma(kb, at[i], 0, t + 3, i);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) dma(vb, vnext[i], 1, t + 2, i);
+#pragma unroll
+        for (int i = 0; i < kI; ++i) vnext[i] = at[i];
+      }
+      if (now) softmax(c, k0 + t * kPrTile);
+      before = now;
+      __builtin_amdgcn_s_barrier();
+    }
+    if (before) products(nt - 1, std::false_type{});
+    if (wave < 4) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_waitcnt(0);  // the DMA of tiles behind the last
+  }
+
+  l_run = pr_sum32(l_run);
+  constexpr float kLn2 = 0.6931471805599453f;
+  if (!whole) {
+    float* p = part + (32 * wave + r) * kD + 8 * hi;
+#pragma unroll
+    for (int n = 0; n < kNb; ++n)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *reinterpret_cast<f32x4*>(p + 32 * n + 16 * (x >> 1) + 4 * (x & 1)) =
+            f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]};
+    if (hi == 0) {
+      part[kPrRows * kD + 2 * (32 * wave + r)] = m_run;
+      part[kPrRows * kD + 2 * (32 * wave + r) + 1] = l_run;
+    }
+  } else if (first + r < rows) {
+    float M = m_run == -kPgInf ? 0.f : m_run, f = 1.f, sum = l_run;
+    if (a.sinks) {
+      const float sk = a.sinks[head] * 1.4426950408889634f;
+      M = fmaxf(m_run, sk);
+      M = M == -kPgInf ? 0.f : M;
+      f = fast_exp2(m_run - M);
+      sum = sum * f + fast_exp2(sk - M);
+    }
+    const float inv = sum > 0.f ? f / sum : 0.f;
+    uint16_t* dst = a.out + qrow * kD + 8 * hi;
+#pragma unroll
+    for (int n = 0; n < kNb; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = o[n][8 * x + i] * inv;
+        *reinterpret_cast<u32x4*>(dst + 32 * n + 16 * x) = u32x4{gqa_pack<kF16>(v[0], v[1]), gqa_pack<kF16>(v[2], v[3]),
+                                                                gqa_pack<kF16>(v[4], v[5]), gqa_pack<kF16>(v[6], v[7])};
+      }
+    if (hi == 0) a.lse[qrow] = sum > 0.f ? (M + fast_log2(sum)) * kLn2 : -kPgInf;
+  }
+}
+
+// The two ways with their sizes.
+template <bool kF16_, int kD_, int kHB>
+struct PgKeys {
+  static constexpr bool kF16 = kF16_;
+  static constexpr int kD = kD_, kR = 16 * kHB, kUnitKeys = kPgUnit, kThreads = kPgThreads;
+  static constexpr int kLds = kPgWaves * 2 * 2 * kPgTile * kD * 2 + kPgWaves * 16 * kHB * 2 * 4;
+  static_assert(16 * kHB * kD * 4 <= 4 * kPgTile * kD * 2, "a wave's sums fit its ring");
+  static __device__ __forceinline__ void item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
+                                              bool whole, float* part, uint8_t* lds) {
+    pg_keys<kF16, kD, kHB>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
+  }
+};
+template <bool kF16_, int kD_>
+struct PgRows {
+  static constexpr bool kF16 = kF16_;
+  static constexpr int kD = kD_, kR = kPrRows, kUnitKeys = kPrTile, kThreads = kPrThreads;
+  static constexpr int kLds = 8 * kPrTile * kD * 2;
+  static __device__ __forceinline__ void item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
+                                              bool whole, float* part, uint8_t* lds) {
+    pg_rows<kF16, kD>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
+    __syncthreads();  // the rings are free for the next item
+  }
+};
+
+// First slot of sequence b, whose rows start at `start`: strictly increasing in b.
 __device__ __forceinline__ int pg_slot(int start, int Hg, int b, int kR) {
   return (int)((int64_t)start * Hg / kR) + b;
 }
-__device__ __forceinline__ int pg_start(const PgArgs& a, int b) {
+// First query row of sequence b; `cu` is a.cu_q or a copy.
+__device__ __forceinline__ int pg_start(const PgArgs& a, const int32_t* cu, int b) {
   if (!a.cu_q) return min(b, a.B) * a.S;
-  return b > 0 ? min(max(a.cu_q[b - 1], 0), a.T) : 0;
+  return b > 0 ? min(max(cu[b - 1], 0), a.T) : 0;
 }
-
-// A tile and all its keys for each workgroup: blockIdx.x = slot, blockIdx.y = group.
-template <bool kF16, int kD, int kHB>
-__global__ __launch_bounds__(kPgThreads) void pg_direct_kernel(PgArgs a) {
-  extern __shared__ __align__(16) uint8_t lds[];
-  constexpr int kR = 16 * kHB;
-  // The causal rows with the most keys first.
-  const int slot = (int)(gridDim.x - 1 - blockIdx.x);
-  int b0 = 0, b1 = a.B;  // the last b whose first slot is not past ours
+// The last sequence whose first slot is not past `slot`.
+__device__ __forceinline__ int pg_find(const PgArgs& a, const int32_t* cu, int slot, int kR) {
+  int b0 = 0, b1 = a.B;
   while (b0 < b1) {
     const int mid = (b0 + b1 + 1) >> 1;
-    if (pg_slot(pg_start(a, mid), a.Hg, mid, kR) <= slot) b0 = mid;
+    if (pg_slot(pg_start(a, cu, mid), a.Hg, mid, kR) <= slot) b0 = mid;
     else b1 = mid - 1;
   }
-  const PgSeq s = pg_seq(a, b0);
-  const int tile = slot - pg_slot(s.start, a.Hg, b0, kR);
-  if (tile < 0 || (int64_t)tile * kR >= (int64_t)s.span * a.Hg) return;
-  int lo = s.lo, hi = s.hi;
+  return b0;
+}
+// The keys [lo, hi) that rows of the tile see; false: the sequence has no such tile.
+__device__ __forceinline__ bool pg_range(const PgArgs& a, const PgSeq& s, int tile, int kR, int& lo, int& hi) {
+  if (tile < 0 || (int64_t)tile * kR >= (int64_t)s.span * a.Hg) return false;
+  lo = s.lo;
+  hi = s.hi;
   const int first = (tile * kR) / a.Hg, last = min(((tile + 1) * kR - 1) / a.Hg, s.span - 1);
   if (a.causal) hi = max(min(hi, s.n - s.len + last + 1), 0);
   if (a.win >= 0) lo = max(lo, (max(s.n - s.len + first, 0) - a.win) & ~(kPgTile - 1));
-  pg_item<kF16, kD, kHB>(a, s, b0, tile, (int)blockIdx.y, min(lo, hi), hi, true, nullptr, lds);
+  lo = min(lo, hi);
+  return true;
 }
 
-// Units (128 keys) of each tile of the sequence, at least one: a tile without keys writes its zeros.
-__device__ __forceinline__ int pg_units(const PgSeq& s) { return max(1, (s.hi - s.lo + kPgUnit - 1) / kPgUnit); }
-__device__ __forceinline__ int pg_tiles(const PgArgs& a, const PgSeq& s, int kR) {
-  return (int)(((int64_t)s.span * a.Hg + kR - 1) / kR);
+// A tile and all its keys for each workgroup.  Group fastest, so that the workgroups of an XCD (every eighth) read few
+// groups' caches; the causal rows with the most keys first.
+template <class W>
+__global__ __launch_bounds__(W::kThreads) void pg_direct_kernel(PgArgs a) {
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int rank = blockIdx.x / a.G, kvg = blockIdx.x - rank * a.G;
+  const int slot = a.slots - 1 - rank;
+  const int b = pg_find(a, a.cu_q, slot, W::kR);
+  const PgSeq s = pg_seq(a, b);
+  const int tile = slot - pg_slot(s.start, a.Hg, b, W::kR);
+  int lo, hi;
+  if (!pg_range(a, s, tile, W::kR, lo, hi)) return;
+  W::item(a, s, b, tile, kvg, lo, hi, true, nullptr, lds);
 }
 
-// The line of units, shared by the split kernel and the join: thread t sums sequences [t * per, (t + 1) * per).
-// Returns the thread's exclusive prefix; `total` is the line's length.
-__device__ __forceinline__ int64_t pg_line(const PgArgs& a, int kR, int64_t& total, int64_t* scratch) {
-  const int per = (a.B + 1 + kPgThreads - 1) / kPgThreads;
-  const int b0 = threadIdx.x * per;
-  int64_t sum = 0;
-  for (int i = 0; i < per; ++i) {
-    if (b0 + i > a.B) break;
-    const PgSeq s = pg_seq(a, b0 + i);
-    sum += (int64_t)pg_tiles(a, s, kR) * a.G * pg_units(s);
-  }
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  int64_t incl = sum;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t v = __shfl_up(incl, o, kWave);
-    if (lane >= o) incl += v;
-  }
-  if (lane == kWave - 1) scratch[wave] = incl;
+// The line of units: slot x takes units [at[x], at[x + 1]) of each group.  Every workgroup of the split kernel and the
+// join makes it alike, in LDS.
+struct PgLine {
+  int64_t at[kPgMaxSlots + 1];
+  int seq[kPgMaxSlots];
+  int32_t cu[kPgMaxSlots];
+};
+static_assert(sizeof(PgLine) <= 16 * 1024 + 8, "LDS of the line");
+
+template <class W>
+__device__ __forceinline__ void pg_line(const PgArgs& a, PgLine& line, int threads) {
+  const int tid = threadIdx.x;
+  if (a.cu_q)
+    for (int b = tid; b < a.B; b += threads) line.cu[b] = a.cu_q[b];  // B < slots
   __syncthreads();
-  int64_t base = 0;
-  total = 0;
+  for (int x = tid; x < a.slots; x += threads) {
+    const int b = pg_find(a, line.cu, x, W::kR);
+    const PgSeq s = pg_seq(a, b);
+    int lo, hi, units = 0;
+    // A tile without keys takes a unit too: it writes its zeros.
+    if (pg_range(a, s, x - pg_slot(s.start, a.Hg, b, W::kR), W::kR, lo, hi))
+      units = max(1, (int)(((int64_t)hi - lo + W::kUnitKeys - 1) / W::kUnitKeys));
+    line.seq[x] = b;
+    line.at[x + 1] = units;
+  }
+  if (tid == 0) line.at[0] = 0;
+  __syncthreads();
+  if (tid < kWave) {
+    int64_t sum = 0;
+    for (int x = tid; x < ((a.slots + kWave - 1) & ~(kWave - 1)); x += kWave) {
+      int64_t v = x < a.slots ? line.at[x + 1] : 0;
 #pragma unroll
-  for (int w = 0; w < kPgWaves; ++w) {
-    if (w < wave) base += scratch[w];
-    total += scratch[w];
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int64_t u = __shfl_up(v, o, kWave);
+        if (tid >= o) v += u;
+      }
+      if (x < a.slots) line.at[x + 1] = sum + v;
+      sum += __shfl(v, kWave - 1, kWave);
+    }
   }
   __syncthreads();
-  return base + incl - sum;
 }
 
 // Units of a workgroup's part of the line.
-__device__ __forceinline__ int64_t pg_share(int64_t total, int wgs) { return max((total + wgs - 1) / wgs, (int64_t)1); }
+__device__ __forceinline__ int64_t pg_share(const PgArgs& a, const PgLine& line) {
+  const int64_t total = line.at[a.slots] * a.G;
+  return max((total + a.wgs - 1) / a.wgs, (int64_t)1);
+}
 
-template <bool kF16, int kD, int kHB>
-__global__ __launch_bounds__(kPgThreads) void pg_split_kernel(PgArgs a) {
+template <class W>
+__global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
-  constexpr int kR = 16 * kHB;
-  int64_t* scratch = reinterpret_cast<int64_t*>(lds);
-  int64_t total;
-  const int64_t before = pg_line(a, kR, total, scratch);
-  const int64_t share = pg_share(total, a.wgs);
+  PgLine& line = *reinterpret_cast<PgLine*>(lds + W::kLds);
+  pg_line<W>(a, line, W::kThreads);
+  const int64_t share = pg_share(a, line), total = line.at[a.slots] * a.G;
   int64_t u = (int64_t)blockIdx.x * share;
   const int64_t end = min(u + share, total);
-  if (u >= end) return;
-  // The sequence that unit u lies in, and the line's units before it.
+  int x = 0;  // the slot that unit u lies in: the last whose units start at or before u and that has any
   {
-    const int per = (a.B + 1 + kPgThreads - 1) / kPgThreads;
-    int64_t at = before;
-    for (int i = 0; i < per; ++i) {
-      const int b = threadIdx.x * per + i;
-      if (b > a.B) break;
-      const PgSeq s = pg_seq(a, b);
-      const int64_t len = (int64_t)pg_tiles(a, s, kR) * a.G * pg_units(s);
-      if (u >= at && u < at + len) {
-        scratch[8] = at;
-        scratch[9] = b;
-      }
-      at += len;
+    int x1 = a.slots - 1;
+    while (x < x1) {
+      const int mid = (x + x1 + 1) >> 1;
+      if (line.at[mid] * a.G <= u) x = mid;
+      else x1 = mid - 1;
     }
   }
-  __syncthreads();
-  int64_t at = scratch[8];
-  int b = (int)scratch[9];
-  __syncthreads();
-  at = ((int64_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-  b = __builtin_amdgcn_readfirstlane(b);
+  x = __builtin_amdgcn_readfirstlane(x);
   while (u < end) {
+    const int64_t from = line.at[x], units = line.at[x + 1] - from;
+    if (units == 0) {
+      ++x;
+      continue;
+    }
+    const int b = __builtin_amdgcn_readfirstlane(line.seq[x]);
     const PgSeq s = pg_seq(a, b);
-    const int units = pg_units(s);
-    const int64_t items = (int64_t)pg_tiles(a, s, kR) * a.G;
-    while (u < end && u < at + items * units) {
-      const int item = (int)((u - at) / units);
-      const int64_t u0 = at + (int64_t)item * units;  // the item's units on the line: [u0, u0 + units)
+    const int tile = x - pg_slot(s.start, a.Hg, b, W::kR);
+    int lo, hi;
+    if (!pg_range(a, s, tile, W::kR, lo, hi)) return;  // not reached: the slot has units
+    for (int kvg = (int)((u - from * a.G) / units); kvg < a.G && u < end; ++kvg) {
+      const int64_t u0 = from * a.G + kvg * units;  // the item's units on the line: [u0, u0 + units)
       const int64_t stop = min(end, u0 + units);
       const bool whole = u == u0 && stop == u0 + units;
-      const int tile = item / a.G, kvg = item - tile * a.G;
-      const int k0 = s.lo + (int)(u - u0) * kPgUnit;
-      const int k1 = (int)min((int64_t)s.hi, s.lo + (stop - u0) * kPgUnit);
-      const int64_t id = (int64_t)(pg_slot(s.start, a.Hg, b, kR) + tile) * a.G + kvg;
-      pg_item<kF16, kD, kHB>(a, s, b, tile, kvg, min(k0, k1), k1, whole,
-                             whole ? nullptr : a.part + (id + blockIdx.x) * pg_part_floats<kHB, kD>(), lds);
+      const int k0 = (int)min((int64_t)hi, lo + (u - u0) * W::kUnitKeys);
+      const int k1 = (int)min((int64_t)hi, lo + (stop - u0) * W::kUnitKeys);
+      float* part = a.part + ((int64_t)x * a.G + kvg + blockIdx.x) * pg_part_floats<W::kR, W::kD>();
+      W::item(a, s, b, tile, kvg, __builtin_amdgcn_readfirstlane(k0), __builtin_amdgcn_readfirstlane(k1), whole, part,
+              lds);
       u = stop;
     }
-    at += items * units;
-    ++b;
+    ++x;
   }
 }
 
-// Joins the parts of each tile whose units lie in more than one workgroup's share: workgroup = (slot, group).
-template <bool kF16, int kD, int kHB>
+// Joins the parts of each tile whose units lie in more than one workgroup's share: workgroup = (slot and group, rows).
+template <class W>
 __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
-  constexpr int kR = 16 * kHB;
-  __shared__ int64_t scratch[16];
-  int64_t total;
-  const int64_t before = pg_line(a, kR, total, scratch);
-  const int64_t share = pg_share(total, a.wgs);
-  const int slot = blockIdx.x, kvg = blockIdx.y;
-  if (threadIdx.x == 0) scratch[9] = -1;
-  __syncthreads();
-  {
-    const int per = (a.B + 1 + kPgThreads - 1) / kPgThreads;
-    int64_t at = before;
-    for (int i = 0; i < per; ++i) {
-      const int b = threadIdx.x * per + i;
-      if (b > a.B) break;
-      const PgSeq s = pg_seq(a, b);
-      const int tiles = pg_tiles(a, s, kR), first = pg_slot(s.start, a.Hg, b, kR);
-      if (slot >= first && slot < first + tiles) {
-        scratch[8] = at;
-        scratch[9] = b;
-      }
-      at += (int64_t)tiles * a.G * pg_units(s);
-    }
-  }
-  __syncthreads();
-  const int b = (int)scratch[9];
-  if (b < 0) return;
+  constexpr int kR = W::kR, kD = W::kD, kPart = pg_part_floats<kR, kD>();
+  __shared__ PgLine line;
+  pg_line<W>(a, line, kPgThreads);
+  const int64_t share = pg_share(a, line);
+  const int x = blockIdx.x / a.G, kvg = blockIdx.x - x * a.G;
+  const int64_t units = line.at[x + 1] - line.at[x];
+  if (units == 0) return;
+  const int64_t u0 = line.at[x] * a.G + kvg * units;
+  const int w0 = (int)(u0 / share), np = (int)((u0 + units - 1) / share) - w0 + 1;
+  if (np == 1) return;
+  const int b = line.seq[x];
   const PgSeq s = pg_seq(a, b);
-  const int units = pg_units(s), tile = slot - pg_slot(s.start, a.Hg, b, kR);
-  const int64_t u0 = scratch[8] + ((int64_t)tile * a.G + kvg) * units;
-  const int w0 = (int)(u0 / share), w1 = (int)((u0 + units - 1) / share);
-  if (w0 == w1) return;
-  const int64_t id = (int64_t)slot * a.G + kvg;
-  const float* base = a.part + (id + w0) * pg_part_floats<kHB, kD>();
+  const int tile = x - pg_slot(s.start, a.Hg, b, kR);
+  const float* base = a.part + ((int64_t)x * a.G + kvg + w0) * kPart;
   constexpr int kPerRow = kD / 8;
   constexpr int kRowsPass = kPgThreads / kPerRow;
   constexpr float kLn2 = 0.6931471805599453f;
-  const int rows = s.span * a.Hg;
+  const int hh = blockIdx.y * kRowsPass + threadIdx.x / kPerRow, c0 = 8 * (threadIdx.x % kPerRow);
+  const int rho = tile * kR + hh;
+  if (hh >= kR || rho >= s.span * a.Hg) return;
+  const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
+  float M = -kPgInf;
+#pragma unroll 4
+  for (int p = 0; p < np; ++p) M = fmaxf(M, base[(int64_t)p * kPart + kR * kD + 2 * hh]);
+  const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
+  M = fmaxf(M, sk);
+  const float M_use = M == -kPgInf ? 0.f : M;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = fast_exp2(sk - M_use);
+#pragma unroll 4
+  for (int p = 0; p < np; ++p) {
+    const float* pp = base + (int64_t)p * kPart;
+    const float f = fast_exp2(pp[kR * kD + 2 * hh] - M_use);
+    sum += f * pp[kR * kD + 2 * hh + 1];
+    const f32x4 x0 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
+    const f32x4 x1 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0 + 4);
 #pragma unroll
-  for (int r0 = 0; r0 < kR; r0 += kRowsPass) {
-    const int hh = r0 + threadIdx.x / kPerRow, c0 = 8 * (threadIdx.x % kPerRow);
-    const int rho = tile * kR + hh;
-    if (hh >= kR || rho >= rows) continue;
-    const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
-    const int np = w1 - w0 + 1;
-    float M = -kPgInf;
-    for (int p = 0; p < np; ++p) M = fmaxf(M, base[(int64_t)p * pg_part_floats<kHB, kD>() + kR * kD + 2 * hh]);
-    const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
-    M = fmaxf(M, sk);
-    const float M_use = M == -kPgInf ? 0.f : M;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = fast_exp2(sk - M_use);
-    for (int p = 0; p < np; ++p) {
-      const float* pp = base + (int64_t)p * pg_part_floats<kHB, kD>();
-      const float f = fast_exp2(pp[kR * kD + 2 * hh] - M_use);
-      sum += f * pp[kR * kD + 2 * hh + 1];
-      const f32x4 x0 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
-      const f32x4 x1 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0 + 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        acc[k] += f * x0[k];
-        acc[4 + k] += f * x1[k];
-      }
+    for (int k = 0; k < 4; ++k) {
+      acc[k] += f * x0[k];
+      acc[4 + k] += f * x1[k];
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const int64_t orow = (int64_t)(s.start + i) * a.H + h;
-    *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
-        u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
-              gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-    if (c0 == 0) a.lse[orow] = sum > 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
   }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const int64_t orow = (int64_t)(s.start + i) * a.H + h;
+  constexpr bool kF16 = W::kF16;
+  *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
+      u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
+            gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
+  if (c0 == 0) a.lse[orow] = sum > 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
 }
 
 // The launch of a call, from sizes that the host knows: T tokens, B sequences, at most `most` keys each.
 struct PgPlan {
-  int hb;         // 16-row blocks of a tile
+  int rows;       // of a tile: 16, 32 (pg_keys) or 256 (pg_rows)
   int64_t slots;  // tiles at most, in each group
   int wgs;        // workgroups that share the line of units; 0: a tile each
 };
@@ -562,50 +975,54 @@ struct PgPlan {
 static PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) {
   PgPlan p;
   const int64_t Hg = H / G;
-  p.hb = T * Hg > 16 * B ? 2 : 1;
-  p.slots = T * Hg / (16 * p.hb) + B + 1;
+  p.rows = T * Hg <= 16 * B ? 16 : T * Hg <= 32 * B ? 32 : kPrRows;
+  p.slots = T * Hg / p.rows + B + 1;
   p.wgs = 0;
-  if (p.slots * G < 1024) {
-    const int64_t units = p.slots * G * ((most + kPgUnit - 1) / kPgUnit + 1);
+  // One workgroup fits a CU: fewer than two rounds of tiles share the line.
+  if (p.slots <= kPgMaxSlots && p.slots * G < 512) {
+    const int64_t unit = p.rows == kPrRows ? kPrTile : kPgUnit;
+    const int64_t units = p.slots * G * ((most + unit - 1) / unit + 1);
     p.wgs = (int)(units < 256 ? units : 256);
   }
   return p;
 }
 
-static int pg_floats(int hb, int64_t D) { return 16 * hb * ((int)D + 2); }
-
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
   const PgPlan p = pg_plan(T, B, H, G, most);
   if (p.wgs == 0) return 0;
-  return (size_t)(p.slots * G + p.wgs) * pg_floats(p.hb, D) * sizeof(float);
+  return (size_t)(p.slots * G + p.wgs) * p.rows * (D + 2) * sizeof(float);
 }
 
-template <bool kF16, int kD, int kHB>
-static hipError_t pg_launch(PgArgs& a, const PgPlan& p, hipStream_t stream) {
-  constexpr int lds = pg_lds_bytes<kHB, kD>();
-  static_assert(lds <= 160 * 1024 && 16 * kHB * kD * 4 <= 4 * kPgTile * kD * 2, "a wave's sums fit its ring");
-  const dim3 tiles((unsigned)p.slots, (unsigned)a.G);
+template <class W>
+static hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
+  constexpr int split_lds = W::kLds + (int)sizeof(PgLine);
+  static_assert(W::kLds % 16 == 0 && split_lds <= 160 * 1024, "LDS");
+  const dim3 tiles((unsigned)((int64_t)a.slots * a.G));
   hipError_t e;
-  if (p.wgs == 0) {
-    e = set_dynamic_lds_once<pg_direct_kernel<kF16, kD, kHB>>(lds);
+  if (a.wgs == 0) {
+    e = set_dynamic_lds_once<pg_direct_kernel<W>>(W::kLds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((pg_direct_kernel<kF16, kD, kHB>), tiles, dim3(kPgThreads), lds, stream, a);
+    hipLaunchKernelGGL((pg_direct_kernel<W>), tiles, dim3(W::kThreads), W::kLds, stream, a);
     return hipGetLastError();
   }
-  e = set_dynamic_lds_once<pg_split_kernel<kF16, kD, kHB>>(lds);
+  e = set_dynamic_lds_once<pg_split_kernel<W>>(split_lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((pg_split_kernel<kF16, kD, kHB>), dim3(p.wgs), dim3(kPgThreads), lds, stream, a);
-  hipLaunchKernelGGL((pg_join_kernel<kF16, kD, kHB>), tiles, dim3(kPgThreads), 0, stream, a);
+  hipLaunchKernelGGL((pg_split_kernel<W>), dim3(a.wgs), dim3(W::kThreads), split_lds, stream, a);
+  constexpr int kRowsPass = kPgThreads / (W::kD / 8);
+  const dim3 join(tiles.x, (W::kR + kRowsPass - 1) / kRowsPass);
+  hipLaunchKernelGGL((pg_join_kernel<W>), join, dim3(kPgThreads), 0, stream, a);
   return hipGetLastError();
 }
 
 template <bool kF16, int kD>
-static hipError_t pg_dispatch(PgArgs& a, const PgPlan& p, hipStream_t stream) {
-  return p.hb == 2 ? pg_launch<kF16, kD, 2>(a, p, stream) : pg_launch<kF16, kD, 1>(a, p, stream);
+static hipError_t pg_dispatch(const PgArgs& a, int rows, hipStream_t stream) {
+  if (rows == kPrRows) return pg_launch<PgRows<kF16, kD>>(a, stream);
+  return rows == 32 ? pg_launch<PgKeys<kF16, kD, 2>>(a, stream) : pg_launch<PgKeys<kF16, kD, 1>>(a, stream);
 }
 
-// Caller validated: D in {64, 128}, H a multiple of G, T * H < 2^31, G <= 65535, pool rows < 2^31,
-// max_blocks * block_size <= 2^31 - 1 - 1024, sm_scale > 0, the workspace as paged_gqa_workspace_bytes says.
+// Caller validated: D in {64, 128}, H a multiple of G, T * H < 2^31 - 65536, pool rows < 2^31,
+// max_blocks * block_size <= 2^31 - 1 - 4096, (T * H / 16 + B + 1) * G < 2^31, sm_scale > 0, the workspace as
+// paged_gqa_workspace_bytes says.
 hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
                             const int32_t* cu_q, const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B,
                             int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
@@ -637,9 +1054,18 @@ hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const vo
   a.causal = causal;
   a.win = win_left < max_blocks * block_size ? (int)win_left : -1;  // a window as long as the cache is none
   a.wgs = p.wgs;
+  a.slots = (int)p.slots;
+  a.div_mul = 0;
+  a.div_shift = 0;
+  if (block_size > 1) {
+    int l = 0;
+    while (((int64_t)1 << l) < block_size) ++l;
+    a.div_mul = (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)block_size) + 1);
+    a.div_shift = l - 1;
+  }
   a.scale_log2 = sm_scale * 1.4426950408889634f;
-  if (D == 128) return is_fp16 ? pg_dispatch<true, 128>(a, p, stream) : pg_dispatch<false, 128>(a, p, stream);
-  return is_fp16 ? pg_dispatch<true, 64>(a, p, stream) : pg_dispatch<false, 64>(a, p, stream);
+  if (D == 128) return is_fp16 ? pg_dispatch<true, 128>(a, p.rows, stream) : pg_dispatch<false, 128>(a, p.rows, stream);
+  return is_fp16 ? pg_dispatch<true, 64>(a, p.rows, stream) : pg_dispatch<false, 64>(a, p.rows, stream);
 }
 
 }  // namespace dsa
