@@ -408,6 +408,15 @@ __device__ __forceinline__ float pr_sum32(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// f(integral_constant) for kFrom .. kTo - 1.
+template <int kFrom, int kTo, class F>
+__device__ __forceinline__ void pr_each(F&& f) {
+  if constexpr (kFrom < kTo) {
+    f(std::integral_constant<int, kFrom>{});
+    pr_each<kFrom + 1, kTo>(f);
+  }
+}
+
 constexpr int kPrWaves = 8;
 constexpr int kPrThreads = kPrWaves * kWave;
 constexpr int kPrRows = 32 * kPrWaves;  // 256
@@ -419,7 +428,7 @@ constexpr int kPrTile = 64;             // keys
 // t + 2, into the stages of K(t - 1) and V(t - 2), whose last reads (in C(t - 1) of the later waves) lie before the
 // barrier ahead of X(t) of the earlier ones; the wait at the end of C(t) leaves only what X(t - 1) started in flight,
 // so that behind the next barrier K(t + 1) and V(t) are whole.
-template <bool kF16, int kD>
+template <bool kF16, int kD, bool kEven>
 __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
   constexpr int kRow = kD * 2;
@@ -445,19 +454,14 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
   const int pos = s.n - s.len + tok;
   const int lim = tok < s.len ? (a.causal ? min(pos, s.n - 1) : s.n - 1) : -1;  // the row sees keys low .. lim
   const int low = a.win >= 0 ? max(pos, 0) - a.win : 0;
-  int lim_min = lim, lim_max = lim, low_min = low, low_max = low;
+  int lim_min = lim, low_max = low;  // tiles in which every row sees every key skip the comparisons
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     lim_min = min(lim_min, __shfl_xor(lim_min, o, kWave));
-    lim_max = max(lim_max, __shfl_xor(lim_max, o, kWave));
-    low_min = min(low_min, __shfl_xor(low_min, o, kWave));
     low_max = max(low_max, __shfl_xor(low_max, o, kWave));
   }
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-  lim_max = __builtin_amdgcn_readfirstlane(lim_max);
-  low_min = __builtin_amdgcn_readfirstlane(low_min);
   low_max = __builtin_amdgcn_readfirstlane(low_max);
-  if (first >= rows) lim_max = -1;  // no rows: this wave only moves tiles
 
   f32x16 o[kNb];
 #pragma unroll
@@ -478,37 +482,53 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     const uint8_t *kb = reinterpret_cast<const uint8_t*>(a.kc), *vb = reinterpret_cast<const uint8_t*>(a.vc);
     const int crow = lane / kChunks, cpos = lane % kChunks;
     const uint8_t* zero = kPgZeroRow + 16 * (cpos & 15);
-    // Page of this lane's key in DMA instruction i of tile t (read without a condition: the waits below count
-    // instructions) and the key's place in it; -1: no key.
+    // DMA instruction i of a wave moves kRpi keys from key first_key(t, i) on; chunk positions repeat every 32 keys.
+    const int swz = 16 * (cpos ^ pr_swz<kD>(wave * kRpi + crow));
+    auto first_key = [&](int t, int i) { return k0 + t * kPrTile + (wave + kPrWaves * i) * kRpi; };
+    auto to_lds = [&](const uint8_t* src, int ring, int t, int i) {
+      __builtin_amdgcn_global_load_lds((gqa_gbl_void*)src,
+                                       (gqa_lds_void*)(lds + (4 * ring + (t & 3)) * kTileBytes + (wave + kPrWaves * i) * 1024),
+                                       16, 0, 0);
+    };
+    // Where the keys of an instruction lie.  kEven: in one page (block_size is a multiple of 8, k0 of 32), whose number
+    // is a scalar load; the row is that of the first key, -1 without a page, `left` the keys before k1.
+    // Otherwise each lane looks up its own key (a load without a condition), and the row is the lane's, -1 without a key.
     struct Look {
-      int page, rem;
+      int page, rem, left;
+    };
+    struct Place {
+      int row, left;
     };
     auto look = [&](int t, int i) {
-      const int j = k0 + t * kPrTile + (wave + kPrWaves * i) * kRpi + crow;
-      const int jc = min(j, k1 - 1), blk = pg_block(a, jc);
-      return Look{bt[blk], j < k1 ? jc - blk * a.block_size : -1};
+      const int j = first_key(t, i) + (kEven ? 0 : crow), jc = min(j, k1 - 1), blk = pg_block(a, jc);
+      typedef const __attribute__((address_space(4))) int32_t const_i32;
+      const int page = kEven ? *(const_i32*)(bt + __builtin_amdgcn_readfirstlane(blk)) : bt[blk];
+      return Look{page, jc - blk * a.block_size, k1 - j};
     };
-    // Row of the caches, -1 where there is no key.
-    auto row_of = [&](const Look& l) {
-      const bool ok = l.rem >= 0 && (uint32_t)l.page < (uint32_t)a.num_blocks;
-      return ok ? l.page * a.block_size + l.rem : -1;
+    auto place = [&](const Look& l) {
+      const bool ok = l.left > 0 && (uint32_t)l.page < (uint32_t)a.num_blocks;
+      return Place{ok ? l.page * a.block_size + l.rem : -1, l.left};
     };
-    auto dma = [&](const uint8_t* cache, int row, int ring, int t, int i) {
-      const int n = wave + kPrWaves * i;
-      const int64_t at = ((int64_t)row * a.G + kvg) * kRow + 16 * (cpos ^ pr_swz<kD>(n * kRpi + crow));
-      const uint8_t* src = row >= 0 ? cache + at : zero;
-      __builtin_amdgcn_global_load_lds((gqa_gbl_void*)src,
-                                       (gqa_lds_void*)(lds + (4 * ring + (t & 3)) * kTileBytes + n * 1024), 16, 0, 0);
+    const int64_t row_bytes = (int64_t)a.G * kRow;
+    const int lane_off = crow * a.G * kRow + swz;
+    auto dma = [&](const uint8_t* cache, const Place& p, int ring, int t, int i) {
+      if constexpr (kEven) {
+        const uint8_t* base = cache + p.row * row_bytes + kvg * kRow;
+        if (p.row >= 0 && p.left >= kRpi) to_lds(base + lane_off, ring, t, i);
+        else to_lds(p.row >= 0 && crow < p.left ? base + lane_off : zero, ring, t, i);
+      } else {
+        to_lds(p.row >= 0 ? cache + p.row * row_bytes + kvg * kRow + swz : zero, ring, t, i);
+      }
     };
-    Look next[kI];  // of tile t + 3
-    int vnext[kI];  // of tile t + 2
+    Look next[kI];    // of tile t + 3
+    Place vnext[kI];  // of tile t + 2
     {
-      int at0[kI], at1[kI];
+      Place at0[kI], at1[kI];
 #pragma unroll
       for (int i = 0; i < kI; ++i) {
-        at0[i] = row_of(look(0, i));
-        at1[i] = row_of(look(1, i));
-        vnext[i] = row_of(look(2, i));
+        at0[i] = place(look(0, i));
+        at1[i] = place(look(1, i));
+        vnext[i] = place(look(2, i));
         next[i] = look(3, i);
       }
 #pragma unroll
@@ -522,6 +542,19 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
 #pragma unroll
       for (int i = 0; i < kI; ++i) dma(kb, vnext[i], 0, 2, i);
     }
+    auto advance = [&](int t) {  // what X(t) starts
+      Place at[kI];
+#pragma unroll
+      for (int i = 0; i < kI; ++i) at[i] = place(next[i]);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) next[i] = look(t + 4, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(kb, at[i], 0, t + 3, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) dma(vb, vnext[i], 1, t + 2, i);
+#pragma unroll
+      for (int i = 0; i < kI; ++i) vnext[i] = at[i];
+    };
 
     const uint32_t lds0 = gqa_lds_u32(lds);
     // K operand (A), step st, key block kb: key 32 kb + r, dims 16 st + 8 hi .. + 7.
@@ -534,88 +567,66 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     const uint32_t v_at =
         lds0 + 4 * kTileBytes + vk * kRow + 16 * ((2 * h + (q & 1)) ^ pr_swz<kD>(vk)) + 8 * ((q >> 1) & 1);
 
+    // A body's LDS reads, in batches of four: batches 0 .. kNk - 1 the K operands of two steps of both key blocks, then
+    // the V operands of two column blocks and 16 keys.  Three batches are in flight ahead of the one multiplied.
+    constexpr int kNk = kSt / 2, kNv = 2 * kNb;
+    u32x4 kop[kNk][4];
+    u32x2 vop[kNv][4];
     u32x4 pb[4];
-    u32x4 kop[2][4];
-    u32x2 vop[2][2 * kNb];
-    // Scores: batch i holds the operands of steps 2 i, 2 i + 1 of both key blocks.
-    auto k_read = [&](int t, auto batch) {
+    f32x16 c[2];
+    auto read = [&](int t, auto batch) {
       constexpr int i = decltype(batch)::value;
-      const uint32_t at = k_at + (t & 3) * kTileBytes;
-      gqa_b128<0>(kop[i & 1][0], at ^ (64 * i));
-      gqa_b128<32 * kRow>(kop[i & 1][1], at ^ (64 * i));
-      gqa_b128<0>(kop[i & 1][2], at ^ (64 * i + 32));
-      gqa_b128<32 * kRow>(kop[i & 1][3], at ^ (64 * i + 32));
-    };
-    f32x16 none;  // no sums yet
-#pragma unroll
-    for (int i = 0; i < 16; ++i) none[i] = 0.f;
-    auto k_mul = [&](f32x16(&c)[2], auto batch) {
-      constexpr int i = decltype(batch)::value;
-      c[0] = pr_mfma<kF16>(kop[i & 1][0], qb[2 * i], i == 0 ? none : c[0]);
-      c[1] = pr_mfma<kF16>(kop[i & 1][1], qb[2 * i], i == 0 ? none : c[1]);
-      c[0] = pr_mfma<kF16>(kop[i & 1][2], qb[2 * i + 1], c[0]);
-      c[1] = pr_mfma<kF16>(kop[i & 1][3], qb[2 * i + 1], c[1]);
-    };
-    auto v_read = [&](int t, auto step) {
-      constexpr int u = decltype(step)::value;
-      const uint32_t at = v_at + (t & 3) * kTileBytes;
-#pragma unroll
-      for (int p = 0; p < kNb; ++p) {
-        gqa_tr<16 * u * kRow>(vop[u & 1][2 * p], at ^ (64 * p + 16 * ((2 * u) & 3)));
-        gqa_tr<(16 * u + 8) * kRow>(vop[u & 1][2 * p + 1], at ^ (64 * p + 16 * ((2 * u + 1) & 3)));
-      }
-    };
-    auto v_mul = [&](auto step) {
-      constexpr int u = decltype(step)::value;
-#pragma unroll
-      for (int p = 0; p < kNb; ++p) {
-        const u32x2 x = vop[u & 1][2 * p], y = vop[u & 1][2 * p + 1];
-        o[p] = pr_mfma<kF16>(u32x4{x.x, x.y, y.x, y.y}, pb[u], o[p]);
-      }
-    };
-    constexpr std::integral_constant<int, 0> c0{};
-    constexpr std::integral_constant<int, 1> c1{};
-    constexpr std::integral_constant<int, 2> c2{};
-    constexpr std::integral_constant<int, 3> c3{};
-    constexpr int kV = 2 * kNb;  // LDS reads of a step
-    // The scores of tile t; the reads of tile pv's first V step go out under its last products (pv < 0: none).
-    auto scores = [&](f32x16(&c)[2], int t, auto with_v) {
-      k_read(t, c0);
-      k_read(t, c1);
-      pr_lds_wait<4>(kop[0]);
-      k_mul(c, c0);
-      if constexpr (kD == 128) {
-        k_read(t, c2);
-        pr_lds_wait<4>(kop[1]);
-        k_mul(c, c1);
-        k_read(t, c3);
-        pr_lds_wait<4>(kop[0]);
-        k_mul(c, c2);
-      }
-      if constexpr (decltype(with_v)::value) {
-        v_read(t - 1, c0);
-        pr_lds_wait<kV>(kop[1]);
+      if constexpr (i < kNk) {
+        const uint32_t at = k_at + (t & 3) * kTileBytes;
+        gqa_b128<0>(kop[i][0], at ^ (64 * i));
+        gqa_b128<32 * kRow>(kop[i][1], at ^ (64 * i));
+        gqa_b128<0>(kop[i][2], at ^ (64 * i + 32));
+        gqa_b128<32 * kRow>(kop[i][3], at ^ (64 * i + 32));
       } else {
-        pr_lds_wait<0>(kop[1]);
+        constexpr int u = (i - kNk) / (kNb / 2), p = 2 * ((i - kNk) % (kNb / 2));
+        const uint32_t at = v_at + ((t - 1) & 3) * kTileBytes;
+        gqa_tr<16 * u * kRow>(vop[i - kNk][0], at ^ (64 * p + 16 * ((2 * u) & 3)));
+        gqa_tr<(16 * u + 8) * kRow>(vop[i - kNk][1], at ^ (64 * p + 16 * ((2 * u + 1) & 3)));
+        gqa_tr<16 * u * kRow>(vop[i - kNk][2], at ^ (64 * p + 64 + 16 * ((2 * u) & 3)));
+        gqa_tr<(16 * u + 8) * kRow>(vop[i - kNk][3], at ^ (64 * p + 64 + 16 * ((2 * u + 1) & 3)));
       }
-      if constexpr (kD == 128) k_mul(c, c3);
-      else k_mul(c, c1);
     };
-    auto products = [&](int t, auto started) {
-      if constexpr (!decltype(started)::value) v_read(t, c0);
-      v_read(t, c1);
-      pr_lds_wait<kV>(vop[0]);
-      v_mul(c0);
-      v_read(t, c2);
-      pr_lds_wait<kV>(vop[1]);
-      v_mul(c1);
-      v_read(t, c3);
-      pr_lds_wait<kV>(vop[0]);
-      v_mul(c2);
-      pr_lds_wait<0>(vop[1]);
-      v_mul(c3);
+    auto mul = [&](auto batch) {
+      constexpr int i = decltype(batch)::value;
+      if constexpr (i < kNk) {
+        if constexpr (i == 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) c[k][e] = 0.f;
+        }
+        c[0] = pr_mfma<kF16>(kop[i][0], qb[2 * i], c[0]);
+        c[1] = pr_mfma<kF16>(kop[i][1], qb[2 * i], c[1]);
+        c[0] = pr_mfma<kF16>(kop[i][2], qb[2 * i + 1], c[0]);
+        c[1] = pr_mfma<kF16>(kop[i][3], qb[2 * i + 1], c[1]);
+      } else {
+        constexpr int u = (i - kNk) / (kNb / 2), p = 2 * ((i - kNk) % (kNb / 2));
+        const u32x2(&v)[4] = vop[i - kNk];
+        o[p] = pr_mfma<kF16>(u32x4{v[0].x, v[0].y, v[1].x, v[1].y}, pb[u], o[p]);
+        o[p + 1] = pr_mfma<kF16>(u32x4{v[2].x, v[2].y, v[3].x, v[3].y}, pb[u], o[p + 1]);
+      }
     };
-    auto softmax = [&](f32x16(&c)[2], int j0) {
+    // Batches kFrom .. kTo - 1: scores of tile t, products of tile t - 1.
+    auto body = [&](int t, auto from, auto to) {
+      constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
+      pr_each<kFrom, (kTo - kFrom < 3 ? kTo : kFrom + 3)>([&](auto i) { read(t, i); });
+      pr_each<kFrom, kTo>([&](auto i) {
+        constexpr int n = decltype(i)::value, left = kTo - 1 - n < 3 ? kTo - 1 - n : 3;
+        if constexpr (n + 3 < kTo) read(t, std::integral_constant<int, n + 3>{});
+        if constexpr (n < kNk) pr_lds_wait<4 * left>(kop[n]);
+        else pr_lds_wait<4 * left>(vop[n - kNk]);
+        mul(i);
+      });
+    };
+    constexpr std::integral_constant<int, 0> kFirst{};
+    constexpr std::integral_constant<int, kNk> kMid{};
+    constexpr std::integral_constant<int, kNk + kNv> kAll{};
+    auto softmax = [&](int j0) {
       if (holes || j0 + kPrTile - 1 > lim_min || j0 < low_max) {
         uint64_t there = ~(uint64_t)0;  // keys in pages of the pool
         if (holes) there = __ballot((uint32_t)bt[pg_block(a, min(j0 + lane, k1 - 1))] < (uint32_t)a.num_blocks);
@@ -663,50 +674,39 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
                       gqa_pack<kF16>(e[x + 4], e[x + 5]), gqa_pack<kF16>(e[x + 6], e[x + 7])};
       }
     };
-    // Tiles that no row of the wave sees take no part in its sums.
-    auto seen = [&](int t) {
-      const int j0 = k0 + t * kPrTile;
-      return j0 <= lim_max && j0 + kPrTile - 1 >= low_min;
-    };
-
+    const auto turn = [] { __builtin_amdgcn_s_barrier(); };
     gqa_wait_vmcnt<4 * kI>();
-    __builtin_amdgcn_s_barrier();
-    if (wave >= 4) __builtin_amdgcn_s_barrier();
-    bool before = false;  // tile t - 1 was seen
-    for (int t = 0; t < nt; ++t) {
-      const bool now = seen(t);
-      f32x16 c[2];
+    turn();
+    if (wave >= 4) turn();
+    if (first < rows) {
       __builtin_amdgcn_s_setprio(1);
-      if (now && before) {
-        scores(c, t, std::true_type{});
-        products(t - 1, std::true_type{});
-      } else if (now) {
-        scores(c, t, std::false_type{});
-      } else if (before) {
-        products(t - 1, std::false_type{});
-      }
+      body(0, kFirst, kMid);
       __builtin_amdgcn_s_setprio(0);
       gqa_wait_vmcnt<2 * kI>();
-      __builtin_amdgcn_s_barrier();
-      {
-        int at[kI];
-#pragma unroll
-        for (int i = 0; i < kI; ++i) at[i] = row_of(next[i]);
-#pragma unroll
-        for (int i = 0; i < kI; ++i) next[i] = look(t + 4, i);
-#pragma unroll
-        for (int i = 0; i < kI; ++i) dma(kb, at[i], 0, t + 3, i);
-#pragma unroll
-        for (int i = 0; i < kI; ++i) dma(vb, vnext[i], 1, t + 2, i);
-#pragma unroll
-        for (int i = 0; i < kI; ++i) vnext[i] = at[i];
+      turn();
+      advance(0);
+      softmax(k0);
+      turn();
+      for (int t = 1; t < nt; ++t) {
+        __builtin_amdgcn_s_setprio(1);
+        body(t, kFirst, kAll);
+        __builtin_amdgcn_s_setprio(0);
+        gqa_wait_vmcnt<2 * kI>();
+        turn();
+        advance(t);
+        softmax(k0 + t * kPrTile);
+        turn();
       }
-      if (now) softmax(c, k0 + t * kPrTile);
-      before = now;
-      __builtin_amdgcn_s_barrier();
+      body(nt, kMid, kAll);
+    } else {  // no rows: this wave only moves tiles
+      for (int t = 0; t < nt; ++t) {
+        gqa_wait_vmcnt<2 * kI>();
+        turn();
+        advance(t);
+        turn();
+      }
     }
-    if (before) products(nt - 1, std::false_type{});
-    if (wave < 4) __builtin_amdgcn_s_barrier();
+    if (wave < 4) turn();
     __builtin_amdgcn_s_waitcnt(0);  // the DMA of tiles behind the last
   }
 
@@ -761,14 +761,14 @@ struct PgKeys {
     pg_keys<kF16, kD, kHB>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
   }
 };
-template <bool kF16_, int kD_>
+template <bool kF16_, int kD_, bool kEven>
 struct PgRows {
   static constexpr bool kF16 = kF16_;
   static constexpr int kD = kD_, kR = kPrRows, kUnitKeys = kPrTile, kThreads = kPrThreads;
   static constexpr int kLds = 8 * kPrTile * kD * 2;
   static __device__ __forceinline__ void item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                               bool whole, float* part, uint8_t* lds) {
-    pg_rows<kF16, kD>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
+    pg_rows<kF16, kD, kEven>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
     __syncthreads();  // the rings are free for the next item
   }
 };
@@ -1016,7 +1016,8 @@ static hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
 
 template <bool kF16, int kD>
 static hipError_t pg_dispatch(const PgArgs& a, int rows, hipStream_t stream) {
-  if (rows == kPrRows) return pg_launch<PgRows<kF16, kD>>(a, stream);
+  if (rows == kPrRows && a.block_size % 8 == 0) return pg_launch<PgRows<kF16, kD, true>>(a, stream);
+  if (rows == kPrRows) return pg_launch<PgRows<kF16, kD, false>>(a, stream);
   return rows == 32 ? pg_launch<PgKeys<kF16, kD, 2>>(a, stream) : pg_launch<PgKeys<kF16, kD, 1>>(a, stream);
 }
 
