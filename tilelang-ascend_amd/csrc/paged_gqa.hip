@@ -40,7 +40,7 @@ constexpr int kPgTile = 32;                 // keys a wave of pg_keys takes at o
 constexpr int kPgWaves = 4;
 constexpr int kPgThreads = kPgWaves * kWave;
 constexpr int kPgUnit = kPgWaves * kPgTile;  // 128 keys
-constexpr int kPgMaxSlots = 1024;            // of a call whose tiles share the line of units
+constexpr int kPgMaxSlots = 4096;            // of a call whose tiles share the line of units
 constexpr float kPgInf = __builtin_huge_valf();
 
 struct PgArgs {
@@ -473,11 +473,13 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
   const int32_t* bt = a.table + (int64_t)b * a.max_blocks;
   const int nt = k1 > k0 ? (k1 - k0 + kPrTile - 1) / kPrTile : 0;
   if (nt > 0) {
-    // Pages outside the pool hide their keys: looked for once, the comparisons look again where there are any.
+    // Pages outside the pool hide their keys: looked for once, the comparisons look again where there are any.  The
+    // first load of a thread is judged behind the first DMA.
+    const int last_blk = pg_block(a, k1 - 1), my_blk = pg_block(a, k0) + tid;
+    const int my_page = bt[min(my_blk, last_blk)];
     int outside = 0;
-    for (int blk = pg_block(a, k0) + tid; blk <= pg_block(a, k1 - 1); blk += kPrThreads)
+    for (int blk = my_blk + kPrThreads; blk <= last_blk; blk += kPrThreads)
       outside |= (uint32_t)bt[blk] >= (uint32_t)a.num_blocks;
-    const bool holes = __syncthreads_or(outside) != 0;
 
     const uint8_t *kb = reinterpret_cast<const uint8_t*>(a.kc), *vb = reinterpret_cast<const uint8_t*>(a.vc);
     const int crow = lane / kChunks, cpos = lane % kChunks;
@@ -626,6 +628,16 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     constexpr std::integral_constant<int, 0> kFirst{};
     constexpr std::integral_constant<int, kNk> kMid{};
     constexpr std::integral_constant<int, kNk + kNv> kAll{};
+    const auto turn = [] { __builtin_amdgcn_s_barrier(); };
+    gqa_wait_vmcnt<4 * kI>();
+    // The waves' findings pass through LDS by hand: a fence or a plain access would wait for the DMA.
+    const uint32_t flags = gqa_lds_u32(lds + 8 * kTileBytes);
+    const bool found = __any(outside | ((uint32_t)my_page >= (uint32_t)a.num_blocks));
+    __asm__ __volatile__("ds_write_b8 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(flags + wave), "v"((int)found) : "memory");
+    turn();
+    u32x2 seen;
+    __asm__ __volatile__("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(seen) : "v"(flags) : "memory");
+    const bool holes = __builtin_amdgcn_readfirstlane((int)(seen.x | seen.y)) != 0;
     auto softmax = [&](int j0) {
       if (holes || j0 + kPrTile - 1 > lim_min || j0 < low_max) {
         uint64_t there = ~(uint64_t)0;  // keys in pages of the pool
@@ -674,9 +686,6 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
                       gqa_pack<kF16>(e[x + 4], e[x + 5]), gqa_pack<kF16>(e[x + 6], e[x + 7])};
       }
     };
-    const auto turn = [] { __builtin_amdgcn_s_barrier(); };
-    gqa_wait_vmcnt<4 * kI>();
-    turn();
     if (wave >= 4) turn();
     if (first < rows) {
       __builtin_amdgcn_s_setprio(1);
@@ -765,7 +774,7 @@ template <bool kF16_, int kD_, bool kEven>
 struct PgRows {
   static constexpr bool kF16 = kF16_;
   static constexpr int kD = kD_, kR = kPrRows, kUnitKeys = kPrTile, kThreads = kPrThreads;
-  static constexpr int kLds = 8 * kPrTile * kD * 2;
+  static constexpr int kLds = 8 * kPrTile * kD * 2 + 16;  // two rings of four stages, the waves' flags
   static __device__ __forceinline__ void item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                               bool whole, float* part, uint8_t* lds) {
     pg_rows<kF16, kD, kEven>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
@@ -819,40 +828,43 @@ __global__ __launch_bounds__(W::kThreads) void pg_direct_kernel(PgArgs a) {
   W::item(a, s, b, tile, kvg, lo, hi, true, nullptr, lds);
 }
 
-// The line of units: slot x takes units [at[x], at[x + 1]) of each group.  Every workgroup of the split kernel and the
-// join makes it alike, in LDS.
+// The line of units: slot x takes [at[x], at[x + 1]) of each group, a tile's first kExtra for what it costs beside
+// its keys (start and end, three units' time in either way).  Every workgroup of the split kernel and the join makes
+// it alike, in LDS.
+constexpr int kPgExtra = 3;
+constexpr int kPgLineCu = 1024;
 struct PgLine {
-  int64_t at[kPgMaxSlots + 1];
-  int seq[kPgMaxSlots];
-  int32_t cu[kPgMaxSlots];
+  int at[kPgMaxSlots + 1];
+  uint16_t seq[kPgMaxSlots];
+  int32_t cu[kPgLineCu];
 };
-static_assert(sizeof(PgLine) <= 16 * 1024 + 8, "LDS of the line");
 
 template <class W>
 __device__ __forceinline__ void pg_line(const PgArgs& a, PgLine& line, int threads) {
   const int tid = threadIdx.x;
-  if (a.cu_q)
-    for (int b = tid; b < a.B; b += threads) line.cu[b] = a.cu_q[b];  // B < slots
+  const bool copy = a.cu_q && a.B <= kPgLineCu;
+  if (copy)
+    for (int b = tid; b < a.B; b += threads) line.cu[b] = a.cu_q[b];
   __syncthreads();
   for (int x = tid; x < a.slots; x += threads) {
-    const int b = pg_find(a, line.cu, x, W::kR);
+    const int b = pg_find(a, copy ? line.cu : a.cu_q, x, W::kR);
     const PgSeq s = pg_seq(a, b);
     int lo, hi, units = 0;
     // A tile without keys takes a unit too: it writes its zeros.
     if (pg_range(a, s, x - pg_slot(s.start, a.Hg, b, W::kR), W::kR, lo, hi))
-      units = max(1, (int)(((int64_t)hi - lo + W::kUnitKeys - 1) / W::kUnitKeys));
-    line.seq[x] = b;
+      units = kPgExtra + max(1, (hi - lo + W::kUnitKeys - 1) / W::kUnitKeys);
+    line.seq[x] = (uint16_t)b;
     line.at[x + 1] = units;
   }
   if (tid == 0) line.at[0] = 0;
   __syncthreads();
   if (tid < kWave) {
-    int64_t sum = 0;
+    int sum = 0;
     for (int x = tid; x < ((a.slots + kWave - 1) & ~(kWave - 1)); x += kWave) {
-      int64_t v = x < a.slots ? line.at[x + 1] : 0;
+      int v = x < a.slots ? line.at[x + 1] : 0;
 #pragma unroll
       for (int o = 1; o < kWave; o <<= 1) {
-        const int64_t u = __shfl_up(v, o, kWave);
+        const int u = __shfl_up(v, o, kWave);
         if (tid >= o) v += u;
       }
       if (x < a.slots) line.at[x + 1] = sum + v;
@@ -863,9 +875,16 @@ __device__ __forceinline__ void pg_line(const PgArgs& a, PgLine& line, int threa
 }
 
 // Units of a workgroup's part of the line.
-__device__ __forceinline__ int64_t pg_share(const PgArgs& a, const PgLine& line) {
-  const int64_t total = line.at[a.slots] * a.G;
-  return max((total + a.wgs - 1) / a.wgs, (int64_t)1);
+__device__ __forceinline__ int pg_share(const PgArgs& a, const PgLine& line) {
+  const int total = line.at[a.slots] * a.G;
+  return max((total + a.wgs - 1) / a.wgs, 1);
+}
+
+// A workgroup has at most two tiles that others share: one begun before its part of the line, and one that goes on
+// behind it.
+template <class W>
+__device__ __forceinline__ float* pg_part(const PgArgs& a, int wg, bool begun_before) {
+  return a.part + (int64_t)(2 * wg + (begun_before ? 0 : 1)) * pg_part_floats<W::kR, W::kD>();
 }
 
 template <class W>
@@ -873,79 +892,77 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   PgLine& line = *reinterpret_cast<PgLine*>(lds + W::kLds);
   pg_line<W>(a, line, W::kThreads);
-  const int64_t share = pg_share(a, line), total = line.at[a.slots] * a.G;
-  int64_t u = (int64_t)blockIdx.x * share;
-  const int64_t end = min(u + share, total);
-  int x = 0;  // the slot that unit u lies in: the last whose units start at or before u and that has any
+  const int share = pg_share(a, line), total = line.at[a.slots] * a.G;
+  const int begin = min((int)min((int64_t)blockIdx.x * share, (int64_t)total), total);
+  const int end = (int)min((int64_t)begin + share, (int64_t)total);
+  int x = 0;  // the last slot whose line starts at or before `begin`
   {
     int x1 = a.slots - 1;
     while (x < x1) {
       const int mid = (x + x1 + 1) >> 1;
-      if (line.at[mid] * a.G <= u) x = mid;
+      if (line.at[mid] * a.G <= begin) x = mid;
       else x1 = mid - 1;
     }
   }
   x = __builtin_amdgcn_readfirstlane(x);
-  while (u < end) {
-    const int64_t from = line.at[x], units = line.at[x + 1] - from;
-    if (units == 0) {
-      ++x;
-      continue;
-    }
-    const int b = __builtin_amdgcn_readfirstlane(line.seq[x]);
+  for (; x < a.slots; ++x) {
+    const int from = __builtin_amdgcn_readfirstlane(line.at[x]) * a.G;
+    if (from >= end) break;
+    const int length = __builtin_amdgcn_readfirstlane(line.at[x + 1] - line.at[x]);
+    if (length == 0) continue;
+    const int b = __builtin_amdgcn_readfirstlane((int)line.seq[x]);
     const PgSeq s = pg_seq(a, b);
     const int tile = x - pg_slot(s.start, a.Hg, b, W::kR);
     int lo, hi;
-    if (!pg_range(a, s, tile, W::kR, lo, hi)) return;  // not reached: the slot has units
-    for (int kvg = (int)((u - from * a.G) / units); kvg < a.G && u < end; ++kvg) {
-      const int64_t u0 = from * a.G + kvg * units;  // the item's units on the line: [u0, u0 + units)
-      const int64_t stop = min(end, u0 + units);
-      const bool whole = u == u0 && stop == u0 + units;
-      const int k0 = (int)min((int64_t)hi, lo + (u - u0) * W::kUnitKeys);
-      const int k1 = (int)min((int64_t)hi, lo + (stop - u0) * W::kUnitKeys);
-      float* part = a.part + ((int64_t)x * a.G + kvg + blockIdx.x) * pg_part_floats<W::kR, W::kD>();
-      W::item(a, s, b, tile, kvg, __builtin_amdgcn_readfirstlane(k0), __builtin_amdgcn_readfirstlane(k1), whole, part,
-              lds);
-      u = stop;
+    if (!pg_range(a, s, tile, W::kR, lo, hi)) break;  // not reached: the slot has units
+    for (int kvg = max(0, (begin - from) / length); kvg < a.G; ++kvg) {
+      const int u0 = from + kvg * length + kPgExtra, u1 = u0 + length - kPgExtra;  // the tile's units on the line
+      if (u0 - kPgExtra >= end) break;
+      const int c0 = max(u0, begin), c1 = min(u1, end);
+      if (c0 >= c1) continue;
+      const int k0 = (int)min((int64_t)hi, lo + (int64_t)(c0 - u0) * W::kUnitKeys);
+      const int k1 = (int)min((int64_t)hi, lo + (int64_t)(c1 - u0) * W::kUnitKeys);
+      W::item(a, s, b, tile, kvg, k0, k1, c0 == u0 && c1 == u1, pg_part<W>(a, blockIdx.x, u0 < begin), lds);
     }
-    ++x;
   }
 }
 
 // Joins the parts of each tile whose units lie in more than one workgroup's share: workgroup = (slot and group, rows).
+// A row's threads find the maximum together, then take 8 columns each.
 template <class W>
 __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
-  constexpr int kR = W::kR, kD = W::kD, kPart = pg_part_floats<kR, kD>();
+  constexpr int kR = W::kR, kD = W::kD;
   __shared__ PgLine line;
   pg_line<W>(a, line, kPgThreads);
-  const int64_t share = pg_share(a, line);
+  const int share = pg_share(a, line);
   const int x = blockIdx.x / a.G, kvg = blockIdx.x - x * a.G;
-  const int64_t units = line.at[x + 1] - line.at[x];
-  if (units == 0) return;
-  const int64_t u0 = line.at[x] * a.G + kvg * units;
-  const int w0 = (int)(u0 / share), np = (int)((u0 + units - 1) / share) - w0 + 1;
+  const int length = line.at[x + 1] - line.at[x];
+  if (length == 0) return;
+  const int u0 = line.at[x] * a.G + kvg * length + kPgExtra, u1 = u0 + length - kPgExtra;
+  const int w0 = u0 / share, np = (u1 - 1) / share - w0 + 1;
   if (np == 1) return;
   const int b = line.seq[x];
   const PgSeq s = pg_seq(a, b);
   const int tile = x - pg_slot(s.start, a.Hg, b, kR);
-  const float* base = a.part + ((int64_t)x * a.G + kvg + w0) * kPart;
   constexpr int kPerRow = kD / 8;
   constexpr int kRowsPass = kPgThreads / kPerRow;
   constexpr float kLn2 = 0.6931471805599453f;
-  const int hh = blockIdx.y * kRowsPass + threadIdx.x / kPerRow, c0 = 8 * (threadIdx.x % kPerRow);
+  const int hh = blockIdx.y * kRowsPass + threadIdx.x / kPerRow, t = threadIdx.x % kPerRow, c0 = 8 * t;
   const int rho = tile * kR + hh;
-  if (hh >= kR || rho >= s.span * a.Hg) return;
+  if (hh >= kR || rho >= s.span * a.Hg) return;  // a row's threads together
   const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
+  const auto part = [&](int p) { return pg_part<W>(a, w0 + p, u0 < (w0 + p) * share); };
   float M = -kPgInf;
-#pragma unroll 4
-  for (int p = 0; p < np; ++p) M = fmaxf(M, base[(int64_t)p * kPart + kR * kD + 2 * hh]);
+  for (int p = t; p < np; p += kPerRow) M = fmaxf(M, part(p)[kR * kD + 2 * hh]);
+#pragma unroll
+  for (int o = 1; o < kPerRow; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
   const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
   M = fmaxf(M, sk);
   const float M_use = M == -kPgInf ? 0.f : M;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = fast_exp2(sk - M_use);
-#pragma unroll 4
+#pragma unroll 8
   for (int p = 0; p < np; ++p) {
-    const float* pp = base + (int64_t)p * kPart;
+    const float* pp = part(p);
     const float f = fast_exp2(pp[kR * kD + 2 * hh] - M_use);
     sum += f * pp[kR * kD + 2 * hh + 1];
     const f32x4 x0 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
@@ -978,19 +995,19 @@ static PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) 
   p.rows = T * Hg <= 16 * B ? 16 : T * Hg <= 32 * B ? 32 : kPrRows;
   p.slots = T * Hg / p.rows + B + 1;
   p.wgs = 0;
-  // One workgroup fits a CU: fewer than two rounds of tiles share the line.
-  if (p.slots <= kPgMaxSlots && p.slots * G < 512) {
-    const int64_t unit = p.rows == kPrRows ? kPrTile : kPgUnit;
-    const int64_t units = p.slots * G * ((most + unit - 1) / unit + 1);
+  // One workgroup fits a CU.  Fewer than two rounds of tiles share the line, and batches of many sequences, where slots
+  // without a tile lie between the others (a workgroup each for 64 x 8192 keys put the tiles on every other XCD: 330 us
+  // instead of 199).
+  const int64_t unit = p.rows == kPrRows ? kPrTile : kPgUnit;
+  const int64_t units = p.slots * G * ((most + unit - 1) / unit + 1 + kPgExtra);
+  if (p.slots <= kPgMaxSlots && units < ((int64_t)1 << 30) && (p.slots * G < 512 || 4 * (B + 1) > p.slots))
     p.wgs = (int)(units < 256 ? units : 256);
-  }
   return p;
 }
 
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
   const PgPlan p = pg_plan(T, B, H, G, most);
-  if (p.wgs == 0) return 0;
-  return (size_t)(p.slots * G + p.wgs) * p.rows * (D + 2) * sizeof(float);
+  return (size_t)(2 * p.wgs) * p.rows * (D + 2) * sizeof(float);
 }
 
 template <class W>
