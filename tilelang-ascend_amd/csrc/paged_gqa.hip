@@ -54,7 +54,8 @@ struct PgArgs {
   const float* sinks;     // [H] or null
   uint16_t* out;          // [T, H, D]
   float* lse;             // [T, H]
-  float* part;            // parts: sums [16 kHB, D], then (maximum, sum) [16 kHB, 2]
+  float* part;            // parts: sums [kR, D], then (maximum, sum) [kR, 2]
+  int32_t* line;          // [slots + 1] the line's `at`, then [slots] its `seq`, for the join
   int T, B, S, H, G, Hg, block_size, max_blocks, num_blocks, causal, win, wgs;
   int slots;              // of the call
   uint32_t div_mul;       // j / block_size = umulhi(j, div_mul) >> div_shift for 0 <= j < 2^31; 0: block_size is 1
@@ -829,8 +830,8 @@ __global__ __launch_bounds__(W::kThreads) void pg_direct_kernel(PgArgs a) {
 }
 
 // The line of units: slot x takes [at[x], at[x + 1]) of each group, a tile's first kExtra for what it costs beside
-// its keys (start and end, three units' time in either way).  Every workgroup of the split kernel and the join makes
-// it alike, in LDS.
+// its keys (start and end, three units' time in either way).  Every workgroup of the split kernel makes it alike, in
+// LDS; the first writes it out for the join.
 constexpr int kPgExtra = 3;
 constexpr int kPgLineCu = 1024;
 struct PgLine {
@@ -875,10 +876,7 @@ __device__ __forceinline__ void pg_line(const PgArgs& a, PgLine& line, int threa
 }
 
 // Units of a workgroup's part of the line.
-__device__ __forceinline__ int pg_share(const PgArgs& a, const PgLine& line) {
-  const int total = line.at[a.slots] * a.G;
-  return max((total + a.wgs - 1) / a.wgs, 1);
-}
+__device__ __forceinline__ int pg_share(const PgArgs& a, int total) { return max((total + a.wgs - 1) / a.wgs, 1); }
 
 // A workgroup has at most two tiles that others share: one begun before its part of the line, and one that goes on
 // behind it.
@@ -892,7 +890,13 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
   PgLine& line = *reinterpret_cast<PgLine*>(lds + W::kLds);
   pg_line<W>(a, line, W::kThreads);
-  const int share = pg_share(a, line), total = line.at[a.slots] * a.G;
+  if (blockIdx.x == 0) {
+    for (int x = threadIdx.x; x <= a.slots; x += W::kThreads) {
+      a.line[x] = line.at[x];
+      if (x < a.slots) a.line[a.slots + 1 + x] = line.seq[x];
+    }
+  }
+  const int total = line.at[a.slots] * a.G, share = pg_share(a, total);
   const int begin = min((int)min((int64_t)blockIdx.x * share, (int64_t)total), total);
   const int end = (int)min((int64_t)begin + share, (int64_t)total);
   int x = 0;  // the last slot whose line starts at or before `begin`
@@ -928,58 +932,97 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
 }
 
 // Joins the parts of each tile whose units lie in more than one workgroup's share: workgroup = (slot and group, rows).
-// A row's threads find the maximum together, then take 8 columns each.
+// kGroups groups of threads take every kGroups-th part of a pass's rows, 8 columns a thread, and are summed through
+// LDS: four for the tiles of few rows, whose keys may lie in many parts, one for those of 256, which have many rows.
+template <class W>
+struct PgJoin {
+  static constexpr int kPerRow = W::kD / 8;
+  static constexpr int kGroups = W::kR == kPrRows ? 1 : 4;
+  static constexpr int kPass = kPgThreads / kGroups / kPerRow;  // rows of a pass
+  static constexpr int kRows = W::kR == kPrRows ? 64 : kPass;   // rows of a workgroup
+  static_assert(W::kR % kRows == 0 && kRows % kPass == 0, "whole groups of rows");
+};
 template <class W>
 __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
+  typedef PgJoin<W> J;
   constexpr int kR = W::kR, kD = W::kD;
-  __shared__ PgLine line;
-  pg_line<W>(a, line, kPgThreads);
-  const int share = pg_share(a, line);
+  constexpr bool kF16 = W::kF16;
   const int x = blockIdx.x / a.G, kvg = blockIdx.x - x * a.G;
-  const int length = line.at[x + 1] - line.at[x];
+  const int from = a.line[x], length = a.line[x + 1] - from, share = pg_share(a, a.line[a.slots] * a.G);
+  const int b = a.line[a.slots + 1 + x];
   if (length == 0) return;
-  const int u0 = line.at[x] * a.G + kvg * length + kPgExtra, u1 = u0 + length - kPgExtra;
+  const int u0 = from * a.G + kvg * length + kPgExtra, u1 = u0 + length - kPgExtra;
   const int w0 = u0 / share, np = (u1 - 1) / share - w0 + 1;
   if (np == 1) return;
-  const int b = line.seq[x];
   const PgSeq s = pg_seq(a, b);
   const int tile = x - pg_slot(s.start, a.Hg, b, kR);
-  constexpr int kPerRow = kD / 8;
-  constexpr int kRowsPass = kPgThreads / kPerRow;
   constexpr float kLn2 = 0.6931471805599453f;
-  const int hh = blockIdx.y * kRowsPass + threadIdx.x / kPerRow, t = threadIdx.x % kPerRow, c0 = 8 * t;
-  const int rho = tile * kR + hh;
-  if (hh >= kR || rho >= s.span * a.Hg) return;  // a row's threads together
-  const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
+  const int group = threadIdx.x / (kPgThreads / J::kGroups), in = threadIdx.x % (kPgThreads / J::kGroups);
+  const int t = in % J::kPerRow, c0 = 8 * t;
   const auto part = [&](int p) { return pg_part<W>(a, w0 + p, u0 < (w0 + p) * share); };
-  float M = -kPgInf;
-  for (int p = t; p < np; p += kPerRow) M = fmaxf(M, part(p)[kR * kD + 2 * hh]);
+  __shared__ float sums[J::kGroups][9][kPgThreads / J::kGroups];
+  for (int r0 = 0; r0 < J::kRows; r0 += J::kPass) {
+    const int hh = blockIdx.y * J::kRows + r0 + in / J::kPerRow;
+    const int rho = tile * kR + hh;
+    if (rho - in / J::kPerRow >= s.span * a.Hg) break;  // no row of the pass
+    const bool live = rho < s.span * a.Hg;
+    float M = -kPgInf;
+    for (int p = t; p < np; p += J::kPerRow) M = fmaxf(M, part(p)[kR * kD + 2 * hh]);
 #pragma unroll
-  for (int o = 1; o < kPerRow; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
-  const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
-  M = fmaxf(M, sk);
-  const float M_use = M == -kPgInf ? 0.f : M;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = fast_exp2(sk - M_use);
-#pragma unroll 8
-  for (int p = 0; p < np; ++p) {
-    const float* pp = part(p);
-    const float f = fast_exp2(pp[kR * kD + 2 * hh] - M_use);
-    sum += f * pp[kR * kD + 2 * hh + 1];
-    const f32x4 x0 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
-    const f32x4 x1 = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0 + 4);
+    for (int o = 1; o < J::kPerRow; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
+    const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
+    const float sk = a.sinks && live ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
+    M = fmaxf(M, sk);
+    const float M_use = M == -kPgInf ? 0.f : M;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+    constexpr int kAhead = J::kGroups == 1 ? 2 : 8;  // parts whose loads are in flight together
+    for (int p0 = group; p0 < np; p0 += J::kGroups * kAhead) {
+      f32x4 x0[kAhead], x1[kAhead];
+      float m[kAhead], l[kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      acc[k] += f * x0[k];
-      acc[4 + k] += f * x1[k];
+      for (int j = 0; j < kAhead; ++j) {
+        const float* pp = part(min(p0 + J::kGroups * j, np - 1));
+        x0[j] = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
+        x1[j] = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0 + 4);
+        m[j] = pp[kR * kD + 2 * hh];
+        l[j] = pp[kR * kD + 2 * hh + 1];
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float f = p0 + J::kGroups * j < np ? fast_exp2(m[j] - M_use) : 0.f;
+        sum += f * l[j];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          acc[k] += f * x0[j][k];
+          acc[4 + k] += f * x1[j][k];
+        }
+      }
     }
+    if constexpr (J::kGroups > 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[group][k][in] = acc[k];
+      sums[group][8][in] = sum;
+      __syncthreads();
+      if (group > 0) return;  // one pass
+      sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < J::kGroups; ++w) {
+        sum += sums[w][8][in];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += sums[w][k][in];
+      }
+    }
+    if (!live) continue;
+    sum += fast_exp2(sk - M_use);
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t orow = (int64_t)(s.start + i) * a.H + h;
+    *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
+        u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
+              gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
+    if (c0 == 0) a.lse[orow] = sum > 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const int64_t orow = (int64_t)(s.start + i) * a.H + h;
-  constexpr bool kF16 = W::kF16;
-  *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
-      u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
-            gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-  if (c0 == 0) a.lse[orow] = sum > 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
 }
 
 // The launch of a call, from sizes that the host knows: T tokens, B sequences, at most `most` keys each.
@@ -1005,9 +1048,12 @@ static PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) 
   return p;
 }
 
+static size_t pg_part_bytes(const PgPlan& p, int64_t D) { return (size_t)(2 * p.wgs) * p.rows * (D + 2) * sizeof(float); }
+
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
   const PgPlan p = pg_plan(T, B, H, G, most);
-  return (size_t)(2 * p.wgs) * p.rows * (D + 2) * sizeof(float);
+  if (p.wgs == 0) return 0;
+  return pg_part_bytes(p, D) + (size_t)(2 * p.slots + 1) * sizeof(int32_t);
 }
 
 template <class W>
@@ -1025,8 +1071,7 @@ static hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
   e = set_dynamic_lds_once<pg_split_kernel<W>>(split_lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((pg_split_kernel<W>), dim3(a.wgs), dim3(W::kThreads), split_lds, stream, a);
-  constexpr int kRowsPass = kPgThreads / (W::kD / 8);
-  const dim3 join(tiles.x, (W::kR + kRowsPass - 1) / kRowsPass);
+  const dim3 join(tiles.x, W::kR / PgJoin<W>::kRows);
   hipLaunchKernelGGL((pg_join_kernel<W>), join, dim3(kPgThreads), 0, stream, a);
   return hipGetLastError();
 }
@@ -1060,6 +1105,7 @@ hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const vo
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   a.part = static_cast<float*>(workspace);
+  a.line = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + pg_part_bytes(p, D));
   a.T = (int)T;
   a.B = (int)B;
   a.S = (int)S;
