@@ -425,10 +425,10 @@ constexpr int kPrTile = 64;             // keys
 
 // As pg_keys, for 256 rows.  Body t of a wave is C(t): scores of tile t and the products of tile t - 1 with V, a
 // barrier, X(t): exponentials of tile t, a barrier; waves 4 to 7 run one barrier behind, so that on each SIMD one
-// wave is in C while the other is in X.  Rings of four stages: X(t) starts the DMA of K of tile t + 3 and V of tile
+// wave is in C while the other is in X.  Rings of four stages: C(t) starts the DMA of K of tile t + 3 and V of tile
 // t + 2, into the stages of K(t - 1) and V(t - 2), whose last reads (in C(t - 1) of the later waves) lie before the
-// barrier ahead of X(t) of the earlier ones; the wait at the end of C(t) leaves only what X(t - 1) started in flight,
-// so that behind the next barrier K(t + 1) and V(t) are whole.
+// barrier ahead of C(t) of the earlier ones.  The wait at the end of C(t) leaves only what C(t) started in flight:
+// behind two barriers more K(t + 2) and V(t + 1) are whole, so that the end of X(t) may read ahead of C(t + 1).
 template <bool kF16, int kD, bool kEven>
 __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
@@ -515,16 +515,11 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     const int64_t row_bytes = (int64_t)a.G * kRow;
     const int lane_off = crow * a.G * kRow + swz;
     auto dma = [&](const uint8_t* cache, const Place& p, int ring, int t, int i) {
-      if constexpr (kEven) {
-        const uint8_t* base = cache + p.row * row_bytes + kvg * kRow;
-        if (p.row >= 0 && p.left >= kRpi) to_lds(base + lane_off, ring, t, i);
-        else to_lds(p.row >= 0 && crow < p.left ? base + lane_off : zero, ring, t, i);
-      } else {
-        to_lds(p.row >= 0 ? cache + p.row * row_bytes + kvg * kRow + swz : zero, ring, t, i);
-      }
+      const uint8_t* base = cache + p.row * row_bytes + kvg * kRow;
+      if constexpr (kEven) to_lds(p.row >= 0 && crow < p.left ? base + lane_off : zero, ring, t, i);
+      else to_lds(p.row >= 0 ? base + swz : zero, ring, t, i);
     };
-    Look next[kI];    // of tile t + 3
-    Place vnext[kI];  // of tile t + 2
+    Place knext[kI], vnext[kI];  // of tiles t + 3 and t + 2
     {
       Place at0[kI], at1[kI];
 #pragma unroll
@@ -532,7 +527,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         at0[i] = place(look(0, i));
         at1[i] = place(look(1, i));
         vnext[i] = place(look(2, i));
-        next[i] = look(3, i);
+        knext[i] = place(look(3, i));
       }
 #pragma unroll
       for (int i = 0; i < kI; ++i) dma(kb, at0[i], 0, 0, i);
@@ -545,18 +540,16 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
 #pragma unroll
       for (int i = 0; i < kI; ++i) dma(kb, vnext[i], 0, 2, i);
     }
-    auto advance = [&](int t) {  // what X(t) starts
-      Place at[kI];
+    auto dma_k = [&](int t) {
 #pragma unroll
-      for (int i = 0; i < kI; ++i) at[i] = place(next[i]);
+      for (int i = 0; i < kI; ++i) dma(kb, knext[i], 0, t + 3, i);
+    };
+    auto dma_v = [&](int t) {
 #pragma unroll
-      for (int i = 0; i < kI; ++i) next[i] = look(t + 4, i);
-#pragma unroll
-      for (int i = 0; i < kI; ++i) dma(kb, at[i], 0, t + 3, i);
-#pragma unroll
-      for (int i = 0; i < kI; ++i) dma(vb, vnext[i], 1, t + 2, i);
-#pragma unroll
-      for (int i = 0; i < kI; ++i) vnext[i] = at[i];
+      for (int i = 0; i < kI; ++i) {
+        dma(vb, vnext[i], 1, t + 2, i);
+        vnext[i] = knext[i];
+      }
     };
 
     const uint32_t lds0 = gqa_lds_u32(lds);
@@ -614,17 +607,33 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         o[p + 1] = pr_mfma<kF16>(u32x4{v[2].x, v[2].y, v[3].x, v[3].y}, pb[u], o[p + 1]);
       }
     };
-    // Batches kFrom .. kTo - 1: scores of tile t, products of tile t - 1.
+    // Batches kFrom .. kTo - 1: scores of tile t, products of tile t - 1; the first three are read ahead by `start`.
+    auto start = [&](int t, auto from) {
+      constexpr int kFrom = decltype(from)::value;
+      pr_each<kFrom, kFrom + 3>([&](auto i) { read(t, i); });
+    };
     auto body = [&](int t, auto from, auto to) {
       constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
-      pr_each<kFrom, (kTo - kFrom < 3 ? kTo : kFrom + 3)>([&](auto i) { read(t, i); });
       pr_each<kFrom, kTo>([&](auto i) {
-        constexpr int n = decltype(i)::value, left = kTo - 1 - n < 3 ? kTo - 1 - n : 3;
-        if constexpr (n + 3 < kTo) read(t, std::integral_constant<int, n + 3>{});
+        // Twelve reads are out: the counter of them holds fifteen.
+        constexpr int n = decltype(i)::value, left = kTo - 1 - n < 2 ? kTo - 1 - n : 2;
         if constexpr (n < kNk) pr_lds_wait<4 * left>(kop[n]);
         else pr_lds_wait<4 * left>(vop[n - kNk]);
+        if constexpr (n + 3 < kTo) read(t, std::integral_constant<int, n + 3>{});
+        mul(i);
+        if constexpr (n == 0) dma_k(t);
+        if constexpr (n == 1) dma_v(t);
+      });
+    };
+    auto scores_only = [&](int t) {  // batches 0 and 1 are on their way
+      pr_each<0, kNk>([&](auto i) {
+        constexpr int n = decltype(i)::value;
+        pr_lds_wait<n + 1 < kNk ? 4 : 0>(kop[n]);
+        if constexpr (n + 2 < kNk) read(t, std::integral_constant<int, n + 2>{});
         mul(i);
       });
+      dma_k(t);
+      dma_v(t);
     };
     constexpr std::integral_constant<int, 0> kFirst{};
     constexpr std::integral_constant<int, kNk> kMid{};
@@ -655,9 +664,11 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
           }
         }
       }
-      float mx = fmaxf(c[0][0], c[1][0]);
+      // `maximum` needs no quieting of its operands beforehand, as fmaxf does: v_maximum3_f32.
+      float mx = __builtin_elementwise_maximum(c[0][0], c[1][0]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(c[0][i], c[1][i]));
+      for (int i = 1; i < 16; ++i)
+        mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, c[0][i]), c[1][i]);
       mx = pr_max32(mx) * a.scale_log2;  // sm_scale > 0
       // The reference moves only when it falls 2^8 behind: a probability is at most 2^8 then, in the range of every
       // type here, and most tiles leave the sums as they are.
@@ -688,31 +699,52 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       }
     };
     if (wave >= 4) turn();
+    Look seen_ahead[kI];
+    auto look_first = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) seen_ahead[i] = look(t + 4, i);
+    };
+    auto look_last = [&] {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) knext[i] = place(seen_ahead[i]);
+    };
+    auto look_ahead = [&](int t) {
+      look_first(t);
+      look_last();
+    };
+    auto exponentials = [&](int t) {
+      look_first(t);
+      softmax(k0 + t * kPrTile);
+      look_last();
+    };
     if (first < rows) {
-      __builtin_amdgcn_s_setprio(1);
-      body(0, kFirst, kMid);
-      __builtin_amdgcn_s_setprio(0);
+      // C(0) reads its scores' operands at once: with two batches (64-wide heads) no V is read ahead of it.
+      read(0, kFirst);
+      read(0, std::integral_constant<int, 1>{});
+      scores_only(0);
       gqa_wait_vmcnt<2 * kI>();
       turn();
-      advance(0);
-      softmax(k0);
-      turn();
+      exponentials(0);
       for (int t = 1; t < nt; ++t) {
+        start(t, kFirst);
+        turn();
         __builtin_amdgcn_s_setprio(1);
         body(t, kFirst, kAll);
         __builtin_amdgcn_s_setprio(0);
         gqa_wait_vmcnt<2 * kI>();
         turn();
-        advance(t);
-        softmax(k0 + t * kPrTile);
-        turn();
+        exponentials(t);
       }
+      turn();
+      start(nt, kMid);
       body(nt, kMid, kAll);
     } else {  // no rows: this wave only moves tiles
       for (int t = 0; t < nt; ++t) {
+        dma_k(t);
+        dma_v(t);
         gqa_wait_vmcnt<2 * kI>();
         turn();
-        advance(t);
+        look_ahead(t);
         turn();
       }
     }
