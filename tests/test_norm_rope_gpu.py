@@ -103,6 +103,32 @@ def test_paged(dsa, dev, T, H, G, D, R, interleaved):
         assert torch.equal(a, kc) and torch.equal(b, vc)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_tokens(dsa, dev, interleaved):
+    """Enough rows that a group takes several heads of a token; 29 rows a token, in sets that do not end with it."""
+    T, H, G, D, R, bs = 9101, 23, 3, 64, 48, 128
+    g = torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn(T, n, D, generator=g).bfloat16() for n in (H, G, G))
+    qw, kw = torch.randn(D, generator=g), torch.randn(D, generator=g)
+    cos, sin = _tables(T, R)
+    pos = torch.randperm(T, generator=g).to(torch.int32)
+    nb = T // bs + 2
+    slots = torch.randperm(nb * bs, generator=g)[:T].to(torch.int32)
+    kc, vc = torch.zeros(nb, bs, G, D, dtype=torch.bfloat16, device=dev), torch.zeros(nb, bs, G, D, dtype=torch.bfloat16,
+                                                                                     device=dev)
+    up = lambda t: t.to(dev)
+    qo = dsa.qk_norm_rope_paged(up(q), up(k), up(v), up(qw), up(kw), up(pos), up(cos), up(sin), kc, vc, up(slots),
+                                interleaved=interleaved)
+    _within(qo, *ref.norm_rope(q, qw, pos, cos, sin, interleaved=interleaved))
+    at = slots.long()
+    kv, vv = kc.cpu().view(-1, G, D), vc.cpu().view(-1, G, D)
+    _within(kv[at], *ref.norm_rope(k, kw, pos, cos, sin, interleaved=interleaved))
+    assert torch.equal(vv[at], v)
+    rest = torch.ones(nb * bs, dtype=torch.bool)
+    rest[at] = False
+    assert (kv[rest] == 0).all() and (vv[rest] == 0).all()
+
+
 def test_wide_slots_do_not_wrap(dsa, dev):
     """64-bit slots and positions past 32 bits mark padding, they do not come back as small ones."""
     q = torch.ones(2, 1, 16, dtype=torch.bfloat16, device=dev)
