@@ -143,15 +143,15 @@ __global__ __launch_bounds__(kQmmRowWaves * kWave) void qmm_rows_kernel(QmmArgs 
 }
 
 // More tokens: kBM x kBN of the output a workgroup, bound by the matrix cores.  The operands' rows stream into
-// LDS by DMA, 128 bytes of each at a time, two stages; a wave multiplies kTM tokens by 64 channels (32x32x32
+// LDS by DMA, 128 bytes of each at a time, two to four stages; a wave multiplies kTM tokens by 64 channels (32x32x32
 // products, channels on the M axis).  Chunk c (16 bytes) of row r lies at c ^ ((r >> 2) & 7), so that the 32 rows
 // a half wave reads at one c fall on distinct banks; the DMA fetches the chunks in that order.  Rows start on 16
 // bytes and hold whole chunks (qmm_pack_kernel sees to it where they do not); chunks past K come from a row of zeros.
 // 16384 x 9216 x 7168: 1089 us, 1988 TOP/s; the DMA alone takes 836 us there, the LDS reads 495, and the matrix cores
 // reach 3200 to 3700 on random operands (clock), a library's 8192^3 2089.
 // With kSplit the steps are dealt to gridDim.z workgroups, which leave int32 sums for qmm_join_kernel.
-constexpr int kQmmStep = 128;                    // whole lines of a row: with 64 (four stages) 16384 x 9216 x 7168
-constexpr int kQmmStages = 2;                    // took 1120 us, 1089 with 128
+// Whole lines of a row: with 64 bytes (and four stages) 16384 x 9216 x 7168 took 1120 us, 1089 with 128.
+constexpr int kQmmStep = 128;
 constexpr int kQmmLanes = kQmmStep / 16;         // of a row in a DMA instruction
 constexpr int kQmmRows = kWave / kQmmLanes;      // rows of a DMA instruction
 constexpr int kQmmParts = kQmmStep / 32;
@@ -176,6 +176,13 @@ __device__ __forceinline__ void qmm_lds_wait(u32x4 (&v)[N]) {
   for (int i = 0; i < N; ++i) __asm__ __volatile__("" : "+v"(v[i]));
 }
 
+// s_waitcnt with only vmcnt constrained.
+template <int N>
+__device__ __forceinline__ void qmm_wait_vmcnt() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
 template <int kBM, int kBN, int kWM, int kWN>
 struct QmmShape {
   static constexpr int kWaves = kWM * kWN, kTM = kBM / kWM, kTN = kBN / kWN;
@@ -185,7 +192,7 @@ struct QmmShape {
   static_assert((kBM + kBN) % (kQmmRows * kWaves) == 0 && kBN % 32 == 0, "whole DMA instructions");
 };
 
-template <int kOut, int kBM, int kBN, int kWM, int kWN, bool kSplit>
+template <int kOut, int kBM, int kBN, int kWM, int kWN, int kStages, bool kSplit>
 __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
   typedef QmmShape<kBM, kBN, kWM, kWN> S;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
     src[j] = (is_w ? a.w : a.x) + at * a.K + chunks[j] + (int64_t)s0 * kQmmStep;
   }
   auto dma = [&](int s) {
-    uint8_t* dst = lds + (s & 1) * S::kStage;
+    uint8_t* dst = lds + s % kStages * S::kStage;
     if ((s + 1) * kQmmStep <= a.K) {
 #pragma unroll
       for (int j = 0; j < S::kInstr; ++j) {
@@ -258,7 +265,7 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
   constexpr int kR = S::kFN + S::kFM;
   u32x4 v[2][kR];
   auto read = [&](u32x4(&o)[kR], int s, int q) {
-    const uint32_t st = (s & 1) * S::kStage, w = lw + st + off[q], x = lx + st + off[q];
+    const uint32_t st = s % kStages * S::kStage, w = lw + st + off[q], x = lx + st + off[q];
     qmm_b128<0>(o[0], w);
     qmm_b128<32 * kQmmStep>(o[1], w);
     qmm_b128<0>(o[2], x);
@@ -275,15 +282,20 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, o[i]),
                                                           __builtin_bit_cast(i32x4, o[S::kFN + j]), acc[i][j], 0, 0, 0);
   };
-  // This wave's part of the youngest stage is in LDS; behind the barrier everyone's is, and all reads of the stage
-  // before it are done.
-  auto turn = [&] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  // This wave's part of step s is in LDS (up to kStages - 2 younger steps may be in flight); behind the barrier
+  // everyone's is, and all reads of the step before it are done.
+  auto turn = [&](int s) {
+    const int younger = min(kStages - 2, s1 - 1 - s);
+    if (kStages > 3 && younger == 2) qmm_wait_vmcnt<2 * S::kInstr>();
+    else if (kStages > 2 && younger == 1) qmm_wait_vmcnt<S::kInstr>();
+    else qmm_wait_vmcnt<0>();
     __builtin_amdgcn_s_barrier();
   };
-  dma(s0);
-  turn();
-  if (s0 + 1 < s1) dma(s0 + 1);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i)
+    if (s0 + i < s1) dma(s0 + i);
+  turn(s0);
+  if (s0 + kStages - 1 < s1) dma(s0 + kStages - 1);
   read(v[0], s0, 0);
   auto parts = [&](int s) {  // all products of the stage but the last part's, whose operands are left in v[1]
 #pragma unroll
@@ -296,8 +308,8 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
   };
   for (int s = s0; s + 1 < s1; ++s) {
     parts(s);
-    turn();
-    if (s + 2 < s1) dma(s + 2);
+    turn(s + 1);
+    if (s + kStages < s1) dma(s + kStages);
     read(v[0], s + 1, 0);
     mul(v[1]);
   }
@@ -378,6 +390,7 @@ struct QmmPlan {
   int tile;    // 16: the kernel for few tokens; 32, 64, 128: tokens of a tile of 128 channels; 256: of 256 channels
   bool pack;   // operands copied to aligned rows first
   int splits;  // workgroups that share a tile's K
+  bool deep;   // tiles of 128 with four stages, one workgroup a CU
   size_t pack_bytes, part_bytes;
 };
 
@@ -385,9 +398,9 @@ static int64_t qmm_ld(int64_t K) { return (K + 127) / 128 * 128; }
 
 // `odd`: rows do not start on 16 bytes or hold no whole number of chunks.
 static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
-  QmmPlan p = {16, false, 1, 0, 0};
+  QmmPlan p = {16, false, 1, false, 0, 0};
   // Up to 16 tokens every workgroup reads all of x beside its 16 rows of w: one token of 9216 x 7168 takes 15.6 us
-  // (19.7 with split tiles), 16 tokens 21.6 (20.5); 32 tokens 33 against 21.4, 64 (7168 x 8192) 28.8 against 20.7.
+  // (19.7 with split tiles), 16 tokens 21.6 (20.5); 32 tokens 33 against 20.7, 64 (7168 x 8192) 28.8 against 18.0.
   if (M <= 16) return p;
   p.pack = odd;
   if (odd) p.pack_bytes = (size_t)((M + N) * qmm_ld(K));
@@ -402,9 +415,13 @@ static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
     p.tile = 256;
     return p;
   }
-  // Few tiles share their K, up to two workgroups a CU and eight steps each.
-  const int64_t steps = (K + kQmmStep - 1) / kQmmStep;
-  while (p.splits < 8 && small * p.splits * 2 <= 512 && steps >= 8 * p.splits) p.splits *= 2;
+  // Few tiles share their K, eight steps each at least, up to about one workgroup a CU: with up to two, what the
+  // join reads costs more (64 tokens of 7168 x 8192: 22.0 us instead of 18.0; 512: 57.2 instead of 51).  Tiles of 128
+  // may pass 256 a little (1021 x 2113 x 4099: 42.5 us with 136 workgroups, 38.1 with 272).
+  const int64_t steps = (K + kQmmStep - 1) / kQmmStep, most = p.tile == 128 ? 320 : 256;
+  while (p.splits < 8 && small * p.splits * 2 <= most && steps >= 8 * p.splits) p.splits *= 2;
+  // A workgroup alone on its CU keeps three steps in flight (512 tokens: 65.0 -> 52 us).
+  p.deep = p.tile == 128 && small * p.splits <= 256;
   if (p.splits > 1) p.part_bytes = (size_t)(p.splits * M * ((N + 3) / 4 * 4) * 4);
   return p;
 }
@@ -419,21 +436,22 @@ size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, bool aligne
   return p.pack_bytes + p.part_bytes;
 }
 
-template <int kOut, int kBM, int kBN, int kWM, int kWN, bool kSplit>
+template <int kOut, int kBM, int kBN, int kWM, int kWN, int kStages, bool kSplit>
 static hipError_t qmm_launch_tile(const QmmArgs& a, int splits, hipStream_t stream) {
-  constexpr int lds = kQmmStages * QmmShape<kBM, kBN, kWM, kWN>::kStage;
-  static_assert(lds <= 160 * 1024, "LDS");
-  const hipError_t e = set_dynamic_lds_once<qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kSplit>>(lds);
+  constexpr int lds = kStages * QmmShape<kBM, kBN, kWM, kWN>::kStage;
+  static_assert(kStages >= 2 && kStages <= 4 && lds <= 160 * 1024, "LDS");
+  const hipError_t e = set_dynamic_lds_once<qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kStages, kSplit>>(lds);
   if (e != hipSuccess) return e;
   const dim3 grid((unsigned)(((a.M + kBM - 1) / kBM) * ((a.N + kBN - 1) / kBN)), 1, splits);
-  hipLaunchKernelGGL((qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kSplit>), grid, dim3(kWM * kWN * kWave), lds, stream, a);
+  hipLaunchKernelGGL((qmm_tile_kernel<kOut, kBM, kBN, kWM, kWN, kStages, kSplit>), grid, dim3(kWM * kWN * kWave), lds,
+                     stream, a);
   return hipGetLastError();
 }
 
-template <int kOut, int kBM, int kWM, int kWN>
+template <int kOut, int kBM, int kWM, int kWN, int kStages>
 static hipError_t qmm_launch_shared(const QmmArgs& a, int splits, hipStream_t stream) {
-  if (splits == 1) return qmm_launch_tile<kOut, kBM, 128, kWM, kWN, false>(a, 1, stream);
-  const hipError_t e = qmm_launch_tile<kOut, kBM, 128, kWM, kWN, true>(a, splits, stream);
+  if (splits == 1) return qmm_launch_tile<kOut, kBM, 128, kWM, kWN, kStages, false>(a, 1, stream);
+  const hipError_t e = qmm_launch_tile<kOut, kBM, 128, kWM, kWN, kStages, true>(a, splits, stream);
   if (e != hipSuccess) return e;
   const int64_t quads = (int64_t)a.M * (a.part_ld / 4);
   hipLaunchKernelGGL((qmm_join_kernel<kOut>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
@@ -461,10 +479,12 @@ static hipError_t qmm_launch(QmmArgs a, void* workspace, hipStream_t stream) {
     a.K = ld;
   }
   switch (p.tile) {
-    case 32: return qmm_launch_shared<kOut, 32, 1, 2>(a, p.splits, stream);
-    case 64: return qmm_launch_shared<kOut, 64, 2, 2>(a, p.splits, stream);
-    case 128: return qmm_launch_shared<kOut, 128, 2, 2>(a, p.splits, stream);
-    default: return qmm_launch_tile<kOut, 256, 256, 2, 4, false>(a, 1, stream);
+    case 32: return qmm_launch_shared<kOut, 32, 1, 2, 3>(a, p.splits, stream);
+    case 64: return qmm_launch_shared<kOut, 64, 2, 2, 3>(a, p.splits, stream);
+    case 128:
+      if (p.deep) return qmm_launch_shared<kOut, 128, 2, 2, 4>(a, p.splits, stream);
+      return qmm_launch_shared<kOut, 128, 2, 2, 2>(a, p.splits, stream);
+    default: return qmm_launch_tile<kOut, 256, 256, 2, 4, 2, false>(a, 1, stream);
   }
 }
 
