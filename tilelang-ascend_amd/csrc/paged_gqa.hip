@@ -552,6 +552,17 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       }
     };
 
+    // Where K of tile t + 4 lies: asked at the start of C(t), taken at its end.
+    Look asked[kI];
+    auto ask = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) asked[i] = look(t + 4, i);
+    };
+    auto take = [&] {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) knext[i] = place(asked[i]);
+    };
+
     const uint32_t lds0 = gqa_lds_u32(lds);
     // K operand (A), step st, key block kb: key 32 kb + r, dims 16 st + 8 hi .. + 7.
     const uint32_t k_at = lds0 + r * kRow + 16 * (hi ^ pr_swz<kD>(r));
@@ -614,6 +625,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     };
     auto body = [&](int t, auto from, auto to) {
       constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
+      if constexpr (kFrom == 0) ask(t);
       pr_each<kFrom, kTo>([&](auto i) {
         // Twelve reads are out: the counter of them holds fifteen.
         constexpr int n = decltype(i)::value, left = kTo - 1 - n < 2 ? kTo - 1 - n : 2;
@@ -624,8 +636,10 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         if constexpr (n == 0) dma_k(t);
         if constexpr (n == 1) dma_v(t);
       });
+      if constexpr (kFrom == 0) take();
     };
     auto scores_only = [&](int t) {  // batches 0 and 1 are on their way
+      ask(t);
       pr_each<0, kNk>([&](auto i) {
         constexpr int n = decltype(i)::value;
         pr_lds_wait<n + 1 < kNk ? 4 : 0>(kop[n]);
@@ -634,6 +648,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       });
       dma_k(t);
       dma_v(t);
+      take();
     };
     constexpr std::integral_constant<int, 0> kFirst{};
     constexpr std::integral_constant<int, kNk> kMid{};
@@ -699,24 +714,6 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       }
     };
     if (wave >= 4) turn();
-    Look seen_ahead[kI];
-    auto look_first = [&](int t) {
-#pragma unroll
-      for (int i = 0; i < kI; ++i) seen_ahead[i] = look(t + 4, i);
-    };
-    auto look_last = [&] {
-#pragma unroll
-      for (int i = 0; i < kI; ++i) knext[i] = place(seen_ahead[i]);
-    };
-    auto look_ahead = [&](int t) {
-      look_first(t);
-      look_last();
-    };
-    auto exponentials = [&](int t) {
-      look_first(t);
-      softmax(k0 + t * kPrTile);
-      look_last();
-    };
     if (first < rows) {
       // C(0) reads its scores' operands at once: with two batches (64-wide heads) no V is read ahead of it.
       read(0, kFirst);
@@ -724,27 +721,34 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       scores_only(0);
       gqa_wait_vmcnt<2 * kI>();
       turn();
-      exponentials(0);
+      // The first reads of C(t + 1) go out ahead of the exponentials of tile t, while the SIMD's other wave is in C.
+      start(1, kFirst);
+      softmax(k0);
       for (int t = 1; t < nt; ++t) {
-        start(t, kFirst);
         turn();
         __builtin_amdgcn_s_setprio(1);
         body(t, kFirst, kAll);
         __builtin_amdgcn_s_setprio(0);
         gqa_wait_vmcnt<2 * kI>();
         turn();
-        exponentials(t);
+        start(t + 1, kFirst);
+        softmax(k0 + t * kPrTile);
       }
+      pr_lds_wait<0>(kop[0]);  // of a tile behind the last
+      pr_lds_wait<0>(kop[1]);
+      if constexpr (kNk > 2) pr_lds_wait<0>(kop[2]);
+      else pr_lds_wait<0>(vop[0]);
       turn();
       start(nt, kMid);
       body(nt, kMid, kAll);
     } else {  // no rows: this wave only moves tiles
       for (int t = 0; t < nt; ++t) {
+        ask(t);
         dma_k(t);
         dma_v(t);
+        take();
         gqa_wait_vmcnt<2 * kI>();
         turn();
-        look_ahead(t);
         turn();
       }
     }
