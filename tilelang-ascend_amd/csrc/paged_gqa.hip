@@ -618,27 +618,46 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         o[p + 1] = pr_mfma<kF16>(u32x4{v[2].x, v[2].y, v[3].x, v[3].y}, pb[u], o[p + 1]);
       }
     };
-    // Batches kFrom .. kTo - 1: scores of tile t, products of tile t - 1; the first three are read ahead by `start`.
-    auto start = [&](int t, auto from) {
-      constexpr int kFrom = decltype(from)::value;
-      pr_each<kFrom, kFrom + 3>([&](auto i) { read(t, i); });
+    // C(t) takes a batch of scores and two of products in turn, so that the transposing reads, the slowest, are spread
+    // over all its products: n-th batch.
+    const auto nth = [](int n) constexpr { return n % 3 == 0 ? n / 3 : kNk + n - n / 3 - 1; };
+    static_assert(kNv == 2 * kNk, "a batch of scores and two of products in turn");
+    auto wait_for = [&](auto left, auto batch) {
+      constexpr int i = decltype(batch)::value;
+      if constexpr (i < kNk) pr_lds_wait<decltype(left)::value>(kop[i]);
+      else pr_lds_wait<decltype(left)::value>(vop[i - kNk]);
     };
-    auto body = [&](int t, auto from, auto to) {
-      constexpr int kFrom = decltype(from)::value, kTo = decltype(to)::value;
-      if constexpr (kFrom == 0) ask(t);
-      pr_each<kFrom, kTo>([&](auto i) {
+    auto start = [&](int t) {  // the first three batches of C(t)
+      read(t, std::integral_constant<int, nth(0)>{});
+      read(t, std::integral_constant<int, nth(1)>{});
+      read(t, std::integral_constant<int, nth(2)>{});
+    };
+    auto body = [&](int t) {
+      ask(t);
+      constexpr int kAll = kNk + kNv;
+      pr_each<0, kAll>([&](auto i) {
         // Twelve reads are out: the counter of them holds fifteen.
-        constexpr int n = decltype(i)::value, left = kTo - 1 - n < 2 ? kTo - 1 - n : 2;
-        if constexpr (n < kNk) pr_lds_wait<4 * left>(kop[n]);
-        else pr_lds_wait<4 * left>(vop[n - kNk]);
-        if constexpr (n + 3 < kTo) read(t, std::integral_constant<int, n + 3>{});
-        mul(i);
+        constexpr int n = decltype(i)::value, left = kAll - 1 - n < 2 ? kAll - 1 - n : 2;
+        wait_for(std::integral_constant<int, 4 * left>{}, std::integral_constant<int, nth(n)>{});
+        if constexpr (n + 3 < kAll) read(t, std::integral_constant<int, nth(n + 3)>{});
+        mul(std::integral_constant<int, nth(n)>{});
         if constexpr (n == 0) dma_k(t);
         if constexpr (n == 1) dma_v(t);
       });
-      if constexpr (kFrom == 0) take();
+      take();
     };
-    auto scores_only = [&](int t) {  // batches 0 and 1 are on their way
+    auto products_only = [&](int t) {  // of tile t - 1
+      pr_each<kNk, kNk + 3>([&](auto i) { read(t, i); });
+      pr_each<kNk, kNk + kNv>([&](auto i) {
+        constexpr int n = decltype(i)::value, left = kNk + kNv - 1 - n < 2 ? kNk + kNv - 1 - n : 2;
+        wait_for(std::integral_constant<int, 4 * left>{}, i);
+        if constexpr (n + 3 < kNk + kNv) read(t, std::integral_constant<int, n + 3>{});
+        mul(i);
+      });
+    };
+    auto scores_only = [&](int t) {
+      read(t, std::integral_constant<int, 0>{});
+      read(t, std::integral_constant<int, 1>{});
       ask(t);
       pr_each<0, kNk>([&](auto i) {
         constexpr int n = decltype(i)::value;
@@ -650,9 +669,6 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       dma_v(t);
       take();
     };
-    constexpr std::integral_constant<int, 0> kFirst{};
-    constexpr std::integral_constant<int, kNk> kMid{};
-    constexpr std::integral_constant<int, kNk + kNv> kAll{};
     const auto turn = [] { __builtin_amdgcn_s_barrier(); };
     gqa_wait_vmcnt<4 * kI>();
     // The waves' findings pass through LDS by hand: a fence or a plain access would wait for the DMA.
@@ -715,32 +731,27 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
     };
     if (wave >= 4) turn();
     if (first < rows) {
-      // C(0) reads its scores' operands at once: with two batches (64-wide heads) no V is read ahead of it.
-      read(0, kFirst);
-      read(0, std::integral_constant<int, 1>{});
       scores_only(0);
       gqa_wait_vmcnt<2 * kI>();
       turn();
       // The first reads of C(t + 1) go out ahead of the exponentials of tile t, while the SIMD's other wave is in C.
-      start(1, kFirst);
+      start(1);
       softmax(k0);
       for (int t = 1; t < nt; ++t) {
         turn();
         __builtin_amdgcn_s_setprio(1);
-        body(t, kFirst, kAll);
+        body(t);
         __builtin_amdgcn_s_setprio(0);
         gqa_wait_vmcnt<2 * kI>();
         turn();
-        start(t + 1, kFirst);
+        start(t + 1);
         softmax(k0 + t * kPrTile);
       }
-      pr_lds_wait<0>(kop[0]);  // of a tile behind the last
-      pr_lds_wait<0>(kop[1]);
-      if constexpr (kNk > 2) pr_lds_wait<0>(kop[2]);
-      else pr_lds_wait<0>(vop[0]);
+      wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(0)>{});  // of a tile behind the last
+      wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(1)>{});
+      wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(2)>{});
       turn();
-      start(nt, kMid);
-      body(nt, kMid, kAll);
+      products_only(nt);
     } else {  // no rows: this wave only moves tiles
       for (int t = 0; t < nt; ++t) {
         ask(t);
