@@ -128,6 +128,50 @@ def test_what_lies_behind_the_last_key(dsa, dev, seqs, what):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("seqs,win", [([(50, 300)], None), ([(1, 300), (3, 77)], 64), ([(200, 200), (90, 333)], 100),
+                                      ([(1, 20), (1, 500)], 10)])
+@pytest.mark.parametrize("D,dtype", [(64, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_values_that_a_row_does_not_see(dsa, dev, seqs, win, D, dtype, what):
+    """Infinities and NaN among a sequence's own keys reach the rows that see them, in their columns, and no others."""
+    H, G, bs = 8, 2, 16
+    q, kc, vc, table = _setup(seqs, H, G, D, bs, dtype, seed=12)
+    clean, _ = _run(dsa, dev, seqs, q, kc, vc, table, win=win)
+    kc2, vc2 = kc.clone(), vc.clone()
+    bad_v, bad_k = [], []
+    rows = []
+    for b, (s, n) in enumerate(seqs):
+        # A key before any row's window (if there is one), the first token's own, one in the middle, the last.
+        for j, c in {(max(n - s - 12, 0), 3), (n - s, 17), (n - s // 2 - 1, 40), (n - 1, D - 1)}:
+            vc2[table[b, j // bs], j % bs, j % G, c] = what
+            bad_v.append((b, j, j % G, c))
+        rows += [(b, n - s + i) for i in range(s)]
+    got, _ = _run(dsa, dev, seqs, q, kc, vc2, table, win=win)
+    sees = lambda row, b, j: row[0] == b and j <= row[1] and (win is None or j >= row[1] - win)
+    want = clean.cpu().clone()
+    hit = torch.zeros(want.shape, dtype=torch.bool)
+    for b, j, g, c in bad_v:
+        for t, row in enumerate(rows):
+            if sees(row, b, j):
+                hit[t, g * (H // G):(g + 1) * (H // G), c] = True
+    got = got.cpu()
+    assert torch.equal(got[~hit], want[~hit])
+    assert not torch.isfinite(got[hit]).any()
+    if math.isnan(what):  # a key: the whole row of a head that sees it
+        for b, (s, n) in enumerate(seqs):
+            j = n - s // 2 - 1
+            kc2[table[b, j // bs], j % bs, 1, 5] = what
+            bad_k.append((b, j))
+        got, lse = (x.cpu() for x in _run(dsa, dev, seqs, q, kc2, vc, table, win=win))
+        hit = torch.zeros(want.shape[:2], dtype=torch.bool)
+        for b, j in bad_k:
+            for t, row in enumerate(rows):
+                if sees(row, b, j):
+                    hit[t, H // G:] = True
+        assert torch.equal(got[~hit], want[~hit]) and torch.isfinite(lse[~hit]).all()
+        assert torch.isnan(got[hit]).all()
+
+
 def test_pages_outside_the_pool_hide_their_keys(dsa, dev):
     seqs = [(1, 300), (20, 200), (1, 64)]
     q, kc, vc, table = _setup(seqs, 8, 2, 64, 32, torch.bfloat16, seed=7)

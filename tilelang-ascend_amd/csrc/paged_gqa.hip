@@ -107,6 +107,30 @@ __device__ __forceinline__ int pg_block(const PgArgs& a, int j) {
   return a.div_mul ? (int)(__umulhi((uint32_t)j, a.div_mul) >> a.div_shift) : j;
 }
 
+// Values that a row does not see must not reach it, whatever they hold, but 0 times an infinity or a NaN is a NaN in
+// the product of probabilities and V.  So tiles that some row sees in part are searched for such values (unseen
+// ones of other tiles do not exist); where there are any, the product takes zeros in their place, and rows that do
+// see them get them added by hand.
+// Of a pair of 16-bit values: bit 15 (and 31) set where the value is infinite or NaN: the exponent's ones plus one.
+template <bool kF16>
+__device__ __forceinline__ uint32_t pg_not_finite(uint32_t w) {
+  constexpr uint32_t kOnes = kF16 ? 0x7c007c00u : 0x7f807f80u, kOne = kF16 ? 0x04000400u : 0x00800080u;
+  return ((w & kOnes) + kOne) & 0x80008000u;
+}
+template <bool kF16>
+__device__ __forceinline__ void pg_clean(u32x2& v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] &= ~((pg_not_finite<kF16>(v[i]) >> 15) * 0xffffu);
+}
+// x where it is not finite, else 0.
+template <bool kF16>
+__device__ __forceinline__ float pg_only_bad(uint32_t w, int hi) {
+  const uint16_t u = (uint16_t)(hi ? w >> 16 : w);
+  if (!(pg_not_finite<kF16>(u) & 0x8000u)) return 0.f;
+  if constexpr (kF16) return (float)__builtin_bit_cast(_Float16, u);
+  else return __uint_as_float((uint32_t)u << 16);
+}
+
 // Keys behind a sequence's last one, and of pages outside the pool, load this row: 0 times what lies there need
 // not be 0.
 static __device__ __align__(128) uint8_t kPgZeroRow[256];
@@ -251,7 +275,8 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
         for (int st = 0; st < kSt; ++st) acc = gqa_mfma<kF16>(kop[k * kSt + st], qb[hb][st], acc);
         c[hb][k] = acc;
       }
-    if (ok_cur != 0xffffffffu || j0 + kPgTile - 1 > all_lim || j0 < all_low) {
+    const bool partly = ok_cur != 0xffffffffu || j0 + kPgTile - 1 > all_lim || j0 < all_low;
+    if (partly) {
 #pragma unroll
       for (int hb = 0; hb < kHB; ++hb)
 #pragma unroll
@@ -288,6 +313,34 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
       for (int i = 0; i < kNb; ++i) o[hb][i] *= alpha;
       pb[hb] = u32x4{gqa_pack<kF16>(pv[0], pv[1]), gqa_pack<kF16>(pv[2], pv[3]), gqa_pack<kF16>(pv[4], pv[5]),
                      gqa_pack<kF16>(pv[6], pv[7])};
+    }
+    if (partly) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < kNb; ++i)
+        bad |= pg_not_finite<kF16>(vop[i][0].x) | pg_not_finite<kF16>(vop[i][0].y) | pg_not_finite<kF16>(vop[i][1].x) |
+               pg_not_finite<kF16>(vop[i][1].y);
+      if (__any(bad != 0)) {
+#pragma unroll
+        for (int i = 0; i < kNb; ++i) {
+          pg_clean<kF16>(vop[i][0]);
+          pg_clean<kF16>(vop[i][1]);
+        }
+        const uint8_t* vt = ring + (e & 1) * 2 * kTileBytes + kTileBytes;
+        for (int j = 0; j < kPgTile; ++j) {
+          if (!((ok_cur >> j) & 1u)) continue;
+#pragma unroll
+          for (int p = 0; p < kSt; ++p) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(vt + j * kRow + 16 * ((4 * p + g) ^ pg_swz<kD>(j)));
+#pragma unroll
+            for (int hb = 0; hb < kHB; ++hb) {
+              const bool see = j0 + j <= lim[hb] && j0 + j >= low[hb];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[hb][2 * p + (i >> 2)][i & 3] += see ? pg_only_bad<kF16>(w[i / 2], i & 1) : 0.f;
+            }
+          }
+        }
+      }
     }
     // O^T += V^T P^T: lane (g, r) of block 2p + h accumulates row r, columns 32 p + 8 g + 4 h .. + 3.
 #pragma unroll
@@ -463,6 +516,10 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
   }
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
   low_max = __builtin_amdgcn_readfirstlane(low_max);
+  // Tiles of keys in [part_lo, part_hi] are seen whole by every token of the workgroup's rows.
+  const int tok0 = tile * kPrRows / a.Hg, tok1 = min(((tile + 1) * kPrRows - 1) / a.Hg, s.len - 1);
+  const int part_hi = a.causal ? min(s.n - s.len + tok0, s.n - 1) : s.n - 1;
+  const int part_lo = a.win >= 0 ? max(s.n - s.len + tok1, 0) - a.win : 0;
 
   f32x16 o[kNb];
 #pragma unroll
@@ -670,16 +727,18 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       take();
     };
     const auto turn = [] { __builtin_amdgcn_s_barrier(); };
-    gqa_wait_vmcnt<4 * kI>();
+    gqa_wait_vmcnt<3 * kI>();
     // The waves' findings pass through LDS by hand: a fence or a plain access would wait for the DMA.
     const uint32_t flags = gqa_lds_u32(lds + 8 * kTileBytes);
     const bool found = __any(outside | ((uint32_t)my_page >= (uint32_t)a.num_blocks));
-    __asm__ __volatile__("ds_write_b8 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(flags + wave), "v"((int)found) : "memory");
+    __asm__ __volatile__("ds_write_b8 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(flags + 16 + wave), "v"((int)found)
+                         : "memory");
     turn();
     u32x2 seen;
-    __asm__ __volatile__("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(seen) : "v"(flags) : "memory");
+    __asm__ __volatile__("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(seen) : "v"(flags + 16) : "memory");
     const bool holes = __builtin_amdgcn_readfirstlane((int)(seen.x | seen.y)) != 0;
-    auto softmax = [&](int j0) {
+    auto softmax = [&](int t) {
+      const int j0 = k0 + t * kPrTile;
       if (holes || j0 + kPrTile - 1 > lim_min || j0 < low_max) {
         uint64_t there = ~(uint64_t)0;  // keys in pages of the pool
         if (holes) there = __ballot((uint32_t)bt[pg_block(a, min(j0 + lane, k1 - 1))] < (uint32_t)a.num_blocks);
@@ -729,45 +788,131 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
                       gqa_pack<kF16>(e[x + 4], e[x + 5]), gqa_pack<kF16>(e[x + 6], e[x + 7])};
       }
     };
-    if (wave >= 4) turn();
-    if (first < rows) {
-      scores_only(0);
-      gqa_wait_vmcnt<2 * kI>();
-      turn();
-      // The first reads of C(t + 1) go out ahead of the exponentials of tile t, while the SIMD's other wave is in C.
-      start(1);
-      softmax(k0);
-      for (int t = 1; t < nt; ++t) {
+    const bool late = wave >= 4;
+    // V of tile t, searched for values that are not finite where some row sees the tile in part: two barriers ahead of
+    // its first use, an eighth by each wave, which notes what it found; one barrier later they are replaced by zeros
+    // in LDS, by every wave (one that reads ahead in the same turn reads its own zeros).  What the rows do see of
+    // them is added behind the loop.  Tiles [part_end, part_begin) are seen whole by all rows.
+    const int part_end = part_lo > k0 ? min((part_lo - k0 + kPrTile - 1) / kPrTile, nt) : 0;
+    const int part_begin = part_hi + 1 > k0 ? min((part_hi + 1 - k0) / kPrTile, nt) : 0;
+    const auto in_part = [&](int t) { return t < nt && (t < part_end || t >= part_begin); };
+    bool any_bad = false;
+    auto search = [&](int t) {
+      if (!in_part(t)) return;
+      const uint32_t at = lds0 + (4 + (t & 3)) * kTileBytes + wave * (kTileBytes / kPrWaves) + 16 * lane;
+      u32x4 w[kTileBytes / kPrWaves / 1024];
+      __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");
+      gqa_b128<0>(w[0], at);
+      if constexpr (kTileBytes / kPrWaves == 2048) gqa_b128<1024>(w[1], at);
+      gqa_lgkm_wait(w);
+      uint32_t bad = 0;
+#pragma unroll
+      for (int n = 0; n < kTileBytes / kPrWaves / 1024; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= pg_not_finite<kF16>(w[n][i]);
+      const int note = __any(bad != 0);
+      __asm__ __volatile__("ds_write_b8 %0, %1\n\ts_waitcnt lgkmcnt(0)" ::"v"(flags + 8 * (t & 1) + wave), "v"(note)
+                           : "memory");
+    };
+    auto scrub = [&](int t) {
+      if (!in_part(t)) return;
+      u32x2 notes;
+      __asm__ __volatile__("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(notes) : "v"(flags + 8 * (t & 1)) : "memory");
+      if (__builtin_amdgcn_readfirstlane((int)(notes.x | notes.y)) == 0) return;
+      any_bad = true;
+      uint8_t* vt = lds + (4 + (t & 3)) * kTileBytes + 8 * lane;
+#pragma unroll 1
+      for (int n = 0; n < kTileBytes; n += 512) {
+        u32x2 w = *reinterpret_cast<u32x2*>(vt + n);
+        pg_clean<kF16>(w);
+        *reinterpret_cast<u32x2*>(vt + n) = w;
+      }
+      __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    // Bodies t0 .. t1 - 1 behind C(0) and X(0); without `checked` no tile t0 .. t1 is seen in part.
+    auto bodies = [&](int t0, int t1, auto checked) {
+      constexpr bool kChecked = decltype(checked)::value;
+      for (int t = t0; t < t1; ++t) {
         turn();
+        if (kChecked && late) scrub(t);
         __builtin_amdgcn_s_setprio(1);
         body(t);
         __builtin_amdgcn_s_setprio(0);
         gqa_wait_vmcnt<2 * kI>();
+        if (kChecked && !late) search(t);
         turn();
+        if (kChecked && !late) scrub(t);
+        // The first reads of C(t + 1) go out ahead of the exponentials, while the SIMD's other wave is in C.
         start(t + 1);
-        softmax(k0 + t * kPrTile);
+        softmax(t);
+        if (kChecked && late) search(t + 1);
       }
+    };
+    if (first < rows) {
+      if (late) {
+        search(0);
+        turn();
+        scrub(0);
+      }
+      scores_only(0);
+      gqa_wait_vmcnt<2 * kI>();
+      if (!late) search(0);
+      turn();
+      if (!late) scrub(0);
+      start(1);
+      softmax(0);
+      if (late) search(1);
+      const int whole0 = max(part_end, 1), whole1 = max(part_begin - 1, whole0);
+      bodies(1, min(whole0, nt), std::true_type{});
+      bodies(whole0, min(whole1, nt), std::false_type{});
+      bodies(max(whole1, 1), nt, std::true_type{});
       wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(0)>{});  // of a tile behind the last
       wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(1)>{});
       wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(2)>{});
       turn();
       products_only(nt);
-    } else {  // no rows: this wave only moves tiles
+      if (any_bad) {
+        for (int t = 0; t < nt; ++t) {
+          if (!in_part(t)) continue;
+          for (int j = k0 + t * kPrTile; j < min(k0 + (t + 1) * kPrTile, k1); ++j) {
+            const int blk = pg_block(a, j), page = bt[blk];
+            if ((uint32_t)page >= (uint32_t)a.num_blocks) continue;
+            const uint8_t* vr = vb + (page * a.block_size + j - blk * a.block_size) * row_bytes + kvg * kRow;
+            const bool see = j <= lim && j >= low;
+#pragma unroll
+            for (int p = 0; p < kNb; ++p)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(vr + 16 * (4 * p + 2 * x + hi));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[p][8 * x + i] += see ? pg_only_bad<kF16>(w[i / 2], i & 1) : 0.f;
+              }
+          }
+        }
+      }
+    } else {  // no rows: this wave only moves tiles and searches its part of them
+      if (late) {
+        search(0);
+        turn();
+      }
       for (int t = 0; t < nt; ++t) {
         ask(t);
         dma_k(t);
         dma_v(t);
         take();
         gqa_wait_vmcnt<2 * kI>();
+        if (!late) search(t);
         turn();
+        if (late) search(t + 1);
         turn();
       }
     }
-    if (wave < 4) turn();
+    if (!late) turn();
     __builtin_amdgcn_s_waitcnt(0);  // the DMA of tiles behind the last
   }
 
   l_run = pr_sum32(l_run);
+  const bool none = l_run == 0.f;  // a row that saw nothing: its sums may be 0 times anything
   constexpr float kLn2 = 0.6931471805599453f;
   if (!whole) {
     float* p = part + (32 * wave + r) * kD + 8 * hi;
@@ -776,7 +921,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         *reinterpret_cast<f32x4*>(p + 32 * n + 16 * (x >> 1) + 4 * (x & 1)) =
-            f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]};
+            none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{o[n][4 * x], o[n][4 * x + 1], o[n][4 * x + 2], o[n][4 * x + 3]};
     if (hi == 0) {
       part[kPrRows * kD + 2 * (32 * wave + r)] = m_run;
       part[kPrRows * kD + 2 * (32 * wave + r) + 1] = l_run;
@@ -798,7 +943,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       for (int x = 0; x < 2; ++x) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = o[n][8 * x + i] * inv;
+        for (int i = 0; i < 8; ++i) v[i] = none ? 0.f : o[n][8 * x + i] * inv;
         *reinterpret_cast<u32x4*>(dst + 32 * n + 16 * x) = u32x4{gqa_pack<kF16>(v[0], v[1]), gqa_pack<kF16>(v[2], v[3]),
                                                                 gqa_pack<kF16>(v[4], v[5]), gqa_pack<kF16>(v[6], v[7])};
       }
@@ -822,7 +967,7 @@ template <bool kF16_, int kD_, bool kEven>
 struct PgRows {
   static constexpr bool kF16 = kF16_;
   static constexpr int kD = kD_, kR = kPrRows, kUnitKeys = kPrTile, kThreads = kPrThreads;
-  static constexpr int kLds = 8 * kPrTile * kD * 2 + 16;  // two rings of four stages, the waves' flags
+  static constexpr int kLds = 8 * kPrTile * kD * 2 + 32;  // two rings of four stages, the waves' notes
   static __device__ __forceinline__ void item(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                               bool whole, float* part, uint8_t* lds) {
     pg_rows<kF16, kD, kEven>(a, s, b, tile, kvg, k0, k1, whole, part, lds);
