@@ -207,3 +207,5 @@ def test_refusals(dsa, dev):
         paged(v=q[:, :1])
     with pytest.raises(ValueError, match="required"):
         paged(v=None)
+    with pytest.raises(ValueError, match="caches of their own"):
+        paged(vc=kc)

@@ -104,6 +104,36 @@ def test_many_rows(dsa, dev, H, G):
     _check(_run(dsa, dev, seqs, *args), _want(seqs, *args))
 
 
+@pytest.mark.parametrize("bs", [64, 20])
+def test_a_tile_for_each_workgroup(dsa, dev, bs):
+    """More tiles of rows than two rounds of workgroups, few sequences: no line to share."""
+    seqs = [(1500, 1700), (1201, 1201)]
+    args = _setup(seqs, 64, 1, 64, bs, torch.bfloat16, seed=bs)
+    _check(_run(dsa, dev, seqs, *args, win=700), _want(seqs, *args, win=700))
+
+
+def test_thousands_of_sequences(dsa, dev):
+    """More slots than the line holds: decode tiles a workgroup each.  All sequences are alike but in their pages."""
+    B, n, H, D, bs = 4300, 21, 4, 64, 16
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(B, 1, H, D, generator=g).bfloat16()
+    kc, vc = torch.randn(2 * B, bs, 1, D, generator=g).bfloat16(), torch.randn(2 * B, bs, 1, D, generator=g).bfloat16()
+    table = torch.randperm(2 * B, generator=g).to(torch.int32).view(B, 2)
+    kl = torch.full((B,), n, dtype=torch.int32)
+    out, lse = dsa.paged_gqa_fwd(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), actual_seq_lengths_kv=kl.to(dev))
+    k, v = (c[table.long()].view(B, 2 * bs, D)[:, :n].double() for c in (kc, vc))
+    s = torch.matmul(q.view(B, H, D).double(), k.transpose(1, 2)) * D ** -0.5
+    w = torch.softmax(s, -1)
+    u = ref.half_step(torch.bfloat16)
+    # As in ref.attention: the weights' and the output's rounding, scores within (D + 4) half steps of their terms' sum.
+    ds = (D + 4) * ref.F32 * torch.matmul(q.view(B, H, D).double().abs(), k.transpose(1, 2).abs()).max() * D ** -0.5
+    want = torch.matmul(w, v)
+    tol = (u + 2 * ds + (n + 64) * ref.F32 + 4e-7) * torch.matmul(w, v.abs()) + u * want.abs()
+    ref.assert_within(out.view(B, H, D), want, tol, "out")
+    l = torch.logsumexp(s, -1)
+    ref.assert_within(lse.view(B, H), l, ds + (n + 64) * ref.F32 + 1e-6 + 4 * ref.F32 * l.abs(), "lse")
+
+
 @pytest.mark.parametrize("scale", [8.0, 40.0])
 def test_large_scores(dsa, dev, scale):
     """Rows that one key decides, with scores of hundreds either way."""
@@ -172,10 +202,12 @@ def test_values_that_a_row_does_not_see(dsa, dev, seqs, win, D, dtype, what):
         assert torch.isnan(got[hit]).all()
 
 
-def test_pages_outside_the_pool_hide_their_keys(dsa, dev):
-    seqs = [(1, 300), (20, 200), (1, 64)]
-    q, kc, vc, table = _setup(seqs, 8, 2, 64, 32, torch.bfloat16, seed=7)
-    table[0, 2], table[1, 0], table[2, 0], table[2, 1] = -1, kc.shape[0], -5, 2**31 - 1
+@pytest.mark.parametrize("chunk", [20, 150])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_outside_the_pool_hide_their_keys(dsa, dev, chunk, D):
+    seqs = [(1, 300), (chunk, 200), (1, 64)]
+    q, kc, vc, table = _setup(seqs, 8, 2, D, 32, torch.bfloat16, seed=7)
+    table[0, 2], table[1, 0], table[1, 5], table[2, 0], table[2, 1] = -1, kc.shape[0], -1, -5, 2**31 - 1
     got = _run(dsa, dev, seqs, q, kc, vc, table)
     _check(got, _want(seqs, q, kc, vc, table))
     assert (got[0][-1] == 0).all() and torch.isinf(got[1][-1]).all()

@@ -553,8 +553,8 @@ int dsa_sparse_attn_sink(int kind, const void* q, const void* kv, const int32_t*
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 static int check_quant_matmul(int64_t M, int64_t N, int64_t K) {
-  // A grid dimension of 128-row tiles; int32 sums of products of at most 2^14.
-  if (M < 0 || N < 0 || M > 8388480 || N > kMaxInt - 4096) return reject("quant_matmul: bad M / N");
+  // int32 sums of products of at most 2^14; a grid of 128 x 128 tiles.
+  if (M < 0 || N < 0 || M > kMaxInt - 4096 || N > kMaxInt - 4096) return reject("quant_matmul: bad M / N");
   if (K < 1 || K > 131071) return reject("quant_matmul: K must be in [1, 131071]");
   if (((M + 127) / 128) * ((N + 127) / 128) > kMaxInt || (M + N) * K > ((int64_t)1 << 42))
     return reject("quant_matmul: sizes out of range");
@@ -605,6 +605,7 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
   if (!aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) ||
       (paged && (!aligned16(v) || !aligned16(v_out))))
     return reject("qk_norm_rope: rows must start on 16 bytes");
+  if (k_out && (k_out == v_out || k_out == q_out)) return reject("qk_norm_rope: the outputs must be arrays of their own");
   return ok(dsa::launch_qk_norm_rope(kind == DSA_KIND_FP16, q, q_stride, k, k_stride, v, v_stride, q_weight, k_weight,
                                      weight_kind == DSA_KIND_FP32, positions, cos, sin, table_len, T, H, G, D, R, eps,
                                      interleaved ? 1 : 0, slots, cache_rows, q_out, k_out, v_out,
@@ -614,7 +615,8 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
 // Sizes that both the workspace query and the call need in range.
 static bool paged_gqa_sizes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
   return T >= 0 && B >= 1 && B <= 65535 && H >= 1 && G >= 1 && H % G == 0 && G <= 65535 && T <= kMaxInt &&
-         H <= 65535 && T * H <= kMaxInt - 65536 && (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096;
+         H <= 65535 && T * H <= kMaxInt - 65536 && (T * (H / G) / 16 + B + 1) * G <= kMaxInt &&  // a grid of tiles
+         (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096;
 }
 
 size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {

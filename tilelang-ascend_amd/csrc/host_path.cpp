@@ -549,7 +549,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (paged)
     DSA_PLAIN(heads_ok(*val.t, dev, st, T, D, vs) && val.t->size(1) == G && kc.t->dim() == 4 &&
               plain(*kc.t, dev, st) && plain(*vc.t, dev, st) && kc.t->sizes() == vc.t->sizes() &&
-              kc.t->size(2) == G && kc.t->size(3) == D && plain(*slots.t, dev, at::kInt) && slots.t->numel() == T);
+              kc.t->size(2) == G && kc.t->size(3) == D && plain(*slots.t, dev, at::kInt) && slots.t->numel() == T &&
+              kc.t->data_ptr() != vc.t->data_ptr());
   const double eps = PyFloat_AS_DOUBLE(v[11]);
   DSA_PLAIN(eps >= 0);
   const bool pairs = v[12] == Py_True;

@@ -85,6 +85,8 @@ def _run(q, k, v, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slo
                     raise ValueError(f"{name} must be [blocks, block_size, {G}, {D}] {q.dtype}, got {tuple(c.shape)} "
                                      f"{c.dtype}")
                 _lib.require_contiguous(name, c)
+            if k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
+                raise ValueError("k_cache and v_cache must be caches of their own")
             rows = k_cache.shape[0] * k_cache.shape[1]
         q_out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
         k_out = torch.empty((T, G, D), dtype=q.dtype, device=dev) if k_cache is None else k_cache

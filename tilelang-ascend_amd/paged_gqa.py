@@ -34,7 +34,8 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     j <= p (``is_causal``) and j >= p - win_left (``win_left`` None: all).  ``sinks`` [H] fp32 adds exp(sink) to
     each head's denominator.  sm_scale defaults to D^-0.5.  Rows that see nothing -- padding rows, rows behind the
     last packed sequence -- give out = 0 and lse = -inf (or the sink).  A table entry outside the pool hides its keys.
-    Within a sequence's keys the caches hold finite values; what lies behind them does not matter.
+    Keys that a row does not see do not reach it, whatever the caches hold there (infinities and NaN too).  Lengths
+    stay on the device and are cut to what the table and q hold.
     """
     scale = q.shape[-1] ** -0.5 if sm_scale is None and q.dim() >= 3 and q.shape[-1] > 0 else sm_scale
     win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
