@@ -350,39 +350,41 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
   }
 }
 
-// Sums of the splits, scaled and biased: four channels a thread.
-template <int kOut>
+// Sums of the splits, scaled and biased: four channels a thread where rows of the output start on them, one otherwise
+// (neighbouring lanes then store neighbouring elements: 1021 x 2113 fp32 takes 12.4 us by fours).
+template <int kOut, int kPer>
 __global__ __launch_bounds__(256) void qmm_join_kernel(QmmArgs a, int splits) {
-  const int quads = a.part_ld / 4;
+  const int per_row = kPer == 4 ? a.part_ld / 4 : a.N;
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)a.M * quads) return;
-  const int m = (int)(t / quads), n = 4 * (int)(t - (int64_t)m * quads);
-  i32x4 sum = {0, 0, 0, 0};
-  for (int z = 0; z < splits; ++z)
-    sum += *reinterpret_cast<const i32x4*>(a.part + ((int64_t)z * a.M + m) * a.part_ld + n);
+  if (t >= (int64_t)a.M * per_row) return;
+  const int m = (int)(t / per_row), n = kPer * (int)(t - (int64_t)m * per_row);
+  const int* from = a.part + (int64_t)m * a.part_ld + n;
+  const int64_t step = (int64_t)a.M * a.part_ld, at = (int64_t)m * a.N + n;
   const float sx = a.sx[m];
-  float v[4];
+  if constexpr (kPer == 4) {
+    i32x4 sum = {0, 0, 0, 0};
+    for (int z = 0; z < splits; ++z) sum += *reinterpret_cast<const i32x4*>(from + z * step);
+    float v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, sum[e], min(n + e, a.N - 1), sx);
-  const int64_t at = (int64_t)m * a.N + n;
-  if ((a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+    for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, sum[e], n + e, sx);
     qmm_store4<kOut>(a.out, at, v);
   } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < a.N) qmm_store1<kOut>(a.out, at + e, v[e]);
+    int sum = 0;
+    for (int z = 0; z < splits; ++z) sum += from[z * step];
+    qmm_store1<kOut>(a.out, at, qmm_value(a, sum, n, sx));
   }
 }
 
-// Rows of K bytes anywhere to rows of ld bytes (a multiple of 128) on 16 bytes, zeros behind K: a chunk a thread.
+// Rows of K bytes anywhere to rows of ld bytes (a multiple of 128) on 16 bytes, zeros behind K: a wave a row.
 __global__ __launch_bounds__(256) void qmm_pack_kernel(const uint8_t* x, int64_t M, const uint8_t* w, int64_t N, int K,
                                                        int ld, uint8_t* to) {
-  const int chunks = ld / 16;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (M + N) * chunks) return;
-  const int64_t row = t / chunks;
-  const int k = 16 * (int)(t - row * chunks);
-  *reinterpret_cast<u32x4*>(to + t * 16) = qmm_chunk(row < M ? x + row * K : w + (row - M) * K, k, K);
+  const int64_t row = (int64_t)blockIdx.x * (256 / kWave) + threadIdx.x / kWave;
+  if (row >= M + N) return;
+  const uint8_t* src = row < M ? x + row * K : w + (row - M) * K;
+  uint8_t* dst = to + row * ld;
+#pragma unroll 4
+  for (int k = 16 * (threadIdx.x & (kWave - 1)); k < ld; k += 16 * kWave)
+    *reinterpret_cast<u32x4*>(dst + k) = qmm_chunk(src, k, K);
 }
 
 // The launch of a call: which kernel, and the workspace's parts.
@@ -453,8 +455,13 @@ static hipError_t qmm_launch_shared(const QmmArgs& a, int splits, hipStream_t st
   if (splits == 1) return qmm_launch_tile<kOut, kBM, 128, kWM, kWN, kStages, false>(a, 1, stream);
   const hipError_t e = qmm_launch_tile<kOut, kBM, 128, kWM, kWN, kStages, true>(a, splits, stream);
   if (e != hipSuccess) return e;
-  const int64_t quads = (int64_t)a.M * (a.part_ld / 4);
-  hipLaunchKernelGGL((qmm_join_kernel<kOut>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
+  if ((a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
+    const int64_t quads = (int64_t)a.M * (a.part_ld / 4);
+    hipLaunchKernelGGL((qmm_join_kernel<kOut, 4>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
+  } else {
+    const int64_t all = (int64_t)a.M * a.N;
+    hipLaunchKernelGGL((qmm_join_kernel<kOut, 1>), dim3((unsigned)((all + 255) / 256)), dim3(256), 0, stream, a, splits);
+  }
   return hipGetLastError();
 }
 
@@ -471,9 +478,8 @@ static hipError_t qmm_launch(QmmArgs a, void* workspace, hipStream_t stream) {
   a.part_ld = (a.N + 3) / 4 * 4;
   if (p.pack) {
     const int ld = (int)qmm_ld(a.K);
-    const int64_t chunks = ((int64_t)a.M + a.N) * (ld / 16);
-    hipLaunchKernelGGL(qmm_pack_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, stream, a.x, (int64_t)a.M,
-                       a.w, (int64_t)a.N, a.K, ld, ws);
+    hipLaunchKernelGGL(qmm_pack_kernel, dim3((unsigned)(((int64_t)a.M + a.N + 3) / 4)), dim3(256), 0, stream, a.x,
+                       (int64_t)a.M, a.w, (int64_t)a.N, a.K, ld, ws);
     a.x = ws;
     a.w = ws + (int64_t)a.M * ld;
     a.K = ld;
