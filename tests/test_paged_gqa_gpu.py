@@ -199,7 +199,7 @@ def test_values_that_a_row_does_not_see(dsa, dev, seqs, win, D, dtype, what):
                 if sees(row, b, j):
                     hit[t, H // G:] = True
         assert torch.equal(got[~hit], want[~hit]) and torch.isfinite(lse[~hit]).all()
-        assert torch.isnan(got[hit]).all()
+        assert torch.isnan(got[hit]).all() and torch.isnan(lse[hit]).all()
 
 
 @pytest.mark.parametrize("chunk", [20, 150])

@@ -137,7 +137,8 @@ static __device__ __align__(128) uint8_t kPgZeroRow[256];
 
 // The keys [k0, k1) of tile `tile` of sequence s, group kvg; `whole`: these are all its keys (the result goes to
 // out and lse, otherwise to the part).  Two stages of K and V of 32 keys a wave; the merge reuses a wave's ring, its
-// (maximum, sum) lie behind.
+// (maximum, sum) lie behind.  Bound by the caches' bytes: 64 tokens over 8192 keys each, 64 heads over 4 of 128: 201 us,
+// 5.4 TB/s; one token over 4097: 9 us and the join's 7, latencies.
 template <bool kF16, int kD, int kHB>
 __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
@@ -413,11 +414,11 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
         f = fast_exp2(M - M2);
         sum = sum * f + fast_exp2(sk - M2);
       }
-      const float inv = sum > 0.f ? f / sum : 0.f;
+      const float inv = sum != 0.f ? f / sum : 0.f;
       *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
           u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
                 gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-      if (c0 == 0) a.lse[orow] = sum > 0.f ? (M2 + fast_log2(sum)) * kLn2 : -kPgInf;
+      if (c0 == 0) a.lse[orow] = sum != 0.f ? (M2 + fast_log2(sum)) * kLn2 : -kPgInf;
     }
   }
   __syncthreads();  // the rings are free for the next item
@@ -481,7 +482,10 @@ constexpr int kPrTile = 64;             // keys
 // wave is in C while the other is in X.  Rings of four stages: C(t) starts the DMA of K of tile t + 3 and V of tile
 // t + 2, into the stages of K(t - 1) and V(t - 2), whose last reads (in C(t - 1) of the later waves) lie before the
 // barrier ahead of C(t) of the earlier ones.  The wait at the end of C(t) leaves only what C(t) started in flight:
-// behind two barriers more K(t + 2) and V(t + 1) are whole, so that the end of X(t) may read ahead of C(t + 1).
+// behind two barriers more K(t + 2) and V(t + 1) are whole, so that X(t) may begin with the first reads of C(t + 1).
+// One barrier a body instead of two, the halves still apart: 64-wide heads 2631 -> 2474 us, 128-wide 3916 -> 4079 (16K
+// prompts, 64 heads over 4); both halves in phase: 4409.  As it is: 3875 us for 128-wide heads, 1135 TFLOP/s; 512 tokens
+// over 65536 keys 1009 us, 1086.  A tile's LDS reads (64 + 64 KB by eight waves) take about 70% of a body's time.
 template <bool kF16, int kD, bool kEven>
 __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
@@ -935,7 +939,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       f = fast_exp2(m_run - M);
       sum = sum * f + fast_exp2(sk - M);
     }
-    const float inv = sum > 0.f ? f / sum : 0.f;
+    const float inv = sum != 0.f ? f / sum : 0.f;
     uint16_t* dst = a.out + qrow * kD + 8 * hi;
 #pragma unroll
     for (int n = 0; n < kNb; ++n)
@@ -947,7 +951,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         *reinterpret_cast<u32x4*>(dst + 32 * n + 16 * x) = u32x4{gqa_pack<kF16>(v[0], v[1]), gqa_pack<kF16>(v[2], v[3]),
                                                                 gqa_pack<kF16>(v[4], v[5]), gqa_pack<kF16>(v[6], v[7])};
       }
-    if (hi == 0) a.lse[qrow] = sum > 0.f ? (M + fast_log2(sum)) * kLn2 : -kPgInf;
+    if (hi == 0) a.lse[qrow] = sum != 0.f ? (M + fast_log2(sum)) * kLn2 : -kPgInf;
   }
 }
 
@@ -1208,12 +1212,12 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
     }
     if (!live) continue;
     sum += fast_exp2(sk - M_use);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
     const int64_t orow = (int64_t)(s.start + i) * a.H + h;
     *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
         u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
               gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-    if (c0 == 0) a.lse[orow] = sum > 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
+    if (c0 == 0) a.lse[orow] = sum != 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
   }
 }
 
