@@ -41,6 +41,7 @@ constexpr int kPgWaves = 4;
 constexpr int kPgThreads = kPgWaves * kWave;
 constexpr int kPgUnit = kPgWaves * kPgTile;  // 128 keys
 constexpr int kPgMaxSlots = 4096;            // of a call whose tiles share the line of units
+constexpr int kPgFewSlots = 256;             // of all groups: the join takes a pass a workgroup
 constexpr float kPgInf = __builtin_huge_valf();
 
 struct PgArgs {
@@ -1130,13 +1131,16 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
 // Joins the parts of each tile whose units lie in more than one workgroup's share: workgroup = (slot and group, rows).
 // kGroups groups of threads take every kGroups-th part of a pass's rows, 8 columns a thread, and are summed through
 // LDS: four for the tiles of few rows, whose keys may lie in many parts, one for those of 256, which have many rows.
+// Those have a workgroup a pass as long as the slots are few (64 queries of 64 heads over 30000 keys: 16 parts a tile,
+// 21.7 us with four passes a workgroup, 8.8 with one), and four passes a workgroup where most slots may hold no tile
+// (800 sequences of 5 tokens: 79.7 us with one pass, 21.1 with four).
 template <class W>
 struct PgJoin {
   static constexpr int kPerRow = W::kD / 8;
   static constexpr int kGroups = W::kR == kPrRows ? 1 : 4;
   static constexpr int kPass = kPgThreads / kGroups / kPerRow;  // rows of a pass
-  static constexpr int kRows = W::kR == kPrRows ? 64 : kPass;   // rows of a workgroup
-  static_assert(W::kR % kRows == 0 && kRows % kPass == 0, "whole groups of rows");
+  static constexpr int kMost = W::kR == kPrRows ? 4 : 1;        // passes of a workgroup
+  static_assert(W::kR % (kMost * kPass) == 0, "whole groups of rows");
 };
 template <class W>
 __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
@@ -1157,8 +1161,9 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
   const int t = in % J::kPerRow, c0 = 8 * t;
   const auto part = [&](int p) { return pg_part<W>(a, w0 + p, u0 < (w0 + p) * share); };
   __shared__ float sums[J::kGroups][9][kPgThreads / J::kGroups];
-  for (int r0 = 0; r0 < J::kRows; r0 += J::kPass) {
-    const int hh = blockIdx.y * J::kRows + r0 + in / J::kPerRow;
+  const int rows = kR / gridDim.y;  // of the workgroup
+  for (int r0 = 0; r0 < rows; r0 += J::kPass) {
+    const int hh = blockIdx.y * rows + r0 + in / J::kPerRow;
     const int rho = tile * kR + hh;
     if (rho - in / J::kPerRow >= s.span * a.Hg) break;  // no row of the pass
     const bool live = rho < s.span * a.Hg;
@@ -1171,7 +1176,7 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
     M = fmaxf(M, sk);
     const float M_use = M == -kPgInf ? 0.f : M;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-    constexpr int kAhead = J::kGroups == 1 ? 2 : 8;  // parts whose loads are in flight together
+    constexpr int kAhead = J::kGroups == 1 ? 4 : 8;  // parts whose loads are in flight together
     for (int p0 = group; p0 < np; p0 += J::kGroups * kAhead) {
       f32x4 x0[kAhead], x1[kAhead];
       float m[kAhead], l[kAhead];
@@ -1267,7 +1272,8 @@ static hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
   e = set_dynamic_lds_once<pg_split_kernel<W>>(split_lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((pg_split_kernel<W>), dim3(a.wgs), dim3(W::kThreads), split_lds, stream, a);
-  const dim3 join(tiles.x, W::kR / PgJoin<W>::kRows);
+  typedef PgJoin<W> J;
+  const dim3 join(tiles.x, W::kR / J::kPass / (tiles.x > kPgFewSlots ? J::kMost : 1));
   hipLaunchKernelGGL((pg_join_kernel<W>), join, dim3(kPgThreads), 0, stream, a);
   return hipGetLastError();
 }
