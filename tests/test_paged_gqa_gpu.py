@@ -257,6 +257,19 @@ def test_same_bits_each_time(dsa, dev):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("win", [None, 500])
+def test_long_chunks_are_repeated_to_the_bit(dsa, dev, D, win):
+    """Whole and partly seen tiles in turn, a tile that ends inside a page, waves without rows in the last one."""
+    seqs = [(1301, 2777), (1, 40), (270, 270)]
+    args = _setup(seqs, 8, 2, D, 24, torch.bfloat16, seed=D)
+    got = _run(dsa, dev, seqs, *args, win=win)
+    _check(got, _want(seqs, *args, win=-1 if win is None else win))
+    for _ in range(5):
+        again = _run(dsa, dev, seqs, *args, win=win)
+        assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
 def test_lengths_past_the_table_are_cut(dsa, dev):
     """kv lengths above max_blocks * block_size and prefix sums above T are clamped, not followed."""
     seqs = [(4, 64)]

@@ -484,9 +484,12 @@ constexpr int kPrTile = 64;             // keys
 // t + 2, into the stages of K(t - 1) and V(t - 2), whose last reads (in C(t - 1) of the later waves) lie before the
 // barrier ahead of C(t) of the earlier ones.  The wait at the end of C(t) leaves only what C(t) started in flight:
 // behind two barriers more K(t + 2) and V(t + 1) are whole, so that X(t) may begin with the first reads of C(t + 1).
-// One barrier a body instead of two, the halves still apart: 64-wide heads 2631 -> 2474 us, 128-wide 3916 -> 4079 (16K
-// prompts, 64 heads over 4); both halves in phase: 4409.  As it is: 3875 us for 128-wide heads, 1135 TFLOP/s; 512 tokens
-// over 65536 keys 1009 us, 1086.  A tile's LDS reads (64 + 64 KB by eight waves) take about 70% of a body's time.
+// 64-wide heads have one barrier a body instead of two, the halves still apart: between two barriers waves 0 to 3 have
+// C(t) and X(t), waves 4 to 7 X(t - 1) and C(t).  Those read K(t), K(t + 1), V(t - 1) and V(t), whole by the wait at
+// the end of C(t - 1) and the barrier behind it, and the DMA of C(t) goes to K(t - 1) and V(t - 2), last read before
+// that barrier.  16K prompts, 64 heads over 4: 2697 -> 2593 us; 128-wide heads 3970 -> 4152; both halves in phase: 4409.
+// 128-wide heads reach 1135 TFLOP/s there (3875 us); 512 tokens over 65536 keys 1009 us, 1086.  A tile's LDS reads (64 +
+// 64 KB by eight waves) take about 70% of a body's time.
 template <bool kF16, int kD, bool kEven>
 __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
@@ -497,6 +500,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
   constexpr int kI = kPrTile / kRpi / kPrWaves;       // DMA instructions of a wave and tile
   constexpr int kSt = kD / 16;                        // steps of the score product
   constexpr int kNb = kD / 32;                        // 32-column blocks of the output
+  constexpr bool kOne = kD == 64;                     // one barrier a body (64 KB of LDS reads a tile, not 128)
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 31, hi = lane >> 5;
@@ -732,7 +736,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       take();
     };
     const auto turn = [] { __builtin_amdgcn_s_barrier(); };
-    gqa_wait_vmcnt<3 * kI>();
+    gqa_wait_vmcnt<(kOne ? 2 : 3) * kI>();
     // The waves' findings pass through LDS by hand: a fence or a plain access would wait for the DMA.
     const uint32_t flags = gqa_lds_u32(lds + 8 * kTileBytes);
     const bool found = __any(outside | ((uint32_t)my_page >= (uint32_t)a.num_blocks));
@@ -853,28 +857,70 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         if (kChecked && late) search(t + 1);
       }
     };
-    if (first < rows) {
-      if (late) {
-        search(0);
-        turn();
-        scrub(0);
-      }
-      scores_only(0);
-      gqa_wait_vmcnt<2 * kI>();
-      if (!late) search(0);
-      turn();
-      if (!late) scrub(0);
-      start(1);
-      softmax(0);
-      if (late) search(1);
-      const int whole0 = max(part_end, 1), whole1 = max(part_begin - 1, whole0);
-      bodies(1, min(whole0, nt), std::true_type{});
-      bodies(whole0, min(whole1, nt), std::false_type{});
-      bodies(max(whole1, 1), nt, std::true_type{});
-      wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(0)>{});  // of a tile behind the last
+    const auto drop = [&] {  // the reads of a tile behind the last
+      wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(0)>{});
       wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(1)>{});
       wait_for(std::integral_constant<int, 0>{}, std::integral_constant<int, nth(2)>{});
-      turn();
+    };
+    const int whole0 = max(part_end, 1), whole1 = max(part_begin - 1, whole0);
+    if (first < rows) {
+      if constexpr (kOne) {
+        // A tile seen in part is searched and cleaned behind its turn, with a barrier between.
+        const auto check = [&](int t) {
+          if (!in_part(t)) return;
+          search(t);
+          turn();
+          scrub(t);
+        };
+        // Bodies as below, one turn each: before C(t) of waves 0 to 3, between C(t - 1) and X(t - 1) of the others.
+        const auto rest = [&](int t, auto checked) {  // of body t, behind C(t)
+          gqa_wait_vmcnt<2 * kI>();
+          if (late) {
+            turn();
+            if (decltype(checked)::value) check(t + 1);
+          }
+          start(t + 1);
+          softmax(t);
+          if (!late) {
+            turn();
+            if (decltype(checked)::value) check(t + 1);
+          }
+        };
+        check(0);
+        scores_only(0);
+        rest(0, std::true_type{});
+        const auto run = [&](int t0, int t1, auto checked) {
+          for (int t = t0; t < t1; ++t) {
+            __builtin_amdgcn_s_setprio(1);
+            body(t);
+            __builtin_amdgcn_s_setprio(0);
+            rest(t, checked);
+          }
+        };
+        run(1, min(whole0, nt), std::true_type{});
+        run(whole0, min(whole1, nt), std::false_type{});
+        run(max(whole1, 1), nt, std::true_type{});
+        drop();
+      } else {
+        if (late) {
+          search(0);
+          turn();
+          scrub(0);
+        }
+        scores_only(0);
+        gqa_wait_vmcnt<2 * kI>();
+        if (!late) search(0);
+        turn();
+        if (!late) scrub(0);
+        start(1);
+        softmax(0);
+        if (late) search(1);
+        bodies(1, min(whole0, nt), std::true_type{});
+        bodies(whole0, min(whole1, nt), std::false_type{});
+        bodies(max(whole1, 1), nt, std::true_type{});
+        drop();
+        turn();
+      }
       products_only(nt);
       if (any_bad) {
         for (int t = 0; t < nt; ++t) {
@@ -896,11 +942,24 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         }
       }
     } else {  // no rows: this wave only moves tiles and searches its part of them
-      if (late) {
+      if (!kOne && late) {
         search(0);
         turn();
       }
-      for (int t = 0; t < nt; ++t) {
+      for (int t = 0; kOne && t < nt; ++t) {
+        if (t > 0) turn();
+        if (in_part(t)) {
+          search(t);
+          turn();
+        }
+        ask(t);
+        dma_k(t);
+        dma_v(t);
+        take();
+        gqa_wait_vmcnt<2 * kI>();
+      }
+      if (kOne) turn();
+      for (int t = 0; !kOne && t < nt; ++t) {
         ask(t);
         dma_k(t);
         dma_v(t);
@@ -912,7 +971,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         turn();
       }
     }
-    if (!late) turn();
+    if (!kOne && !late) turn();
     __builtin_amdgcn_s_waitcnt(0);  // the DMA of tiles behind the last
   }
 
