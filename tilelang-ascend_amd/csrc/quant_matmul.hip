@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kQmmRowWaves * kWave) void qmm_rows_kernel(QmmArgs 
 // products, channels on the M axis).  Chunk c (16 bytes) of row r lies at c ^ ((r >> 2) & 7), so that the 32 rows
 // a half wave reads at one c fall on distinct banks; the DMA fetches the chunks in that order.  Rows start on 16
 // bytes and hold whole chunks (qmm_pack_kernel sees to it where they do not); chunks past K come from a row of zeros.
-// 16384 x 9216 x 7168: 1089 us, 1988 TOP/s; the DMA alone takes 836 us there, the LDS reads 495, and the matrix cores
+// 16384 x 9216 x 7168: 1051 us, 2060 TOP/s; the DMA alone takes 836 us there, the LDS reads 495, and the matrix cores
 // reach 3200 to 3700 on random operands (clock), a library's 8192^3 2089.
 // With kSplit the steps are dealt to gridDim.z workgroups, which leave int32 sums for qmm_join_kernel.
 // Whole lines of a row: with 64 bytes (and four stages) 16384 x 9216 x 7168 took 1120 us, 1089 with 128.
@@ -317,61 +317,93 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
   mul(v[1]);
 
   // Lane (r, hi) holds channels 8 c + 4 hi + e (c = 0 .. 3, e = 0 .. 3) of token r of a 32 x 32 block.
-  const bool vec = (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  if constexpr (kSplit) {
+    // Rows of the sums are padded to a multiple of 4 channels.
 #pragma unroll
-  for (int j = 0; j < S::kFM; ++j) {
-    const int m = m0 + wm + 32 * j + r;
-    if (m >= a.M) continue;
-    const float sx = a.sx[m];
+    for (int j = 0; j < S::kFM; ++j) {
+      const int m = m0 + wm + 32 * j + r;
+      if (m >= a.M) continue;
 #pragma unroll
-    for (int i = 0; i < S::kFN; ++i)
+      for (int i = 0; i < S::kFN; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = n0 + wn + 32 * i + 8 * c + 4 * hi;
-        if constexpr (kSplit) {
-          // Rows of the sums are padded to a multiple of 4 channels.
+        for (int c = 0; c < 4; ++c) {
+          const int n = n0 + wn + 32 * i + 8 * c + 4 * hi;
           if (n < a.N)
             *reinterpret_cast<i32x4*>(a.part + ((int64_t)blockIdx.z * a.M + m) * a.part_ld + n) =
                 i32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
-        } else {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, acc[i][j][4 * c + e], min(n + e, a.N - 1), sx);
-          const int64_t at = (int64_t)m * a.N + n;
-          if (vec) {
-            if (n < a.N) qmm_store4<kOut>(a.out, at, v);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < a.N) qmm_store1<kOut>(a.out, at + e, v[e]);
-          }
         }
+    }
+  } else {
+    // A wave turns 32 rows of the output at a time in its own LDS and stores neighbouring channels from neighbouring
+    // lanes, wherever rows start.  Straight from the sums' places, four channels or one a lane: 16384 x 9216 x 7168 1085 us
+    // instead of 1051, 16384 x 9215 x 7168 1306 instead of 1062.
+    constexpr int kLd = S::kTN + 4;  // 16 lanes' writes of 16 bytes meet each bank once
+    static_assert(S::kTN == kWave && S::kWaves * 32 * kLd * 4 <= kStages * S::kStage, "a channel a lane, in the stages");
+    __syncthreads();  // no wave reads its operands any more
+    int* turned = reinterpret_cast<int*>(lds) + wave * 32 * kLd;
+    const int n = n0 + wn + lane;
+#pragma unroll
+    for (int j = 0; j < S::kFM; ++j) {
+      const int m1 = m0 + wm + 32 * j;
+#pragma unroll
+      for (int i = 0; i < S::kFN; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<i32x4*>(turned + r * kLd + 32 * i + 8 * c + 4 * hi) =
+              i32x4{acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]};
+      // A wave's LDS accesses keep their order.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (n < a.N) {
+#pragma unroll 4
+        for (int t = 0; t < min(32, a.M - m1); ++t)
+          qmm_store1<kOut>(a.out, (int64_t)(m1 + t) * a.N + n, qmm_value(a, turned[t * kLd + lane], n, a.sx[m1 + t]));
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 }
 
-// Sums of the splits, scaled and biased: four channels a thread where rows of the output start on them, one otherwise
-// (neighbouring lanes then store neighbouring elements: 1021 x 2113 fp32 takes 12.4 us by fours).
-template <int kOut, int kPer>
+// Sums of the splits, scaled and biased: four channels a thread where rows of the output start on them, otherwise four
+// elements 256 apart (neighbouring lanes then store neighbouring elements).  Split products have at most 320 tiles, so
+// elements are counted in 32 bits.
+template <int kOut, bool kQuad>
 __global__ __launch_bounds__(256) void qmm_join_kernel(QmmArgs a, int splits) {
-  const int per_row = kPer == 4 ? a.part_ld / 4 : a.N;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (int64_t)a.M * per_row) return;
-  const int m = (int)(t / per_row), n = kPer * (int)(t - (int64_t)m * per_row);
-  const int* from = a.part + (int64_t)m * a.part_ld + n;
-  const int64_t step = (int64_t)a.M * a.part_ld, at = (int64_t)m * a.N + n;
-  const float sx = a.sx[m];
-  if constexpr (kPer == 4) {
+  const uint32_t per_row = kQuad ? a.part_ld / 4 : a.N, all = (uint32_t)a.M * per_row;
+  const int64_t step = (int64_t)a.M * a.part_ld;
+  if constexpr (kQuad) {
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= all) return;
+    const uint32_t m = t / per_row, n = 4 * (t - m * per_row);
+    const int* from = a.part + (int64_t)m * a.part_ld + n;
+    const float sx = a.sx[m];
     i32x4 sum = {0, 0, 0, 0};
+#pragma unroll 2
     for (int z = 0; z < splits; ++z) sum += *reinterpret_cast<const i32x4*>(from + z * step);
     float v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, sum[e], n + e, sx);
-    qmm_store4<kOut>(a.out, at, v);
+    qmm_store4<kOut>(a.out, (int64_t)m * a.N + n, v);
   } else {
-    int sum = 0;
-    for (int z = 0; z < splits; ++z) sum += from[z * step];
-    qmm_store1<kOut>(a.out, at, qmm_value(a, sum, n, sx));
+    const uint32_t t0 = blockIdx.x * 1024 + threadIdx.x;
+    uint32_t m[4], n[4];
+    int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t t = min(t0 + 256 * e, all - 1);
+      m[e] = t / per_row;
+      n[e] = t - m[e] * per_row;
+    }
+    for (int z = 0; z < splits; ++z)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += a.part[z * step + (int64_t)m[e] * a.part_ld + n[e]];
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = qmm_value(a, sum[e], n[e], a.sx[m[e]]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (t0 + 256 * e < all) qmm_store1<kOut>(a.out, (int64_t)(t0 + 256 * e), v[e]);
   }
 }
 
@@ -457,10 +489,10 @@ static hipError_t qmm_launch_shared(const QmmArgs& a, int splits, hipStream_t st
   if (e != hipSuccess) return e;
   if ((a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0) {
     const int64_t quads = (int64_t)a.M * (a.part_ld / 4);
-    hipLaunchKernelGGL((qmm_join_kernel<kOut, 4>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
+    hipLaunchKernelGGL((qmm_join_kernel<kOut, true>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, a, splits);
   } else {
     const int64_t all = (int64_t)a.M * a.N;
-    hipLaunchKernelGGL((qmm_join_kernel<kOut, 1>), dim3((unsigned)((all + 255) / 256)), dim3(256), 0, stream, a, splits);
+    hipLaunchKernelGGL((qmm_join_kernel<kOut, false>), dim3((unsigned)((all + 1023) / 1024)), dim3(256), 0, stream, a, splits);
   }
   return hipGetLastError();
 }
