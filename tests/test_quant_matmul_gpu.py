@@ -38,6 +38,16 @@ def test_against_64_bits(dsa, dev, M, N, K, dtype):
     _check(out, x, w, xs, ws, bias, dtype)
 
 
+@pytest.mark.parametrize("M,N,K", [(1100, 1981, 4160), (1030, 2012, 4113), (700, 2689, 4099)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_three_shares_of_a_long_k(dsa, dev, M, N, K, dtype):
+    """Tiles for more than half and at most two thirds of the CUs."""
+    g = torch.Generator().manual_seed(M + N + K)
+    (x, xs), (w, ws) = _rows(g, M, K), _rows(g, N, K)
+    out = dsa.quant_matmul(x.to(dev), w.to(dev), xs.to(dev), ws.to(dev), dtype=dtype)
+    _check(out, x, w, xs, ws, None, dtype)
+
+
 @pytest.mark.parametrize("M", [1, 5, 40, 130, 600])
 def test_fp16_and_leading_dimensions(dsa, dev, M):
     g = torch.Generator().manual_seed(M)

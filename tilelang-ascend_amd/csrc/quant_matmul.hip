@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kWM* kWN* kWave) void qmm_tile_kernel(QmmArgs a) {
 }
 
 // Sums of the splits, scaled and biased: four channels a thread where rows of the output start on them, otherwise four
-// elements 256 apart (neighbouring lanes then store neighbouring elements).  Split products have at most 320 tiles, so
+// elements 256 apart (neighbouring lanes then store neighbouring elements).  Split products have at most 170 tiles, so
 // elements are counted in 32 bits.
 template <int kOut, bool kQuad>
 __global__ __launch_bounds__(256) void qmm_join_kernel(QmmArgs a, int splits) {
@@ -450,10 +450,13 @@ static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
     return p;
   }
   // Few tiles share their K, eight steps each at least, up to about one workgroup a CU: with up to two, what the
-  // join reads costs more (64 tokens of 7168 x 8192: 22.0 us instead of 18.0; 512: 57.2 instead of 51).  Tiles of 128
-  // may pass 256 a little (1021 x 2113 x 4099: 42.5 us with 136 workgroups, 38.1 with 272).
-  const int64_t steps = (K + kQmmStep - 1) / kQmmStep, most = p.tile == 128 ? 320 : 256;
-  while (p.splits < 8 && small * p.splits * 2 <= most && steps >= 8 * p.splits) p.splits *= 2;
+  // join reads costs more (64 tokens of 7168 x 8192: 22.0 us instead of 18.0; 512: 57.2 instead of 51).  More than
+  // half as many tiles of 128 as CUs share a long K by three, two workgroups a CU (1021 x 2113 x 4099: 39.7 us with one,
+  // 37.6 with two, 35.8 with three; 1024 x 2112 x 7168: 41.4, 40.5, 35.6; 1280 x 1920 x 4096: 27.8, 31.0, 29.1).
+  const int64_t steps = (K + kQmmStep - 1) / kQmmStep;
+  if (p.tile == 128 && small > 128 && small <= 170 && steps > 32) p.splits = 3;
+  else
+    while (p.splits < 8 && small * p.splits * 2 <= 256 && steps >= 8 * p.splits) p.splits *= 2;
   // A workgroup alone on its CU keeps three steps in flight (512 tokens: 65.0 -> 52 us).
   p.deep = p.tile == 128 && small * p.splits <= 256;
   if (p.splits > 1) p.part_bytes = (size_t)(p.splits * M * ((N + 3) / 4 * 4) * 4);
