@@ -1,0 +1,61 @@
+"""Corners of the dense layer's operators on the GPU: wide integers, sinks, padding, other routes, threads, devices."""
+import math
+
+import pytest
+import torch
+
+import dense_layer_ref as ref
+from test_paged_gqa_gpu import _check, _run, _setup, _want
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("chunk", [1, 90])
+def test_wide_table_entries_do_not_wrap(dsa, dev, chunk):
+    """64-bit page numbers past 32 bits lie outside the pool; they do not come back as pages of it."""
+    seqs = [(chunk, 150), (1, 70)]
+    q, kc, vc, table = _setup(seqs, 8, 2, 64, 16, torch.bfloat16, seed=21)
+    hidden, wide = table.clone(), table.long()
+    for at, page in [((0, 1), 2**32), ((0, 3), -2**63), ((0, 4), 2**63 - 1), ((1, 0), 2**32 + int(table[1, 0])),
+                     ((1, 2), 2**31), ((0, 6), -2**32 + 1)]:
+        hidden[at], wide[at] = -1, page
+    want = _run(dsa, dev, seqs, q, kc, vc, hidden)
+    _check(want, _want(seqs, q, kc, vc, hidden))
+    got = _run(dsa, dev, seqs, q, kc, vc, wide)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    got = dsa.load_torch_ops().paged_gqa_fwd(q.to(dev), kc.to(dev), vc.to(dev), wide.to(dev), i32([150, 70]), 64 ** -0.5,
+                                             i32([chunk, chunk + 1]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("where", ["device", "host", "list"])
+def test_wide_lengths_do_not_wrap(dsa, dev, where):
+    """64-bit lengths past 32 bits are cut to what the table and q hold, as smaller ones past it are."""
+    seqs = [(4, 64)]
+    q, kc, vc, table = (t.to(dev) for t in _setup(seqs, 4, 1, 64, 16, torch.bfloat16, seed=22))
+    whole = _run(dsa, dev, seqs, q, kc, vc, table)
+    place = {"device": lambda x: torch.tensor(x, device=dev), "host": torch.tensor, "list": list}[where]
+    ops = dsa.load_torch_ops()
+    for cu, kl in [([2**32 + 2], [2**32 + 5]), ([2**63 - 1], [2**31])]:
+        got = dsa.paged_gqa_fwd(q, kc, vc, table, actual_seq_lengths_query=place(cu), actual_seq_lengths_kv=place(kl))
+        assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])
+        if where == "device":
+            got = ops.paged_gqa_fwd(q, kc, vc, table, place(kl), 64 ** -0.5, place(cu))
+            assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])
+    low = place([-2**63 + 5])
+    out, lse = dsa.paged_gqa_fwd(q, kc, vc, table, actual_seq_lengths_query=low, actual_seq_lengths_kv=low)
+    assert (out == 0).all() and torch.isinf(lse).all()
+
+
+@pytest.mark.parametrize("dtype,big", [(torch.uint32, 2**32 - 3), (torch.uint64, 2**63 + 5), (torch.uint16, 2**16 - 1),
+                                       (torch.uint8, 255)])
+def test_unsigned_lengths(dsa, dev, dtype, big):
+    """Lengths of unsigned types are cut as signed ones are."""
+    seqs = [(4, 64)]
+    q, kc, vc, table = (t.to(dev) for t in _setup(seqs, 4, 1, 64, 16, torch.bfloat16, seed=23))
+    whole = _run(dsa, dev, seqs, q, kc, vc, table)
+    n = torch.tensor([big], dtype=dtype)
+    for place in (n, n.to(dev)):
+        got = dsa.paged_gqa_fwd(q, kc, vc, table, actual_seq_lengths_query=place, actual_seq_lengths_kv=place)
+        assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])

@@ -89,3 +89,16 @@ def test_lds_waits_cover_their_reads(tmp_path_factory, name, nkernels):
     kernels, findings = asm_lds.check_asm(_asm(tmp_path_factory, name))
     assert len(kernels) >= nkernels, kernels
     assert not findings, "\n".join(map(str, findings[:20]))
+
+
+def test_integers_past_32_bits_saturate(dsa):
+    """A helper of the wrappers: what does not fit 32 bits stays at its end of them."""
+    cast = dsa._lib.saturated_int32
+    top, low = 2**31 - 1, -2**31
+    for dtype, given, want in [(torch.int64, [2**32 + 5, -2**63, 2**63 - 1, -7, 2**31, 4], [top, low, top, -7, top, 4]),
+                               (torch.uint32, [2**32 - 1, 2**31, 9], [top, top, 9]),
+                               (torch.uint64, [2**64 - 1, 2**63 + 5, 2**32, 9], [top, top, top, 9]),
+                               (torch.int32, [low, top], [low, top]), (torch.uint16, [65535], [65535]),
+                               (torch.uint8, [255], [255]), (torch.int8, [-1], [-1])]:
+        got = cast(torch.tensor(given, dtype=dtype))
+        assert got.dtype == torch.int32 and got.tolist() == want, dtype

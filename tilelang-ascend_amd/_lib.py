@@ -212,3 +212,16 @@ def require_device(*tensors: Optional[torch.Tensor]) -> torch.device:
 def require_contiguous(name: str, t: torch.Tensor) -> None:
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+_WIDE_INTS = (torch.int64, torch.uint32, torch.uint64)
+
+
+def saturated_int32(t: torch.Tensor) -> torch.Tensor:
+    """An integer tensor as int32, values past 32 bits at the ends of the range instead of wrapped into it."""
+    if t.dtype in _WIDE_INTS:
+        wide = t.to(torch.int64)
+        if t.dtype == torch.uint64:  # values past 63 bits have come out negative
+            wide = wide.masked_fill(wide < 0, 2**31 - 1)
+        t = wide.clamp(-2**31, 2**31 - 1)
+    return t.to(torch.int32)

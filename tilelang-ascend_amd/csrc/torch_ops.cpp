@@ -84,6 +84,15 @@ c10::optional<at::Tensor> aux_i32(const c10::optional<at::Tensor>& t, const at::
   return aux_i32(*t, main, n, name);
 }
 
+// Integers whose values past 32 bits lie at the ends of that range: cast as they are they would wrap into it.
+at::Tensor saturated_i32(const at::Tensor& t) {
+  const at::ScalarType st = t.scalar_type();
+  if (st != at::kLong && st != at::kUInt32 && st != at::kUInt64) return t;
+  at::Tensor wide = t.to(at::kLong);
+  if (st == at::kUInt64) wide = wide.masked_fill(wide < 0, 0x7fffffff);  // values past 63 bits have come out negative
+  return wide.clamp(-0x80000000LL, 0x7fffffffLL).to(at::kInt);
+}
+
 // A float argument: on main's device, `n` elements, made contiguous fp32.
 at::Tensor aux_f32(const at::Tensor& t, const at::Tensor& main, int64_t n, const char* name) {
   require_on(t, main, name);
@@ -457,10 +466,9 @@ void norm_rope(const at::Tensor& q, const at::Tensor& k, const c10::optional<at:
   TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), "dsa.qk_norm_rope: cos and sin must be [positions, R / 2]");
   auto c = aux_f32(cos, q, cos.numel(), "cos"), s = aux_f32(sin, q, sin.numel(), "sin");
   auto qw = aux_f32(q_weight, q, D, "q_weight"), kw = aux_f32(k_weight, q, D, "k_weight");
-  // 64-bit values past 32 bits mark padding; cast as they are they would come back as small ones.
-  const auto fit = [](const at::Tensor& t) { return t.scalar_type() == at::kLong ? t.clamp(-1, 0x7fffffff) : t; };
-  auto pos = aux_i32(fit(positions), q, T, "positions");
-  auto at_rows = aux_i32(slots ? c10::make_optional(fit(*slots)) : slots, q, T, "slots");
+  // 64-bit values past 32 bits mark padding.
+  auto pos = aux_i32(saturated_i32(positions), q, T, "positions");
+  auto at_rows = aux_i32(slots ? c10::make_optional(saturated_i32(*slots)) : slots, q, T, "slots");
   if (T == 0) return;
   check_rc(dsa_qk_norm_rope(kind_of(q), ptr(q), qs, ptr(k), ks, ptr_or_null<void>(v), vs, ptr_or_null<void>(qw),
                             ptr_or_null<void>(kw), DSA_KIND_FP32, static_cast<int32_t*>(ptr(pos)),
@@ -542,9 +550,12 @@ std::tuple<at::Tensor, at::Tensor> paged_gqa_fwd(const at::Tensor& q, const at::
   TORCH_CHECK(packed ? actual_seq_lengths_query.has_value() : q.size(0) == B,
               "dsa.paged_gqa_fwd: packed queries need prefix sums, padded ones one row of block_table per sequence");
   c10::OptionalDeviceGuard guard(q.device());
-  auto bt = aux_i32(block_table, q, -1, "block_table");
-  auto kl = aux_i32(actual_seq_lengths_kv, q, B, "actual_seq_lengths_kv");
-  auto ql = aux_i32(actual_seq_lengths_query, q, B, "actual_seq_lengths_query");
+  // Pages past 32 bits lie outside the pool, lengths past them are cut as smaller ones are.
+  auto bt = aux_i32(saturated_i32(block_table), q, -1, "block_table");
+  auto kl = aux_i32(saturated_i32(actual_seq_lengths_kv), q, B, "actual_seq_lengths_kv");
+  auto ql = aux_i32(actual_seq_lengths_query ? c10::make_optional(saturated_i32(*actual_seq_lengths_query))
+                                             : actual_seq_lengths_query,
+                    q, B, "actual_seq_lengths_query");
   const int64_t H = q.size(-2), D = q.size(-1), G = k_cache.size(2);
   auto sk = aux_f32(sinks, q, H, "sinks");
   auto out = at::empty(q.sizes(), q.options());

@@ -69,9 +69,7 @@ def _run(q, k, v, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slo
     def ints(name, t):
         if t.numel() != T or t.dtype not in (torch.int32, torch.int64, torch.int16, torch.uint8, torch.int8):
             raise ValueError(f"{name} must hold one integer per token ({T}), got {tuple(t.shape)} {t.dtype}")
-        if t.dtype == torch.int64:  # values past 32 bits mark padding, as they did
-            t = t.clamp(-1, 2**31 - 1)
-        return t.to(torch.int32).contiguous()
+        return _lib.saturated_int32(t).contiguous()  # values past 32 bits mark padding, as they did
 
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")

@@ -88,12 +88,12 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         t = torch.as_tensor(x)
         if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool or t.numel() != B:
             raise ValueError(f"{name} must hold B={B} integers, got {tuple(t.shape)} {t.dtype}")
-        return t.to(device=dev, dtype=torch.int32).reshape(-1).contiguous()
+        return _lib.saturated_int32(t).to(dev).reshape(-1).contiguous()
 
     with torch.cuda.device(dev):
         ql = lens("actual_seq_lengths_query", actual_seq_lengths_query)
         kl = lens("actual_seq_lengths_kv", actual_seq_lengths_kv)
-        bt = block_table.to(torch.int32).contiguous()
+        bt = _lib.saturated_int32(block_table).contiguous()
         sk = None if sinks is None else sinks.contiguous()
         T = q.shape[0] if packed else B * q.shape[1]
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
