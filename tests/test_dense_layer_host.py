@@ -102,3 +102,11 @@ def test_integers_past_32_bits_saturate(dsa):
                                (torch.uint8, [255], [255]), (torch.int8, [-1], [-1])]:
         got = cast(torch.tensor(given, dtype=dtype))
         assert got.dtype == torch.int32 and got.tolist() == want, dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.bool, torch.complex64])
+def test_block_tables_hold_integers(dsa, dtype):
+    q, c = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    n = torch.ones(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="block_table must hold integers"):
+        dsa.paged_gqa_fwd(q, c, c, torch.zeros(1, 4, dtype=dtype), actual_seq_lengths_query=n, actual_seq_lengths_kv=n)

@@ -214,6 +214,10 @@ def require_contiguous(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+def is_integer(t: torch.Tensor) -> bool:
+    return not (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool)
+
+
 _WIDE_INTS = (torch.int64, torch.uint32, torch.uint64)
 
 

@@ -61,6 +61,8 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         raise ValueError(f"the caches must hold at least one row, got {tuple(k_cache.shape)}")
     if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
         raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
+    if not _lib.is_integer(block_table):
+        raise ValueError(f"block_table must hold integers, got {block_table.dtype}")
     B = block_table.shape[0]
     if actual_seq_lengths_kv is None:
         raise ValueError("actual_seq_lengths_kv is required")
@@ -86,7 +88,7 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         if x is None:
             return None
         t = torch.as_tensor(x)
-        if t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool or t.numel() != B:
+        if not _lib.is_integer(t) or t.numel() != B:
             raise ValueError(f"{name} must hold B={B} integers, got {tuple(t.shape)} {t.dtype}")
         return _lib.saturated_int32(t).to(dev).reshape(-1).contiguous()
 
