@@ -410,6 +410,8 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
  *  the denominator; out [T, H, D]; lse [T, H] fp32, natural log, sink included.  Rows that see nothing (padding
  *  rows, rows behind cu_q[B - 1] too) get out = 0 and lse = -inf (or the sink).  Keys that a row does not see do
  *  not reach it, whatever their pages hold.  Lengths are read on the device and cut to what the table and q hold.
+ *  cu_q must not decrease (a sequence without new tokens repeats the sum before it): nothing out of range is read or
+ *  written where it does, but rows of out and lse are then undefined.
  *  max_keys of the workspace query is max_blocks * block_size.
  */
 size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys);

@@ -110,3 +110,15 @@ def test_block_tables_hold_integers(dsa, dtype):
     n = torch.ones(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="block_table must hold integers"):
         dsa.paged_gqa_fwd(q, c, c, torch.zeros(1, 4, dtype=dtype), actual_seq_lengths_query=n, actual_seq_lengths_kv=n)
+
+
+@pytest.mark.parametrize("sums", [[3, 1], torch.tensor([3, 0]), torch.tensor([2**32, 4]),
+                                  torch.tensor([3, -1], dtype=torch.int32)])
+def test_prefix_sums_on_the_host_do_not_decrease(dsa, sums):
+    q, c = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    call = lambda cu: dsa.paged_gqa_fwd(q, c, c, torch.zeros(2, 4, dtype=torch.int32), actual_seq_lengths_query=cu,
+                                        actual_seq_lengths_kv=[4, 4])
+    with pytest.raises(ValueError, match="non-decreasing"):
+        call(sums)
+    with pytest.raises(ValueError, match="HIP"):  # the next check: host tensors
+        call([3, 3])

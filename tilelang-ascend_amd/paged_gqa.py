@@ -35,7 +35,9 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     each head's denominator.  sm_scale defaults to D^-0.5.  Rows that see nothing -- padding rows, rows behind the
     last packed sequence -- give out = 0 and lse = -inf (or the sink).  A table entry outside the pool hides its keys.
     Keys that a row does not see do not reach it, whatever the caches hold there (infinities and NaN too).  Lengths
-    stay on the device and are cut to what the table and q hold.
+    stay on the device and are cut to what the table and q hold.  Prefix sums must not decrease (a sequence without
+    new tokens repeats the one before it): on the host that is checked; on the device sums that do decrease leave
+    rows of out and lse undefined.
     """
     scale = q.shape[-1] ** -0.5 if sm_scale is None and q.dim() >= 3 and q.shape[-1] > 0 else sm_scale
     win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
@@ -75,6 +77,19 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         raise ValueError(f"win_left must be None or a key count, got {win_left}")
     if not 0 < scale <= 1e30:
         raise ValueError(f"sm_scale must be positive, got {sm_scale}")
+
+    def lens(name, x):
+        if x is None:
+            return None
+        t = torch.as_tensor(x)
+        if not _lib.is_integer(t) or t.numel() != B:
+            raise ValueError(f"{name} must hold B={B} integers, got {tuple(t.shape)} {t.dtype}")
+        return _lib.saturated_int32(t).reshape(-1)
+
+    ql = lens("actual_seq_lengths_query", actual_seq_lengths_query)
+    kl = lens("actual_seq_lengths_kv", actual_seq_lengths_kv)
+    if packed and ql.device.type == "cpu" and bool((ql[1:] < ql[:-1]).any()):
+        raise ValueError("actual_seq_lengths_query must be non-decreasing prefix sums")
     dev = _lib.require_device(q, k_cache, v_cache, block_table, sinks)
     if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (H,)):
         raise ValueError(f"sinks must be [{H}] float32, got {tuple(sinks.shape)} {sinks.dtype}")
@@ -84,17 +99,8 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         if t.data_ptr() % 16 != 0:
             raise ValueError(f"{name} must start on 16 bytes")
 
-    def lens(name, x):
-        if x is None:
-            return None
-        t = torch.as_tensor(x)
-        if not _lib.is_integer(t) or t.numel() != B:
-            raise ValueError(f"{name} must hold B={B} integers, got {tuple(t.shape)} {t.dtype}")
-        return _lib.saturated_int32(t).to(dev).reshape(-1).contiguous()
-
     with torch.cuda.device(dev):
-        ql = lens("actual_seq_lengths_query", actual_seq_lengths_query)
-        kl = lens("actual_seq_lengths_kv", actual_seq_lengths_kv)
+        ql, kl = (None if x is None else x.to(dev).contiguous() for x in (ql, kl))
         bt = _lib.saturated_int32(block_table).contiguous()
         sk = None if sinks is None else sinks.contiguous()
         T = q.shape[0] if packed else B * q.shape[1]
