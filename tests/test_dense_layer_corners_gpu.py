@@ -59,3 +59,22 @@ def test_unsigned_lengths(dsa, dev, dtype, big):
     for place in (n, n.to(dev)):
         got = dsa.paged_gqa_fwd(q, kc, vc, table, actual_seq_lengths_query=place, actual_seq_lengths_kv=place)
         assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])
+
+
+# Batches in which whole sequences, single rows of a tile, or rows of a tile that several workgroups share see no key.
+NOTHING = {"decode": [(1, 0), (1, 40), (1, 0)], "tokens before the keys": [(40, 20), (1, 5)], "shared": [(300, 280)],
+           "none": [(90, 0)]}
+
+
+@pytest.mark.parametrize("name", list(NOTHING))
+@pytest.mark.parametrize("H,G,D", [(8, 2, 64), (16, 1, 128)])
+def test_rows_that_see_nothing_keep_their_sink(dsa, dev, name, H, G, D):
+    """lse is the sink however small or large its exponential is."""
+    seqs = NOTHING[name]
+    args = _setup(seqs, H, G, D, 16, torch.bfloat16, seed=24)
+    sinks = torch.tensor([-200.0, -80.0, -1e4, torch.finfo(torch.float32).min, 0.0, 3.0, 100.0, 500.0]).repeat(H // 8)
+    out, tol, lse, ltol = _want(seqs, *args, sinks=sinks)
+    # Beside a large sink a row's keys have the factor 2^(m - sink) in fp32, which is 0 below 2^-126: the sum of at most n
+    # weights of at most 1 times v, over a denominator of at least 1 (the sink's own), is then off by 2^-126 n |v|.
+    tol = tol + 2.0 ** -126 * max(n for _, n in seqs) * args[2].double().abs().max()
+    _check(_run(dsa, dev, seqs, *args, sinks=sinks), (out, tol, lse, ltol))

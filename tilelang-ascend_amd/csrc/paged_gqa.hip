@@ -136,6 +136,25 @@ __device__ __forceinline__ float pg_only_bad(uint32_t w, int hi) {
 // not be 0.
 static __device__ __align__(128) uint8_t kPgZeroRow[256];
 
+// What becomes of a row's sums o, taken beside the maximum m (base 2), whose weights add up to l: out = o * scale.  A
+// row that saw nothing (l = 0) has its sink for lse as it is, whatever its exponential is.
+struct PgEnd {
+  float scale, lse;
+};
+__device__ __forceinline__ PgEnd pg_end(const PgArgs& a, float m, float l, int head) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  if (l == 0.f) return {0.f, a.sinks ? a.sinks[head] : -kPgInf};
+  if (m == -kPgInf) m = 0.f;
+  float f = 1.f;
+  if (a.sinks) {
+    const float sk = a.sinks[head] * kLog2e, top = fmaxf(m, sk);
+    f = fast_exp2(m - top);
+    l = l * f + fast_exp2(sk - top);
+    m = top;
+  }
+  return {f / l, (m + fast_log2(l)) * kLn2};
+}
+
 // The keys [k0, k1) of tile `tile` of sequence s, group kvg; `whole`: these are all its keys (the result goes to
 // out and lse, otherwise to the part).  Two stages of K and V of 32 keys a wave; the merge reuses a wave's ring, its
 // (maximum, sum) lie behind.  Bound by the caches' bytes: 64 tokens over 8192 keys each, 64 heads over 4 of 128: 201 us,
@@ -374,7 +393,6 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
   __syncthreads();
   constexpr int kPerRow = kD / 8;                  // threads of a row
   constexpr int kRowsPass = kPgThreads / kPerRow;  // 16 or 32
-  constexpr float kLn2 = 0.6931471805599453f;
 #pragma unroll
   for (int r0 = 0; r0 < 16 * kHB; r0 += kRowsPass) {
     const int hh = r0 + tid / kPerRow, c0 = 8 * (tid % kPerRow);
@@ -407,19 +425,12 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
     } else if (rho < rows) {
       const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
       const int64_t orow = (int64_t)(s.start + i) * a.H + h;
-      float M2 = M_use, f = 1.f;
-      if (a.sinks) {
-        const float sk = a.sinks[h] * 1.4426950408889634f;
-        M2 = fmaxf(M, sk);
-        M2 = M2 == -kPgInf ? 0.f : M2;
-        f = fast_exp2(M - M2);
-        sum = sum * f + fast_exp2(sk - M2);
-      }
-      const float inv = sum != 0.f ? f / sum : 0.f;
+      const PgEnd e = pg_end(a, M, sum, h);
+      const float inv = e.scale;
       *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
           u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
                 gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-      if (c0 == 0) a.lse[orow] = sum != 0.f ? (M2 + fast_log2(sum)) * kLn2 : -kPgInf;
+      if (c0 == 0) a.lse[orow] = e.lse;
     }
   }
   __syncthreads();  // the rings are free for the next item
@@ -977,7 +988,6 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
 
   l_run = pr_sum32(l_run);
   const bool none = l_run == 0.f;  // a row that saw nothing: its sums may be 0 times anything
-  constexpr float kLn2 = 0.6931471805599453f;
   if (!whole) {
     float* p = part + (32 * wave + r) * kD + 8 * hi;
 #pragma unroll
@@ -991,15 +1001,8 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       part[kPrRows * kD + 2 * (32 * wave + r) + 1] = l_run;
     }
   } else if (first + r < rows) {
-    float M = m_run == -kPgInf ? 0.f : m_run, f = 1.f, sum = l_run;
-    if (a.sinks) {
-      const float sk = a.sinks[head] * 1.4426950408889634f;
-      M = fmaxf(m_run, sk);
-      M = M == -kPgInf ? 0.f : M;
-      f = fast_exp2(m_run - M);
-      sum = sum * f + fast_exp2(sk - M);
-    }
-    const float inv = sum != 0.f ? f / sum : 0.f;
+    const PgEnd e = pg_end(a, m_run, l_run, head);
+    const float inv = e.scale;
     uint16_t* dst = a.out + qrow * kD + 8 * hi;
 #pragma unroll
     for (int n = 0; n < kNb; ++n)
@@ -1011,7 +1014,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
         *reinterpret_cast<u32x4*>(dst + 32 * n + 16 * x) = u32x4{gqa_pack<kF16>(v[0], v[1]), gqa_pack<kF16>(v[2], v[3]),
                                                                 gqa_pack<kF16>(v[4], v[5]), gqa_pack<kF16>(v[6], v[7])};
       }
-    if (hi == 0) a.lse[qrow] = sum != 0.f ? (M + fast_log2(sum)) * kLn2 : -kPgInf;
+    if (hi == 0) a.lse[qrow] = e.lse;
   }
 }
 
@@ -1215,7 +1218,6 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
   if (np == 1) return;
   const PgSeq s = pg_seq(a, b);
   const int tile = x - pg_slot(s.start, a.Hg, b, kR);
-  constexpr float kLn2 = 0.6931471805599453f;
   const int group = threadIdx.x / (kPgThreads / J::kGroups), in = threadIdx.x % (kPgThreads / J::kGroups);
   const int t = in % J::kPerRow, c0 = 8 * t;
   const auto part = [&](int p) { return pg_part<W>(a, w0 + p, u0 < (w0 + p) * share); };
@@ -1231,8 +1233,6 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
 #pragma unroll
     for (int o = 1; o < J::kPerRow; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
     const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
-    const float sk = a.sinks && live ? a.sinks[h] * 1.4426950408889634f : -kPgInf;
-    M = fmaxf(M, sk);
     const float M_use = M == -kPgInf ? 0.f : M;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
     constexpr int kAhead = J::kGroups == 1 ? 4 : 8;  // parts whose loads are in flight together
@@ -1275,13 +1275,13 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
       }
     }
     if (!live) continue;
-    sum += fast_exp2(sk - M_use);
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    const PgEnd e = pg_end(a, M, sum, h);
+    const float inv = e.scale;
     const int64_t orow = (int64_t)(s.start + i) * a.H + h;
     *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
         u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
               gqa_pack<kF16>(acc[4] * inv, acc[5] * inv), gqa_pack<kF16>(acc[6] * inv, acc[7] * inv)};
-    if (c0 == 0) a.lse[orow] = sum != 0.f ? (M_use + fast_log2(sum)) * kLn2 : -kPgInf;
+    if (c0 == 0) a.lse[orow] = e.lse;
   }
 }
 
