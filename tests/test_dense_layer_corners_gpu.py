@@ -78,3 +78,21 @@ def test_rows_that_see_nothing_keep_their_sink(dsa, dev, name, H, G, D):
     # weights of at most 1 times v, over a denominator of at least 1 (the sink's own), is then off by 2^-126 n |v|.
     tol = tol + 2.0 ** -126 * max(n for _, n in seqs) * args[2].double().abs().max()
     _check(_run(dsa, dev, seqs, *args, sinks=sinks), (out, tol, lse, ltol))
+
+
+@pytest.mark.parametrize("name", list(NOTHING))
+@pytest.mark.parametrize("H,G,D", [(8, 2, 64), (16, 1, 128)])
+def test_sinks_that_are_not_finite(dsa, dev, name, H, G, D):
+    """A sink of +infinity takes all the weight: out = 0, lse = +infinity.  One of -infinity takes none; NaN stays in
+    its head's sums."""
+    seqs = NOTHING[name]
+    args = _setup(seqs, H, G, D, 16, torch.bfloat16, seed=25)
+    free = _run(dsa, dev, seqs, *args)
+    sinks = torch.full((H,), -math.inf)
+    sinks[1], sinks[3], sinks[4] = math.inf, math.nan, 3e38
+    out, lse = _run(dsa, dev, seqs, *args, sinks=sinks)
+    assert (out[:, 1] == 0).all() and (lse[:, 1] == math.inf).all()
+    assert torch.isnan(lse[:, 3]).all()
+    assert (out[:, 4] == 0).all() and (lse[:, 4] == sinks[4].item()).all()
+    rest = [h for h in range(H) if h not in (1, 3, 4)]
+    assert torch.equal(out[:, rest], free[0][:, rest]) and torch.equal(lse[:, rest], free[1][:, rest])

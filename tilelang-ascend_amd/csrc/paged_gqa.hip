@@ -137,7 +137,8 @@ __device__ __forceinline__ float pg_only_bad(uint32_t w, int hi) {
 static __device__ __align__(128) uint8_t kPgZeroRow[256];
 
 // What becomes of a row's sums o, taken beside the maximum m (base 2), whose weights add up to l: out = o * scale.  A
-// row that saw nothing (l = 0) has its sink for lse as it is, whatever its exponential is.
+// row that saw nothing (l = 0) has its sink for lse as it is, whatever its exponential is.  So has a row whose sink is
+// infinite in base 2: all the weight is the sink's.
 struct PgEnd {
   float scale, lse;
 };
@@ -149,7 +150,8 @@ __device__ __forceinline__ PgEnd pg_end(const PgArgs& a, float m, float l, int h
   if (a.sinks) {
     const float sk = a.sinks[head] * kLog2e, top = fmaxf(m, sk);
     f = fast_exp2(m - top);
-    l = l * f + fast_exp2(sk - top);
+    l = l * f + (sk == kPgInf ? 1.f : fast_exp2(sk - top));
+    if (sk == kPgInf && l == 1.f) return {0.f, a.sinks[head]};
     m = top;
   }
   return {f / l, (m + fast_log2(l)) * kLn2};
