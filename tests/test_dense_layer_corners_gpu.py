@@ -96,3 +96,52 @@ def test_sinks_that_are_not_finite(dsa, dev, name, H, G, D):
     assert (out[:, 4] == 0).all() and (lse[:, 4] == sinks[4].item()).all()
     rest = [h for h in range(H) if h not in (1, 3, 4)]
     assert torch.equal(out[:, rest], free[0][:, rest]) and torch.equal(lse[:, rest], free[1][:, rest])
+
+
+def _us(f, n=5):
+    f()
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(n):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) / n * 1e3)
+    return sorted(times)[2]
+
+
+@pytest.mark.parametrize("S,lens,keys", [(300, [1, 0, 120], [2000, 900, 500]), (17, [1, 3, 17], [777, 3, 400]),
+                                         (1100, [40, 1, 700], [40, 3000, 800])])
+@pytest.mark.parametrize("win", [None, 50])
+def test_padding_over_long_contexts(dsa, dev, S, lens, keys, win):
+    """Tiles that hold padding only, beside sequences of many keys, with sinks."""
+    B, H, G, D, bs = 3, 8, 2, 64, 16
+    q, kc, vc, table = _setup([(S, n) for n in keys], H, G, D, bs, torch.bfloat16, seed=S)
+    sinks = torch.randn(H, generator=torch.Generator().manual_seed(S))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    out, lse = dsa.paged_gqa_fwd(q.view(B, S, H, D).to(dev), kc.to(dev), vc.to(dev), table.to(dev),
+                                 actual_seq_lengths_query=i32(lens), actual_seq_lengths_kv=i32(keys), win_left=win,
+                                 sinks=sinks.to(dev))
+    want = ref.attention(q, kc, vc, table, [b * S for b in range(B)], [S] * B, lens, keys, D ** -0.5,
+                         win=-1 if win is None else win, sinks=sinks)
+    _check((out.view(B * S, H, D), lse.view(B * S, H)), want)
+    for b in range(B):
+        assert (out[b, lens[b]:] == 0).all()
+
+
+@pytest.mark.parametrize("B,S", [(2, 1024), (8, 2048)])
+def test_padding_reads_no_keys(dsa, dev, B, S):
+    """A batch padded to S rows a sequence, one of them real, takes a fraction of the full batch's time (a share of
+    the work of at most 1/32; a third allows for the launches and for workgroups that walk their keys alone)."""
+    H, G, D, bs, n = 32, 2, 128, 64, 16384
+    q = torch.randn(B, S, H, D, device=dev).bfloat16()
+    kc, vc = (torch.randn(B * n // bs, bs, G, D, device=dev).bfloat16() for _ in range(2))
+    table = torch.arange(B * n // bs, dtype=torch.int32, device=dev).view(B, -1)
+    i32 = lambda x: torch.tensor([x] * B, dtype=torch.int32, device=dev)
+    kl = i32(n)
+    time = lambda ql: _us(lambda: dsa.paged_gqa_fwd(q, kc, vc, table, actual_seq_lengths_query=ql,
+                                                    actual_seq_lengths_kv=kl))
+    one, full = time(i32(1)), time(i32(S))
+    assert one < full / 3, f"one token of {S}: {one:.0f} us, all: {full:.0f} us"

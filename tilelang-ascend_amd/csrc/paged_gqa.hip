@@ -1063,13 +1063,15 @@ __device__ __forceinline__ int pg_find(const PgArgs& a, const int32_t* cu, int s
   }
   return b0;
 }
-// The keys [lo, hi) that rows of the tile see; false: the sequence has no such tile.
+// The keys [lo, hi) that rows of the tile see, none for a tile that holds padding only; false: the sequence has no such
+// tile.
 __device__ __forceinline__ bool pg_range(const PgArgs& a, const PgSeq& s, int tile, int kR, int& lo, int& hi) {
   if (tile < 0 || (int64_t)tile * kR >= (int64_t)s.span * a.Hg) return false;
   lo = s.lo;
   hi = s.hi;
-  const int first = (tile * kR) / a.Hg, last = min(((tile + 1) * kR - 1) / a.Hg, s.span - 1);
-  if (a.causal) hi = max(min(hi, s.n - s.len + last + 1), 0);
+  const int first = (tile * kR) / a.Hg, last = min(((tile + 1) * kR - 1) / a.Hg, s.len - 1);
+  if (first >= s.len) hi = lo;
+  else if (a.causal) hi = max(min(hi, s.n - s.len + last + 1), 0);
   if (a.win >= 0) lo = max(lo, (max(s.n - s.len + first, 0) - a.win) & ~(kPgTile - 1));
   lo = min(lo, hi);
   return true;
