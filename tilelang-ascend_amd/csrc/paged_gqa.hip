@@ -136,25 +136,19 @@ __device__ __forceinline__ float pg_only_bad(uint32_t w, int hi) {
 // not be 0.
 static __device__ __align__(128) uint8_t kPgZeroRow[256];
 
-// What becomes of a row's sums o, taken beside the maximum m (base 2), whose weights add up to l: out = o * scale.  A
-// row that saw nothing (l = 0) has its sink for lse as it is, whatever its exponential is.  So has a row whose sink is
-// infinite in base 2: all the weight is the sink's.
+// What becomes of a row's sums o, taken beside the maximum m (base 2), whose weights add up to l: out = o * scale.
+// `sink` is -infinity where there is none.  A row that saw nothing (l = 0) has its sink for lse as it is, whatever its
+// exponential is.  So has a row whose sink is infinite in base 2: all the weight is the sink's.
 struct PgEnd {
   float scale, lse;
 };
-__device__ __forceinline__ PgEnd pg_end(const PgArgs& a, float m, float l, int head) {
+__device__ __forceinline__ float pg_sink(const PgArgs& a, int head) { return a.sinks ? a.sinks[head] : -kPgInf; }
+__device__ __forceinline__ PgEnd pg_end(float m, float l, float sink) {
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-  if (l == 0.f) return {0.f, a.sinks ? a.sinks[head] : -kPgInf};
-  if (m == -kPgInf) m = 0.f;
-  float f = 1.f;
-  if (a.sinks) {
-    const float sk = a.sinks[head] * kLog2e, top = fmaxf(m, sk);
-    f = fast_exp2(m - top);
-    l = l * f + (sk == kPgInf ? 1.f : fast_exp2(sk - top));
-    if (sk == kPgInf && l == 1.f) return {0.f, a.sinks[head]};
-    m = top;
-  }
-  return {f / l, (m + fast_log2(l)) * kLn2};
+  const float sk = sink * kLog2e, top = fmaxf(m, sk), beside = top == -kPgInf ? 0.f : top;
+  const float f = fast_exp2(m - beside), sum = l * f + (sk == kPgInf ? 1.f : fast_exp2(sk - beside));
+  const bool only = l == 0.f || (sk == kPgInf && sum == 1.f);
+  return {only ? 0.f : f / sum, only ? sink : (beside + fast_log2(sum)) * kLn2};
 }
 
 // The keys [k0, k1) of tile `tile` of sequence s, group kvg; `whole`: these are all its keys (the result goes to
@@ -427,7 +421,7 @@ __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, 
     } else if (rho < rows) {
       const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
       const int64_t orow = (int64_t)(s.start + i) * a.H + h;
-      const PgEnd e = pg_end(a, M, sum, h);
+      const PgEnd e = pg_end(M, sum, pg_sink(a, h));
       const float inv = e.scale;
       *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
           u32x4{gqa_pack<kF16>(acc[0] * inv, acc[1] * inv), gqa_pack<kF16>(acc[2] * inv, acc[3] * inv),
@@ -1003,7 +997,7 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
       part[kPrRows * kD + 2 * (32 * wave + r) + 1] = l_run;
     }
   } else if (first + r < rows) {
-    const PgEnd e = pg_end(a, m_run, l_run, head);
+    const PgEnd e = pg_end(m_run, l_run, pg_sink(a, head));
     const float inv = e.scale;
     uint16_t* dst = a.out + qrow * kD + 8 * hi;
 #pragma unroll
@@ -1237,7 +1231,7 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
 #pragma unroll
     for (int o = 1; o < J::kPerRow; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
     const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
-    const float M_use = M == -kPgInf ? 0.f : M;
+    const float M_use = M == -kPgInf ? 0.f : M, sink = live ? pg_sink(a, h) : -kPgInf;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
     constexpr int kAhead = J::kGroups == 1 ? 4 : 8;  // parts whose loads are in flight together
     for (int p0 = group; p0 < np; p0 += J::kGroups * kAhead) {
@@ -1279,7 +1273,7 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
       }
     }
     if (!live) continue;
-    const PgEnd e = pg_end(a, M, sum, h);
+    const PgEnd e = pg_end(M, sum, sink);
     const float inv = e.scale;
     const int64_t orow = (int64_t)(s.start + i) * a.H + h;
     *reinterpret_cast<u32x4*>(a.out + orow * kD + c0) =
