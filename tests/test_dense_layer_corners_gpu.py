@@ -145,3 +145,41 @@ def test_padding_reads_no_keys(dsa, dev, B, S):
                                                     actual_seq_lengths_kv=kl))
     one, full = time(i32(1)), time(i32(S))
     assert one < full / 3, f"one token of {S}: {one:.0f} us, all: {full:.0f} us"
+
+
+@pytest.mark.parametrize("route", ["native", "64-bit", "registered"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_each_route_writes_the_cache_rows(dsa, dev, route, interleaved):
+    """From caches of its own, each route writes every slot's key and value row and no other."""
+    T, H, G, D, R, bs, nb = 21, 8, 2, 64, 32, 16, 5
+    g = torch.Generator().manual_seed(31)
+    q, k, v = (torch.randn(T, n, D, generator=g).bfloat16() for n in (H, G, G))
+    qw, kw = torch.randn(D, generator=g), torch.randn(D, generator=g)
+    ang = torch.arange(100).double().view(-1, 1) * 10000.0 ** (-torch.arange(0, R, 2).double() / R)
+    cos, sin = ang.cos().float(), ang.sin().float()
+    pos = torch.randint(0, 100, (T,), generator=g).to(torch.int32)
+    slots = torch.randperm(nb * bs, generator=g)[:T].to(torch.int32)
+    pos[1], slots[4], slots[5] = -1, -1, nb * bs
+    kc0, vc0 = torch.randn(nb, bs, G, D, generator=g).bfloat16(), torch.randn(nb, bs, G, D, generator=g).bfloat16()
+    kc, vc = kc0.clone().to(dev), vc0.clone().to(dev)
+    a = [t.to(dev) for t in (q, k, v, qw, kw)]
+    p, c, s, sl = (t.to(dev) for t in (pos, cos, sin, slots))
+    if route == "native":
+        qo = dsa.qk_norm_rope_paged(*a, p, c, s, kc, vc, sl, interleaved=interleaved)
+    elif route == "64-bit":
+        qo = dsa.qk_norm_rope_paged(*a, p.long(), c, s, kc, vc, sl.long(), interleaved=interleaved)
+    else:
+        qo = dsa.load_torch_ops().qk_norm_rope_paged(*a, p, c, s, kc, vc, sl, 1e-6, interleaved)
+    u = ref.half_step(torch.bfloat16)
+    within = lambda got, want, tol, what: ref.assert_within(got, want, tol + u * (want.abs() + tol), what)
+    within(qo, *ref.norm_rope(q, qw, pos, cos, sin, interleaved=interleaved), "queries")
+    wk, tol = ref.norm_rope(k, kw, pos, cos, sin, interleaved=interleaved)
+    live = [t for t in range(T) if t not in (1, 4, 5)]
+    at = slots[live].long()
+    got_k, got_v = kc.cpu().view(-1, G, D), vc.cpu().view(-1, G, D)
+    assert (got_k[at] != kc0.view(-1, G, D)[at]).flatten(1).any(1).all()
+    within(got_k[at], wk[live], tol[live], "keys")
+    assert torch.equal(got_v[at], v[live])
+    rest = torch.ones(nb * bs, dtype=torch.bool)
+    rest[at] = False
+    assert torch.equal(got_k[rest], kc0.view(-1, G, D)[rest]) and torch.equal(got_v[rest], vc0.view(-1, G, D)[rest])
