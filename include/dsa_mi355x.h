@@ -390,6 +390,7 @@ int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_
  * and v may be parts of one projection's output).  Weights [D] fp32 or of `kind`, or NULL (ones).
  * slots NULL: k_out [T, G, D].  Else k_out and v_out are caches of cache_rows rows [G, D]: token t's keys and
  * values (v unchanged) go to row slots[t]; slots outside [0, cache_rows) write nothing; slots in it must differ.
+ * With cache_rows 0 the caches may be NULL.
  * A position outside [0, table_len) marks padding: q_out and k_out rows of zeros, nothing to a cache.
  * bf16 or fp16; D a multiple of 8 up to 512, R a multiple of 16 up to D; rows start on 16 bytes.
  */

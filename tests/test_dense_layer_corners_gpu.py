@@ -183,3 +183,15 @@ def test_each_route_writes_the_cache_rows(dsa, dev, route, interleaved):
     rest = torch.ones(nb * bs, dtype=torch.bool)
     rest[at] = False
     assert torch.equal(got_k[rest], kc0.view(-1, G, D)[rest]) and torch.equal(got_v[rest], vc0.view(-1, G, D)[rest])
+
+
+def test_caches_without_rows(dsa, dev):
+    """Every slot lies outside a cache of no blocks: nothing is written, the queries come back."""
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(3, 2, 16, generator=g).bfloat16().to(dev)
+    pos = torch.arange(3, dtype=torch.int32, device=dev)
+    cos, sin = torch.rand(8, 8, generator=g).to(dev), torch.rand(8, 8, generator=g).to(dev)
+    want, _ = dsa.qk_norm_rope(q, q, None, None, pos, cos, sin)
+    kc, vc = (torch.empty(0, 16, 2, 16, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    for f in (dsa.qk_norm_rope_paged, dsa.load_torch_ops().qk_norm_rope_paged):
+        assert torch.equal(f(q, q, q, None, None, pos, cos, sin, kc, vc, pos), want)

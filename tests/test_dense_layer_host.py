@@ -122,3 +122,11 @@ def test_prefix_sums_on_the_host_do_not_decrease(dsa, sums):
         call(sums)
     with pytest.raises(ValueError, match="HIP"):  # the next check: host tensors
         call([3, 3])
+
+
+def test_norms_need_caches_only_for_rows(dsa):
+    """Null caches are refused where they have rows."""
+    lib = dsa.load_library()
+    call = lambda rows: lib.dsa_qk_norm_rope(1, 16, 128, 16, 128, 16, 128, None, None, 1, 16, 16, 16, 8, 4, 1, 1, 64, 64,
+                                             1e-6, 0, 16, rows, 16, None, None, None)
+    assert call(8) == 1 and b"null" in lib.dsa_last_error_message()

@@ -597,7 +597,7 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
   if (T * (H + G) == 0) return 0;
   const bool paged = slots != nullptr;
   if (!positions || (R > 0 && table_len > 0 && (!cos || !sin)) || (H > 0 && (!q || !q_out)) ||
-      (G > 0 && (!k || !k_out || (paged && (!v || !v_out)))))
+      (G > 0 && (!k || (paged ? !v || (cache_rows > 0 && (!k_out || !v_out)) : !k_out))))
     return reject("qk_norm_rope: null pointer");
   if (q_stride % 8 != 0 || k_stride % 8 != 0 || (paged && v_stride % 8 != 0) || q_stride < 0 || k_stride < 0 ||
       (paged && v_stride < 0))
