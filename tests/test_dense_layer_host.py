@@ -130,3 +130,21 @@ def test_norms_need_caches_only_for_rows(dsa):
     call = lambda rows: lib.dsa_qk_norm_rope(1, 16, 128, 16, 128, 16, 128, None, None, 1, 16, 16, 16, 8, 4, 1, 1, 64, 64,
                                              1e-6, 0, 16, rows, 16, None, None, None)
     assert call(8) == 1 and b"null" in lib.dsa_last_error_message()
+
+
+def test_grids_past_32_bits_of_threads_are_refused(dsa):
+    """Sizes within every other bound whose launch would pass 2^32 threads."""
+    lib = dsa.load_library()
+    refused = lambda rc: rc == 1 and b"range" in lib.dsa_last_error_message()
+    qmm = lambda M, N, K, x=16, ws=None, n=0: lib.dsa_quant_matmul(1, x, 16, 16, 16, None, M, N, K, 16, ws, n, None)
+    assert refused(qmm(1, 2**27 + 16, 16))  # 16 channels a workgroup of 512
+    assert refused(qmm(2**26, 32, 17, ws=16, n=2**62))  # copies, a wave a row
+    assert refused(qmm(2**26, 32, 16, x=24, ws=16, n=2**62))
+    rope = lambda T, H, D: lib.dsa_qk_norm_rope(1, 16, H * D, 16, H * D, None, 0, None, None, 1, 16, 16, 16, 8, T, H, 0, D, 0,
+                                                1e-6, 0, None, 0, 16, 16, None, None)
+    assert refused(rope(2**24, 127, 512))
+    # Decode tiles of 256 threads: a slot for each of 65535 sequences and their rows, in each of 1024 groups.
+    attn = lambda T, B, H, G: lib.dsa_paged_gqa_fwd(1, 16, 16, 16, 16, 16, None, 16, T, B, 0, H, G, 64, 4, 16, 2, 1, -1, None,
+                                                    1.0, 16, 16, 16, 2**62, None)
+    assert refused(attn(2**15, 65535, 4096, 4096))
+    assert lib.dsa_paged_gqa_workspace_size(2**15, 65535, 4096, 4096, 64, 32) == 0

@@ -58,6 +58,9 @@ hipError_t launch_qk_norm_rope(int is_fp16, const void* q, int64_t q_stride, con
                                int64_t T, int64_t H, int64_t G, int64_t D, int64_t R, float eps, int interleaved,
                                const int32_t* slots, int64_t rows, void* q_out, void* k_out, void* v_out,
                                hipStream_t stream);
+bool quant_matmul_fits(int64_t M, int64_t N, int64_t K, bool aligned);
+bool qk_norm_rope_fits(int64_t T, int64_t heads, int64_t D);
+bool paged_gqa_fits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most);
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most);
 hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
                             const int32_t* cu_q, const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B,
@@ -553,7 +556,7 @@ int dsa_sparse_attn_sink(int kind, const void* q, const void* kv, const int32_t*
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 static int check_quant_matmul(int64_t M, int64_t N, int64_t K) {
-  // int32 sums of products of at most 2^14; a grid of 128 x 128 tiles.
+  // int32 sums of products of at most 2^14.
   if (M < 0 || N < 0 || M > kMaxInt - 4096 || N > kMaxInt - 4096) return reject("quant_matmul: bad M / N");
   if (K < 1 || K > 131071) return reject("quant_matmul: K must be in [1, 131071]");
   if (((M + 127) / 128) * ((N + 127) / 128) > kMaxInt || (M + N) * K > ((int64_t)1 << 42))
@@ -572,6 +575,8 @@ int dsa_quant_matmul(int out_kind, const void* x, const void* w, const float* x_
   if (out_kind != DSA_KIND_BF16 && out_kind != DSA_KIND_FP16 && out_kind != DSA_KIND_FP32)
     return reject("quant_matmul: output kind must be bf16, fp16 or fp32");
   if (const int rc = check_quant_matmul(M, N, K)) return rc;
+  if (M > 0 && N > 0 && !dsa::quant_matmul_fits(M, N, K, aligned16(x) && aligned16(w)))
+    return reject("quant_matmul: sizes out of range");
   if (M > 0 && N > 0 && (!x || !w || !x_scale || !w_scale || !out)) return reject("quant_matmul: null pointer");
   const size_t need = dsa_quant_matmul_workspace_size(M, N, K, aligned16(x) && aligned16(w));
   if (workspace_bytes < need) return reject("quant_matmul: workspace too small");
@@ -596,6 +601,7 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
   if (!(eps >= 0.f)) return reject("qk_norm_rope: eps must not be negative");
   if (T * (H + G) == 0) return 0;
   const bool paged = slots != nullptr;
+  if (!dsa::qk_norm_rope_fits(T, H + (paged ? 2 : 1) * G, D)) return reject("qk_norm_rope: sizes out of range");
   if (!positions || (R > 0 && table_len > 0 && (!cos || !sin)) || (H > 0 && (!q || !q_out)) ||
       (G > 0 && (!k || (paged ? !v || (cache_rows > 0 && (!k_out || !v_out)) : !k_out))))
     return reject("qk_norm_rope: null pointer");
@@ -615,8 +621,8 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
 // Sizes that both the workspace query and the call need in range.
 static bool paged_gqa_sizes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
   return T >= 0 && B >= 1 && B <= 65535 && H >= 1 && G >= 1 && H % G == 0 && G <= 65535 && T <= kMaxInt &&
-         H <= 65535 && T * H <= kMaxInt - 65536 && (T * (H / G) / 16 + B + 1) * G <= kMaxInt &&  // a grid of tiles
-         (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096;
+         H <= 65535 && T * H <= kMaxInt - 65536 && (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096 &&
+         dsa::paged_gqa_fits(T, B, H, G, most);
 }
 
 size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {

@@ -168,16 +168,25 @@ static void nr_launch_rows(const NormRopeArgs& a, hipStream_t stream) {
 }
 
 // Four heads a group where 2048 workgroups are left, one otherwise.
+static bool nr_many(int64_t T, int64_t heads, int lanes) { return T * heads * lanes >= (int64_t)2048 * 256 * 4; }
+
+// The grid lies within the 2^32 threads of a launch; `heads`: rows of a token.
+bool qk_norm_rope_fits(int64_t T, int64_t heads, int64_t D) {
+  const int lanes = D <= 64 ? 8 : D <= 128 ? 16 : D <= 256 ? 32 : 64;
+  const int64_t sets = T * (nr_many(T, heads, lanes) ? (heads + 3) / 4 : heads);
+  return sets * lanes <= ((int64_t)1 << 32) - 512;
+}
+
 template <bool kF16, int kL>
 static hipError_t nr_launch(const NormRopeArgs& a, bool pairs, hipStream_t stream) {
-  const bool many = (int64_t)a.T * a.heads * kL >= (int64_t)2048 * 256 * 4;
+  const bool many = nr_many(a.T, a.heads, kL);
   if (pairs) many ? nr_launch_rows<kF16, kL, true, 4>(a, stream) : nr_launch_rows<kF16, kL, true, 1>(a, stream);
   else many ? nr_launch_rows<kF16, kL, false, 4>(a, stream) : nr_launch_rows<kF16, kL, false, 1>(a, stream);
   return hipGetLastError();
 }
 
 // Caller validated: D a multiple of 8 in [8, 512], R a multiple of 16 in [0, D], strides multiples of 8, 16-byte
-// aligned pointers, T * (H + 2 G) < 2^31.
+// aligned pointers, T * (H + 2 G) < 2^31, qk_norm_rope_fits.
 template <bool kF16>
 static hipError_t nr_dispatch(const NormRopeArgs& a, bool pairs, hipStream_t stream) {
   const int chunks = a.D / 8;

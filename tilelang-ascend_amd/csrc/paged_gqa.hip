@@ -1306,6 +1306,13 @@ static PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) 
   return p;
 }
 
+// The largest grid, of tiles in each group, within the 2^32 threads of a launch (the shared line's and the join's are
+// smaller).  T * H < 2^31, B, G <= 65535.
+bool paged_gqa_fits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) {
+  const PgPlan p = pg_plan(T, B, H, G, most);
+  return p.slots * G < ((int64_t)1 << 32) / (p.rows == kPrRows ? kPrThreads : kPgThreads);
+}
+
 static size_t pg_part_bytes(const PgPlan& p, int64_t D) { return (size_t)(2 * p.wgs) * p.rows * (D + 2) * sizeof(float); }
 
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
@@ -1343,7 +1350,7 @@ static hipError_t pg_dispatch(const PgArgs& a, int rows, hipStream_t stream) {
 }
 
 // Caller validated: D in {64, 128}, H a multiple of G, T * H < 2^31 - 65536, pool rows < 2^31,
-// max_blocks * block_size <= 2^31 - 1 - 4096, (T * H / 16 + B + 1) * G < 2^31, sm_scale > 0, the workspace as
+// max_blocks * block_size <= 2^31 - 1 - 4096, paged_gqa_fits, sm_scale > 0, the workspace as
 // paged_gqa_workspace_bytes says.
 hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
                             const int32_t* cu_q, const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B,

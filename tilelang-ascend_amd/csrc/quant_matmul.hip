@@ -453,6 +453,17 @@ static bool qmm_odd_rows(const void* x, const void* w, int64_t K) {
   return K % 16 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) != 0;
 }
 
+// The largest grid within the 2^32 threads of a launch: 16 channels or a tile a workgroup, the copies a row a wave (a
+// join's is smaller than its tiles').
+bool quant_matmul_fits(int64_t M, int64_t N, int64_t K, bool aligned) {
+  const QmmPlan p = qmm_plan(M, N, K, !aligned || K % 16 != 0);
+  const int64_t most = ((int64_t)1 << 32) - 1024;
+  if (p.tile == 16) return (N + 15) / 16 * kQmmRowWaves * kWave <= most;
+  if (p.pack && (M + N) * kWave > most) return false;
+  const int64_t bm = p.tile, bn = p.tile == 256 ? 256 : 128, threads = p.tile == 256 ? 512 : p.tile == 32 ? 128 : 256;
+  return ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * threads <= most;
+}
+
 // `aligned`: the operands start on 16 bytes.
 size_t quant_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K, bool aligned) {
   const QmmPlan p = qmm_plan(M, N, K, !aligned || K % 16 != 0);
@@ -515,7 +526,7 @@ static hipError_t qmm_launch(QmmArgs a, void* workspace, hipStream_t stream) {
   }
 }
 
-// Caller validated: 1 <= K <= 131071, M and N within the grids, out_kind in {bf16, fp16, fp32}, a workspace of
+// Caller validated: 1 <= K <= 131071, quant_matmul_fits, out_kind in {bf16, fp16, fp32}, a workspace of
 // quant_matmul_workspace_bytes.
 hipError_t launch_quant_matmul(int out_kind, const void* x, const void* w, const float* sx, const float* sw,
                                const float* bias, int64_t M, int64_t N, int64_t K, void* out, void* workspace,
