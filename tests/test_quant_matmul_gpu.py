@@ -153,3 +153,27 @@ def test_refusals(dsa, dev):
     with pytest.raises(ValueError, match="K must be"):
         dsa.quant_matmul(torch.zeros(1, 131072, dtype=torch.int8, device=dev),
                          torch.zeros(1, 131072, dtype=torch.int8, device=dev), s[:1], s[:1])
+
+
+def test_fewer_tokens_take_no_longer(dsa, dev):
+    """128 tokens of a wide product are half the work of 256: they must not be put into tiles that they half fill."""
+    N, K = 32768, 4096
+    g = torch.Generator(device=dev).manual_seed(5)
+    x = torch.randint(-127, 128, (256, K), dtype=torch.int8, device=dev, generator=g)
+    w = torch.randint(-127, 128, (N, K), dtype=torch.int8, device=dev, generator=g)
+    xs, ws = torch.rand(256, device=dev, generator=g), torch.rand(N, device=dev, generator=g)
+
+    def us(M):
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                dsa.quant_matmul(x[:M], w, xs[:M], ws)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 100)
+        return sorted(times)[2]
+
+    half, all_ = us(128), us(256)
+    assert half < 1.1 * all_, f"128 tokens {half:.0f} us, 256 {all_:.0f}"

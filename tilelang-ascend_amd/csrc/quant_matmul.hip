@@ -427,11 +427,13 @@ static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
   p.tile = M <= 32 ? 32 : M <= 64 ? 64 : 128;
   const int64_t small = ((M + p.tile - 1) / p.tile) * ((N + 127) / 128);
   const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-  // The larger tile multiplies 1.2 times as fast (8192^3: 1932 against 1595 TOP/s) where the rounds of 256
-  // workgroups it makes are as full as the rounds of 512 of the smaller one.
-  const double full_big = (double)big / (double)((big + 255) / 256 * 256);
-  const double full_small = (double)small / (double)((small + 511) / 512 * 512);
-  if (p.tile == 128 && full_big > 0.82 * full_small && big >= 128) {
+  // The larger tile multiplies 1.2 times as fast (8192^3: 1932 against 1595 TOP/s); a round of 256 of them takes what
+  // two rounds of 512 of the smaller one would at one speed.  Rounds count the rows past M that a tile multiplies too.
+  // Smaller and larger tile, us: with K = 4096, 128 x 32768 41 and 69, 128 x 131072 148 and 172, 300 x 32768 87 and 77,
+  // 300 x 131072 298 and 304, 520 x 32768 128 and 137, 6144 x 6144 196 and 208 (the one of these that the rule misses);
+  // with K = 7168, 1100 x 9216 126 and 107, 2100 x 9216 193 and 209, 4096 x 9216 372 and 342.
+  const int64_t rounds_big = (big + 255) / 256, rounds_small = (small + 511) / 512;
+  if (p.tile == 128 && 0.82 * 2 * (double)rounds_big < (double)rounds_small) {
     p.tile = 256;
     return p;
   }
