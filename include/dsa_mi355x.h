@@ -410,7 +410,8 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
  *  [B, max_blocks]; query heads g*H/G .. read KV head g; sinks [H] fp32 (natural-log units) or NULL, added to
  *  the denominator; out [T, H, D]; lse [T, H] fp32, natural log, sink included.  Rows that see nothing (padding
  *  rows, rows behind cu_q[B - 1] too) get out = 0 and lse = -inf (or the sink).  Keys that a row does not see do
- *  not reach it, whatever their pages hold.  Lengths are read on the device and cut to what the table and q hold.
+ *  not reach it, whatever their pages hold; a value that it sees and that is not finite makes its column infinite or
+ *  NaN (NaN where its weight rounds to 0).  Lengths are read on the device and cut to what the table and q hold.
  *  cu_q must not decrease (a sequence without new tokens repeats the sum before it): nothing out of range is read or
  *  written where it does, but rows of out and lse are then undefined.
  *  max_keys of the workspace query is max_blocks * block_size.

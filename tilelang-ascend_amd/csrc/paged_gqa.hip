@@ -111,7 +111,8 @@ __device__ __forceinline__ int pg_block(const PgArgs& a, int j) {
 // Values that a row does not see must not reach it, whatever they hold, but 0 times an infinity or a NaN is a NaN in
 // the product of probabilities and V.  So tiles that some row sees in part are searched for such values (unseen
 // ones of other tiles do not exist); where there are any, the product takes zeros in their place, and rows that do
-// see them get them added by hand.
+// see them get them added by hand.  In tiles that all rows see whole the product takes them as they are: an infinity
+// whose weight rounds to 0 gives NaN there and an infinity here, neither of them finite.
 // Of a pair of 16-bit values: bit 15 (and 31) set where the value is infinite or NaN: the exponent's ones plus one.
 template <bool kF16>
 __device__ __forceinline__ uint32_t pg_not_finite(uint32_t w) {

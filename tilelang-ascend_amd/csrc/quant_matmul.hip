@@ -419,8 +419,10 @@ static int64_t qmm_ld(int64_t K) { return (K + 127) / 128 * 128; }
 // `odd`: rows do not start on 16 bytes or hold no whole number of chunks.
 static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
   QmmPlan p = {16, false, 1, false, 0, 0};
-  // Up to 16 tokens every workgroup reads all of x beside its 16 rows of w: one token of 9216 x 7168 takes 15.6 us
-  // (19.7 with split tiles), 16 tokens 21.6 (20.5); 32 tokens 33 against 20.7, 64 (7168 x 8192) 28.8 against 18.0.
+  // Up to 16 tokens every workgroup reads all of x beside its 16 rows of w.  Rows and (shared) tiles, us: one token of
+  // 9216 x 7168 15.5 and 19.2, of 4096 x 4096 5.7 and 9.5; 16 tokens of 4096 x 7168 8.5 and 12.0, of 8192 x 4096 9.8 and
+  // 11.8, but of 9216 x 7168 21.8 and 20.1, of 7168 x 8192 18.4 and 16.1: from 12 tokens on tiles are up to 3 us ahead
+  // where the weights come from memory, as much behind where a cache holds them.  Past 16 this kernel has no form.
   if (M <= 16) return p;
   p.pack = odd;
   if (odd) p.pack_bytes = (size_t)((M + N) * qmm_ld(K));
@@ -439,8 +441,16 @@ static QmmPlan qmm_plan(int64_t M, int64_t N, int64_t K, bool odd) {
   }
   // Few tiles share their K, eight steps each at least, up to about one workgroup a CU: with up to two, what the
   // join reads costs more (64 tokens of 7168 x 8192: 22.0 us instead of 18.0; 512: 57.2 instead of 51).  More than
-  // half as many tiles of 128 as CUs share a long K by three, two workgroups a CU (1021 x 2113 x 4099: 39.7 us with one,
-  // 37.6 with two, 35.8 with three; 1024 x 2112 x 7168: 41.4, 40.5, 35.6; 1280 x 1920 x 4096: 27.8, 31.0, 29.1).
+  // half as many tiles of 128 as CUs, and at most 170, whose three shares fill two workgroups a CU, share a long K by
+  // three.  Aligned rows, us with one share and with three, by steps of K:
+  //   tiles                20          32          33          36          40          56          72
+  //   136 (1024 x 2112)    21.1 24.8   28.0 27.3   30.3 27.7   29.4 27.1   33.5 29.6   41.0 35.1   52.0 39.5
+  //   154 (1408 x 1792)    22.2 25.8   28.7 30.2   28.3 27.7   29.5 28.3   34.4 31.7   41.8 37.3   52.5 43.0
+  //   169 (1664 x 1664)    22.4 27.6   29.2 31.4   28.2 28.6   29.7 29.5   35.0 32.9   42.8 38.6   53.7 44.6
+  //   170 (256 x 10880)    22.3 30.1   30.4 34.3   30.4 32.1   32.0 33.2   37.9 39.5   45.0 44.4   55.9 51.4
+  // so the sides cross between 31 steps (fewest tiles) and 38 (most); the wide product of two rows of tiles, bound by its
+  // weights, crosses at 56.  Copied rows gain from about 20 steps on but for such wide ones (136 tiles, 27 steps: 33.5 and
+  // 30.5; 169: 34.8 and 33.0; 170, 256 x 10880: 44.5 and 47.2); they keep to the same bound.
   const int64_t steps = (K + kQmmStep - 1) / kQmmStep;
   if (p.tile == 128 && small > 128 && small <= 170 && steps > 32) p.splits = 3;
   else

@@ -34,7 +34,8 @@ def paged_gqa_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     j <= p (``is_causal``) and j >= p - win_left (``win_left`` None: all).  ``sinks`` [H] fp32 adds exp(sink) to
     each head's denominator.  sm_scale defaults to D^-0.5.  Rows that see nothing -- padding rows, rows behind the
     last packed sequence -- give out = 0 and lse = -inf (or the sink).  A table entry outside the pool hides its keys.
-    Keys that a row does not see do not reach it, whatever the caches hold there (infinities and NaN too).  Lengths
+    Keys that a row does not see do not reach it, whatever the caches hold there (infinities and NaN too); a value
+    that it does see and that is not finite makes its column infinite or NaN (NaN where its weight rounds to 0).  Lengths
     stay on the device and are cut to what the table and q hold.  Prefix sums must not decrease (a sequence without
     new tokens repeats the one before it): on the host that is checked; on the device sums that do decrease leave
     rows of out and lse undefined.
