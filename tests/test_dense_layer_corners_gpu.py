@@ -1,5 +1,6 @@
 """Corners of the dense layer's operators on the GPU: wide integers, sinks, padding, other routes, threads, devices."""
 import math
+import threading
 
 import pytest
 import torch
@@ -195,3 +196,50 @@ def test_caches_without_rows(dsa, dev):
     kc, vc = (torch.empty(0, 16, 2, 16, dtype=torch.bfloat16, device=dev) for _ in range(2))
     for f in (dsa.qk_norm_rope_paged, dsa.load_torch_ops().qk_norm_rope_paged):
         assert torch.equal(f(q, q, q, None, None, pos, cos, sin, kc, vc, pos), want)
+
+
+def _step(dsa, dev, seed):
+    """A projection and an attention call of their own inputs."""
+    g = torch.Generator().manual_seed(seed)
+    x, w = (torch.randint(-127, 128, s, dtype=torch.int8, generator=g).to(dev) for s in ((40, 260), (300, 260)))
+    xs, ws = torch.rand(40, generator=g).to(dev), torch.rand(300, generator=g).to(dev)
+    seqs = [(1, 900), (33, 400 + seed), (1, 10)]
+    args = [t.to(dev) for t in _setup(seqs, 16, 2, 128, 64, torch.bfloat16, seed=seed)]
+    return lambda: (dsa.quant_matmul(x, w, xs, ws), *_run(dsa, dev, seqs, *args))
+
+
+def test_calls_from_several_threads(dsa, dev):
+    """Threads with streams of their own, calls at once: each gives what it gives alone."""
+    steps = [_step(dsa, dev, i) for i in range(4)]
+    want = [s() for s in steps]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in steps], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i].append(steps[i]())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # pragma: no cover - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(steps))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(len(steps)):
+        assert len(got[i]) == 10
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
+
+
+def test_another_device_than_the_current_one(dsa, dev):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device here")
+    want = _step(dsa, dev, 1)()
+    with torch.cuda.device(0):
+        got = _step(dsa, torch.device("cuda:1"), 1)()
+    assert all(b.device.index == 1 and torch.equal(a.cpu(), b.cpu()) for a, b in zip(want, got))
