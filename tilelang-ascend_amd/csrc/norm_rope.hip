@@ -10,7 +10,7 @@
 // A head's row is held by a group of kL lanes, 8 elements (16 bytes) a lane, as many lanes as the row has chunks
 // (rounded up to a power of two), so a 256-byte row takes 16 lanes and a wave works on four tokens' rows at once.  A
 // group takes kRows heads of one token, whose loads all go out before the first is used and which share the token's
-// angles (32768 tokens of 72 rows of 128: 492 us with a head a group, 218 with four, 5.6 TB/s).  The partner of an
+// angles (32768 tokens of 72 rows of 128: 492 us with a head a group, 222 with four, 5.5 TB/s).  The partner of an
 // element of the first form lies R/2 elements away: R/16 lanes, one shuffle an element.
 #include "common.hpp"
 

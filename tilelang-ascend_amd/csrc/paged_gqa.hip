@@ -28,8 +28,9 @@
 // second launch joins.
 //
 // S^T = K Q^T with keys on the M axis, so that a lane holds many scores of one row; softmax in base 2; O^T += V^T P^T
-// with V^T through transposing LDS reads.  Probabilities are rounded to the caches' 16 bits for that product, the sum
-// of them is taken before the rounding, in fp32, as maxima and all sums are.
+// with V^T through transposing LDS reads.  Probabilities are rounded to the caches' 16 bits for that product, whose matrix
+// instructions take them so (bf16 outputs: 0.0019 to 0.0024 off where an fp32 form rounded once has 0.0015 to 0.0017); the
+// sum of them is taken before the rounding, in fp32, as maxima and all sums are.
 #include <type_traits>
 
 #include "gqa_common.hpp"
@@ -154,8 +155,8 @@ __device__ __forceinline__ PgEnd pg_end(float m, float l, float sink) {
 
 // The keys [k0, k1) of tile `tile` of sequence s, group kvg; `whole`: these are all its keys (the result goes to
 // out and lse, otherwise to the part).  Two stages of K and V of 32 keys a wave; the merge reuses a wave's ring, its
-// (maximum, sum) lie behind.  Bound by the caches' bytes: 64 tokens over 8192 keys each, 64 heads over 4 of 128: 201 us,
-// 5.4 TB/s; one token over 4097: 9 us and the join's 7, latencies.
+// (maximum, sum) lie behind.  Bound by the caches' bytes: 64 tokens over 8192 keys each, 64 heads over 4 of 128: 200 us,
+// 5.4 TB/s; one token over 4097: 9 us and the join's 6, latencies.
 template <bool kF16, int kD, int kHB>
 __device__ __forceinline__ void pg_keys(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,
                                         bool whole, float* part, uint8_t* lds) {
@@ -496,7 +497,8 @@ constexpr int kPrTile = 64;             // keys
 // C(t) and X(t), waves 4 to 7 X(t - 1) and C(t).  Those read K(t), K(t + 1), V(t - 1) and V(t), whole by the wait at
 // the end of C(t - 1) and the barrier behind it, and the DMA of C(t) goes to K(t - 1) and V(t - 2), last read before
 // that barrier.  16K prompts, 64 heads over 4: 2697 -> 2593 us; 128-wide heads 3970 -> 4152; both halves in phase: 4409.
-// 128-wide heads reach 1135 TFLOP/s there (3875 us); 512 tokens over 65536 keys 1009 us, 1086.  A tile's LDS reads (64 +
+// 128-wide heads reach 1123 TFLOP/s there (3915 us, 3875 to 4010 by card); 512 tokens over 65536 keys 1038 us, 1055;
+// 64-wide heads 878 at the prompt (2504 us).  A tile's LDS reads (64 +
 // 64 KB by eight waves) take about 70% of a body's time.
 template <bool kF16, int kD, bool kEven>
 __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, int tile, int kvg, int k0, int k1,

@@ -61,7 +61,7 @@ __device__ __forceinline__ float qmm_value(const QmmArgs& a, int sum, int n, flo
 // waves share the rows' bytes, 128 of each row at a time, and load straight into the product's operands, four such
 // units ahead (two: 16 tokens of 9216 x 7168 took 23.6 us instead of 21.6; eight: 24.1): nothing is shared between
 // waves but the sums, joined through LDS.  Rows may start at any byte; the unit that K ends in is read by chunks that
-// are cut there.  One token of 9216 x 7168: 15.6 us, 4.2 TB/s.
+// are cut there.  One token of 9216 x 7168: 14.2 us, 4.7 TB/s (back to back, 15.5 over weights that no cache holds).
 constexpr int kQmmRowWaves = 8;
 constexpr int kQmmUnit = 128;
 constexpr int kQmmDeep = 4;
@@ -147,8 +147,8 @@ __global__ __launch_bounds__(kQmmRowWaves * kWave) void qmm_rows_kernel(QmmArgs 
 // products, channels on the M axis).  Chunk c (16 bytes) of row r lies at c ^ ((r >> 2) & 7), so that the 32 rows
 // a half wave reads at one c fall on distinct banks; the DMA fetches the chunks in that order.  Rows start on 16
 // bytes and hold whole chunks (qmm_pack_kernel sees to it where they do not); chunks past K come from a row of zeros.
-// 16384 x 9216 x 7168: 1051 us, 2060 TOP/s; the DMA alone takes 836 us there, the LDS reads 495, and the matrix cores
-// reach 3200 to 3700 on random operands (clock), a library's 8192^3 2089.
+// 16384 x 9216 x 7168: 1042 us (1016 to 1064 by card), 2078 TOP/s; the DMA alone takes 836 us there, the LDS reads 495,
+// and the matrix cores reach 3200 to 3700 on random operands (clock); a library 2360 at 8192^3, 2413 at 16384^3.
 // With kSplit the steps are dealt to gridDim.z workgroups, which leave int32 sums for qmm_join_kernel.
 // Whole lines of a row: with 64 bytes (and four stages) 16384 x 9216 x 7168 took 1120 us, 1089 with 128.
 constexpr int kQmmStep = 128;
