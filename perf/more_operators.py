@@ -1,0 +1,574 @@
+"""Measured calls of a decoding step over a tree of drafted tokens, through the public entry points.
+
+A serving step that checks several drafted continuations at once: pages, slots, positions and the tree's masks are made on
+the GPU from request lengths (``paged_plan``, undone by ``paged_free``), each drafted token attends to the paged cache and
+to its ancestors (``paged_tree_fwd``), the model's choices are followed through the tree (``tree_accept``) and the cache
+rows of the accepted tokens are put in order (``paged_commit``).  ``own`` false: ``run`` computes the operators in elementary
+torch operations in 32 bits; ``own`` true: it calls the package.  ``exact`` is the definition, in 64 bits where it computes.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+_DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+_SIZE = {"bf16": 2, "fp16": 2, "fp32": 4}
+
+
+def listed():
+    return [
+        # The smallest plan: a decode step of 8 sequences, a token each, no tree.
+        dict(name="plan_decode", kind="plan", lens="8x1:8191", block=64, max_blocks=256, tree=False, win=-1),
+        # A step of 64 sequences with drafted trees of 1 to 61 nodes, and some without any new token.
+        dict(name="plan_tree", kind="plan", lens="13x61:8190 20x24:5001 20x7:12345 8x1:77 3x0:640", block=64,
+             max_blocks=256, tree=True, win=-1),
+        # Whole prompts and chunks beside each other, small pages: the largest step.
+        dict(name="plan_prompts", kind="plan", lens="16384:0 1021:30011 1:9001 12001:17 2049:4096 1:0", block=16,
+             max_blocks=2048, tree=False, win=-1),
+        # The smallest attention call: a chain and a branch of 8 nodes of one sequence.
+        dict(name="tree_one", kind="attn", lens="8:4097", H=64, G=4, D=128, block=64, win=-1, sinks=False, dtype="bf16"),
+        # A serving step's mixed batch: single tokens, small and large trees, window of 1024 keys, sinks, odd lengths.
+        dict(name="tree_mixed", kind="attn", lens="4x1:7001 24:44444 7:123 127:257 61:9001 5:30001 1:0 13:0", H=64, G=8,
+             D=64, block=128, win=1023, sinks=True, dtype="fp16"),
+        # Few sequences of long contexts.
+        dict(name="tree_long", kind="attn", lens="4x64:65536", H=64, G=8, D=128, block=64, win=-1, sinks=False,
+             dtype="bf16"),
+        # A decode batch, trees of 61 nodes: the largest call.
+        dict(name="tree_batch", kind="attn", lens="32x61:8192", H=64, G=4, D=128, block=64, win=-1, sinks=False,
+             dtype="bf16"),
+        # A drafted chain of five for each of three sequences, a vocabulary of odd size kept in 32 bits.
+        dict(name="accept_chain", kind="accept", lens="3x5:0", V=50021, accept=3, dtype="fp32", scores=True),
+        # A decode batch's trees: scores of 3904 rows, of which about four a sequence lie on the path.
+        dict(name="accept_batch", kind="accept", lens="64x61:0", V=131072, accept=4, dtype="bf16", scores=True),
+        # One layer's cache of one sequence.
+        dict(name="commit_one", kind="commit", lens="8:4097", caches=2, row=512, block=64, accept=3, dtype="bf16"),
+        # All layers' caches of a batch.
+        dict(name="commit_layers", kind="commit", lens="64x61:60", caches=32, row=512, block=64, accept=5,
+             dtype="bf16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    """An integer spread over the logarithm of [lo, hi]."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def _lens(case):
+    """(new tokens, committed tokens) of each sequence, from "count x new:committed" words."""
+    out = []
+    for word in case["lens"].split():
+        times, _, pair = word.rpartition("x")
+        out += [tuple(int(n) for n in pair.split(":"))] * int(times or 1)
+    return out
+
+
+def _words(pairs):
+    return " ".join("%d:%d" % p for p in pairs)
+
+
+def draw(rng):
+    case = _draw(rng)
+    # No more than the largest listed case of its kind: sequences are left out, a single one is cut.
+    most = [work(c) for c in listed() if c["kind"] == case["kind"]]
+    while any(work(case)[k] > max(w[k] for w in most) for k in ("bytes", "flops")):
+        lens = _lens(case)
+        case["lens"] = _words(lens[:-1] if len(lens) > 1 else [(max(1, lens[0][0] // 2), lens[0][1] // 2)])
+    return case
+
+
+def _draw(rng):
+    kind = rng.choice(["plan", "attn", "attn", "accept", "commit"])
+    dt = rng.choice(["bf16", "bf16", "fp16"])
+    if kind == "plan":
+        tree = rng.random() < 0.6
+        block = rng.choice([16, 64, 128])
+        B = _log_int(rng, 1, 200)
+        most = min(200 if tree else 16384, 32000 // B)
+        pairs = [(0 if b > 0 and rng.random() < 0.1 else _log_int(rng, 1, most), _log_int(rng, 1, 16000) - 1)
+                 for b in range(B)]
+        return dict(kind="plan", lens=_words(pairs), block=block, max_blocks=32768 // block, tree=tree,
+                    win=rng.choice([-1, -1, 2, 40]) if tree else -1)
+    if kind == "attn":
+        G, D = rng.choice([1, 2, 4, 8]), rng.choice([64, 128, 128])
+        H = G * rng.choice([m for m in (1, 4, 5, 8, 16) if G * m <= 64])
+        B = _log_int(rng, 1, 32)
+        pairs = [(_log_int(rng, 1, rng.choice([8, 64, 150])), _log_int(rng, 1, 60000 // max(1, B // 4)) - 1)
+                 for _ in range(B)]
+        return dict(kind="attn", lens=_words(pairs), H=H, G=G, D=D, block=rng.choice([16, 64, 128]),
+                    win=rng.choice([-1, -1, -1, 127, 1023]), sinks=rng.random() < 0.3, dtype=dt)
+    B = _log_int(rng, 1, 64)
+    nodes = [_log_int(rng, 1, rng.choice([8, 61])) for _ in range(B)]
+    accept = rng.randint(2, 6)
+    if kind == "accept":
+        return dict(kind="accept", lens=_words([(s, 0) for s in nodes]), V=_log_int(rng, 1000, 131072), accept=accept,
+                    dtype=rng.choice([dt, "fp32"]), scores=rng.random() < 0.8)
+    block = rng.choice([16, 64, 128])
+    return dict(kind="commit", lens=_words([(s, rng.randint(0, 150)) for s in nodes]), caches=_log_int(rng, 1, 64),
+                row=rng.choice([576, 512, 512, 128]), block=block, accept=accept, dtype=rng.choice([dt, "fp32"]))
+
+
+# ------------------------------------------------------------------------------- inputs
+
+
+def _gen(seed):
+    dev = torch.device("cuda")
+    return dev, torch.Generator(device=dev).manual_seed(seed), random.Random(seed)
+
+
+def _normal(g, dev, shape, dtype, scale=1.0):
+    return torch.randn(shape, generator=g, device=dev, dtype=dtype).mul_(scale)
+
+
+def _i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def _parents(rng, S):
+    """A tree of S nodes, each behind its parent: node 0 the root, breadth and depth both growing with S."""
+    return [-1] + [rng.randint((i - 1) // 4, max((i - 1) // 4, (2 * i - 1) // 3)) for i in range(1, S)] if S else []
+
+
+def _ancestors(parents):
+    """For each node the list of itself and its ancestors, itself first."""
+    out = []
+    for i, p in enumerate(parents):
+        out.append([i] + (out[p] if 0 <= p < i else []))
+    return out
+
+
+def _mask_words(chains, W, win=-1):
+    """[nodes, W] int64: bit a of a node's row is set where a is the node or one of its ancestors (to win steps up)."""
+    bits = np.zeros((len(chains), W), dtype=np.uint64)
+    for i, chain in enumerate(chains):
+        for a in chain[:win + 1] if win >= 0 else chain:
+            bits[i, a // 64] |= np.uint64(1 << (a % 64))
+    return torch.from_numpy(bits.view(np.int64))
+
+
+def _path(rng, S, A):
+    """A nodes on the way down from the root, those behind it among the later nodes."""
+    A = max(1, min(A, (S + 1) // 2))
+    return [0] + sorted(rng.sample(range(A, S), A - 1))
+
+
+def prepare(case, seed):
+    dev, g, rng = _gen(seed)
+    c = dict(case)
+    lens = _lens(c)
+    B, T = len(lens), sum(s for s, _ in lens)
+    st = {"case": c}
+    if own:
+        from __graft_entry__ import load_package
+
+        st["pkg"] = load_package()
+        st["pkg"].load_library()
+    if c["kind"] == "plan":
+        bs, mb = c["block"], c["max_blocks"]
+        st["new"], st["ctx"] = _i32([s for s, _ in lens], dev), _i32([n for _, n in lens], dev)
+        held = [-(-n // bs) for _, n in lens]
+        fresh = [-(-(n + s) // bs) - h for (s, n), h in zip(lens, held)]
+        total = sum(held) + sum(fresh) + 37
+        order = torch.randperm(total, generator=g, device=dev).to(torch.int32)
+        st["table"] = torch.full((B, mb), -1, dtype=torch.int32, device=dev)
+        at = 0
+        for b, h in enumerate(held):
+            st["table"][b, :h] = order[at:at + h]
+            at += h
+        # The pages that no sequence holds are listed, the rest of the list is room for those that come back.
+        st["free"] = torch.full((total,), -1, dtype=torch.int32, device=dev)
+        st["free"][:total - at] = order[at:]
+        st["count"] = _i32([total - at], dev)
+        st["max_nodes"] = max([s for s, _ in lens] + [1])
+        st["parents"] = _i32([p for s, _ in lens for p in _parents(rng, s)], dev) if c["tree"] else None
+        st["T"] = T
+    elif c["kind"] == "attn":
+        dt = _DT[c["dtype"]]
+        G, H, D, bs = c["G"], c["H"], c["D"], c["block"]
+        nb = [-(-(s + n) // bs) for s, n in lens]
+        total = sum(nb) + 1
+        st["q"] = _normal(g, dev, (T, H, D), dt)
+        st["kc"] = _normal(g, dev, (total, bs, G, D), dt)
+        st["vc"] = _normal(g, dev, (total, bs, G, D), dt)
+        order = torch.randperm(total, generator=g, device=dev).to(torch.int32)
+        st["table"] = torch.zeros((B, max(nb)), dtype=torch.int32, device=dev)
+        at = 0
+        for b, n in enumerate(nb):
+            st["table"][b, :n] = order[at:at + n]
+            at += n
+        st["cu"] = torch.tensor([s for s, _ in lens], device=dev).cumsum(0).to(torch.int32)
+        st["kvl"] = _i32([s + n for s, n in lens], dev)
+        W = max(-(-s // 64) for s, _ in lens)
+        chains = [_ancestors(_parents(rng, s)) for s, _ in lens]
+        st["mask"] = torch.cat([_mask_words(x, W, c["win"]) for x in chains]).to(dev)
+        st["pos"] = _i32([n + len(x) - 1 for (_, n), seq in zip(lens, chains) for x in seq], dev)
+        st["sinks"] = _normal(g, dev, (H,), torch.float32) if c["sinks"] else None
+    elif c["kind"] == "accept":
+        V = c["V"]
+        st["cu"] = torch.tensor([s for s, _ in lens], device=dev).cumsum(0).to(torch.int32)
+        st["max_path"] = max([s for s, _ in lens] + [1])
+        parents, tokens, targets = [], [], []
+        for s, _ in lens:
+            par, path = _parents(rng, s), _path(rng, s, c["accept"])
+            tok, tgt = [rng.randrange(V) for _ in range(s)], [rng.randrange(V) for _ in range(s)]
+            for up, at in zip(path, path[1:]):  # the model agrees with the draft along the path
+                par[at], tgt[up] = up, tok[at]
+            parents += par
+            tokens += tok
+            targets += tgt
+        st["parents"], st["tokens"] = _i32(parents, dev), _i32(tokens, dev)
+        st["scores"] = _i32(targets, dev)
+        if c["scores"]:
+            x = _normal(g, dev, (T, V), _DT[c["dtype"]], 2.0)
+            st["scores"] = x.scatter_(1, st["scores"].long().view(-1, 1), 14.0)
+    else:
+        dt, bs = _DT[c["dtype"]], c["block"]
+        nb = [-(-(s + n) // bs) for s, n in lens]
+        total = sum(nb) + 1
+        wide = (total, bs, 1, c["row"])
+        st["caches"] = [_normal(g, dev, wide, dt) for _ in range(c["caches"])]
+        order = torch.randperm(total, generator=g, device=dev).to(torch.int32)
+        st["table"] = torch.full((B, max(nb) + 1), -1, dtype=torch.int32, device=dev)
+        at = 0
+        for b, n in enumerate(nb):
+            st["table"][b, :n] = order[at:at + n]
+            at += n
+        st["ctx"] = _i32([n for _, n in lens], dev)
+        # No row is both read and written: a pass repeated on the same caches leaves them as the first did.
+        paths = [_path(rng, s, c["accept"]) for s, _ in lens]
+        most = max(len(p) for p in paths)
+        st["path"] = _i32([p + [-1] * (most - len(p)) for p in paths], dev)
+        st["accepted"] = _i32([len(p) for p in paths], dev)
+    return st
+
+
+# ------------------------------------------------------------------------------- one pass
+
+
+def run(st):
+    kind = st["case"]["kind"]
+    if own:
+        return {"plan": _own_plan, "attn": _own_attn, "accept": _own_accept, "commit": _own_commit}[kind](st)
+    return {"plan": _plain_plan, "attn": _plain_attn, "accept": _plain_accept, "commit": _plain_commit}[kind](st)
+
+
+def _own_plan(st):
+    """A step's plan, and the pages handed back (nothing of the step was kept)."""
+    c, pkg = st["case"], st["pkg"]
+    more = dict(parents=st["parents"], max_nodes=st["max_nodes"]) if c["tree"] else {}
+    if c["win"] >= 0:
+        more["win_left"] = c["win"]
+    p = pkg.paged_plan(st["new"], st["ctx"], st["table"], st["free"], st["count"], c["block"], st["T"], **more)
+    pkg.paged_free(st["ctx"], st["table"], st["free"], st["count"], c["block"])
+    out = (p.cu_seqlens, p.kv_lens, p.positions, p.slots, p.missing, st["table"], st["free"], st["count"])
+    return out + ((p.tree_mask,) if c["tree"] else ())
+
+
+def _own_attn(st):
+    c, win = st["case"], st["case"]["win"]
+    more = dict(positions=st["pos"], win_left=win) if win >= 0 else {}
+    return st["pkg"].paged_tree_fwd(st["q"], st["kc"], st["vc"], st["table"], st["mask"],
+                                    actual_seq_lengths_query=st["cu"], actual_seq_lengths_kv=st["kvl"],
+                                    sinks=st["sinks"], **more)
+
+
+def _own_accept(st):
+    return st["pkg"].tree_accept(st["scores"], st["tokens"], st["parents"], actual_seq_lengths_query=st["cu"],
+                                 max_path=st["max_path"])
+
+
+def _own_commit(st):
+    st["pkg"].paged_commit(st["caches"], st["table"], st["ctx"], st["path"], st["accepted"])
+    return st["caches"]
+
+
+def _sequence_of_rows(cu, T):
+    """Sequence of each of T packed rows and the row's place in it."""
+    t = torch.arange(T, device=cu.device)
+    b = torch.searchsorted(cu.long(), t, right=True)
+    starts = torch.cat((cu.new_zeros(1), cu[:-1])).long()
+    return b, t - starts[b]
+
+
+def _plain_plan(st):
+    c = st["case"]
+    bs, T, table, free, count = c["block"], st["T"], st["table"], st["free"], st["count"]
+    new, ctx = st["new"].long(), st["ctx"].long()
+    dev = new.device
+    cu = new.cumsum(0)
+    block = torch.arange(table.shape[1], device=dev).view(1, -1)
+    touched = (block >= (ctx // bs).view(-1, 1)) & (block * bs < (ctx + new).view(-1, 1)) & (new > 0).view(-1, 1)
+    lack = touched & (table < 0)
+    rank = lack.view(-1).cumsum(0).view(lack.shape) - 1
+    take = lack & (rank < count)
+    page = free[(count - 1 - rank).clamp(min=0)]
+    table.copy_(torch.where(take, page, table))
+    missing = (lack & ~take).sum(dim=1)
+    count.copy_((count - lack.sum()).clamp(min=0))
+    b, i = _sequence_of_rows(cu, T)
+    depth = torch.zeros(T, dtype=torch.long, device=dev)
+    out = []
+    if c["tree"]:
+        W = -(-st["max_nodes"] // 64)
+        t = torch.arange(T, device=dev)
+        up = st["parents"].long()
+        has = (up >= 0) & (up < i)
+        node = torch.arange(64 * W, device=dev).view(1, -1)
+        sees, depth, at = node == i.view(-1, 1), has.long(), torch.where(has, t - i + up, t)
+        for _ in range((st["max_nodes"] - 1).bit_length()):  # twice as far up in each turn; a root points to itself
+            sees, depth, at = sees | sees[at], depth + depth[at], at[at]
+        if c["win"] >= 0:
+            far = depth.view(-1, 1) - depth[((t - i).view(-1, 1) + node).clamp(max=T - 1)]
+            sees = sees & (far <= c["win"])
+        out = [(sees.view(T, W, 64).long() << torch.arange(64, device=dev)).sum(dim=-1)]
+    key = ctx[b] + i
+    there = table[b, key // bs].long()
+    slots = torch.where(there >= 0, there * bs + key % bs, -1)
+    # The step's pages go back: in the order that undoes the plan.
+    keep = -(-ctx // bs)
+    held = (table < 0).int().argmax(dim=1)
+    held = torch.where((table < 0).any(dim=1), held, table.shape[1])
+    back = (block >= keep.view(-1, 1)) & (block < held.view(-1, 1))
+    n = back.sum()
+    order = n - back.view(-1).cumsum(0).view(back.shape)
+    room = torch.cat((free, free.new_zeros(1)))
+    room.scatter_(0, torch.where(back, count + order, free.numel()).view(-1).long(), table.view(-1))
+    free.copy_(room[:-1])
+    # A page that was handed out and came back lies where it lay.
+    table.masked_fill_(back, -1)
+    count.add_(n)
+    i32 = [x.to(torch.int32) for x in (cu, ctx + new, ctx[b] + depth, slots, missing)]
+    return tuple(i32) + (table, free, count) + tuple(out)
+
+
+def _tree_sees(st, t0, S):
+    """[S, S]: whether node i sees node a, from the masks."""
+    a = torch.arange(S, device=st["mask"].device)
+    return ((st["mask"][t0:t0 + S][:, a // 64] >> (a % 64)) & 1).bool()
+
+
+def _plain_attn(st):
+    c = st["case"]
+    H, G, D, bs, win = c["H"], c["G"], c["D"], c["block"], c["win"]
+    dev, dt = st["q"].device, st["q"].dtype
+    out = torch.empty(st["q"].shape, dtype=dt, device=dev)
+    lse = torch.empty(st["q"].shape[:2], dtype=torch.float32, device=dev)
+    t0 = 0
+    for b, (S, ctx) in enumerate(_lens(c)):
+        n = ctx + S
+        rows = st["table"][b, :-(-n // bs)].long()
+        k = st["kc"][rows].view(-1, G, D)[:n].float().permute(1, 2, 0).contiguous()
+        v = st["vc"][rows].view(-1, G, D)[:n].float().permute(1, 0, 2).contiguous()
+        q = st["q"][t0:t0 + S].float().view(S, G, H // G, D).permute(1, 0, 2, 3).reshape(G, -1, D)
+        x = torch.bmm(q, k).mul_(D ** -0.5).view(G, S, H // G, n)
+        hide = torch.zeros((S, n), dtype=torch.bool, device=dev)
+        hide[:, ctx:] = ~_tree_sees(st, t0, S)
+        if win >= 0:
+            hide[:, :ctx] = torch.arange(ctx, device=dev).view(1, -1) < st["pos"][t0:t0 + S].view(-1, 1) - win
+        x.masked_fill_(hide.view(1, S, 1, n), -math.inf)
+        top = x.amax(dim=-1, keepdim=True)
+        if st["sinks"] is not None:
+            sink = st["sinks"].view(G, 1, H // G, 1)
+            top = torch.maximum(top, sink)
+        e = x.sub_(top).exp_()
+        total = e.sum(dim=-1, keepdim=True)
+        if st["sinks"] is not None:
+            total = total + torch.exp(sink - top)
+        o = torch.bmm(e.view(G, -1, n), v).view(G, S, H // G, D).div_(total)
+        out[t0:t0 + S] = o.permute(1, 0, 2, 3).reshape(S, H, D).to(dt)
+        lse[t0:t0 + S] = (top + torch.log(total)).squeeze(-1).permute(1, 0, 2).reshape(S, H)
+        t0 += S
+    return out, lse
+
+
+def _plain_accept(st):
+    scores, tokens, parents, cu = st["scores"], st["tokens"], st["parents"], st["cu"].long()
+    dev, T, B, P = tokens.device, tokens.shape[0], cu.shape[0], st["max_path"]
+    if scores.dim() == 2:
+        target = torch.empty(T, dtype=torch.int32, device=dev)
+        V = scores.shape[1]
+        step = max(1, (1 << 28) // V)
+        at = torch.arange(V, device=dev, dtype=torch.int32)
+        for t in range(0, T, step):
+            x = scores[t:t + step].float()
+            target[t:t + step] = torch.where(x == x.amax(dim=1, keepdim=True), at, V).amin(dim=1)
+    else:
+        target = scores
+    seq, i = _sequence_of_rows(cu, T)
+    first = torch.arange(T, device=dev) - i
+    start = torch.cat((cu.new_zeros(1), cu[:-1]))
+    up = parents.long()
+    # A node agrees where its parent's choice is its token.
+    agrees = (up >= 0) & (up < i)
+    agrees = agrees & (target[(first + up).clamp(min=0)] == tokens)
+    path = torch.full((B, P), -1, dtype=torch.int32, device=dev)
+    chosen = torch.full((B, P), -1, dtype=torch.int32, device=dev)
+    at, alive = torch.zeros(B, dtype=torch.long, device=dev), cu > start
+    accepted = torch.zeros(B, dtype=torch.int32, device=dev)
+    for k in range(P):
+        path[:, k] = torch.where(alive, at, -1)
+        chosen[:, k] = torch.where(alive, target[(start + at).clamp(max=T - 1)], -1)
+        accepted += alive
+        child = agrees & (up == at[seq]) & alive[seq]
+        nxt = torch.full((B,), T, dtype=torch.long, device=dev)
+        nxt.scatter_reduce_(0, seq, torch.where(child, i, T), "amin")
+        alive = nxt < T
+        at = torch.where(alive, nxt, 0)
+    return accepted, path, chosen
+
+
+def _plain_commit(st):
+    bs = st["case"]["block"]
+    ctx, path, table = st["ctx"].long(), st["path"].long(), st["table"].long()
+    k = torch.arange(path.shape[1], device=path.device).view(1, -1)
+    moves = (k < st["accepted"].view(-1, 1)) & (path > k)
+    b = torch.arange(path.shape[0], device=path.device).view(-1, 1).expand_as(path)[moves]
+    to, src = (ctx.view(-1, 1) + k)[moves], (ctx.view(-1, 1) + path)[moves]
+    to, src = (table[b, x // bs] * bs + x % bs for x in (to, src))
+    for cache in st["caches"]:
+        rows = cache.view(-1, cache.shape[-1])
+        rows[to] = rows[src]
+    return st["caches"]
+
+
+# ------------------------------------------------------------------------------- what a pass cannot do without
+
+
+def work(case):
+    c = case
+    lens = _lens(c)
+    B, T = len(lens), sum(s for s, _ in lens)
+    if c["kind"] == "plan":
+        bs = c["block"]
+        touched = sum((n + s - 1) // bs - n // bs + 1 for s, n in lens if s)
+        fresh = sum(-(-(n + s) // bs) - -(-n // bs) for s, n in lens)
+        W = -(-max([s for s, _ in lens] + [1]) // 64)
+        row = 4 + 4 + (4 + 8 * W if c["tree"] else 0)
+        return {"bytes": 20 * B + 4 * touched + 20 * fresh + T * row, "flops": 0}
+    sz = _SIZE[c["dtype"]]
+    if c["kind"] == "attn":
+        win, row = c["win"], c["G"] * c["D"] * sz
+        W = max(-(-s // 64) for s, _ in lens)
+        keys = sum(s + (min(n, win) if win >= 0 else n) for s, n in lens)
+        # A node sees itself at least; with a window the deepest node that S nodes allow sees the fewest keys.
+        pairs = sum(s * (1 + (min(n, max(0, win - s + 1)) if win >= 0 else n)) for s, n in lens)
+        return {"bytes": T * (c["H"] * (2 * c["D"] * sz + 4) + 8 * W) + 2 * keys * row, "flops": 4 * c["H"] * c["D"] * pairs}
+    path = [max(1, min(c["accept"], (s + 1) // 2)) for s, _ in lens]
+    if c["kind"] == "accept":
+        return {"bytes": sum(path) * (c["V"] * sz if c["scores"] else 4) + 8 * T + 8 * sum(path) + 8 * B, "flops": 0}
+    return {"bytes": 2 * sum(a - 1 for a in path) * c["row"] * sz * c["caches"] + 12 * B, "flops": 0}
+
+
+# ------------------------------------------------------------------------------- the definitions
+
+
+def _exact_plan(st):
+    c, bs = st["case"], st["case"]["block"]
+    new, ctx = st["new"].tolist(), st["ctx"].tolist()
+    table, free, n = st["table"].cpu().numpy().copy(), st["free"].cpu().numpy(), int(st["count"])
+    before = table.copy()
+    par = st["parents"].tolist() if c["tree"] else None
+    cu, pos, slots, missing, masks, t = [], [], [], [], [], 0
+    W = -(-st["max_nodes"] // 64)
+    for b, (S, at) in enumerate(zip(new, ctx)):
+        short = 0
+        for j in range(at // bs, (at + S - 1) // bs + 1 if S else 0):
+            if table[b, j] < 0:
+                if n > 0:
+                    n -= 1
+                    table[b, j] = free[n]
+                else:
+                    short += 1
+        missing.append(short)
+        chains = _ancestors(par[t:t + S]) if c["tree"] else [[i] for i in range(S)]
+        if c["tree"]:
+            masks.append(_mask_words(chains, W, c["win"]))
+        pos += [at + len(x) - 1 if c["tree"] else at for x in chains]
+        for i in range(S):
+            page = int(table[b, (at + i) // bs])
+            slots.append(page * bs + (at + i) % bs if page >= 0 else -1)
+        t += S
+        cu.append(t)
+    ints = [torch.tensor(x) for x in (cu, [a + s for a, s in zip(ctx, new)], pos, slots, missing)]
+    # All pages of the step are back: the lists are as before it.
+    out = ints + [torch.from_numpy(before), st["free"].clone(), st["count"].clone()]
+    return tuple(out) + ((torch.cat(masks),) if c["tree"] else ())
+
+
+def _exact_attn(st):
+    """One head at a time: softmax(q k^T / sqrt(D)) v over the keys a node sees, a sink's mass beside it."""
+    c = st["case"]
+    H, G, D, bs, win = c["H"], c["G"], c["D"], c["block"], c["win"]
+    dev = st["q"].device
+    out = torch.empty(st["q"].shape, dtype=torch.float64, device=dev)
+    lse = torch.empty(st["q"].shape[:2], dtype=torch.float64, device=dev)
+    first = 0
+    for b, (S, ctx) in enumerate(_lens(c)):
+        j = torch.arange(ctx + S, device=dev)
+        row = st["table"][b].long()[j // bs] * bs + j % bs
+        node = (j - ctx).clamp(min=0)
+        see = ((st["mask"][first:first + S][:, node // 64] >> (node % 64)) & 1) == 1
+        old = (j < ctx).view(1, -1)
+        near = (j >= st["pos"][first:first + S].view(-1, 1) - win) if win >= 0 else torch.ones_like(see)
+        see = torch.where(old, near, see)
+        for h in range(H):
+            g = h // (H // G)
+            kt = st["kc"].view(-1, G, D)[row, g].double().t().contiguous()
+            v = st["vc"].view(-1, G, D)[row, g].double()
+            w = torch.where(see, (st["q"][first:first + S, h].double() @ kt) / math.sqrt(D), -math.inf)
+            l = torch.logsumexp(w, dim=1)
+            if st["sinks"] is not None:
+                l = torch.logaddexp(l, st["sinks"][h].double())
+            out[first:first + S, h] = torch.exp(w - l.view(-1, 1)) @ v
+            lse[first:first + S, h] = l
+        first += S
+    return out, lse
+
+
+def _exact_accept(st):
+    tokens, parents, P = st["tokens"].tolist(), st["parents"].tolist(), st["max_path"]
+    scores = st["scores"]
+    accepted, paths, chosen, t = [], [], [], 0
+    for end in st["cu"].tolist():
+        path, out, at = [], [], 0
+        while end > t and len(path) < P:
+            if scores.dim() == 2:
+                x = scores[t + at].cpu().double()
+                want = int(torch.nonzero(x == x.max())[0])
+            else:
+                want = int(scores[t + at])
+            path.append(at)
+            out.append(want)
+            at = next((i for i in range(at + 1, end - t) if parents[t + i] == at and tokens[t + i] == want), -1)
+            if at < 0:
+                break
+        accepted.append(len(path))
+        paths.append(path + [-1] * (P - len(path)))
+        chosen.append(out + [-1] * (P - len(out)))
+        t = end
+    return torch.tensor(accepted), torch.tensor(paths), torch.tensor(chosen)
+
+
+def _exact_commit(st):
+    """Rows are moved, not computed: one by one, in the order of the path."""
+    bs, table = st["case"]["block"], st["table"].tolist()
+    paths, counts = st["path"].tolist(), st["accepted"].tolist()
+    where = lambda b, j: table[b][j // bs] * bs + j % bs
+    moves = []
+    for b, at in enumerate(st["ctx"].tolist()):
+        moves += [(where(b, at + k), where(b, at + paths[b][k])) for k in range(counts[b]) if paths[b][k] != k]
+    out = []
+    for cache in st["caches"]:
+        rows = cache.clone()
+        flat = rows.view(-1, rows.shape[-1])
+        for to, src in moves:
+            flat[to] = flat[src].clone()
+        out.append(rows.double())
+    return out
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    return {"plan": _exact_plan, "attn": _exact_attn, "accept": _exact_accept, "commit": _exact_commit}[case["kind"]](st)
