@@ -34,6 +34,7 @@ extern "C" {
 #define DSA_KIND_FP16 2
 #define DSA_KIND_FP32 3 /* act_quant input */
 #define DSA_KIND_INT8 4 /* act_quant output */
+#define DSA_KIND_INT32 5 /* tree_accept: choices instead of scores */
 
 /* Library ABI version (major * 100 + minor). */
 int dsa_abi_version(void);
@@ -423,6 +424,83 @@ int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* 
                       int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                       int64_t max_blocks, int is_causal, int64_t win_left, const float* sinks, float sm_scale,
                       void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A decoding step that checks trees of drafted tokens: dsa_paged_plan before the layers, dsa_qk_norm_rope and
+ * dsa_paged_tree_fwd in each, dsa_tree_accept behind the last and dsa_paged_commit over all layers' caches.  A sequence's
+ * new tokens are the nodes of its tree, node i with key context_len + i; parents[t] is the place of a node's parent in its
+ * sequence, less than its own (anything else: the node has none).  Single tokens and chunks are trees without `parents`.
+ *
+ * The plan: from the sequences' lengths, of what they hold in the cache (context_lens) and of what they get (new_lens, rows
+ * of the packed step in order, cut to T), on the device:
+ *  - pages: negative entries of block_table [B, max_blocks] among the blocks that the new rows touch get pages off the
+ *    end of free_blocks (free_blocks[*free_count - 1] first), in the order (sequence, block); *free_count falls by them;
+ *  - cu_seqlens [B] inclusive sums of the new lengths, kv_lens [B] = context + new;
+ *  - positions [T] = context + depth in the tree (+ place without one), slots [T] = page * block_size + key % block_size;
+ *    rows behind the last sequence get -1, slots without a page too;
+ *  - missing [B]: pages that a sequence lacks, since the list ran out or its table ended (its step is not whole then);
+ *  - tree_mask [T, mask_words] (with parents): bit a % 64 of word a / 64 of a node's row is set where node a of the
+ *    sequence is the node or an ancestor, with win_left >= 0 at most win_left steps up.
+ * block_table and free_count change in place.  Lengths below 0 count as 0, above 2^30 as 2^30.  B <= 16384, T < 2^30.
+ */
+int dsa_paged_plan(const int32_t* new_lens, const int32_t* context_lens, int32_t* block_table,
+                   const int32_t* free_blocks, int32_t* free_count, const int32_t* parents, int64_t B, int64_t T,
+                   int64_t max_blocks, int64_t block_size, int64_t free_room, int64_t mask_words, int64_t win_left,
+                   int32_t* cu_seqlens, int32_t* kv_lens, int32_t* positions, int32_t* slots, int32_t* missing,
+                   uint64_t* tree_mask, void* stream);
+
+/*
+ * Pages back to the list: those of the blocks behind keep_lens[b] keys, up to the first negative entry of the row, which
+ * becomes -1.  Of n pages in the order (sequence, block) the i-th goes to free_blocks[*free_count + n - 1 - i], so that
+ * giving back what a plan took restores the list; *free_count rises by n.  Pages that free_room entries do not hold stay
+ * in the table.  Pages are counted by no one: each must stand in one row only.
+ */
+int dsa_paged_free(const int32_t* keep_lens, int32_t* block_table, int32_t* free_blocks, int32_t* free_count,
+                   int64_t B, int64_t max_blocks, int64_t block_size, int64_t free_room, void* stream);
+
+/*
+ * dsa_paged_gqa_fwd for the nodes of trees.  Sequence b brings the last len_b of its kv_len[b] keys, first = kv_len - len_b;
+ * node i sees the keys j < first (with a window those of them with j >= positions[t] - win_left; positions are taken into
+ * [first, kv_len)) and the keys first + a of the nodes a whose bits are set in its row of tree_mask [T, mask_words].
+ * The other arguments, limits, the treatment of pages outside the pool, of rows that see nothing and of values that are
+ * not finite are those of dsa_paged_gqa_fwd.  Without cu_q S is at most 64 * mask_words; packed nodes past that many have no
+ * bits.  mask_words in [1, 64].
+ */
+size_t dsa_paged_tree_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys);
+
+int dsa_paged_tree_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                       const uint64_t* tree_mask, int64_t mask_words, const int32_t* positions, const int32_t* cu_q,
+                       const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T, int64_t B, int64_t S,
+                       int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                       int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
+ * The path that a model's choices take through each tree.  Node 0 of a sequence is on it (the token chosen by the step
+ * before); behind a node comes the lowest later node whose parent it is and whose token is the choice at it; it ends
+ * where there is none, and at max_path nodes.  The choice at a row is the place of its largest score, the lowest of equal
+ * ones; NaN and -infinity are never it (-1 where a row holds nothing else, which no token matches).
+ *  scores [T, V] bf16, fp16 or fp32, rows row_stride elements apart, or with DSA_KIND_INT32 the choices [T] themselves;
+ *  tokens, parents [T]; cu_seqlens [B] inclusive sums.  accepted [B]: nodes on the path; path [B, max_path]: their
+ *  places; chosen [B, max_path]: the choices at them, that is the tokens the step yields, the last one not in the cache
+ *  yet; both -1 behind the path.
+ */
+size_t dsa_tree_accept_workspace_size(int kind, int64_t T, int64_t V);
+
+int dsa_tree_accept(int kind, const void* scores, int64_t row_stride, int64_t T, int64_t V, const int32_t* tokens,
+                    const int32_t* parents, const int32_t* cu_seqlens, int64_t B, int64_t max_path, int32_t* accepted,
+                    int32_t* path, int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The accepted nodes' rows to the front: in every cache, for k = 0 .. accepted[b] - 1 one after the other, the row of key
+ * context_lens[b] + path[b, k] is copied to that of key context_lens[b] + k where path[b, k] > k; rows without a page in
+ * [0, num_blocks) are left.  caches and row_bytes are host arrays of num_caches: caches [num_blocks, block_size] rows of
+ * row_bytes (a multiple of 4; 16 is faster), of any type, which must not overlap.  All of them go in one launch for each
+ * 128 caches.  A sequence's new tokens must lie in pages of its own.
+ */
+int dsa_paged_commit(void* const* caches, const int64_t* row_bytes, int64_t num_caches, const int32_t* block_table,
+                     const int32_t* context_lens, const int32_t* path, const int32_t* accepted, int64_t B,
+                     int64_t max_path, int64_t num_blocks, int64_t block_size, int64_t max_blocks, void* stream);
 
 #ifdef __cplusplus
 }

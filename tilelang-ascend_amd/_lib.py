@@ -22,6 +22,7 @@ KIND_BF16 = 1
 KIND_FP16 = 2
 KIND_FP32 = 3
 KIND_INT8 = 4
+KIND_INT32 = 5
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -95,6 +96,15 @@ SIGNATURES = {
     "dsa_paged_gqa_fwd": (_c_int, [_c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64,
                                    _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_vp, _c_float,
                                    _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "dsa_paged_plan": (_c_int, [_c_vp] * 6 + [_c_i64] * 7 + [_c_vp] * 7),
+    "dsa_paged_free": (_c_int, [_c_vp] * 4 + [_c_i64] * 4 + [_c_vp]),
+    "dsa_paged_tree_workspace_size": (_c_size, [_c_i64] * 6),
+    "dsa_paged_tree_fwd": (_c_int, [_c_int] + [_c_vp] * 5 + [_c_i64] + [_c_vp] * 4 + [_c_i64] * 10 +
+                           [_c_vp, _c_float, _c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "dsa_tree_accept_workspace_size": (_c_size, [_c_int, _c_i64, _c_i64]),
+    "dsa_tree_accept": (_c_int, [_c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp,
+                                 _c_vp, _c_vp, _c_size, _c_vp]),
+    "dsa_paged_commit": (_c_int, [_c_vp, _c_vp, _c_i64] + [_c_vp] * 4 + [_c_i64] * 5 + [_c_vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -218,12 +228,12 @@ def is_integer(t: torch.Tensor) -> bool:
     return not (t.dtype.is_floating_point or t.dtype.is_complex or t.dtype == torch.bool)
 
 
-_WIDE_INTS = (torch.int64, torch.uint32, torch.uint64)
+WIDE_INTS = (torch.int64, torch.uint32, torch.uint64)
 
 
 def saturated_int32(t: torch.Tensor) -> torch.Tensor:
     """An integer tensor as int32, values past 32 bits at the ends of the range instead of wrapped into it."""
-    if t.dtype in _WIDE_INTS:
+    if t.dtype in WIDE_INTS:
         wide = t.to(torch.int64)
         if t.dtype == torch.uint64:  # values past 63 bits have come out negative
             wide = wide.masked_fill(wide < 0, 2**31 - 1)

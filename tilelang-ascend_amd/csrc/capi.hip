@@ -1,6 +1,9 @@
 // C ABI entry points: argument validation, then the kernel launchers.
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
+#include <utility>
+#include <vector>
 
 #include "../../include/dsa_mi355x.h"
 #include "common.hpp"
@@ -67,6 +70,25 @@ hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const vo
                             int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                             int64_t max_blocks, int causal, int64_t win_left, const float* sinks, float sm_scale,
                             void* out, float* lse, void* workspace, hipStream_t stream);
+hipError_t launch_paged_tree(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
+                             const uint64_t* mask, int64_t words, const int32_t* pos, const int32_t* cu_q,
+                             const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B, int64_t S, int64_t H,
+                             int64_t G, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                             int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse,
+                             void* workspace, hipStream_t stream);
+hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_t* table, const int32_t* free_list,
+                             int32_t* free_count, const int32_t* parents, int64_t B, int64_t T, int64_t max_blocks,
+                             int64_t block_size, int64_t room, int64_t words, int64_t win, int32_t* cu, int32_t* kv,
+                             int32_t* positions, int32_t* slots, int32_t* missing, uint64_t* mask, hipStream_t stream);
+hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_list, int32_t* free_count, int64_t B,
+                             int64_t max_blocks, int64_t block_size, int64_t room, hipStream_t stream);
+size_t tree_accept_workspace_bytes(int size, int64_t T, int64_t V);
+hipError_t launch_tree_accept(int kind, const void* scores, int64_t stride, int64_t T, int64_t V, const int32_t* tokens,
+                              const int32_t* parents, const int32_t* cu, int64_t B, int64_t P, int32_t* accepted,
+                              int32_t* path, int32_t* chosen, void* workspace, hipStream_t stream);
+hipError_t launch_paged_commit(void* const* caches, const int64_t* row_bytes, int64_t num_caches, const int32_t* table,
+                               const int32_t* ctx, const int32_t* path, const int32_t* accepted, int64_t B, int64_t P,
+                               int64_t num_blocks, int64_t block_size, int64_t max_blocks, hipStream_t stream);
 hipError_t launch_sparse_flash_mla(int is_fp16, const void* q, int64_t T, int64_t H, int64_t B,
                                    const int32_t* q_start, const int32_t* q_len, const int32_t* kv_len,
                                    const void* ori_kv, int64_t ori_blocks, int64_t ori_bs, const int32_t* ori_bt,
@@ -630,34 +652,185 @@ size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, 
   return dsa::paged_gqa_workspace_bytes(T, B, H, G, D, max_keys);
 }
 
+// What the two attentions over pages ask alike of their arguments; `who` names the entry.
+static int check_paged(const char* who, int kind, const void* q, const void* k_cache, const void* v_cache,
+                       const int32_t* block_table, const int32_t* cu_q, const int32_t* actual_kv_len, int64_t T,
+                       int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
+                       int64_t max_blocks, int64_t win_left, float sm_scale, const void* out, const float* lse,
+                       const void* workspace, size_t workspace_bytes) {
+  char text[96];
+  const auto no = [&](const char* what) {
+    std::snprintf(text, sizeof(text), "%s: %s", who, what);
+    return reject(text);
+  };
+  if (kind != DSA_KIND_BF16 && kind != DSA_KIND_FP16) return no("kind must be bf16 or fp16");
+  if (D != 64 && D != 128) return no("D must be 64 or 128");
+  if (G < 1 || H < 1 || H % G != 0) return no("H must be a multiple of kv_group");
+  if (block_size < 1 || max_blocks < 1 || num_blocks < 1 || block_size > kMaxInt || max_blocks > kMaxInt ||
+      num_blocks > kMaxInt / block_size)
+    return no("bad page sizes");
+  if (max_blocks > (kMaxInt - 4096) / block_size || !paged_gqa_sizes(T, B, H, G, D, max_blocks * block_size))
+    return no("sizes out of range");
+  if (!cu_q && (S < 0 || S > kMaxInt || B * S != T)) return no("T must be B * S without cu_q");
+  if (win_left < -1 || win_left > kMaxInt - 4096) return no("win_left must be -1 (none) or a key count");
+  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return no("sm_scale must be positive");
+  if (T == 0) return 0;
+  if (!q || !k_cache || !v_cache || !block_table || !actual_kv_len || !out || !lse) return no("null pointer");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return no("rows must start on 16 bytes");
+  const size_t need = dsa_paged_gqa_workspace_size(T, B, H, G, D, max_blocks * block_size);
+  if (workspace_bytes < need) return no("workspace too small");
+  if (need > 0 && (!workspace || !aligned16(workspace))) return no("null or unaligned workspace");
+  return 0;
+}
+
 int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                       const int32_t* cu_q, const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T,
                       int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                       int64_t max_blocks, int is_causal, int64_t win_left, const float* sinks, float sm_scale,
                       void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  if (kind != DSA_KIND_BF16 && kind != DSA_KIND_FP16) return reject("paged_gqa: kind must be bf16 or fp16");
-  if (D != 64 && D != 128) return reject("paged_gqa: D must be 64 or 128");
-  if (G < 1 || H < 1 || H % G != 0) return reject("paged_gqa: H must be a multiple of kv_group");
-  if (block_size < 1 || max_blocks < 1 || num_blocks < 1 || block_size > kMaxInt || max_blocks > kMaxInt ||
-      num_blocks > kMaxInt / block_size)
-    return reject("paged_gqa: bad page sizes");
-  if (max_blocks > (kMaxInt - 4096) / block_size || !paged_gqa_sizes(T, B, H, G, D, max_blocks * block_size))
-    return reject("paged_gqa: sizes out of range");
-  if (!cu_q && (S < 0 || S > kMaxInt || B * S != T)) return reject("paged_gqa: T must be B * S without cu_q");
-  if (win_left < -1 || win_left > kMaxInt - 4096) return reject("paged_gqa: win_left must be -1 (none) or a key count");
-  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return reject("paged_gqa: sm_scale must be positive");
+  if (const int rc = check_paged("paged_gqa", kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
+                                 num_blocks, block_size, max_blocks, win_left, sm_scale, out, lse, workspace,
+                                 workspace_bytes))
+    return rc;
   if (T == 0) return 0;
-  if (!q || !k_cache || !v_cache || !block_table || !actual_kv_len || !out || !lse)
-    return reject("paged_gqa: null pointer");
-  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
-    return reject("paged_gqa: rows must start on 16 bytes");
-  const size_t need = dsa_paged_gqa_workspace_size(T, B, H, G, D, max_blocks * block_size);
-  if (workspace_bytes < need) return reject("paged_gqa: workspace too small");
-  if (need > 0 && (!workspace || !aligned16(workspace))) return reject("paged_gqa: null or unaligned workspace");
   return ok(dsa::launch_paged_gqa(kind == DSA_KIND_FP16, q, k_cache, v_cache, block_table, cu_q, actual_q_len,
                                   actual_kv_len, T, B, S, H, G, D, num_blocks, block_size, max_blocks,
                                   is_causal ? 1 : 0, win_left, sinks, sm_scale, out, lse, workspace,
                                   static_cast<hipStream_t>(stream)));
+}
+
+size_t dsa_paged_tree_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {
+  return dsa_paged_gqa_workspace_size(T, B, H, G, D, max_keys);
+}
+
+int dsa_paged_tree_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                       const uint64_t* tree_mask, int64_t mask_words, const int32_t* positions, const int32_t* cu_q,
+                       const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T, int64_t B, int64_t S,
+                       int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                       int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  if (mask_words < 1 || mask_words > 64) return reject("paged_tree: mask_words must be in [1, 64]");
+  if (const int rc = check_paged("paged_tree", kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
+                                 num_blocks, block_size, max_blocks, win_left, sm_scale, out, lse, workspace,
+                                 workspace_bytes))
+    return rc;
+  if (!cu_q && S > 64 * mask_words) return reject("paged_tree: S must be at most 64 * mask_words");
+  if (T == 0) return 0;
+  if (!tree_mask || (win_left >= 0 && !positions)) return reject("paged_tree: null pointer");
+  if (reinterpret_cast<uintptr_t>(tree_mask) & 7) return reject("paged_tree: tree_mask must start on 8 bytes");
+  return ok(dsa::launch_paged_tree(kind == DSA_KIND_FP16, q, k_cache, v_cache, block_table, tree_mask, mask_words,
+                                   positions, cu_q, actual_q_len, actual_kv_len, T, B, S, H, G, D, num_blocks,
+                                   block_size, max_blocks, win_left, sinks, sm_scale, out, lse, workspace,
+                                   static_cast<hipStream_t>(stream)));
+}
+
+// The limits of the page lists: the sums of a call's sequences lie in one workgroup's LDS, lengths in 30 bits.
+constexpr int64_t kPlanSeqs = 16384, kPlanRows = ((int64_t)1 << 30) - 1;
+
+static int check_lists(const char* who, int64_t B, int64_t max_blocks, int64_t block_size, int64_t room) {
+  char text[96];
+  const char* what = nullptr;
+  if (B < 1 || B > kPlanSeqs) what = "B must be in [1, 16384]";
+  else if (block_size < 1 || block_size > kMaxInt || max_blocks < 1 || max_blocks > kMaxInt / B || room < 0 || room > kMaxInt)
+    what = "bad page sizes";
+  if (!what) return 0;
+  std::snprintf(text, sizeof(text), "%s: %s", who, what);
+  return reject(text);
+}
+
+int dsa_paged_plan(const int32_t* new_lens, const int32_t* context_lens, int32_t* block_table,
+                   const int32_t* free_blocks, int32_t* free_count, const int32_t* parents, int64_t B, int64_t T,
+                   int64_t max_blocks, int64_t block_size, int64_t free_room, int64_t mask_words, int64_t win_left,
+                   int32_t* cu_seqlens, int32_t* kv_lens, int32_t* positions, int32_t* slots, int32_t* missing,
+                   uint64_t* tree_mask, void* stream) {
+  if (const int rc = check_lists("paged_plan", B, max_blocks, block_size, free_room)) return rc;
+  if (T < 0 || T > kPlanRows) return reject("paged_plan: T must be in [0, 2^30)");
+  if (parents && (mask_words < 1 || mask_words > 64)) return reject("paged_plan: mask_words must be in [1, 64]");
+  if (win_left < -1 || win_left > kMaxInt) return reject("paged_plan: win_left must be -1 (none) or a count");
+  if (!new_lens || !context_lens || !block_table || !free_count || (free_room > 0 && !free_blocks) || !cu_seqlens ||
+      !kv_lens || !missing || (T > 0 && (!positions || !slots || (parents && !tree_mask))))
+    return reject("paged_plan: null pointer");
+  return ok(dsa::launch_paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, parents, B, T,
+                                   max_blocks, block_size, free_room, parents ? mask_words : 0, win_left, cu_seqlens,
+                                   kv_lens, positions, slots, missing, tree_mask, static_cast<hipStream_t>(stream)));
+}
+
+int dsa_paged_free(const int32_t* keep_lens, int32_t* block_table, int32_t* free_blocks, int32_t* free_count,
+                   int64_t B, int64_t max_blocks, int64_t block_size, int64_t free_room, void* stream) {
+  if (const int rc = check_lists("paged_free", B, max_blocks, block_size, free_room)) return rc;
+  if (!keep_lens || !block_table || !free_count || (free_room > 0 && !free_blocks))
+    return reject("paged_free: null pointer");
+  return ok(dsa::launch_paged_free(keep_lens, block_table, free_blocks, free_count, B, max_blocks, block_size, free_room,
+                                   static_cast<hipStream_t>(stream)));
+}
+
+static int check_accept(int kind, int64_t T, int64_t V) {
+  if (kind != DSA_KIND_BF16 && kind != DSA_KIND_FP16 && kind != DSA_KIND_FP32 && kind != DSA_KIND_INT32)
+    return reject("tree_accept: kind must be bf16, fp16, fp32 or int32 (choices)");
+  if (T < 0 || T > kPlanRows) return reject("tree_accept: T must be in [0, 2^30)");
+  if (kind != DSA_KIND_INT32 && (V < 1 || V > kPlanRows)) return reject("tree_accept: V must be in [1, 2^30)");
+  return 0;
+}
+
+size_t dsa_tree_accept_workspace_size(int kind, int64_t T, int64_t V) {
+  if (T <= 0 || check_accept(kind, T, V) || kind == DSA_KIND_INT32) return 0;
+  return dsa::tree_accept_workspace_bytes(kind == DSA_KIND_FP32 ? 4 : 2, T, V);
+}
+
+int dsa_tree_accept(int kind, const void* scores, int64_t row_stride, int64_t T, int64_t V, const int32_t* tokens,
+                    const int32_t* parents, const int32_t* cu_seqlens, int64_t B, int64_t max_path, int32_t* accepted,
+                    int32_t* path, int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_accept(kind, T, V)) return rc;
+  if (B < 1 || B > 65535 || max_path < 1 || max_path > kMaxInt / B) return reject("tree_accept: bad B / max_path");
+  if (!cu_seqlens || !accepted || !path || !chosen || (T > 0 && (!scores || !tokens || !parents)))
+    return reject("tree_accept: null pointer");
+  const int size = kind == DSA_KIND_FP32 || kind == DSA_KIND_INT32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(scores) % size) return reject("tree_accept: scores must start on an element");
+  if (kind != DSA_KIND_INT32 && row_stride < V && T > 1) return reject("tree_accept: rows of scores must not overlap");
+  if (T > 0 && row_stride > ((int64_t)1 << 60) / T) return reject("tree_accept: row_stride out of range");
+  const size_t need = dsa_tree_accept_workspace_size(kind, T, V);
+  if (workspace_bytes < need) return reject("tree_accept: workspace too small");
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7)))
+    return reject("tree_accept: null or unaligned workspace");
+  return ok(dsa::launch_tree_accept(kind == DSA_KIND_INT32 ? 0 : kind, scores, row_stride, T, V, tokens, parents,
+                                    cu_seqlens, B, max_path, accepted, path, chosen, workspace,
+                                    static_cast<hipStream_t>(stream)));
+}
+
+int dsa_paged_commit(void* const* caches, const int64_t* row_bytes, int64_t num_caches, const int32_t* block_table,
+                     const int32_t* context_lens, const int32_t* path, const int32_t* accepted, int64_t B,
+                     int64_t max_path, int64_t num_blocks, int64_t block_size, int64_t max_blocks, void* stream) {
+  if (num_caches < 0 || num_caches > 65536) return reject("paged_commit: bad number of caches");
+  if (B < 1 || B > 65535 || max_path < 0 || max_path > kMaxInt / B) return reject("paged_commit: bad B / max_path");
+  if (block_size < 1 || max_blocks < 1 || num_blocks < 1 || block_size > kMaxInt || max_blocks > kMaxInt / B ||
+      num_blocks > kMaxInt / block_size)
+    return reject("paged_commit: bad page sizes");
+  if (num_caches == 0 || max_path == 0) return 0;
+  if (!caches || !row_bytes || !block_table || !context_lens || !path || !accepted)
+    return reject("paged_commit: null pointer");
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  try {
+    spans.reserve((size_t)num_caches);
+  } catch (...) {
+    return reject("paged_commit: out of host memory");
+  }
+  int64_t units = 0;  // waves for each sequence
+  for (int64_t c = 0; c < num_caches; ++c) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(caches[c]);
+    if (!at) return reject("paged_commit: null cache");
+    if (row_bytes[c] < 4 || row_bytes[c] % 4 != 0 || row_bytes[c] > (1 << 22) || at % 4 != 0)
+      return reject("paged_commit: rows must be multiples of 4 bytes up to 4 MB that start on 4 bytes");
+    spans.emplace_back(at, at + (uintptr_t)(num_blocks * block_size * row_bytes[c]));
+    units += (row_bytes[c] + 255) / 256;
+  }
+  if ((units / 4 + 1) * 256 * B >= (int64_t)1 << 32) return reject("paged_commit: sizes out of range");
+  // A row that two caches share would be moved twice.
+  std::sort(spans.begin(), spans.end());
+  for (size_t c = 1; c < spans.size(); ++c)
+    if (spans[c].first < spans[c - 1].second) return reject("paged_commit: caches must not overlap");
+  return ok(dsa::launch_paged_commit(caches, row_bytes, num_caches, block_table, context_lens, path, accepted, B,
+                                     max_path, num_blocks, block_size, max_blocks, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -54,6 +54,13 @@ struct Entries {
   decltype(&dsa_qk_norm_rope) rope;
   decltype(&dsa_paged_gqa_workspace_size) pgqa_ws;
   decltype(&dsa_paged_gqa_fwd) pgqa;
+  decltype(&dsa_paged_tree_workspace_size) tree_ws;
+  decltype(&dsa_paged_tree_fwd) tree;
+  decltype(&dsa_paged_plan) plan;
+  decltype(&dsa_paged_free) free_pages;
+  decltype(&dsa_tree_accept_workspace_size) accept_ws;
+  decltype(&dsa_tree_accept) accept;
+  decltype(&dsa_paged_commit) commit;
 } E;
 bool bound = false;
 
@@ -616,6 +623,206 @@ PyObject* paged_gqa(PyObject*, PyObject* const* v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (q, k_cache, v_cache, block_table, tree_mask, sm_scale, q lengths, kv lengths, positions, win_left, sinks)
+PyObject* paged_tree(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t win = -1;
+  DSA_PLAIN(bound && n == 11 && PyFloat_CheckExact(v[5]) && int_of(v[9], win));
+  for (int i = 0; i < 5; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const at::Tensor &q = THPVariable_Unpack(v[0]), &kc = THPVariable_Unpack(v[1]), &vc = THPVariable_Unpack(v[2]),
+                   &bt = THPVariable_Unpack(v[3]), &mask = THPVariable_Unpack(v[4]);
+  const Arg ql(v[6]), kl(v[7]), pos(v[8]), sinks(v[10]);
+  DSA_PLAIN(q.is_cuda() && (q.dim() == 3 || q.dim() == 4) && kc.dim() == 4 && bt.dim() == 2 && q.numel() > 0 && kl &&
+            !sinks.other && win >= -1 && win < 0x7fffffff - 4096);
+  const c10::Device dev = q.device();
+  const at::ScalarType st = q.scalar_type();
+  const int kind = kind16(st);
+  const bool packed = q.dim() == 3;
+  const int64_t B = bt.size(0), H = q.size(-2), D = q.size(-1), G = kc.size(2), blocks = kc.size(0), bs = kc.size(1),
+                mb = bt.size(1), S = packed ? 0 : q.size(1), T = packed ? q.size(0) : B * S;
+  DSA_PLAIN(kind >= 0 && plain(q, dev, st) && plain(kc, dev, st) && plain(vc, dev, st) && kc.sizes() == vc.sizes() &&
+            plain(bt, dev, at::kInt) && (D == 64 || D == 128) && kc.size(3) == D && G > 0 && H % G == 0 && B > 0 &&
+            mb > 0 && blocks > 0 && bs > 0 && lens_ok(ql, dev, B) && lens_ok(kl, dev, B) && lens_ok(pos, dev, T) &&
+            (packed ? (bool)ql : q.size(0) == B) && (win < 0 || pos));
+  DSA_PLAIN(plain(mask, dev, at::kLong) && mask.dim() == q.dim() - 1 &&
+            mask.sizes().slice(0, q.dim() - 2) == q.sizes().slice(0, q.dim() - 2));
+  const int64_t words = mask.size(-1);
+  DSA_PLAIN(words >= 1 && words <= 64 && (packed || S <= 64 * words));
+  if (sinks) DSA_PLAIN(plain(*sinks.t, dev, at::kFloat) && sinks.t->dim() == 1 && sinks.t->numel() == H);
+  for (const at::Tensor* t : {&q, &kc, &vc}) DSA_PLAIN((reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) == 0);
+  const double scale = PyFloat_AS_DOUBLE(v[5]);
+  DSA_PLAIN(scale > 0 && scale <= 1e30);
+  at::Tensor out, lse, ws;
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    out = make(q.sizes(), st, dev);
+    lse = make(q.sizes().slice(0, q.dim() - 1), at::kFloat, dev);
+    const size_t bytes = E.tree_ws(T, B, H, G, D, mb * bs);
+    if (bytes) ws = make({(int64_t)bytes}, at::kByte, dev);
+    rc = E.tree(kind, q.data_ptr(), kc.data_ptr(), vc.data_ptr(), bt.data_ptr<int32_t>(),
+                reinterpret_cast<const uint64_t*>(mask.data_ptr<int64_t>()), words, pos.ptr<int32_t>(),
+                packed ? ql.ptr<int32_t>() : nullptr, packed ? nullptr : ql.ptr<int32_t>(), kl.ptr<int32_t>(), T, B, S,
+                H, G, D, blocks, bs, mb, win, sinks.ptr<float>(), (float)scale, out.data_ptr(), lse.data_ptr<float>(),
+                bytes ? ws.data_ptr() : nullptr, bytes, stream(dev));
+  }
+  DSA_RC(rc);
+  return pair(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// The table and the free list of a plan, which change in place.
+bool lists_ok(const at::Tensor& bt, const at::Tensor& list, const at::Tensor& count, c10::Device dev) {
+  return bt.dim() == 2 && bt.size(0) >= 1 && bt.size(0) <= 16384 && bt.size(1) >= 1 && plain(bt, dev, at::kInt) &&
+         list.dim() == 1 && plain(list, dev, at::kInt) && count.numel() == 1 && plain(count, dev, at::kInt);
+}
+
+// (new lengths, context lengths, block_table, free_blocks, free_count, block_size, num_tokens, parents, max_nodes,
+// win_left): a tuple of the plan's six parts
+PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t bs = 0, T = 0, nodes = 0, win = -1;
+  DSA_PLAIN(bound && n == 10 && int_of(v[5], bs) && int_of(v[6], T) && int_of(v[8], nodes) && int_of(v[9], win));
+  for (int i = 2; i < 5; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const Arg nl(v[0]), ctx(v[1]), parents(v[7]);
+  const at::Tensor &bt = THPVariable_Unpack(v[2]), &list = THPVariable_Unpack(v[3]), &count = THPVariable_Unpack(v[4]);
+  DSA_PLAIN(nl && ctx && bt.is_cuda() && bs >= 1 && bs <= 0x7fffffff && T >= 1 && T < (1 << 30) && win >= -1 &&
+            win <= 0x7fffffff);
+  const c10::Device dev = bt.device();
+  DSA_PLAIN(lists_ok(bt, list, count, dev));
+  const int64_t B = bt.size(0);
+  DSA_PLAIN(lens_ok(nl, dev, B) && lens_ok(ctx, dev, B) && lens_ok(parents, dev, T) && (win < 0 || parents) &&
+            (!parents || (nodes >= 1 && nodes <= 4096)));
+  const int64_t words = parents ? (nodes + 63) / 64 : 0;
+  at::Tensor out[6];
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    for (int i = 0; i < 5; ++i) out[i] = make({i == 2 || i == 3 ? T : B}, at::kInt, dev);
+    if (parents) out[5] = make({T, words}, at::kLong, dev);
+    int32_t* p[5];
+    for (int i = 0; i < 5; ++i) p[i] = out[i].data_ptr<int32_t>();
+    rc = E.plan(nl.ptr<int32_t>(), ctx.ptr<int32_t>(), bt.data_ptr<int32_t>(), list.data_ptr<int32_t>(),
+                count.data_ptr<int32_t>(), parents.ptr<int32_t>(), B, T, bt.size(1), bs, list.numel(), words, win, p[0],
+                p[1], p[2], p[3], p[4],
+                parents ? reinterpret_cast<uint64_t*>(out[5].data_ptr<int64_t>()) : nullptr, stream(dev));
+  }
+  DSA_RC(rc);
+  PyObject* r = PyTuple_New(6);
+  if (!r) return nullptr;
+  for (int i = 0; i < 6; ++i) {
+    PyObject* o = i == 5 && !parents ? Py_NewRef(Py_None) : wrap(std::move(out[i]));
+    PyTuple_SET_ITEM(r, i, o);
+  }
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// (lengths kept, block_table, free_blocks, free_count, block_size): True
+PyObject* paged_free(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t bs = 0;
+  DSA_PLAIN(bound && n == 5 && int_of(v[4], bs));
+  for (int i = 1; i < 4; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const Arg keep(v[0]);
+  const at::Tensor &bt = THPVariable_Unpack(v[1]), &list = THPVariable_Unpack(v[2]), &count = THPVariable_Unpack(v[3]);
+  DSA_PLAIN(keep && bt.is_cuda() && bs >= 1 && bs <= 0x7fffffff);
+  const c10::Device dev = bt.device();
+  DSA_PLAIN(lists_ok(bt, list, count, dev) && lens_ok(keep, dev, bt.size(0)));
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    rc = E.free_pages(keep.ptr<int32_t>(), bt.data_ptr<int32_t>(), list.data_ptr<int32_t>(), count.data_ptr<int32_t>(),
+                      bt.size(0), bt.size(1), bs, list.numel(), stream(dev));
+  }
+  DSA_RC(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (scores or choices, tokens, parents, sums of the lengths, max_path)
+PyObject* tree_accept(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t P = 0;
+  DSA_PLAIN(bound && n == 5 && int_of(v[4], P));
+  for (int i = 0; i < 4; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const at::Tensor &x = THPVariable_Unpack(v[0]), &tok = THPVariable_Unpack(v[1]), &par = THPVariable_Unpack(v[2]),
+                   &cu = THPVariable_Unpack(v[3]);
+  DSA_PLAIN(x.is_cuda() && x.numel() > 0 && cu.dim() == 1 && cu.numel() >= 1 && cu.numel() <= 65535);
+  const c10::Device dev = x.device();
+  const at::ScalarType st = x.scalar_type();
+  const bool given = st == at::kInt;
+  const int kind = given ? DSA_KIND_INT32 : st == at::kFloat ? DSA_KIND_FP32 : kind16(st);
+  const int64_t T = x.size(0), V = given ? 0 : x.size(-1), B = cu.numel();
+  DSA_PLAIN(kind >= 0 && x.dim() == (given ? 1 : 2) && T < (1 << 30) && V < (1 << 30) && P >= 1 && P <= 0x7fffffff / B);
+  DSA_PLAIN(given ? x.is_contiguous() : x.stride(1) == 1 && (T == 1 || x.stride(0) >= V));
+  DSA_PLAIN(plain(tok, dev, at::kInt) && tok.numel() == T && plain(par, dev, at::kInt) && par.numel() == T &&
+            plain(cu, dev, at::kInt));
+  at::Tensor accepted, path, chosen, ws;
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    accepted = make({B}, at::kInt, dev);
+    path = make({B, P}, at::kInt, dev);
+    chosen = make({B, P}, at::kInt, dev);
+    const size_t bytes = E.accept_ws(kind, T, V);
+    if (bytes) ws = make({(int64_t)bytes}, at::kByte, dev);
+    rc = E.accept(kind, x.data_ptr(), x.stride(0), T, V, tok.data_ptr<int32_t>(), par.data_ptr<int32_t>(),
+                  cu.data_ptr<int32_t>(), B, P, accepted.data_ptr<int32_t>(), path.data_ptr<int32_t>(),
+                  chosen.data_ptr<int32_t>(), bytes ? ws.data_ptr() : nullptr, bytes, stream(dev));
+  }
+  DSA_RC(rc);
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, wrap(std::move(accepted)));
+  PyTuple_SET_ITEM(r, 1, wrap(std::move(path)));
+  PyTuple_SET_ITEM(r, 2, wrap(std::move(chosen)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// (tuple of caches, block_table, context lengths, path, accepted): True
+PyObject* paged_commit(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  DSA_PLAIN(bound && n == 5 && PyTuple_CheckExact(v[0]) && PyTuple_GET_SIZE(v[0]) > 0);
+  for (int i = 1; i < 5; ++i) DSA_PLAIN(THPVariable_CheckExact(v[i]));
+  const at::Tensor &bt = THPVariable_Unpack(v[1]), &path = THPVariable_Unpack(v[3]);
+  const Arg ctx(v[2]), accepted(v[4]);
+  DSA_PLAIN(bt.is_cuda() && bt.dim() == 2 && bt.size(0) >= 1 && bt.size(1) >= 1);
+  const c10::Device dev = bt.device();
+  const int64_t B = bt.size(0), count = PyTuple_GET_SIZE(v[0]);
+  DSA_PLAIN(plain(bt, dev, at::kInt) && path.dim() == 2 && path.size(0) == B && plain(path, dev, at::kInt) &&
+            ctx && accepted && lens_ok(ctx, dev, B) && lens_ok(accepted, dev, B));
+  std::vector<void*> at_cache(count);
+  std::vector<int64_t> bytes(count);
+  int64_t blocks = 0, bs = 0;
+  for (int64_t c = 0; c < count; ++c) {
+    PyObject* o = PyTuple_GET_ITEM(v[0], c);
+    DSA_PLAIN(THPVariable_CheckExact(o));
+    const at::Tensor& t = THPVariable_Unpack(o);
+    DSA_PLAIN(t.device() == dev && t.dim() >= 3 && t.is_contiguous() && t.numel() > 0);
+    if (c == 0) blocks = t.size(0), bs = t.size(1);
+    DSA_PLAIN(t.size(0) == blocks && t.size(1) == bs);
+    at_cache[c] = t.data_ptr();
+    bytes[c] = t.numel() / (blocks * bs) * (int64_t)t.element_size();
+  }
+  int rc;
+  {
+    const NoGil unlocked;
+    const c10::OptionalDeviceGuard guard(dev);
+    rc = E.commit(at_cache.data(), bytes.data(), count, bt.data_ptr<int32_t>(), ctx.ptr<int32_t>(),
+                  path.data_ptr<int32_t>(), accepted.ptr<int32_t>(), B, path.size(1), blocks, bs, bt.size(1),
+                  stream(dev));
+  }
+  DSA_RC(rc);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // ({entry name: address})
 PyObject* bind(PyObject*, PyObject* d) {
   struct Slot {
@@ -643,7 +850,14 @@ PyObject* bind(PyObject*, PyObject* d) {
                {"dsa_quant_matmul", &E.qmm},
                {"dsa_qk_norm_rope", &E.rope},
                {"dsa_paged_gqa_workspace_size", &E.pgqa_ws},
-               {"dsa_paged_gqa_fwd", &E.pgqa}};
+               {"dsa_paged_gqa_fwd", &E.pgqa},
+               {"dsa_paged_tree_workspace_size", &E.tree_ws},
+               {"dsa_paged_tree_fwd", &E.tree},
+               {"dsa_paged_plan", &E.plan},
+               {"dsa_paged_free", &E.free_pages},
+               {"dsa_tree_accept_workspace_size", &E.accept_ws},
+               {"dsa_tree_accept", &E.accept},
+               {"dsa_paged_commit", &E.commit}};
   for (const Slot& s : slots) {
     PyObject* o = PyDict_Check(d) ? PyDict_GetItemString(d, s.name) : nullptr;
     void* p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -672,6 +886,11 @@ PyMethodDef methods[] = {fast<topk>("topk"),
                          fast<quant_matmul>("quant_matmul"),
                          fast<qk_norm_rope>("qk_norm_rope"),
                          fast<paged_gqa>("paged_gqa"),
+                         fast<paged_tree>("paged_tree"),
+                         fast<paged_plan>("paged_plan"),
+                         fast<paged_free>("paged_free"),
+                         fast<tree_accept>("tree_accept"),
+                         fast<paged_commit>("paged_commit"),
                          {"bind", bind, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsa_host_path", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

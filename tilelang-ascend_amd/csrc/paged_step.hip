@@ -1,0 +1,640 @@
+// What a decoding step over a paged cache needs around its attention, gfx950: pages, slots, positions and tree masks from
+// request lengths (the plan) and the pages' way back, the choices of a model followed through a tree of drafted tokens, and
+// the cache rows of the accepted ones put in order.  All lengths, tables and lists stay on the device.
+#include "common.hpp"
+
+namespace dsa {
+
+constexpr int kStepThreads = 1024;
+constexpr int kStepWaves = kStepThreads / kWave;
+
+// ---------------------------------------------------------------------------------------------- plan
+//
+// Sequence b holds ctx_b keys and gets new_b rows of the packed step, cut to the T rows that there are; row i of it is
+// key ctx_b + i.  The blocks it touches are floor(ctx_b / bs) .. floor((ctx_b + new_b - 1) / bs); touched entries of the
+// table that are negative get pages off the end of the free list, in the order (sequence, block).  A row's slot is
+// table[b, key / bs] * bs + key % bs, its position ctx_b + depth (the tree's; i without one), and its mask the bits of
+// itself and its ancestors.
+//
+// Which page an entry gets depends on the entries before it in all sequences, and the table changes in place: one
+// workgroup counts and hands out (plan_pages_kernel), with the sums in LDS.  Its time is a chain of latencies (lengths,
+// sums, entries, list).  Few rows are written by the same workgroup, many by a second launch over the card.
+
+struct PlanArgs {
+  const int32_t* new_lens;   // [B]
+  const int32_t* ctx;        // [B]
+  int32_t* table;            // [B, max_blocks]
+  const int32_t* free_list;  // [room]
+  int32_t* free_count;       // [1]
+  const int32_t* parents;    // [T] place of a row's parent in its sequence, or null: no tree
+  int32_t* cu;               // [B] inclusive sums of the lengths
+  int32_t* kv;               // [B]
+  int32_t* positions;        // [T]
+  int32_t* slots;            // [T]
+  int32_t* missing;          // [B] pages that the list did not have, or past the table
+  uint64_t* mask;            // [T, words]
+  int B, T, max_blocks, block_size, room, words, win;
+};
+
+constexpr int kPlanMost = 1 << 30;  // lengths past it count as this many, so that sums of two stay in 32 bits
+
+__device__ __forceinline__ int plan_len(int x) { return min(max(x, 0), kPlanMost); }
+
+// Inclusive scan of op over the workgroup's threads (kStepThreads of them); `sums` holds kStepWaves values.  Every thread
+// gets its own result and the total.
+template <class Op>
+__device__ __forceinline__ int step_scan(int v, int* sums, int& total, Op op) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int u = __shfl_up(v, o, kWave);
+    if (lane >= o) v = op(u, v);
+  }
+  if (lane == kWave - 1) sums[wave] = v;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < kStepWaves; ++w) {
+    if (w == wave) before = total;
+    total = op(total, sums[w]);
+  }
+  __syncthreads();  // sums may be written again
+  return wave > 0 ? op(before, v) : v;
+}
+
+// The sequence of packed row t: the first whose sum is past it, B where there is none.
+__device__ __forceinline__ int plan_seq(const int* cu, int B, int t) {
+  int b0 = 0, b1 = B;
+  while (b0 < b1) {
+    const int mid = (b0 + b1) >> 1;
+    if (cu[mid] > t) b1 = mid;
+    else b0 = mid + 1;
+  }
+  return b0;
+}
+
+// Row t: `cu` is a.cu or a copy.
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const int* cu, int t) {
+  const int b = plan_seq(cu, a.B, t);
+  int position = -1, slot = -1, i = 0, start = 0;
+  if (b < a.B) {
+    start = b > 0 ? cu[b - 1] : 0;
+    i = t - start;
+    const int ctx = plan_len(a.ctx[b]), key = ctx + i, blk = key / a.block_size;
+    position = key;
+    if (blk < a.max_blocks) {
+      const int page = a.table[(int64_t)b * a.max_blocks + blk];
+      const int64_t at = (int64_t)page * a.block_size + (key - blk * a.block_size);
+      if (page >= 0 && at <= 0x7fffffff) slot = (int)at;
+    }
+    if (a.parents) position = ctx;
+  }
+  if (a.parents) {
+    // Up to the root: parents lie before their children, so the words of the mask come from the last to the first.
+    uint64_t* row = a.mask + (int64_t)t * a.words;
+    int word = a.words - 1, depth = 0;
+    uint64_t bits = 0;
+    if (b < a.B) {
+      for (int n = i;; ++depth) {
+        if ((a.win < 0 || depth <= a.win) && (n >> 6) < a.words) {
+          for (; word > (n >> 6); --word) {
+            row[word] = bits;
+            bits = 0;
+          }
+          bits |= (uint64_t)1 << (n & 63);
+        }
+        const int up = a.parents[start + n];
+        if (up < 0 || up >= n) break;
+        n = up;
+      }
+      position += depth;
+    }
+    for (; word >= 0; --word) {
+      row[word] = bits;
+      bits = 0;
+    }
+  }
+  a.positions[t] = position;
+  a.slots[t] = slot;
+}
+
+// `rows`: this workgroup writes the rows too.
+__global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, int rows) {
+  extern __shared__ __align__(16) int plan_lds[];
+  __shared__ int sums[kStepWaves];
+  int* cu = plan_lds;             // [B] sums of the lengths
+  int* touched = plan_lds + a.B;  // [B] sums of the touched blocks
+  const int tid = threadIdx.x, bs = a.block_size;
+  const int most = a.T;
+  const auto add_rows = [most](int x, int y) { return min(x + y, most); };  // at most T rows: sums that stay there
+  const auto add = [](int x, int y) { return x + y; };
+  int rows_before = 0, blocks_before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
+    const int b = b0 + tid;
+    const bool live = b < a.B;
+    const int ctx = live ? plan_len(a.ctx[b]) : 0;
+    int total;
+    const int sum = add_rows(rows_before, step_scan(live ? min(plan_len(a.new_lens[b]), most) : 0, sums, total, add_rows));
+    // The sum before this one is the neighbour's: through LDS.
+    if (live) cu[b] = sum;
+    __syncthreads();
+    const int len = live ? sum - (b > 0 ? cu[b - 1] : 0) : 0;
+    rows_before = add_rows(rows_before, total);
+    int blocks = 0, past = 0;
+    if (len > 0) {
+      const int first = ctx / bs, last = (ctx + len - 1) / bs;
+      blocks = max(min(last, a.max_blocks - 1) - first + 1, 0);
+      past = last - first + 1 - blocks;
+    }
+    const int upto = blocks_before + step_scan(blocks, sums, total, add);
+    blocks_before += total;
+    if (live) {
+      touched[b] = upto;
+      a.cu[b] = sum;
+      a.kv[b] = ctx + len;
+      a.missing[b] = past;
+    }
+  }
+  __syncthreads();
+  const int count = min(max(a.free_count[0], 0), a.room);
+  int taken = 0;
+  for (int p0 = 0; p0 < blocks_before; p0 += kStepThreads) {
+    const int p = p0 + tid;
+    int32_t* entry = nullptr;
+    int b = 0;
+    if (p < blocks_before) {
+      b = plan_seq(touched, a.B, p);
+      const int blk = plan_len(a.ctx[b]) / bs + p - (b > 0 ? touched[b - 1] : 0);
+      entry = a.table + (int64_t)b * a.max_blocks + blk;
+    }
+    const bool lacks = entry && *entry < 0;
+    int total;
+    const int rank = taken + step_scan(lacks ? 1 : 0, sums, total, add) - 1;
+    taken += total;
+    if (lacks) {
+      if (rank < count) *entry = a.free_list[count - 1 - rank];
+      else atomicAdd(a.missing + b, 1);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) a.free_count[0] = max(count - taken, 0);
+  if (rows)
+    for (int t = tid; t < a.T; t += kStepThreads) plan_row(a, cu, t);
+}
+
+constexpr int kPlanRowThreads = 256;
+constexpr int kPlanRowCu = 2048;
+__global__ __launch_bounds__(kPlanRowThreads) void plan_rows_kernel(PlanArgs a) {
+  __shared__ int copy[kPlanRowCu];
+  const bool copied = a.B <= kPlanRowCu;
+  if (copied) {
+    for (int b = threadIdx.x; b < a.B; b += kPlanRowThreads) copy[b] = a.cu[b];
+    __syncthreads();
+  }
+  const int t = blockIdx.x * kPlanRowThreads + threadIdx.x;
+  if (t < a.T) plan_row(a, copied ? copy : a.cu, t);
+}
+
+// Rows that the workgroup of the plan writes by itself.
+constexpr int kPlanFewRows = 4096;
+
+// Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, sizes and pointers; words >= 1 with parents.
+hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_t* table, const int32_t* free_list,
+                             int32_t* free_count, const int32_t* parents, int64_t B, int64_t T, int64_t max_blocks,
+                             int64_t block_size, int64_t room, int64_t words, int64_t win, int32_t* cu, int32_t* kv,
+                             int32_t* positions, int32_t* slots, int32_t* missing, uint64_t* mask,
+                             hipStream_t stream) {
+  const PlanArgs a = {new_lens, ctx, table, free_list, free_count, parents, cu, kv, positions, slots, missing, mask,
+                      (int)B, (int)T, (int)max_blocks, (int)block_size, (int)room, (int)words, (int)win};
+  const int lds = 2 * (int)B * (int)sizeof(int);
+  hipError_t e = set_dynamic_lds_once<plan_pages_kernel>(2 * 16384 * (int)sizeof(int));
+  if (e != hipSuccess) return e;
+  const bool few = T <= kPlanFewRows;
+  hipLaunchKernelGGL(plan_pages_kernel, dim3(1), dim3(kStepThreads), lds, stream, a, few ? 1 : 0);
+  if (!few)
+    hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((T + kPlanRowThreads - 1) / kPlanRowThreads)),
+                       dim3(kPlanRowThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------- free
+//
+// The pages behind the blocks of keep_b keys, up to the first negative entry, go back to the list: of n pages in the
+// order (sequence, block) the i-th to place count + n - 1 - i, so that giving back what a plan took leaves the list as it
+// was.  Pages that would lie past the list's room stay in the table.  One workgroup: a lane group a sequence counts, the
+// counts are summed, and the groups move the entries.
+
+struct FreeArgs {
+  const int32_t* keep;  // [B]
+  int32_t* table;       // [B, max_blocks]
+  int32_t* free_list;   // [room]
+  int32_t* free_count;  // [1]
+  int B, max_blocks, block_size, room;
+};
+
+// kGroup lanes a sequence.
+template <int kGroup>
+__global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
+  extern __shared__ __align__(16) int upto[];  // [B] pages of the sequences up to this one
+  __shared__ int sums[kStepWaves];
+  constexpr int kSeqs = kStepThreads / kGroup;
+  const int tid = threadIdx.x, in = tid % kGroup, lane = tid & (kWave - 1);
+  const auto first_block = [&](int b) {
+    const int keep = plan_len(a.keep[b]);
+    return keep / a.block_size + (keep % a.block_size ? 1 : 0);
+  };
+  for (int b = tid / kGroup; b < a.B; b += kSeqs) {
+    const int32_t* row = a.table + (int64_t)b * a.max_blocks;
+    const int from = first_block(b);
+    int n = 0;
+    for (int j = from; j < a.max_blocks; j += kGroup) {
+      const bool held = j + in < a.max_blocks && row[j + in] >= 0;
+      const uint64_t group = __ballot(held) >> (lane & ~(kGroup - 1));
+      const uint64_t ends = ~group & (kGroup == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (kGroup & 63)) - 1);
+      if (ends) {
+        n += __ffsll((unsigned long long)ends) - 1;
+        break;
+      }
+      n += kGroup;
+    }
+    if (in == 0) upto[b] = n;
+  }
+  __syncthreads();
+  int all = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
+    const int b = b0 + tid;
+    int total;
+    const int sum = all + step_scan(b < a.B ? upto[b] : 0, sums, total, [](int x, int y) { return x + y; });
+    all += total;
+    if (b < a.B) upto[b] = sum;
+  }
+  __syncthreads();
+  const int count = min(max(a.free_count[0], 0), a.room);
+  __syncthreads();
+  for (int b = tid / kGroup; b < a.B; b += kSeqs) {
+    const int before = b > 0 ? upto[b - 1] : 0, n = upto[b] - before;
+    int32_t* row = a.table + (int64_t)b * a.max_blocks + first_block(b);
+    for (int j = in; j < n; j += kGroup) {
+      const int64_t to = (int64_t)count + all - 1 - (before + j);
+      if (to < a.room) {
+        a.free_list[to] = row[j];
+        row[j] = -1;
+      }
+    }
+  }
+  if (tid == 0) a.free_count[0] = (int)min((int64_t)count + all, (int64_t)a.room);
+}
+
+// Caller validated: 1 <= B <= 16384, B * max_blocks < 2^31, sizes and pointers.
+hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_list, int32_t* free_count, int64_t B,
+                             int64_t max_blocks, int64_t block_size, int64_t room, hipStream_t stream) {
+  const FreeArgs a = {keep, table, free_list, free_count, (int)B, (int)max_blocks, (int)block_size, (int)room};
+  const int lds = (int)B * (int)sizeof(int);
+  const auto run = [&](auto kernel, hipError_t e) {
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kStepThreads), lds, stream, a);
+    return hipGetLastError();
+  };
+  constexpr int kLds = 16384 * (int)sizeof(int);
+  // A pass of the workgroup over the sequences is a round trip: lanes enough for one pass, eight at least.
+  if (B <= kStepThreads / 64) return run(free_pages_kernel<64>, set_dynamic_lds_once<free_pages_kernel<64>>(kLds));
+  if (B <= kStepThreads / 16) return run(free_pages_kernel<16>, set_dynamic_lds_once<free_pages_kernel<16>>(kLds));
+  return run(free_pages_kernel<8>, set_dynamic_lds_once<free_pages_kernel<8>>(kLds));
+}
+
+// ---------------------------------------------------------------------------------------------- accept
+//
+// The walk of sequence b starts at its first row.  At row at: choice = the lowest place of the largest score of the row
+// (NaN and -infinity never; -1 where a row holds nothing else), or the given choice; the next row is the lowest one
+// behind `at` whose parent is `at` and whose drafted token is the choice.
+//
+// Scores are read where the walk comes by: of 61 rows of a sequence some four.  A workgroup a sequence (accept_walk_kernel)
+// reads a row with all its threads, then looks for the child; each step is one row's bytes through one CU and a
+// reduction.  Where all rows together are few, a first launch takes the largest of every row in pieces over the card
+// (row_max_kernel), and the walk only joins pieces.
+
+struct AcceptArgs {
+  const void* scores;      // [T, V], or choices [T]
+  int64_t stride;          // elements between rows
+  const int32_t* tokens;   // [T]
+  const int32_t* parents;  // [T]
+  const int32_t* cu;       // [B] inclusive sums
+  const uint64_t* pieces;  // [T, num_pieces] of the first launch, or null
+  int32_t* accepted;       // [B]
+  int32_t* path;           // [B, P]
+  int32_t* chosen;         // [B, P]
+  int T, B, V, P, num_pieces;
+};
+
+template <int kKind>
+struct Score;  // of 16 bytes: kN values
+template <>
+struct Score<1> {  // bf16
+  static constexpr int kN = 8;
+  typedef uint16_t T;
+  static __device__ __forceinline__ float at(const u32x4& w, int i) {
+    return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  static __device__ __forceinline__ float one(const T* p) { return __uint_as_float((uint32_t)*p << 16); }
+};
+template <>
+struct Score<2> {  // fp16
+  static constexpr int kN = 8;
+  typedef uint16_t T;
+  static __device__ __forceinline__ float at(const u32x4& w, int i) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2]));
+  }
+  static __device__ __forceinline__ float one(const T* p) { return (float)__builtin_bit_cast(_Float16, *p); }
+};
+template <>
+struct Score<3> {  // fp32
+  static constexpr int kN = 4;
+  typedef float T;
+  static __device__ __forceinline__ float at(const u32x4& w, int i) { return __uint_as_float(w[i]); }
+  static __device__ __forceinline__ float one(const T* p) { return *p; }
+};
+
+// The larger value first, then the lower place; 0 where there is none.
+__device__ __forceinline__ uint64_t score_rank(float v, int place) {
+  return v > -__builtin_huge_valf() ? (uint64_t)float_key(v) << 32 | (uint32_t)~place : 0;
+}
+__device__ __forceinline__ int score_place(uint64_t rank) { return rank ? (int)~(uint32_t)rank : -1; }
+
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t u = __shfl_xor((unsigned long long)v, o, kWave);
+    v = u > v ? u : v;
+  }
+  return v;
+}
+
+// The rank of the elements [from, to) of a row, this thread's part of them.  Whole 16-byte chunks in turn, the elements
+// before and behind them one a thread.
+template <class S>
+__device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from, int to, int tid, int threads) {
+  constexpr int kN = S::kN, kAhead = 8;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + from);
+  const int head = min((int)(((16 - (at & 15)) & 15) / sizeof(typename S::T)), to - from);
+  const int chunks = (to - from - head) / kN, tail = from + head + chunks * kN;
+  const u32x4* body = reinterpret_cast<const u32x4*>(row + from + head);
+  float best = -__builtin_huge_valf();
+  int where = -1;
+  for (int c0 = tid; c0 < chunks; c0 += kAhead * threads) {
+    u32x4 w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) w[j] = body[min(c0 + j * threads, chunks - 1)];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (c0 + j * threads >= chunks) break;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const float v = S::at(w[j], i);
+        if (v > best) {
+          best = v;
+          where = (c0 + j * threads) * kN + i;
+        }
+      }
+    }
+  }
+  uint64_t rank = score_rank(best, from + head + where);
+  if (tid < head) {
+    const uint64_t r = score_rank(S::one(row + from + tid), from + tid);
+    rank = r > rank ? r : rank;
+  }
+  if (tid < to - tail) {
+    const uint64_t r = score_rank(S::one(row + tail + tid), tail + tid);
+    rank = r > rank ? r : rank;
+  }
+  return rank;
+}
+
+template <int kKind>
+__global__ __launch_bounds__(256) void row_max_kernel(const void* scores, int64_t stride, int V, int piece, uint64_t* out) {
+  typedef Score<kKind> S;
+  __shared__ uint64_t waves[4];
+  const int from = blockIdx.x * piece, to = min(from + piece, V);
+  const typename S::T* row = static_cast<const typename S::T*>(scores) + blockIdx.y * stride;
+  const uint64_t rank = wave_max_u64(row_rank<S>(row, from, to, threadIdx.x, 256));
+  if ((threadIdx.x & (kWave - 1)) == 0) waves[threadIdx.x / kWave] = rank;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint64_t m = waves[0];
+    for (int w = 1; w < 4; ++w) m = waves[w] > m ? waves[w] : m;
+    out[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = m;
+  }
+}
+
+// kKind 0: choices are given, or pieces of the first launch.
+template <int kKind, int kThreads>
+__global__ __launch_bounds__(kThreads) void accept_walk_kernel(AcceptArgs a) {
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ uint64_t ranks[kWaves];
+  __shared__ int child[3];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int start = b > 0 ? min(max(a.cu[b - 1], 0), a.T) : 0, end = min(max(a.cu[b], start), a.T), S = end - start;
+  int32_t *path = a.path + (int64_t)b * a.P, *chosen = a.chosen + (int64_t)b * a.P;
+  const int32_t *parents = a.parents + start, *tokens = a.tokens + start;
+  // Row tid's, for the first rows; the others are read as the walk goes.
+  const int my_parent = tid < S ? parents[tid] : -1, my_token = tid < S ? tokens[tid] : -1;
+  if (tid < 3) child[tid] = S;
+  __syncthreads();
+  int at = 0, k = 0;
+  while (at < S && k < a.P) {
+    int choice;
+    if constexpr (kKind != 0) {
+      typedef Score<kKind ? kKind : 1> R;
+      const typename R::T* row = static_cast<const typename R::T*>(a.scores) + (start + at) * a.stride;
+      const uint64_t rank = wave_max_u64(row_rank<R>(row, 0, a.V, tid, kThreads));
+      if ((tid & (kWave - 1)) == 0) ranks[tid / kWave] = rank;
+      __syncthreads();
+      uint64_t m = ranks[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) m = ranks[w] > m ? ranks[w] : m;
+      choice = score_place(m);
+    } else if (a.pieces) {
+      uint64_t m = 0;
+      const uint64_t* row = a.pieces + (int64_t)(start + at) * a.num_pieces;
+      for (int i = tid & (kWave - 1); i < a.num_pieces; i += kWave) m = row[i] > m ? row[i] : m;
+      choice = score_place(wave_max_u64(m));
+    } else {
+      choice = static_cast<const int32_t*>(a.scores)[start + at];
+    }
+    if (tid == 0) {
+      path[k] = at;
+      chosen[k] = choice;
+    }
+    int found = S;
+    if (tid > at && tid < S && my_parent == at && my_token == choice && choice >= 0) found = tid;
+    for (int i = tid + kThreads; i < S && found == S; i += kThreads)
+      if (i > at && parents[i] == at && tokens[i] == choice && choice >= 0) found = i;
+    if (found < S) atomicMin(&child[k % 3], found);
+    // The next step's place was last read two steps ago, ahead of the last step's barrier.
+    if (tid == 0) child[(k + 1) % 3] = S;
+    __syncthreads();
+    at = child[k % 3];
+    ++k;
+  }
+  for (int i = k + tid; i < a.P; i += kThreads) path[i] = chosen[i] = -1;
+  if (tid == 0) a.accepted[b] = k;
+}
+
+// Bytes of all rows up to which a first launch reads them all.
+constexpr int64_t kAcceptFewBytes = 32 << 20;
+constexpr int kAcceptPiece = 16384;  // bytes of a workgroup's piece of a row
+
+struct AcceptPlan {
+  bool all;       // every row in a first launch
+  int piece;      // elements
+  int64_t num_pieces;
+};
+static AcceptPlan accept_plan(int size, int64_t T, int64_t V) {
+  AcceptPlan p = {};
+  p.all = T * V * size <= kAcceptFewBytes && T <= 65535;  // a row of the grid each
+  p.piece = kAcceptPiece / size;
+  p.num_pieces = (V + p.piece - 1) / p.piece;
+  return p;
+}
+
+size_t tree_accept_workspace_bytes(int size, int64_t T, int64_t V) {
+  const AcceptPlan p = accept_plan(size, T, V);
+  return p.all ? (size_t)(T * p.num_pieces) * sizeof(uint64_t) : 0;
+}
+
+// kind 0: choices.  Caller validated: T < 2^30, V <= 2^30, B <= 65535, the workspace as tree_accept_workspace_bytes says.
+hipError_t launch_tree_accept(int kind, const void* scores, int64_t stride, int64_t T, int64_t V, const int32_t* tokens,
+                              const int32_t* parents, const int32_t* cu, int64_t B, int64_t P, int32_t* accepted,
+                              int32_t* path, int32_t* chosen, void* workspace, hipStream_t stream) {
+  AcceptArgs a = {scores, stride, tokens, parents, cu, nullptr, accepted, path, chosen,
+                  (int)T, (int)B, (int)V, (int)P, 0};
+  const dim3 grid((unsigned)B);
+  const int size = kind == 3 ? 4 : 2;
+  if (kind != 0) {
+    const AcceptPlan p = accept_plan(size, T, V);
+    if (p.all && T > 0) {
+      uint64_t* pieces = static_cast<uint64_t*>(workspace);
+      const dim3 all((unsigned)p.num_pieces, (unsigned)T);
+      if (kind == 1) hipLaunchKernelGGL(row_max_kernel<1>, all, dim3(256), 0, stream, scores, stride, (int)V, p.piece, pieces);
+      else if (kind == 2) hipLaunchKernelGGL(row_max_kernel<2>, all, dim3(256), 0, stream, scores, stride, (int)V, p.piece, pieces);
+      else hipLaunchKernelGGL(row_max_kernel<3>, all, dim3(256), 0, stream, scores, stride, (int)V, p.piece, pieces);
+      a.pieces = pieces;
+      a.num_pieces = (int)p.num_pieces;
+      kind = 0;
+    }
+  }
+  if (kind == 0) hipLaunchKernelGGL((accept_walk_kernel<0, 256>), grid, dim3(256), 0, stream, a);
+  else if (kind == 1) hipLaunchKernelGGL((accept_walk_kernel<1, 1024>), grid, dim3(1024), 0, stream, a);
+  else if (kind == 2) hipLaunchKernelGGL((accept_walk_kernel<2, 1024>), grid, dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL((accept_walk_kernel<3, 1024>), grid, dim3(1024), 0, stream, a);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------- commit
+//
+// In every cache, for k = 0, 1, ..: row(ctx_b + k) = row(ctx_b + path[b, k]), where path[b, k] > k.  A wave takes up to
+// 1 KB of the columns of a cache's rows of one sequence, a lane 16 bytes of each, so that no lane reads what another one
+// writes.  Eight rows are read before the eight are written: a source lies behind its own place and so behind all places
+// written before, which makes this the same as one row after the other.  Bound by latencies: lengths, path, table, rows.
+
+constexpr int kCommitCaches = 128;  // of a launch: their descriptions are kernel arguments
+constexpr int kCommitWaves = 4;
+
+struct CommitArgs {
+  uint8_t* cache[kCommitCaches];
+  int32_t row_bytes[kCommitCaches];
+  int32_t unit[kCommitCaches + 1];  // first unit of a cache: a wave's columns of its rows
+  const int32_t* table;     // [B, max_blocks]
+  const int32_t* ctx;       // [B]
+  const int32_t* path;      // [B, P]
+  const int32_t* accepted;  // [B]
+  int caches, P, max_blocks, block_size, num_blocks;
+};
+
+template <class V>
+__device__ __forceinline__ void commit_columns(const CommitArgs& a, uint8_t* cache, int row_bytes, int column, int src,
+                                               int dst, int n) {
+  // Lanes hold the rows of n moves; this lane moves the bytes at `column` of each.
+  const bool live = column + (int)sizeof(V) <= row_bytes;
+  for (int k0 = 0; k0 < n; k0 += 8) {
+    V v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int s = __shfl(src, min(k0 + j, kWave - 1), kWave);
+      if (k0 + j < n && s >= 0 && live) v[j] = *reinterpret_cast<const V*>(cache + (int64_t)s * row_bytes + column);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int s = __shfl(src, min(k0 + j, kWave - 1), kWave), d = __shfl(dst, min(k0 + j, kWave - 1), kWave);
+      if (k0 + j < n && s >= 0 && live) *reinterpret_cast<V*>(cache + (int64_t)d * row_bytes + column) = v[j];
+    }
+  }
+}
+
+__global__ __launch_bounds__(kCommitWaves * kWave) void commit_kernel(CommitArgs a) {
+  const int lane = threadIdx.x & (kWave - 1), b = blockIdx.y;
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kCommitWaves + threadIdx.x / kWave);
+  if (unit >= a.unit[a.caches]) return;
+  int c0 = 0, c1 = a.caches - 1;
+  while (c0 < c1) {
+    const int mid = (c0 + c1 + 1) >> 1;
+    if (a.unit[mid] <= unit) c0 = mid;
+    else c1 = mid - 1;
+  }
+  uint8_t* cache = a.cache[c0];
+  const int row_bytes = a.row_bytes[c0], part = unit - a.unit[c0];
+  const bool wide = (row_bytes & 15) == 0 && (reinterpret_cast<uintptr_t>(cache) & 15) == 0;
+  const int ctx = plan_len(a.ctx[b]), n = min(max(a.accepted[b], 0), a.P);
+  const int32_t* table = a.table + (int64_t)b * a.max_blocks;
+  // Row of key j in the pools, -1 without a page.
+  const auto row = [&](int j) {
+    const int blk = j / a.block_size;
+    if (blk >= a.max_blocks) return -1;
+    const int page = table[blk];
+    return (uint32_t)page < (uint32_t)a.num_blocks ? page * a.block_size + (j - blk * a.block_size) : -1;
+  };
+  for (int k0 = 0; k0 < n; k0 += kWave) {
+    const int k = k0 + lane, from = k < n ? a.path[(int64_t)b * a.P + k] : -1;
+    int src = -1, dst = -1;
+    if (from > k && from < kPlanMost) {
+      src = row(ctx + from);
+      dst = row(ctx + k);
+      if (dst < 0) src = -1;
+    }
+    if (__ballot(src >= 0) == 0) continue;
+    if (wide) commit_columns<u32x4>(a, cache, row_bytes, 16 * (part * kWave + lane), src, dst, min(n - k0, kWave));
+    else commit_columns<uint32_t>(a, cache, row_bytes, 4 * (part * kWave + lane), src, dst, min(n - k0, kWave));
+  }
+}
+
+// Caller validated: sizes and pointers; rows are multiples of 4 bytes that start on 4; B <= 65535.
+hipError_t launch_paged_commit(void* const* caches, const int64_t* row_bytes, int64_t num_caches, const int32_t* table,
+                               const int32_t* ctx, const int32_t* path, const int32_t* accepted, int64_t B, int64_t P,
+                               int64_t num_blocks, int64_t block_size, int64_t max_blocks, hipStream_t stream) {
+  for (int64_t c0 = 0; c0 < num_caches; c0 += kCommitCaches) {
+    CommitArgs a;
+    a.caches = (int)(num_caches - c0 < kCommitCaches ? num_caches - c0 : kCommitCaches);
+    int unit = 0;
+    for (int c = 0; c < a.caches; ++c) {
+      a.cache[c] = static_cast<uint8_t*>(caches[c0 + c]);
+      a.row_bytes[c] = (int32_t)row_bytes[c0 + c];
+      a.unit[c] = unit;
+      const bool wide = (a.row_bytes[c] & 15) == 0 && (reinterpret_cast<uintptr_t>(a.cache[c]) & 15) == 0;
+      const int per = (wide ? 16 : 4) * kWave;
+      unit += (a.row_bytes[c] + per - 1) / per;
+    }
+    a.unit[a.caches] = unit;
+    a.table = table;
+    a.ctx = ctx;
+    a.path = path;
+    a.accepted = accepted;
+    a.P = (int)P;
+    a.max_blocks = (int)max_blocks;
+    a.block_size = (int)block_size;
+    a.num_blocks = (int)num_blocks;
+    const dim3 grid((unsigned)((unit + kCommitWaves - 1) / kCommitWaves), (unsigned)B);
+    hipLaunchKernelGGL(commit_kernel, grid, dim3(kCommitWaves * kWave), 0, stream, a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace dsa

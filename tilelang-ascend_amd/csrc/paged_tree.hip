@@ -1,0 +1,27 @@
+// Attention of the nodes of trees of drafted tokens over a paged cache: the launch.  The kernels are those of
+// paged_gqa_kernels.hpp in their tree form.
+#include "paged_gqa_kernels.hpp"
+
+namespace dsa {
+
+// Caller validated: the sizes as launch_paged_gqa has them (its workspace too), mask [T, words] 64-bit words,
+// 1 <= words <= 64, pos [T] where there is a window.
+hipError_t launch_paged_tree(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
+                             const uint64_t* mask, int64_t words, const int32_t* pos, const int32_t* cu_q,
+                             const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B, int64_t S, int64_t H,
+                             int64_t G, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                             int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse,
+                             void* workspace, hipStream_t stream) {
+  if (T == 0 || H == 0) return hipSuccess;
+  const PgPlan p = pg_plan(T, B, H, G, max_blocks * block_size);
+  PgArgs a = pg_args({T, B, S, H, G, D, num_blocks, block_size, max_blocks}, q, kc, vc, table, cu_q, q_len, kv_len,
+                     win_left, sinks, sm_scale, out, lse, workspace, p);
+  a.mask = reinterpret_cast<const uint32_t*>(mask);
+  a.words = 2 * (int)words;
+  a.pos = pos;
+  if (D == 128)
+    return is_fp16 ? pg_dispatch<true, 128, true>(a, p.rows, stream) : pg_dispatch<false, 128, true>(a, p.rows, stream);
+  return is_fp16 ? pg_dispatch<true, 64, true>(a, p.rows, stream) : pg_dispatch<false, 64, true>(a, p.rows, stream);
+}
+
+}  // namespace dsa

@@ -580,6 +580,207 @@ std::tuple<at::Tensor, at::Tensor> paged_gqa_fwd_meta(const at::Tensor& q, const
           at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat))};
 }
 
+// paged_gqa_fwd for the nodes of trees: tree_mask [T, W] or [B, S, W] int64, positions of the rows with a window.
+std::tuple<at::Tensor, at::Tensor> paged_tree_fwd(const at::Tensor& q, const at::Tensor& k_cache,
+                                                  const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                  const at::Tensor& tree_mask, const at::Tensor& actual_seq_lengths_kv,
+                                                  double sm_scale,
+                                                  const c10::optional<at::Tensor>& actual_seq_lengths_query,
+                                                  const c10::optional<at::Tensor>& positions, int64_t win_left,
+                                                  const c10::optional<at::Tensor>& sinks) {
+  require(q, "q");
+  require(k_cache, "k_cache");
+  require(v_cache, "v_cache");
+  require_on(k_cache, q, "k_cache");
+  require_on(v_cache, q, "v_cache");
+  require_on(tree_mask, q, "tree_mask");
+  TORCH_CHECK((q.dim() == 3 || q.dim() == 4) && k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() &&
+                  k_cache.size(3) == q.size(-1) && block_table.dim() == 2,
+              "dsa.paged_tree_fwd: q [T, H, D] or [B, S, H, D], caches [blocks, block_size, G, D], block_table [B, n]");
+  TORCH_CHECK(k_cache.scalar_type() == q.scalar_type() && v_cache.scalar_type() == q.scalar_type(),
+              "dsa.paged_tree_fwd: cache dtypes must equal q dtype");
+  TORCH_CHECK(tree_mask.scalar_type() == at::kLong && tree_mask.dim() == q.dim() - 1 &&
+                  tree_mask.sizes().slice(0, q.dim() - 2) == q.sizes().slice(0, q.dim() - 2),
+              "dsa.paged_tree_fwd: tree_mask must hold int64 words for each of q's rows (got ", tree_mask.sizes(), ")");
+  const bool packed = q.dim() == 3;
+  const int64_t B = block_table.size(0), mb = block_table.size(1), S = packed ? 0 : q.size(1),
+                T = packed ? q.size(0) : B * S;
+  TORCH_CHECK(packed ? actual_seq_lengths_query.has_value() : q.size(0) == B,
+              "dsa.paged_tree_fwd: packed queries need prefix sums, padded ones one row of block_table per sequence");
+  TORCH_CHECK(win_left < 0 || positions.has_value(), "dsa.paged_tree_fwd: win_left needs positions");
+  c10::OptionalDeviceGuard guard(q.device());
+  auto bt = aux_i32(saturated_i32(block_table), q, -1, "block_table");
+  auto kl = aux_i32(saturated_i32(actual_seq_lengths_kv), q, B, "actual_seq_lengths_kv");
+  auto ql = aux_i32(actual_seq_lengths_query ? c10::make_optional(saturated_i32(*actual_seq_lengths_query))
+                                             : actual_seq_lengths_query,
+                    q, B, "actual_seq_lengths_query");
+  auto pos = aux_i32(positions ? c10::make_optional(saturated_i32(*positions)) : positions, q, T, "positions");
+  auto mask = tree_mask.contiguous();
+  const int64_t H = q.size(-2), D = q.size(-1), G = k_cache.size(2);
+  auto sk = aux_f32(sinks, q, H, "sinks");
+  auto out = at::empty(q.sizes(), q.options());
+  auto lse = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat));
+  const size_t bytes = dsa_paged_tree_workspace_size(T, B, H, G, D, mb * k_cache.size(1));
+  auto ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  int32_t* qlp = ptr_or_null<int32_t>(ql);
+  check_rc(dsa_paged_tree_fwd(kind_of(q), ptr(q), ptr(k_cache), ptr(v_cache), static_cast<int32_t*>(ptr(bt)),
+                              static_cast<uint64_t*>(ptr(mask)), mask.size(-1), ptr_or_null<int32_t>(pos),
+                              packed ? qlp : nullptr, packed ? nullptr : qlp, static_cast<int32_t*>(ptr(kl)), T, B, S,
+                              H, G, D, k_cache.size(0), k_cache.size(1), mb, win_left, ptr_or_null<float>(sk),
+                              (float)sm_scale, ptr(out), static_cast<float*>(ptr(lse)), bytes ? ptr(ws) : nullptr, bytes,
+                              stream_of(q)),
+           "paged_tree_fwd");
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_tree_fwd_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&,
+                                                       const at::Tensor&, const at::Tensor&, const at::Tensor&, double,
+                                                       const c10::optional<at::Tensor>&,
+                                                       const c10::optional<at::Tensor>&, int64_t,
+                                                       const c10::optional<at::Tensor>&) {
+  return {at::empty(q.sizes(), q.options()),
+          at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat))};
+}
+
+// A list that changes in place: int32, contiguous, beside the table.
+void require_list(const at::Tensor& t, const at::Tensor& table, const char* name) {
+  require(t, name);
+  require_on(t, table, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt, "dsa: ", name, " changes in place and must be int32 (got ", t.scalar_type(),
+              ")");
+}
+
+typedef std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> Plan;
+Plan plan_outputs(const at::Tensor& table, int64_t T, bool tree, int64_t max_nodes) {
+  TORCH_CHECK(T >= 0 && (!tree || (max_nodes >= 1 && max_nodes <= 4096)),
+              "dsa.paged_plan: num_tokens must be a count, parents need max_nodes in [1, 4096]");
+  const int64_t B = table.size(0);
+  const auto make = [&](at::IntArrayRef n) { return at::empty(n, table.options().dtype(at::kInt)); };
+  return {make({B}), make({B}), make({T}), make({T}), make({B}),
+          at::empty({T, tree ? (max_nodes + 63) / 64 : 0}, table.options().dtype(at::kLong))};
+}
+
+// The plan's parts; without parents the mask has no words.
+Plan paged_plan(const at::Tensor& new_lens, const at::Tensor& context_lens, at::Tensor block_table,
+                const at::Tensor& free_blocks, at::Tensor free_count, int64_t block_size, int64_t num_tokens,
+                const c10::optional<at::Tensor>& parents, int64_t max_nodes, int64_t win_left) {
+  require_list(block_table, block_table, "block_table");
+  require_list(free_blocks, block_table, "free_blocks");
+  require_list(free_count, block_table, "free_count");
+  TORCH_CHECK(block_table.dim() == 2 && free_blocks.dim() == 1 && free_count.numel() == 1,
+              "dsa.paged_plan: block_table [B, max_blocks], free_blocks [room], free_count one number");
+  TORCH_CHECK(parents || win_left < 0, "dsa.paged_plan: win_left cuts tree masks: it needs parents");
+  c10::OptionalDeviceGuard guard(block_table.device());
+  const int64_t B = block_table.size(0);
+  auto nl = aux_i32(saturated_i32(new_lens), block_table, B, "new_lens");
+  auto ctx = aux_i32(saturated_i32(context_lens), block_table, B, "context_lens");
+  auto par = aux_i32(parents ? c10::make_optional(saturated_i32(*parents)) : parents, block_table, num_tokens, "parents");
+  Plan p = plan_outputs(block_table, num_tokens, parents.has_value(), max_nodes);
+  const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(ptr(t)); };
+  check_rc(dsa_paged_plan(i32(nl), i32(ctx), i32(block_table), i32(free_blocks), i32(free_count),
+                          num_tokens ? ptr_or_null<int32_t>(par) : nullptr, B, num_tokens, block_table.size(1),
+                          block_size, free_blocks.numel(), std::get<5>(p).size(1), win_left, i32(std::get<0>(p)),
+                          i32(std::get<1>(p)), i32(std::get<2>(p)), i32(std::get<3>(p)), i32(std::get<4>(p)),
+                          static_cast<uint64_t*>(ptr(std::get<5>(p))), stream_of(block_table)),
+           "paged_plan");
+  return p;
+}
+
+Plan paged_plan_meta(const at::Tensor&, const at::Tensor&, at::Tensor block_table, const at::Tensor&, at::Tensor, int64_t,
+                     int64_t num_tokens, const c10::optional<at::Tensor>& parents, int64_t max_nodes, int64_t) {
+  return plan_outputs(block_table, num_tokens, parents.has_value(), max_nodes);
+}
+
+void paged_free(const at::Tensor& keep_lens, at::Tensor block_table, at::Tensor free_blocks, at::Tensor free_count,
+                int64_t block_size) {
+  require_list(block_table, block_table, "block_table");
+  require_list(free_blocks, block_table, "free_blocks");
+  require_list(free_count, block_table, "free_count");
+  TORCH_CHECK(block_table.dim() == 2 && free_blocks.dim() == 1 && free_count.numel() == 1,
+              "dsa.paged_free: block_table [B, max_blocks], free_blocks [room], free_count one number");
+  c10::OptionalDeviceGuard guard(block_table.device());
+  auto keep = aux_i32(saturated_i32(keep_lens), block_table, block_table.size(0), "keep_lens");
+  const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(ptr(t)); };
+  check_rc(dsa_paged_free(i32(keep), i32(block_table), i32(free_blocks), i32(free_count), block_table.size(0),
+                          block_table.size(1), block_size, free_blocks.numel(), stream_of(block_table)),
+           "paged_free");
+}
+
+void paged_free_meta(const at::Tensor&, at::Tensor, at::Tensor, at::Tensor, int64_t) {}
+
+typedef std::tuple<at::Tensor, at::Tensor, at::Tensor> Accepted;
+Accepted accept_outputs(const at::Tensor& cu, int64_t max_path, const at::Tensor& like) {
+  TORCH_CHECK(max_path >= 1, "dsa.tree_accept: max_path must be a positive count");
+  const auto o = like.options().dtype(at::kInt);
+  return {at::empty({cu.numel()}, o), at::empty({cu.numel(), max_path}, o), at::empty({cu.numel(), max_path}, o)};
+}
+
+// Numbers past 31 bits become -1, which matches nothing.
+at::Tensor token_ids(const at::Tensor& t) {
+  if (t.scalar_type() != at::kLong) return saturated_i32(t);
+  return t.masked_fill(t.lt(0).logical_or(t.gt((int64_t)0x7fffffff)), -1).to(at::kInt);
+}
+
+// scores [T, V] whose rows may lie apart, or [T] integer choices.
+Accepted tree_accept(const at::Tensor& scores, const at::Tensor& tokens, const at::Tensor& parents,
+                     const at::Tensor& actual_seq_lengths_query, int64_t max_path) {
+  TORCH_CHECK(scores.is_cuda(), "dsa: scores must be on a HIP device");
+  const bool given = at::isIntegralType(scores.scalar_type(), /*includeBool=*/false);
+  TORCH_CHECK(scores.dim() == (given ? 1 : 2), "dsa.tree_accept: scores must be [T, V], or [T] integer choices");
+  TORCH_CHECK(actual_seq_lengths_query.dim() == 1, "dsa.tree_accept: actual_seq_lengths_query must be [B]");
+  c10::OptionalDeviceGuard guard(scores.device());
+  const int64_t T = scores.size(0), V = given ? 0 : scores.size(1), B = actual_seq_lengths_query.numel();
+  at::Tensor x = given ? token_ids(scores).contiguous() : scores;
+  if (!given && ((V > 1 && x.stride(1) != 1) || (T > 1 && x.stride(0) < V))) x = x.contiguous();
+  const int kind = given ? DSA_KIND_INT32 : kind_of(x);
+  auto tok = aux_i32(token_ids(tokens), scores, T, "tokens");
+  auto par = aux_i32(saturated_i32(parents), scores, T, "parents");
+  auto cu = aux_i32(saturated_i32(actual_seq_lengths_query), scores, B, "actual_seq_lengths_query");
+  Accepted r = accept_outputs(cu, max_path, scores);
+  const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(ptr(t)); };
+  const size_t bytes = dsa_tree_accept_workspace_size(kind, T, V);
+  auto ws = at::empty({(int64_t)bytes}, scores.options().dtype(at::kByte));
+  check_rc(dsa_tree_accept(kind, ptr(x), given ? 1 : x.stride(0), T, V, i32(tok), i32(par), i32(cu), B, max_path,
+                           i32(std::get<0>(r)), i32(std::get<1>(r)), i32(std::get<2>(r)), bytes ? ptr(ws) : nullptr,
+                           bytes, stream_of(scores)),
+           "tree_accept");
+  return r;
+}
+
+Accepted tree_accept_meta(const at::Tensor& scores, const at::Tensor&, const at::Tensor&, const at::Tensor& cu,
+                          int64_t max_path) {
+  return accept_outputs(cu, max_path, scores);
+}
+
+void paged_commit(at::TensorList caches, const at::Tensor& block_table, const at::Tensor& context_lens,
+                  const at::Tensor& path, const at::Tensor& accepted) {
+  TORCH_CHECK(caches.size() > 0, "dsa.paged_commit: caches must not be empty");
+  TORCH_CHECK(block_table.dim() == 2 && path.dim() == 2, "dsa.paged_commit: block_table [B, max_blocks], path [B, n]");
+  const at::Tensor& first = caches[0];
+  std::vector<void*> at_cache;
+  std::vector<int64_t> bytes;
+  for (const at::Tensor& c : caches) {
+    require(c, "caches");
+    require_on(c, first, "caches");
+    TORCH_CHECK(c.dim() >= 3 && c.numel() > 0 && c.size(0) == first.size(0) && c.size(1) == first.size(1),
+                "dsa.paged_commit: caches must be [blocks, block_size, ...] alike (got ", c.sizes(), ")");
+    at_cache.push_back(ptr(c));
+    bytes.push_back(c.numel() / (c.size(0) * c.size(1)) * (int64_t)c.element_size());
+  }
+  c10::OptionalDeviceGuard guard(first.device());
+  const int64_t B = block_table.size(0), P = path.size(1);
+  auto bt = aux_i32(saturated_i32(block_table), first, -1, "block_table");
+  auto ctx = aux_i32(saturated_i32(context_lens), first, B, "context_lens");
+  auto pa = aux_i32(saturated_i32(path), first, B * P, "path");
+  auto ac = aux_i32(saturated_i32(accepted), first, B, "accepted");
+  const auto i32 = [](const at::Tensor& t) { return static_cast<int32_t*>(ptr(t)); };
+  check_rc(dsa_paged_commit(at_cache.data(), bytes.data(), (int64_t)caches.size(), i32(bt), i32(ctx), i32(pa), i32(ac), B,
+                            P, first.size(0), first.size(1), block_table.size(1), stream_of(first)),
+           "paged_commit");
+}
+
+void paged_commit_meta(at::TensorList, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&) {}
+
 }  // namespace
 
 TORCH_LIBRARY(dsa, m) {
@@ -611,6 +812,22 @@ TORCH_LIBRARY(dsa, m) {
       "paged_gqa_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor actual_seq_lengths_kv, "
       "float sm_scale, Tensor? actual_seq_lengths_query=None, bool is_causal=True, int win_left=-1, "
       "Tensor? sinks=None) -> (Tensor, Tensor)");
+  m.def(
+      "paged_tree_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor tree_mask, "
+      "Tensor actual_seq_lengths_kv, float sm_scale, Tensor? actual_seq_lengths_query=None, Tensor? positions=None, "
+      "int win_left=-1, Tensor? sinks=None) -> (Tensor, Tensor)");
+  m.def(
+      "paged_plan(Tensor new_lens, Tensor context_lens, Tensor(a!) block_table, Tensor free_blocks, "
+      "Tensor(b!) free_count, int block_size, int num_tokens, Tensor? parents=None, int max_nodes=0, int win_left=-1) "
+      "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "paged_free(Tensor keep_lens, Tensor(a!) block_table, Tensor(b!) free_blocks, Tensor(c!) free_count, "
+      "int block_size) -> ()");
+  m.def(
+      "tree_accept(Tensor scores, Tensor tokens, Tensor parents, Tensor actual_seq_lengths_query, int max_path) "
+      "-> (Tensor, Tensor, Tensor)");
+  m.def(
+      "paged_commit(Tensor(a!)[] caches, Tensor block_table, Tensor context_lens, Tensor path, Tensor accepted) -> ()");
   m.def("sparse_attn(Tensor q, Tensor kv, Tensor? attn_sink, Tensor topk_idxs, float softmax_scale) -> (Tensor, Tensor)");
 }
 
@@ -625,6 +842,11 @@ TORCH_LIBRARY_IMPL(dsa, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_paged", &qk_norm_rope_paged);
   m.impl("paged_gqa_fwd", &paged_gqa_fwd);
+  m.impl("paged_tree_fwd", &paged_tree_fwd);
+  m.impl("paged_plan", &paged_plan);
+  m.impl("paged_free", &paged_free);
+  m.impl("tree_accept", &tree_accept);
+  m.impl("paged_commit", &paged_commit);
 }
 
 TORCH_LIBRARY_IMPL(dsa, Meta, m) {
@@ -638,4 +860,9 @@ TORCH_LIBRARY_IMPL(dsa, Meta, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_meta);
   m.impl("qk_norm_rope_paged", &qk_norm_rope_paged_meta);
   m.impl("paged_gqa_fwd", &paged_gqa_fwd_meta);
+  m.impl("paged_tree_fwd", &paged_tree_fwd_meta);
+  m.impl("paged_plan", &paged_plan_meta);
+  m.impl("paged_free", &paged_free_meta);
+  m.impl("tree_accept", &tree_accept_meta);
+  m.impl("paged_commit", &paged_commit_meta);
 }

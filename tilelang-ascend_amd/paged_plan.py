@@ -1,0 +1,130 @@
+"""Pages, slots, positions and tree masks of a serving step from its request lengths, on the GPU, gfx950.
+
+``paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, block_size, num_tokens)`` hands pages from a
+free list to the sequences' new tokens and returns what ``qk_norm_rope_paged`` and ``paged_gqa_fwd`` or
+``paged_tree_fwd`` take; ``paged_free`` gives pages back.  Neither reads anything on the host, so that steps of changing
+lengths replay from one captured graph.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+
+class PagedPlan(NamedTuple):
+    """What a step needs, all int32 but for the mask."""
+
+    cu_seqlens: torch.Tensor  # [B] inclusive prefix sums of the new lengths
+    kv_lens: torch.Tensor  # [B] context and new tokens
+    positions: torch.Tensor  # [T], -1 for rows behind the last sequence
+    slots: torch.Tensor  # [T] cache rows, -1 without one
+    missing: torch.Tensor  # [B] pages that the sequence lacks
+    tree_mask: Optional[torch.Tensor]  # [T, W] int64 with parents: a node's bits
+
+
+def _lists(what: str, block_table, free_blocks, free_count, block_size):
+    """Checks the arguments that change in place; returns their device."""
+    dev = _lib.require_device(block_table, free_blocks, free_count)
+    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
+    for name, t in (("block_table", block_table), ("free_blocks", free_blocks), ("free_count", free_count)):
+        if t.dtype != torch.int32:
+            raise ValueError(f"{what}: {name} changes in place and must be int32, got {t.dtype}")
+        _lib.require_contiguous(name, t)
+    if free_blocks.dim() != 1 or free_count.numel() != 1:
+        raise ValueError(f"free_blocks must be [room] and free_count one number, got {tuple(free_blocks.shape)} and "
+                         f"{tuple(free_count.shape)}")
+    if not isinstance(block_size, int) or not 1 <= block_size < 2**31:
+        raise ValueError(f"block_size must be a positive count, got {block_size}")
+    return dev
+
+
+def _ints(name: str, x, n: int) -> torch.Tensor:
+    t = torch.as_tensor(x)
+    if not _lib.is_integer(t) or t.numel() != n:
+        raise ValueError(f"{name} must hold {n} integers, got {tuple(t.shape)} {t.dtype}")
+    return _lib.saturated_int32(t).reshape(-1)
+
+
+def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: torch.Tensor, free_count: torch.Tensor,
+               block_size: int, num_tokens: int, *, parents: Optional[torch.Tensor] = None, max_nodes: int = 0,
+               win_left: Optional[int] = None) -> PagedPlan:
+    """Plans a step in which sequence b, with ``context_lens[b]`` tokens in the cache, gets ``new_lens[b]`` more.
+
+    The new tokens are packed: T = ``num_tokens`` rows, those of sequence 0 first; rows that the lengths do not fill
+    are padding, lengths past T are cut.  Entries of ``block_table`` [B, max_blocks] that are negative hold no page;
+    where new tokens need one it comes off the end of ``free_blocks`` (the first ``free_count`` entries are free), in the
+    order of sequences and blocks.  ``block_table`` and ``free_count`` (int32) change in place.  ``missing`` of the result
+    counts the pages that a sequence did not get, since the list ran out or its table ended: slots there are -1 (nothing
+    is written), and the step is not whole for that sequence.
+
+    ``parents`` [T] makes each sequence's new tokens a tree of drafted ones: the place of a token's parent in its
+    sequence, less than its own; any other number (-1) marks a root.  Positions are then the context's length and the
+    depth, and ``tree_mask`` [T, W], W = ceil(max_nodes / 64), has the bits of a node and its ancestors, with ``win_left``
+    those at most so many steps up.  ``max_nodes`` (at most 4096) bounds a sequence's nodes; nodes past 64 W are seen by
+    none.  At most 16384 sequences, fewer than 2^30 rows; lengths count up to 2^30.
+    """
+    win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
+    res = _lib.host_path().paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, block_size,
+                                      num_tokens, parents, max_nodes, win)
+    if res is not None:
+        return PagedPlan(*_lib.returned(res, "dsa_paged_plan"))
+    dev = _lists("paged_plan", block_table, free_blocks, free_count, block_size)
+    B = block_table.shape[0]
+    if not isinstance(num_tokens, int) or not 0 <= num_tokens < 2**30:
+        raise ValueError(f"num_tokens must be a count below 2^30, got {num_tokens}")
+    if B > 16384:
+        raise ValueError(f"at most 16384 sequences, got {B}")
+    T, words = num_tokens, 0
+    if parents is not None:
+        if not isinstance(max_nodes, int) or not 1 <= max_nodes <= 4096:
+            raise ValueError(f"parents need max_nodes in [1, 4096], got {max_nodes}")
+        words = -(-max_nodes // 64)
+    elif win_left is not None:
+        raise ValueError("win_left cuts tree masks: it needs parents")
+    if win_left is not None and not (isinstance(win_left, int) and 0 <= win_left < 2**31):
+        raise ValueError(f"win_left must be None or a count, got {win_left}")
+    new, ctx = _ints("new_lens", new_lens, B), _ints("context_lens", context_lens, B)
+    par = None if parents is None else _ints("parents", parents, T)
+    with torch.cuda.device(dev):
+        new, ctx, par = (None if x is None else x.to(dev).contiguous() for x in (new, ctx, par))
+        empty = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=dev)
+        out = PagedPlan(empty(B), empty(B), empty(T), empty(T), empty(B),
+                        None if par is None else empty(T, words, dtype=torch.int64))
+        rc = _lib.load_library().dsa_paged_plan(
+            _lib.ptr(new), _lib.ptr(ctx), _lib.ptr(block_table), _lib.ptr(free_blocks), _lib.ptr(free_count),
+            _lib.ptr(par) if T else None, B, T, block_table.shape[1], block_size, free_blocks.numel(), words,
+            win, _lib.ptr(out.cu_seqlens), _lib.ptr(out.kv_lens),
+            _lib.ptr(out.positions), _lib.ptr(out.slots), _lib.ptr(out.missing), _lib.ptr(out.tree_mask),
+            _lib.stream_handle(dev))
+        _lib.check(rc, "dsa_paged_plan")
+    return out
+
+
+def paged_free(keep_lens, block_table: torch.Tensor, free_blocks: torch.Tensor, free_count: torch.Tensor,
+               block_size: int) -> None:
+    """Gives back the pages behind each sequence's first ``keep_lens[b]`` tokens (0: all of them).
+
+    The pages of a row of ``block_table`` are its entries up to the first negative one; those given back become -1 and
+    go to ``free_blocks`` behind the ``free_count`` free ones, all in place (int32).  They are listed so that giving back
+    what a plan took restores the list.  Pages that the list has no room for stay where they are.  No page is counted: one
+    that stands in two rows would be listed twice.
+    """
+    res = _lib.host_path().paged_free(keep_lens, block_table, free_blocks, free_count, block_size)
+    if res is not None:
+        _lib.returned(res, "dsa_paged_free")
+        return
+    dev = _lists("paged_free", block_table, free_blocks, free_count, block_size)
+    B = block_table.shape[0]
+    if B > 16384:
+        raise ValueError(f"at most 16384 sequences, got {B}")
+    keep = _ints("keep_lens", keep_lens, B)
+    with torch.cuda.device(dev):
+        keep = keep.to(dev).contiguous()
+        rc = _lib.load_library().dsa_paged_free(_lib.ptr(keep), _lib.ptr(block_table), _lib.ptr(free_blocks),
+                                                _lib.ptr(free_count), B, block_table.shape[1], block_size,
+                                                free_blocks.numel(), _lib.stream_handle(dev))
+        _lib.check(rc, "dsa_paged_free")

@@ -1,0 +1,240 @@
+"""Trees of drafted tokens over a paged cache: attention, acceptance and the cache rows' order, gfx950.
+
+``paged_tree_fwd`` is ``paged_gqa_fwd`` for tokens that see their ancestors instead of all tokens before them;
+``tree_accept`` follows a model's choices through the trees; ``paged_commit`` moves the accepted tokens' cache rows
+behind the context, in all layers' caches at once.  ``paged_plan`` makes the masks.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+
+_KINDS = {torch.bfloat16: _lib.KIND_BF16, torch.float16: _lib.KIND_FP16}
+
+
+def paged_tree_fwd(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   tree_mask: torch.Tensor, sm_scale: Optional[float] = None, *,
+                   actual_seq_lengths_query: Optional[torch.Tensor] = None,
+                   actual_seq_lengths_kv: torch.Tensor = None, positions: Optional[torch.Tensor] = None,
+                   win_left: Optional[int] = None,
+                   sinks: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of the nodes of each sequence's tree; returns ``(out, lse)``.
+
+    The arguments are those of ``paged_gqa_fwd``: q [T, H, D] packed (``actual_seq_lengths_query`` inclusive prefix
+    sums) or [B, S, H, D], the caches hold the nodes' keys and values already.  A sequence with n keys and L nodes has
+    first = n - L keys before its tree; node i, whose key is key first + i, sees all of those, and key first + a of node a
+    where bit a % 64 of word a / 64 of its row of ``tree_mask`` is set ([T, W] or [B, S, W] int64; W up to 64, a
+    sequence's nodes past 64 W are seen by none).  With ``win_left`` it sees of the first keys only j >= position -
+    win_left, and ``positions`` ([T] or [B, S], those of ``paged_plan``) are needed; they count as the nearest of
+    first .. n - 1.  The mask is taken as it is: what a window leaves of the ancestors is ``paged_plan``'s to say.  Rows
+    that see nothing, pages outside the pool, values that are not finite and prefix sums are treated as in
+    ``paged_gqa_fwd``.
+    """
+    scale = q.shape[-1] ** -0.5 if sm_scale is None and q.dim() >= 3 and q.shape[-1] > 0 else sm_scale
+    win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
+    res = _lib.host_path().paged_tree(q, k_cache, v_cache, block_table, tree_mask, scale, actual_seq_lengths_query,
+                                      actual_seq_lengths_kv, positions, win, sinks)
+    if res is not None:
+        return _lib.returned(res, "dsa_paged_tree_fwd")
+    if q.dtype not in _KINDS:
+        raise ValueError(f"q must be bfloat16 or float16, got {q.dtype}")
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dtype != q.dtype:
+            raise ValueError(f"{name} dtype {c.dtype} must equal q dtype {q.dtype}")
+    if q.dim() not in (3, 4) or q.shape[-1] not in (64, 128):
+        raise ValueError(f"q must be [T, H, D] or [B, S, H, D] with D = 64 or 128, got {tuple(q.shape)}")
+    H, D = q.shape[-2], q.shape[-1]
+    if k_cache.dim() != 4 or k_cache.shape[3] != D or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache and v_cache must be [blocks, block_size, kv_group, {D}], got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    num_blocks, block_size, G, _ = k_cache.shape
+    if G < 1 or H < 1 or H % G != 0:
+        raise ValueError(f"H={H} must be a multiple of kv_group={G}")
+    if num_blocks < 1 or block_size < 1:
+        raise ValueError(f"the caches must hold at least one row, got {tuple(k_cache.shape)}")
+    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise ValueError(f"block_table must be [B, max_blocks], got {tuple(block_table.shape)}")
+    if not _lib.is_integer(block_table):
+        raise ValueError(f"block_table must hold integers, got {block_table.dtype}")
+    B = block_table.shape[0]
+    if actual_seq_lengths_kv is None:
+        raise ValueError("actual_seq_lengths_kv is required")
+    packed = q.dim() == 3
+    if packed and actual_seq_lengths_query is None:
+        raise ValueError("packed queries need actual_seq_lengths_query (inclusive prefix sums)")
+    if not packed and q.shape[0] != B:
+        raise ValueError(f"q batch {q.shape[0]} does not match block_table batch {B}")
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() != q.dim() - 1 or tree_mask.shape[:-1] != q.shape[:-2]:
+        raise ValueError(f"tree_mask must be {list(q.shape[:-2])} rows of int64 words, got {tuple(tree_mask.shape)} "
+                         f"{tree_mask.dtype}")
+    words = tree_mask.shape[-1]
+    if not 1 <= words <= 64 or (not packed and q.shape[1] > 64 * words):
+        raise ValueError(f"tree_mask must have 1 to 64 words a row, and bits for all S nodes, got {words}")
+    if not (isinstance(win, int) and -1 <= win < 2**31 - 4096) or (win_left is not None and win_left < 0):
+        raise ValueError(f"win_left must be None or a key count, got {win_left}")
+    if win_left is not None and positions is None:
+        raise ValueError("win_left needs positions")
+    if not 0 < scale <= 1e30:
+        raise ValueError(f"sm_scale must be positive, got {sm_scale}")
+    rows = math.prod(q.shape[:-2])
+
+    def ints(name, x, n):
+        if x is None:
+            return None
+        t = torch.as_tensor(x)
+        if not _lib.is_integer(t) or t.numel() != n:
+            raise ValueError(f"{name} must hold {n} integers, got {tuple(t.shape)} {t.dtype}")
+        return _lib.saturated_int32(t).reshape(-1)
+
+    ql = ints("actual_seq_lengths_query", actual_seq_lengths_query, B)
+    kl = ints("actual_seq_lengths_kv", actual_seq_lengths_kv, B)
+    pos = ints("positions", positions, rows)
+    if packed and ql.device.type == "cpu" and bool((ql[1:] < ql[:-1]).any()):
+        raise ValueError("actual_seq_lengths_query must be non-decreasing prefix sums")
+    dev = _lib.require_device(q, k_cache, v_cache, block_table, tree_mask, sinks)
+    if sinks is not None and (sinks.dtype != torch.float32 or tuple(sinks.shape) != (H,)):
+        raise ValueError(f"sinks must be [{H}] float32, got {tuple(sinks.shape)} {sinks.dtype}")
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)):
+        _lib.require_contiguous(name, t)
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.data_ptr() % 16 != 0:
+            raise ValueError(f"{name} must start on 16 bytes")
+
+    with torch.cuda.device(dev):
+        ql, kl, pos = (None if x is None else x.to(dev).contiguous() for x in (ql, kl, pos))
+        bt, mask = _lib.saturated_int32(block_table).contiguous(), tree_mask.contiguous()
+        sk = None if sinks is None else sinks.contiguous()
+        T = rows
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
+        lib = _lib.load_library()
+        ws_bytes = lib.dsa_paged_tree_workspace_size(T, B, H, G, D, bt.shape[1] * block_size)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib.dsa_paged_tree_fwd(_KINDS[q.dtype], _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(bt),
+                                    _lib.ptr(mask), words, _lib.ptr(pos), _lib.ptr(ql) if packed else None,
+                                    None if packed else _lib.ptr(ql), _lib.ptr(kl), T, B, 0 if packed else q.shape[1],
+                                    H, G, D, num_blocks, block_size, bt.shape[1], win, _lib.ptr(sk), float(scale),
+                                    _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), ws_bytes, _lib.stream_handle(dev))
+        _lib.check(rc, "dsa_paged_tree_fwd")
+    return out, lse
+
+
+_SCORES = {torch.bfloat16: _lib.KIND_BF16, torch.float16: _lib.KIND_FP16, torch.float32: _lib.KIND_FP32}
+
+
+def tree_accept(scores: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, *,
+                actual_seq_lengths_query: torch.Tensor,
+                max_path: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Follows a model's choices through the trees; returns ``(accepted [B], path, chosen [B, max_path])``, int32.
+
+    ``scores`` [T, V] are the model's at every node (bf16, fp16 or fp32; rows may lie apart): the choice at a node is the
+    place of the largest score, the lowest of equal ones, NaN and -infinity never (-1 where a row holds nothing else).
+    Or [T] integers: the choices themselves, of any sampler.  ``tokens`` [T] are the drafted tokens, ``parents`` [T] as
+    ``paged_plan`` takes them, ``actual_seq_lengths_query`` [B] the inclusive prefix sums.
+
+    Node 0 of a sequence is always on its path (the token that the step before chose); behind a node comes the lowest
+    later one whose parent it is and whose token is the choice.  ``accepted`` counts the nodes on the path, at most
+    ``max_path``; ``path`` has their places, which ``paged_commit`` takes; ``chosen`` the choices at them, the tokens
+    that the step yields: those of the nodes behind the first, and one more that is not in the cache yet.  Both are -1
+    behind the path.  Tokens and choices that do not lie in [0, 2^31) match nothing.
+    """
+    res = _lib.host_path().tree_accept(scores, tokens, parents, actual_seq_lengths_query, max_path)
+    if res is not None:
+        return _lib.returned(res, "dsa_tree_accept")
+    given = _lib.is_integer(scores)
+    if not given and scores.dtype not in _SCORES:
+        raise ValueError(f"scores must be bfloat16, float16 or float32, or integer choices, got {scores.dtype}")
+    if scores.dim() != (1 if given else 2) or (not given and not 1 <= scores.shape[1] < 2**30):
+        raise ValueError(f"scores must be [T, V], or [T] integer choices, got {tuple(scores.shape)} {scores.dtype}")
+    T = scores.shape[0]
+    cu = torch.as_tensor(actual_seq_lengths_query)
+    if not _lib.is_integer(cu) or cu.dim() != 1 or not 1 <= cu.numel() <= 65535:
+        raise ValueError(f"actual_seq_lengths_query must hold 1 to 65535 prefix sums, got {tuple(cu.shape)} {cu.dtype}")
+    B = cu.numel()
+    if not isinstance(max_path, int) or not 1 <= max_path <= (2**31 - 1) // B:
+        raise ValueError(f"max_path must be a positive count, got {max_path}")
+    for name, t in (("tokens", tokens), ("parents", parents)):
+        if not _lib.is_integer(t) or t.numel() != T:
+            raise ValueError(f"{name} must hold T={T} integers, got {tuple(t.shape)} {t.dtype}")
+    cu = _lib.saturated_int32(cu)
+    if cu.device.type == "cpu" and bool((cu[1:] < cu[:-1]).any()):
+        raise ValueError("actual_seq_lengths_query must be non-decreasing prefix sums")
+    dev = _lib.require_device(scores, tokens, parents)
+
+    def ids(t):  # numbers past 31 bits match nothing
+        t = _lib.saturated_int32(t) if t.dtype not in _lib.WIDE_INTS else _match_none(t)
+        return t.reshape(-1).contiguous()
+
+    with torch.cuda.device(dev):
+        if given:
+            x, kind, V, stride = ids(scores), _lib.KIND_INT32, 0, 1
+        else:
+            x = scores if scores.stride(1) == 1 or scores.shape[1] == 1 else scores.contiguous()
+            if T > 1 and x.stride(0) < x.shape[1]:
+                x = x.contiguous()
+            kind, V, stride = _SCORES[x.dtype], x.shape[1], x.stride(0)
+        tok, par, cu = ids(tokens), _lib.saturated_int32(parents).reshape(-1).contiguous(), cu.to(dev).contiguous()
+        accepted = torch.empty((B,), dtype=torch.int32, device=dev)
+        path, chosen = (torch.empty((B, max_path), dtype=torch.int32, device=dev) for _ in range(2))
+        lib = _lib.load_library()
+        ws_bytes = lib.dsa_tree_accept_workspace_size(kind, T, V)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib.dsa_tree_accept(kind, _lib.ptr(x), stride, T, V, _lib.ptr(tok), _lib.ptr(par), _lib.ptr(cu), B,
+                                 max_path, _lib.ptr(accepted), _lib.ptr(path), _lib.ptr(chosen), _lib.ptr(ws), ws_bytes,
+                                 _lib.stream_handle(dev))
+        _lib.check(rc, "dsa_tree_accept")
+    return accepted, path, chosen
+
+
+def _match_none(t: torch.Tensor) -> torch.Tensor:
+    wide = t.to(torch.int64)
+    return wide.masked_fill((wide < 0) | (wide > 2**31 - 1), -1).to(torch.int32)
+
+
+def paged_commit(caches: Union[torch.Tensor, Sequence[torch.Tensor]], block_table: torch.Tensor, context_lens,
+                 path: torch.Tensor, accepted: torch.Tensor) -> None:
+    """Puts the accepted tokens' cache rows in order, in place.
+
+    In each of ``caches`` ([blocks, block_size, ...], rows of any shape and type; keys and values of all layers, latents,
+    index keys), for k = 0, 1, .. below ``accepted[b]``, the row of key ``context_lens[b] + path[b, k]`` is copied to that
+    of key ``context_lens[b] + k``, where path[b, k] > k (``path`` [B, max_path], as ``tree_accept`` leaves it).  Rows whose
+    page is negative or outside the pool are left.  The context then holds ``context_lens + accepted`` tokens.  Rows must
+    be multiples of 4 bytes; the caches must not overlap, and a sequence's new tokens lie in pages of its own.  One launch
+    for each 128 caches.
+    """
+    caches = (caches,) if isinstance(caches, torch.Tensor) else tuple(caches)
+    res = _lib.host_path().paged_commit(caches, block_table, context_lens, path, accepted)
+    if res is not None:
+        _lib.returned(res, "dsa_paged_commit")
+        return
+    if not caches:
+        raise ValueError("caches must not be empty")
+    dev = _lib.require_device(*caches, block_table, path, accepted)
+    blocks = tuple(caches[0].shape[:2])
+    for c in caches:
+        if c.dim() < 3 or tuple(c.shape[:2]) != blocks or c.numel() == 0:
+            raise ValueError(f"caches must be [blocks, block_size, ...] alike, got {tuple(c.shape)} beside {blocks}")
+        _lib.require_contiguous("caches", c)
+    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1 or not _lib.is_integer(block_table):
+        raise ValueError(f"block_table must be [B, max_blocks] integers, got {tuple(block_table.shape)} {block_table.dtype}")
+    B = block_table.shape[0]
+    if path.dim() != 2 or path.shape[0] != B or not _lib.is_integer(path):
+        raise ValueError(f"path must be [{B}, max_path] integers, got {tuple(path.shape)} {path.dtype}")
+    ctx = torch.as_tensor(context_lens)
+    for name, t in (("context_lens", ctx), ("accepted", accepted)):
+        if not _lib.is_integer(t) or t.numel() != B:
+            raise ValueError(f"{name} must hold B={B} integers, got {tuple(t.shape)} {t.dtype}")
+    row_bytes = [math.prod(c.shape[2:]) * c.element_size() for c in caches]
+    with torch.cuda.device(dev):
+        bt, ctx, pa, ac = (_lib.saturated_int32(t).to(dev).contiguous() for t in (block_table, ctx, path, accepted))
+        n = len(caches)
+        rc = _lib.load_library().dsa_paged_commit((ctypes.c_void_p * n)(*(c.data_ptr() for c in caches)),
+                                                  (ctypes.c_int64 * n)(*row_bytes), n, _lib.ptr(bt), _lib.ptr(ctx),
+                                                  _lib.ptr(pa), _lib.ptr(ac), B, pa.shape[1], *blocks, bt.shape[1],
+                                                  _lib.stream_handle(dev))
+        _lib.check(rc, "dsa_paged_commit")
