@@ -35,7 +35,7 @@ def check_plan(dsa, dev, new, ctx, table, free, count, bs, T, parents=None, max_
     got = dsa.paged_plan(ints(dev, new), ints(dev, ctx), g_table, g_free, g_count, bs, T, **more)
     want = R.plan(new, ctx, table, free, count, bs, T, parents, max_nodes, win)
     for name, g, w in zip(got._fields, got, want):
-        if w is None:
+        if w is None or name == "tree_mask" and max_nodes == 0:
             assert g is None
         else:
             w = w if isinstance(w, torch.Tensor) else torch.tensor(w, dtype=I32)
@@ -126,6 +126,19 @@ def test_free_undoes_a_plan_and_cuts_rows(dsa, dev, B):
         assert t.tolist() == table and f.tolist() == lists and c.tolist() == count
 
 
+@pytest.mark.parametrize("T", [300, 5000])
+def test_plan_positions_without_masks(dsa, dev, T):
+    """Trees whose masks are not made: their depths are."""
+    rng = random.Random(T)
+    new, ctx = [T - 60, 0, 50, 1], [30, 1, 2, 3]
+    table, free = make_lists(rng, ctx, 16, T, T)
+    parents = [p for s in new for p in R.tree(rng, s, 0.1)] + [3] * 9
+    got = check_plan(dsa, dev, new, ctx, table, free, [len(free)], 16, T, parents, 0)[0]
+    assert got.tree_mask is None
+    table, free = make_lists(rng, ctx, 16, T, T)
+    check_plan(dsa, dev, new, ctx, table, free, [len(free)], 16, T, [-1] * T, 0)
+
+
 def test_plan_takes_other_integers_and_hosts(dsa, dev):
     rng = random.Random(2)
     new, ctx, par = [3, 0, 9], [7, 100, 30], [-1, 0, 0, -1, 0, 1, 2, 0, 0, 5, 5, 1]
@@ -144,7 +157,7 @@ def test_plan_takes_other_integers_and_hosts(dsa, dev):
                                         (dict(free_blocks=torch.int64), "free_blocks changes"),
                                         (dict(free_count=torch.int64), "free_count changes"), (dict(block_size=0), "block_size"),
                                         (dict(num_tokens=-1), "num_tokens"), (dict(num_tokens=2**30), "num_tokens"),
-                                        (dict(max_nodes=0), "max_nodes"), (dict(max_nodes=4097), "max_nodes"),
+                                        (dict(max_nodes=-1), "max_nodes"), (dict(max_nodes=4097), "max_nodes"),
                                         (dict(win_left=-1), "win_left"), (dict(parents=None, win_left=3), "win_left"),
                                         (dict(new_lens=[1, 2]), "new_lens must"), (dict(context_lens=[1.0] * 3), "context_lens"),
                                         (dict(parents=[0] * 3), "parents must")])

@@ -746,10 +746,10 @@ int dsa_paged_plan(const int32_t* new_lens, const int32_t* context_lens, int32_t
                    uint64_t* tree_mask, void* stream) {
   if (const int rc = check_lists("paged_plan", B, max_blocks, block_size, free_room)) return rc;
   if (T < 0 || T > kPlanRows) return reject("paged_plan: T must be in [0, 2^30)");
-  if (parents && (mask_words < 1 || mask_words > 64)) return reject("paged_plan: mask_words must be in [1, 64]");
+  if (parents && (mask_words < 0 || mask_words > 64)) return reject("paged_plan: mask_words must be in [0, 64]");
   if (win_left < -1 || win_left > kMaxInt) return reject("paged_plan: win_left must be -1 (none) or a count");
   if (!new_lens || !context_lens || !block_table || !free_count || (free_room > 0 && !free_blocks) || !cu_seqlens ||
-      !kv_lens || !missing || (T > 0 && (!positions || !slots || (parents && !tree_mask))))
+      !kv_lens || !missing || (T > 0 && (!positions || !slots || (parents && mask_words > 0 && !tree_mask))))
     return reject("paged_plan: null pointer");
   return ok(dsa::launch_paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, parents, B, T,
                                    max_blocks, block_size, free_room, parents ? mask_words : 0, win_left, cu_seqlens,

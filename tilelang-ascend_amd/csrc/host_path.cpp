@@ -693,7 +693,7 @@ PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   DSA_PLAIN(lists_ok(bt, list, count, dev));
   const int64_t B = bt.size(0);
   DSA_PLAIN(lens_ok(nl, dev, B) && lens_ok(ctx, dev, B) && lens_ok(parents, dev, T) && (win < 0 || parents) &&
-            (!parents || (nodes >= 1 && nodes <= 4096)));
+            (!parents || (nodes >= 0 && nodes <= 4096)));
   const int64_t words = parents ? (nodes + 63) / 64 : 0;
   at::Tensor out[6];
   int rc;
@@ -701,19 +701,19 @@ PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const NoGil unlocked;
     const c10::OptionalDeviceGuard guard(dev);
     for (int i = 0; i < 5; ++i) out[i] = make({i == 2 || i == 3 ? T : B}, at::kInt, dev);
-    if (parents) out[5] = make({T, words}, at::kLong, dev);
+    if (words) out[5] = make({T, words}, at::kLong, dev);
     int32_t* p[5];
     for (int i = 0; i < 5; ++i) p[i] = out[i].data_ptr<int32_t>();
     rc = E.plan(nl.ptr<int32_t>(), ctx.ptr<int32_t>(), bt.data_ptr<int32_t>(), list.data_ptr<int32_t>(),
                 count.data_ptr<int32_t>(), parents.ptr<int32_t>(), B, T, bt.size(1), bs, list.numel(), words, win, p[0],
                 p[1], p[2], p[3], p[4],
-                parents ? reinterpret_cast<uint64_t*>(out[5].data_ptr<int64_t>()) : nullptr, stream(dev));
+                words ? reinterpret_cast<uint64_t*>(out[5].data_ptr<int64_t>()) : nullptr, stream(dev));
   }
   DSA_RC(rc);
   PyObject* r = PyTuple_New(6);
   if (!r) return nullptr;
   for (int i = 0; i < 6; ++i) {
-    PyObject* o = i == 5 && !parents ? Py_NewRef(Py_None) : wrap(std::move(out[i]));
+    PyObject* o = i == 5 && !words ? Py_NewRef(Py_None) : wrap(std::move(out[i]));
     PyTuple_SET_ITEM(r, i, o);
   }
   return r;

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kPlanRowThreads) void plan_rows_kernel(PlanArgs a) 
 // Rows that the workgroup of the plan writes by itself.
 constexpr int kPlanFewRows = 4096;
 
-// Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, sizes and pointers; words >= 1 with parents.
+// Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, sizes and pointers; words 0 for no masks.
 hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_t* table, const int32_t* free_list,
                              int32_t* free_count, const int32_t* parents, int64_t B, int64_t T, int64_t max_blocks,
                              int64_t block_size, int64_t room, int64_t words, int64_t win, int32_t* cu, int32_t* kv,

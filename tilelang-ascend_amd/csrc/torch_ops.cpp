@@ -652,15 +652,15 @@ void require_list(const at::Tensor& t, const at::Tensor& table, const char* name
 
 typedef std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> Plan;
 Plan plan_outputs(const at::Tensor& table, int64_t T, bool tree, int64_t max_nodes) {
-  TORCH_CHECK(T >= 0 && (!tree || (max_nodes >= 1 && max_nodes <= 4096)),
-              "dsa.paged_plan: num_tokens must be a count, parents need max_nodes in [1, 4096]");
+  TORCH_CHECK(T >= 0 && (!tree || (max_nodes >= 0 && max_nodes <= 4096)),
+              "dsa.paged_plan: num_tokens must be a count, max_nodes in [0, 4096]");
   const int64_t B = table.size(0);
   const auto make = [&](at::IntArrayRef n) { return at::empty(n, table.options().dtype(at::kInt)); };
   return {make({B}), make({B}), make({T}), make({T}), make({B}),
           at::empty({T, tree ? (max_nodes + 63) / 64 : 0}, table.options().dtype(at::kLong))};
 }
 
-// The plan's parts; without parents the mask has no words.
+// The plan's parts; without parents or max_nodes the mask has no words.
 Plan paged_plan(const at::Tensor& new_lens, const at::Tensor& context_lens, at::Tensor block_table,
                 const at::Tensor& free_blocks, at::Tensor free_count, int64_t block_size, int64_t num_tokens,
                 const c10::optional<at::Tensor>& parents, int64_t max_nodes, int64_t win_left) {

@@ -22,7 +22,7 @@ class PagedPlan(NamedTuple):
     positions: torch.Tensor  # [T], -1 for rows behind the last sequence
     slots: torch.Tensor  # [T] cache rows, -1 without one
     missing: torch.Tensor  # [B] pages that the sequence lacks
-    tree_mask: Optional[torch.Tensor]  # [T, W] int64 with parents: a node's bits
+    tree_mask: Optional[torch.Tensor]  # [T, W] int64 with parents and max_nodes: a node's bits
 
 
 def _lists(what: str, block_table, free_blocks, free_count, block_size):
@@ -65,7 +65,7 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
     sequence, less than its own; any other number (-1) marks a root.  Positions are then the context's length and the
     depth, and ``tree_mask`` [T, W], W = ceil(max_nodes / 64), has the bits of a node and its ancestors, with ``win_left``
     those at most so many steps up.  ``max_nodes`` (at most 4096) bounds a sequence's nodes; nodes past 64 W are seen by
-    none.  At most 16384 sequences, fewer than 2^30 rows; lengths count up to 2^30.
+    none.  With 0, the default, no masks are made: those of trees that keep their shape need not be made again.  At most 16384 sequences, fewer than 2^30 rows; lengths count up to 2^30.
     """
     win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
     res = _lib.host_path().paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, block_size,
@@ -80,8 +80,8 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
         raise ValueError(f"at most 16384 sequences, got {B}")
     T, words = num_tokens, 0
     if parents is not None:
-        if not isinstance(max_nodes, int) or not 1 <= max_nodes <= 4096:
-            raise ValueError(f"parents need max_nodes in [1, 4096], got {max_nodes}")
+        if not isinstance(max_nodes, int) or not 0 <= max_nodes <= 4096:
+            raise ValueError(f"max_nodes must be in [0, 4096], got {max_nodes}")
         words = -(-max_nodes // 64)
     elif win_left is not None:
         raise ValueError("win_left cuts tree masks: it needs parents")
@@ -93,7 +93,7 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
         new, ctx, par = (None if x is None else x.to(dev).contiguous() for x in (new, ctx, par))
         empty = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=dev)
         out = PagedPlan(empty(B), empty(B), empty(T), empty(T), empty(B),
-                        None if par is None else empty(T, words, dtype=torch.int64))
+                        empty(T, words, dtype=torch.int64) if words else None)
         rc = _lib.load_library().dsa_paged_plan(
             _lib.ptr(new), _lib.ptr(ctx), _lib.ptr(block_table), _lib.ptr(free_blocks), _lib.ptr(free_count),
             _lib.ptr(par) if T else None, B, T, block_table.shape[1], block_size, free_blocks.numel(), words,
