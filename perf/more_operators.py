@@ -257,7 +257,11 @@ def run(st):
 def _own_plan(st):
     """A step's plan, and the pages handed back (nothing of the step was kept)."""
     c, pkg = st["case"], st["pkg"]
-    more = dict(parents=st["parents"], max_nodes=st["max_nodes"]) if c["tree"] else {}
+    if c["tree"]:
+        more = dict(parents=st["parents"], max_nodes=st["max_nodes"])
+    else:
+        # The plain form has the rows of a step without trees at their contexts' ends, as roots are: so has this call.
+        more = dict(parents=torch.full((st["T"],), -1, dtype=torch.int32, device=st["new"].device))
     if c["win"] >= 0:
         more["win_left"] = c["win"]
     p = pkg.paged_plan(st["new"], st["ctx"], st["table"], st["free"], st["count"], c["block"], st["T"], **more)
