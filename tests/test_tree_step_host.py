@@ -55,8 +55,9 @@ def test_tree_attention_c_checks(dsa):
                     (dict(nws=0), b"workspace"), (dict(ws=None), b"workspace")]:
         assert refused(lib, call(**kw), msg), kw
     assert call(T=0, S=0) == 0
-    assert (lib.dsa_paged_tree_workspace_size(8, 1, 64, 4, 128, 4160)
-            == lib.dsa_paged_gqa_workspace_size(8, 1, 64, 4, 128, 4160))
+    assert lib.dsa_paged_tree_workspace_size(8, 1, 64, 4, 128, 4160) > 0
+    assert lib.dsa_paged_tree_workspace_size(0, 1, 64, 4, 128, 4160) == 0
+    assert lib.dsa_paged_tree_workspace_size(8, 1, 64, 3, 128, 4160) == 0
 
 
 def test_accept_c_checks(dsa):

@@ -70,6 +70,8 @@ hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const vo
                             int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                             int64_t max_blocks, int causal, int64_t win_left, const float* sinks, float sm_scale,
                             void* out, float* lse, void* workspace, hipStream_t stream);
+bool paged_tree_fits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most);
+size_t paged_tree_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most);
 hipError_t launch_paged_tree(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
                              const uint64_t* mask, int64_t words, const int32_t* pos, const int32_t* cu_q,
                              const int32_t* q_len, const int32_t* kv_len, int64_t T, int64_t B, int64_t S, int64_t H,
@@ -641,19 +643,24 @@ int dsa_qk_norm_rope(int kind, const void* q, int64_t q_stride, const void* k, i
 }
 
 // Sizes that both the workspace query and the call need in range.
-static bool paged_gqa_sizes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
+static bool paged_sizes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most, bool tree) {
   return T >= 0 && B >= 1 && B <= 65535 && H >= 1 && G >= 1 && H % G == 0 && G <= 65535 && T <= kMaxInt &&
          H <= 65535 && T * H <= kMaxInt - 65536 && (D == 64 || D == 128) && most >= 0 && most <= kMaxInt - 4096 &&
-         dsa::paged_gqa_fits(T, B, H, G, most);
+         (tree ? dsa::paged_tree_fits(T, B, H, G, most) : dsa::paged_gqa_fits(T, B, H, G, most));
 }
 
 size_t dsa_paged_gqa_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {
-  if (T <= 0 || !paged_gqa_sizes(T, B, H, G, D, max_keys)) return 0;
+  if (T <= 0 || !paged_sizes(T, B, H, G, D, max_keys, false)) return 0;
   return dsa::paged_gqa_workspace_bytes(T, B, H, G, D, max_keys);
 }
 
+size_t dsa_paged_tree_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {
+  if (T <= 0 || !paged_sizes(T, B, H, G, D, max_keys, true)) return 0;
+  return dsa::paged_tree_workspace_bytes(T, B, H, G, D, max_keys);
+}
+
 // What the two attentions over pages ask alike of their arguments; `who` names the entry.
-static int check_paged(const char* who, int kind, const void* q, const void* k_cache, const void* v_cache,
+static int check_paged(const char* who, bool tree, int kind, const void* q, const void* k_cache, const void* v_cache,
                        const int32_t* block_table, const int32_t* cu_q, const int32_t* actual_kv_len, int64_t T,
                        int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                        int64_t max_blocks, int64_t win_left, float sm_scale, const void* out, const float* lse,
@@ -669,7 +676,7 @@ static int check_paged(const char* who, int kind, const void* q, const void* k_c
   if (block_size < 1 || max_blocks < 1 || num_blocks < 1 || block_size > kMaxInt || max_blocks > kMaxInt ||
       num_blocks > kMaxInt / block_size)
     return no("bad page sizes");
-  if (max_blocks > (kMaxInt - 4096) / block_size || !paged_gqa_sizes(T, B, H, G, D, max_blocks * block_size))
+  if (max_blocks > (kMaxInt - 4096) / block_size || !paged_sizes(T, B, H, G, D, max_blocks * block_size, tree))
     return no("sizes out of range");
   if (!cu_q && (S < 0 || S > kMaxInt || B * S != T)) return no("T must be B * S without cu_q");
   if (win_left < -1 || win_left > kMaxInt - 4096) return no("win_left must be -1 (none) or a key count");
@@ -678,7 +685,8 @@ static int check_paged(const char* who, int kind, const void* q, const void* k_c
   if (!q || !k_cache || !v_cache || !block_table || !actual_kv_len || !out || !lse) return no("null pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return no("rows must start on 16 bytes");
-  const size_t need = dsa_paged_gqa_workspace_size(T, B, H, G, D, max_blocks * block_size);
+  const size_t need = (tree ? dsa_paged_tree_workspace_size : dsa_paged_gqa_workspace_size)(T, B, H, G, D,
+                                                                                            max_blocks * block_size);
   if (workspace_bytes < need) return no("workspace too small");
   if (need > 0 && (!workspace || !aligned16(workspace))) return no("null or unaligned workspace");
   return 0;
@@ -689,7 +697,7 @@ int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* 
                       int64_t B, int64_t S, int64_t H, int64_t G, int64_t D, int64_t num_blocks, int64_t block_size,
                       int64_t max_blocks, int is_causal, int64_t win_left, const float* sinks, float sm_scale,
                       void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  if (const int rc = check_paged("paged_gqa", kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
+  if (const int rc = check_paged("paged_gqa", false, kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
                                  num_blocks, block_size, max_blocks, win_left, sm_scale, out, lse, workspace,
                                  workspace_bytes))
     return rc;
@@ -700,10 +708,6 @@ int dsa_paged_gqa_fwd(int kind, const void* q, const void* k_cache, const void* 
                                   static_cast<hipStream_t>(stream)));
 }
 
-size_t dsa_paged_tree_workspace_size(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_keys) {
-  return dsa_paged_gqa_workspace_size(T, B, H, G, D, max_keys);
-}
-
 int dsa_paged_tree_fwd(int kind, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                        const uint64_t* tree_mask, int64_t mask_words, const int32_t* positions, const int32_t* cu_q,
                        const int32_t* actual_q_len, const int32_t* actual_kv_len, int64_t T, int64_t B, int64_t S,
@@ -711,7 +715,7 @@ int dsa_paged_tree_fwd(int kind, const void* q, const void* k_cache, const void*
                        int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse, void* workspace,
                        size_t workspace_bytes, void* stream) {
   if (mask_words < 1 || mask_words > 64) return reject("paged_tree: mask_words must be in [1, 64]");
-  if (const int rc = check_paged("paged_tree", kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
+  if (const int rc = check_paged("paged_tree", true, kind, q, k_cache, v_cache, block_table, cu_q, actual_kv_len, T, B, S, H, G, D,
                                  num_blocks, block_size, max_blocks, win_left, sm_scale, out, lse, workspace,
                                  workspace_bytes))
     return rc;

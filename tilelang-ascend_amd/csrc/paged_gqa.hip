@@ -4,17 +4,12 @@
 
 namespace dsa {
 
-// The largest grid, of tiles in each group, within the 2^32 threads of a launch (the shared line's and the join's are
-// smaller).  T * H < 2^31, B, G <= 65535.
 bool paged_gqa_fits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) {
-  const PgPlan p = pg_plan(T, B, H, G, most);
-  return p.slots * G < ((int64_t)1 << 32) / (p.rows == kPrRows ? kPrThreads : kPgThreads);
+  return pg_fits(pg_plan(T, B, H, G, most, false), G);
 }
 
 size_t paged_gqa_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
-  const PgPlan p = pg_plan(T, B, H, G, most);
-  if (p.wgs == 0) return 0;
-  return pg_part_bytes(p, D) + (size_t)(2 * p.slots + 1) * sizeof(int32_t);
+  return pg_workspace_bytes(pg_plan(T, B, H, G, most, false), D);
 }
 
 // Caller validated: D in {64, 128}, H a multiple of G, T * H < 2^31 - 65536, pool rows < 2^31,
@@ -26,7 +21,7 @@ hipError_t launch_paged_gqa(int is_fp16, const void* q, const void* kc, const vo
                             int64_t max_blocks, int causal, int64_t win_left, const float* sinks, float sm_scale,
                             void* out, float* lse, void* workspace, hipStream_t stream) {
   if (T == 0 || H == 0) return hipSuccess;
-  const PgPlan p = pg_plan(T, B, H, G, max_blocks * block_size);
+  const PgPlan p = pg_plan(T, B, H, G, max_blocks * block_size, false);
   PgArgs a = pg_args({T, B, S, H, G, D, num_blocks, block_size, max_blocks}, q, kc, vc, table, cu_q, q_len, kv_len,
                      win_left, sinks, sm_scale, out, lse, workspace, p);
   a.causal = causal;

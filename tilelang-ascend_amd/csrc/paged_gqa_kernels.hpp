@@ -1030,6 +1030,8 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
 
   l_run = pr_sum32(l_run);
   const bool none = l_run == 0.f;  // a row that saw nothing: its sums may be 0 times anything
+  // Trees leave most rows of a part empty; the join reads none of those (8 nodes of 64 heads over 4, 30000 keys: 43 -> 40 us).
+  if (kTree && !whole && first + r >= rows) return;
   if (!whole) {
     float* p = part + (32 * wave + r) * kD + 8 * hi;
 #pragma unroll
@@ -1241,17 +1243,20 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
 // Those have a workgroup a pass as long as the slots are few (64 queries of 64 heads over 30000 keys: 16 parts a tile,
 // 21.7 us with four passes a workgroup, 8.8 with one), and four passes a workgroup where most slots may hold no tile
 // (800 sequences of 5 tokens: 79.7 us with one pass, 21.1 with four).
-template <class W>
+// Trees of few sequences have few tiles of 256 rows, cut into many parts of few live rows: four groups of threads for them
+// too, up to 24 slots of all groups (4 nodes over 4097 keys, 64 heads over 4, 8 slots: the call 22.8 -> 20.2 us; 61 nodes
+// over 30000, 64-wide over 8, 24 slots: 59.5 -> 58.7; four such sequences over 4097, 56 slots: 40.9 -> 49.3).
+constexpr int kPgTreeFewSlots = 24;
+template <class W, int kGroups_ = W::kR == kPrRows ? 1 : 4>
 struct PgJoin {
   static constexpr int kPerRow = W::kD / 8;
-  static constexpr int kGroups = W::kR == kPrRows ? 1 : 4;
+  static constexpr int kGroups = kGroups_;
   static constexpr int kPass = kPgThreads / kGroups / kPerRow;  // rows of a pass
-  static constexpr int kMost = W::kR == kPrRows ? 4 : 1;        // passes of a workgroup
+  static constexpr int kMost = kGroups == 1 ? 4 : 1;            // passes of a workgroup
   static_assert(W::kR % (kMost * kPass) == 0, "whole groups of rows");
 };
-template <class W>
+template <class J, class W>
 __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
-  typedef PgJoin<W> J;
   constexpr int kR = W::kR, kD = W::kD;
   constexpr bool kF16 = W::kF16;
   const int x = blockIdx.x / a.G, kvg = blockIdx.x - x * a.G;
@@ -1337,7 +1342,11 @@ struct PgPlan {
   int wgs;        // workgroups that share the line of units; 0: a tile each
 };
 
-inline PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) {
+// `tree`, tiles of 256 rows: sequences bring alike numbers of rows, of which the last tile is seldom full, so that a workgroup a tile leaves
+// CUs idle in the last round: the line up to 1199 slots of all groups (32 trees of 61 nodes, 64 heads over 4, 620 slots:
+// 8192 keys 660 -> 562 us; 128 trees of 8 over 2000 keys, 772 slots: 158 -> 129; 200 trees of 8 over 500 keys, 1204 slots:
+// 80 -> 89; 24 nodes each, 2004 slots: 176 -> 197).
+inline PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most, bool tree) {
   PgPlan p;
   const int64_t Hg = H / G;
   p.rows = T * Hg <= 16 * B ? 16 : T * Hg <= 32 * B ? 32 : kPrRows;
@@ -1348,12 +1357,23 @@ inline PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) 
   // instead of 199).
   const int64_t unit = p.rows == kPrRows ? kPrTile : kPgUnit;
   const int64_t units = p.slots * G * ((most + unit - 1) / unit + 1 + kPgExtra);
-  if (p.slots <= kPgMaxSlots && units < ((int64_t)1 << 30) && (p.slots * G < 512 || 4 * (B + 1) > p.slots))
+  if (p.slots <= kPgMaxSlots && units < ((int64_t)1 << 30) && (tree && p.rows == kPrRows ? p.slots * G < 1200 : p.slots * G < 512 || 4 * (B + 1) > p.slots))
     p.wgs = (int)(units < 256 ? units : 256);
   return p;
 }
 
+// The largest grid, of tiles in each group, within the 2^32 threads of a launch (the shared line's and the join's are
+// smaller).  T * H < 2^31, B, G <= 65535.
+inline bool pg_fits(const PgPlan& p, int64_t G) {
+  return p.slots * G < ((int64_t)1 << 32) / (p.rows == kPrRows ? kPrThreads : kPgThreads);
+}
+
 inline size_t pg_part_bytes(const PgPlan& p, int64_t D) { return (size_t)(2 * p.wgs) * p.rows * (D + 2) * sizeof(float); }
+
+inline size_t pg_workspace_bytes(const PgPlan& p, int64_t D) {
+  if (p.wgs == 0) return 0;
+  return pg_part_bytes(p, D) + (size_t)(2 * p.slots + 1) * sizeof(int32_t);
+}
 
 template <class W>
 hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
@@ -1370,9 +1390,18 @@ hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
   e = set_dynamic_lds_once<pg_split_kernel<W>>(split_lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((pg_split_kernel<W>), dim3(a.wgs), dim3(W::kThreads), split_lds, stream, a);
-  typedef PgJoin<W> J;
-  const dim3 join(tiles.x, W::kR / J::kPass / (tiles.x > kPgFewSlots ? J::kMost : 1));
-  hipLaunchKernelGGL((pg_join_kernel<W>), join, dim3(kPgThreads), 0, stream, a);
+  const auto join = [&](auto how) {
+    typedef decltype(how) J;
+    const dim3 grid(tiles.x, W::kR / J::kPass / (tiles.x > kPgFewSlots ? J::kMost : 1));
+    hipLaunchKernelGGL((pg_join_kernel<J, W>), grid, dim3(kPgThreads), 0, stream, a);
+  };
+  if constexpr (W::kTree) {
+    if (tiles.x <= kPgTreeFewSlots) {
+      join(PgJoin<W, 4>{});
+      return hipGetLastError();
+    }
+  }
+  join(PgJoin<W>{});
   return hipGetLastError();
 }
 

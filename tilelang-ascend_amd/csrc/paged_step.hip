@@ -122,19 +122,23 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int* cu, int t
 __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, int rows) {
   extern __shared__ __align__(16) int plan_lds[];
   __shared__ int sums[kStepWaves];
-  int* cu = plan_lds;             // [B] sums of the lengths
-  int* touched = plan_lds + a.B;  // [B] sums of the touched blocks
+  __shared__ int next[kStepThreads];  // the pages handed out first
+  int* cu = plan_lds;                 // [B] sums of the lengths
+  int* touched = plan_lds + a.B;      // [B] sums of the touched blocks
   const int tid = threadIdx.x, bs = a.block_size;
   const int most = a.T;
   const auto add_rows = [most](int x, int y) { return min(x + y, most); };  // at most T rows: sums that stay there
   const auto add = [](int x, int y) { return x + y; };
   int rows_before = 0, blocks_before = 0;
+  const int count = min(max(a.free_count[0], 0), a.room);
   for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
     const int b = b0 + tid;
     const bool live = b < a.B;
-    const int ctx = live ? plan_len(a.ctx[b]) : 0;
+    const int ctx = live ? plan_len(a.ctx[b]) : 0, want = live ? min(plan_len(a.new_lens[b]), most) : 0;
+    // Asked for while the sums are made.
+    if (b0 == 0) next[tid] = tid < count ? a.free_list[count - 1 - tid] : -1;
     int total;
-    const int sum = add_rows(rows_before, step_scan(live ? min(plan_len(a.new_lens[b]), most) : 0, sums, total, add_rows));
+    const int sum = add_rows(rows_before, step_scan(want, sums, total, add_rows));
     // The sum before this one is the neighbour's: through LDS.
     if (live) cu[b] = sum;
     __syncthreads();
@@ -156,7 +160,6 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
     }
   }
   __syncthreads();
-  const int count = min(max(a.free_count[0], 0), a.room);
   int taken = 0;
   for (int p0 = 0; p0 < blocks_before; p0 += kStepThreads) {
     const int p = p0 + tid;
@@ -172,7 +175,7 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
     const int rank = taken + step_scan(lacks ? 1 : 0, sums, total, add) - 1;
     taken += total;
     if (lacks) {
-      if (rank < count) *entry = a.free_list[count - 1 - rank];
+      if (rank < count) *entry = rank < kStepThreads ? next[rank] : a.free_list[count - 1 - rank];
       else atomicAdd(a.missing + b, 1);
     }
   }
@@ -238,6 +241,7 @@ __global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
   extern __shared__ __align__(16) int upto[];  // [B] pages of the sequences up to this one
   __shared__ int sums[kStepWaves];
   constexpr int kSeqs = kStepThreads / kGroup;
+  constexpr int kAhead = kGroup == 64 ? 4 : 1;  // entries a lane in flight: rows of many pages come in groups of 64
   const int tid = threadIdx.x, in = tid % kGroup, lane = tid & (kWave - 1);
   const auto first_block = [&](int b) {
     const int keep = plan_len(a.keep[b]);
@@ -247,15 +251,20 @@ __global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
     const int32_t* row = a.table + (int64_t)b * a.max_blocks;
     const int from = first_block(b);
     int n = 0;
-    for (int j = from; j < a.max_blocks; j += kGroup) {
-      const bool held = j + in < a.max_blocks && row[j + in] >= 0;
-      const uint64_t group = __ballot(held) >> (lane & ~(kGroup - 1));
-      const uint64_t ends = ~group & (kGroup == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (kGroup & 63)) - 1);
-      if (ends) {
-        n += __ffsll((unsigned long long)ends) - 1;
-        break;
+    for (int64_t j = from; j < a.max_blocks; j += kAhead * kGroup) {
+      int page[kAhead];  // negative: none
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) page[u] = row[min(j + u * kGroup + in, (int64_t)a.max_blocks - 1)];
+      bool ended = false;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const bool held = j + u * kGroup + in < a.max_blocks && page[u] >= 0;
+        const uint64_t group = __ballot(held) >> (lane & ~(kGroup - 1));
+        const uint64_t ends = ~group & (kGroup == 64 ? ~(uint64_t)0 : ((uint64_t)1 << (kGroup & 63)) - 1);
+        if (!ended) n += ends ? __ffsll((unsigned long long)ends) - 1 : kGroup;
+        ended = ended || ends;
       }
-      n += kGroup;
+      if (ended) break;
     }
     if (in == 0) upto[b] = n;
   }
@@ -370,7 +379,8 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 }
 
 // The rank of the elements [from, to) of a row, this thread's part of them.  Whole 16-byte chunks in turn, the elements
-// before and behind them one a thread.
+// before and behind them one a thread.  A chunk's largest value is compared with the best so far, and only the best
+// chunk's place is looked up, from the caches: two to three operations an element instead of five.
 template <class S>
 __device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from, int to, int tid, int threads) {
   constexpr int kN = S::kN, kAhead = 8;
@@ -379,25 +389,44 @@ __device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from,
   const int chunks = (to - from - head) / kN, tail = from + head + chunks * kN;
   const u32x4* body = reinterpret_cast<const u32x4*>(row + from + head);
   float best = -__builtin_huge_valf();
-  int where = -1;
+  int where = -1;  // the first chunk that holds it
   for (int c0 = tid; c0 < chunks; c0 += kAhead * threads) {
     u32x4 w[kAhead];
+    float top[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) w[j] = body[min(c0 + j * threads, chunks - 1)];
+    // `maximum` takes three operands an instruction and passes NaN on: one comparison finds whether there is any.
+    float any = best;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (c0 + j * threads >= chunks) break;
+      top[j] = S::at(w[j], 0);
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const float v = S::at(w[j], i);
-        if (v > best) {
-          best = v;
-          where = (c0 + j * threads) * kN + i;
-        }
+      for (int i = 1; i < kN; ++i) top[j] = __builtin_elementwise_maximum(top[j], S::at(w[j], i));
+      any = __builtin_elementwise_maximum(any, top[j]);
+    }
+    if (any != any) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        top[j] = -__builtin_huge_valf();
+#pragma unroll
+        for (int i = 0; i < kN; ++i) top[j] = S::at(w[j], i) > top[j] ? S::at(w[j], i) : top[j];
       }
     }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (top[j] > best) {
+        best = top[j];
+        where = min(c0 + j * threads, chunks - 1);
+      }
   }
-  uint64_t rank = score_rank(best, from + head + where);
+  uint64_t rank = 0;
+  if (where >= 0) {
+    const u32x4 w = body[where];
+    int first = kN - 1;
+#pragma unroll
+    for (int i = kN - 2; i >= 0; --i) first = S::at(w, i) == best ? i : first;
+    rank = score_rank(best, from + head + where * kN + first);
+  }
   if (tid < head) {
     const uint64_t r = score_rank(S::one(row + from + tid), from + tid);
     rank = r > rank ? r : rank;

@@ -4,7 +4,15 @@
 
 namespace dsa {
 
-// Caller validated: the sizes as launch_paged_gqa has them (its workspace too), mask [T, words] 64-bit words,
+bool paged_tree_fits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most) {
+  return pg_fits(pg_plan(T, B, H, G, most, true), G);
+}
+
+size_t paged_tree_workspace_bytes(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t most) {
+  return pg_workspace_bytes(pg_plan(T, B, H, G, most, true), D);
+}
+
+// Caller validated: the sizes as launch_paged_gqa has them, paged_tree_fits and the workspace of these functions, mask [T, words] 64-bit words,
 // 1 <= words <= 64, pos [T] where there is a window.
 hipError_t launch_paged_tree(int is_fp16, const void* q, const void* kc, const void* vc, const int32_t* table,
                              const uint64_t* mask, int64_t words, const int32_t* pos, const int32_t* cu_q,
@@ -13,7 +21,7 @@ hipError_t launch_paged_tree(int is_fp16, const void* q, const void* kc, const v
                              int64_t win_left, const float* sinks, float sm_scale, void* out, float* lse,
                              void* workspace, hipStream_t stream) {
   if (T == 0 || H == 0) return hipSuccess;
-  const PgPlan p = pg_plan(T, B, H, G, max_blocks * block_size);
+  const PgPlan p = pg_plan(T, B, H, G, max_blocks * block_size, true);
   PgArgs a = pg_args({T, B, S, H, G, D, num_blocks, block_size, max_blocks}, q, kc, vc, table, cu_q, q_len, kv_len,
                      win_left, sinks, sm_scale, out, lse, workspace, p);
   a.mask = reinterpret_cast<const uint32_t*>(mask);
