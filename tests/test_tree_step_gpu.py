@@ -203,7 +203,7 @@ def check_accept(dsa, dev, scores, lens, parents, tokens, P, plain=None):
 def test_accept(dsa, dev, dtype, V, rows):
     """Both ways over the scores: all rows in a first launch, and those on the path only."""
     rng = random.Random(V)
-    lens = [5, 1, 0, 61, 8] if rows == "few" else [5, 1, 0, 61, 8] + [40] * (1 + (40 << 20) // (40 * V * 2))
+    lens = [5, 1, 0, 61, 8] if rows == "few" else [5, 1, 0, 61, 8] + [40] * (1 + (64 << 20) // (40 * V * 2))
     if sum(lens) > 60000:  # short rows: any number of them is few bytes, and 65536 is past a grid's rows
         lens = [5, 1, 0, 61, 8] + [4000] * 17
     parents, tokens, choices = trees(rng, lens, V, 0.6)

@@ -1,6 +1,8 @@
 // What a decoding step over a paged cache needs around its attention, gfx950: pages, slots, positions and tree masks from
 // request lengths (the plan) and the pages' way back, the choices of a model followed through a tree of drafted tokens, and
 // the cache rows of the accepted ones put in order.  All lengths, tables and lists stay on the device.
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace dsa {
@@ -318,8 +320,9 @@ hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_
 // behind `at` whose parent is `at` and whose drafted token is the choice.
 //
 // Scores are read where the walk comes by: of 61 rows of a sequence some four.  A workgroup a sequence (accept_walk_kernel)
-// reads a row with all its threads, then looks for the child; each step is one row's bytes through one CU and a
-// reduction.  Where all rows together are few, a first launch takes the largest of every row in pieces over the card
+// reads a row with all its threads, then looks for the child; each step is one row's bytes through one CU (108 GB/s) and
+// 2.5 us of latencies (the first loads, the reductions, the child): 64 sequences of 61 rows, 131072 bf16 scores, four nodes
+// on the path 24.6 us, where reading those rows at the card's rate would take 14 and all 3904 rows 215.  Where all rows together are few, a first launch takes the largest of every row in pieces over the card
 // (row_max_kernel), and the walk only joins pieces.
 
 struct AcceptArgs {
@@ -369,18 +372,31 @@ __device__ __forceinline__ uint64_t score_rank(float v, int place) {
 }
 __device__ __forceinline__ int score_place(uint64_t rank) { return rank ? (int)~(uint32_t)rank : -1; }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor((unsigned long long)v, o, kWave);
+// The largest of the wave's values in all lanes, by moves between lanes within the registers: neighbours 1, 2, 4 and 8 lanes
+// below in rows of 16, then the rows' last lanes; lane 63 holds it.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  const auto take = [&](auto ctrl, auto rows) {
+    const uint32_t u = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
     v = u > v ? u : v;
-  }
-  return v;
+  };
+  using std::integral_constant;
+  take(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  take(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  take(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  take(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  take(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  take(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, kWave - 1);
+}
+// Of ranks: the largest upper half, then the largest lower half beside it.
+__device__ __forceinline__ uint64_t wave_max_rank(uint64_t v) {
+  const uint32_t hi = (uint32_t)(v >> 32), top = wave_max_u32(hi);
+  return (uint64_t)top << 32 | wave_max_u32(hi == top ? (uint32_t)v : 0);
 }
 
 // The rank of the elements [from, to) of a row, this thread's part of them.  Whole 16-byte chunks in turn, the elements
 // before and behind them one a thread.  A chunk's largest value is compared with the best so far, and only the best
-// chunk's place is looked up, from the caches: two to three operations an element instead of five.
+// chunk, which is kept, is searched for the place: three operations an element instead of five.
 template <class S>
 __device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from, int to, int tid, int threads) {
   constexpr int kN = S::kN, kAhead = 8;
@@ -390,6 +406,7 @@ __device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from,
   const u32x4* body = reinterpret_cast<const u32x4*>(row + from + head);
   float best = -__builtin_huge_valf();
   int where = -1;  // the first chunk that holds it
+  u32x4 kept = {0, 0, 0, 0};
   for (int c0 = tid; c0 < chunks; c0 += kAhead * threads) {
     u32x4 w[kAhead];
     float top[kAhead];
@@ -417,14 +434,14 @@ __device__ __forceinline__ uint64_t row_rank(const typename S::T* row, int from,
       if (top[j] > best) {
         best = top[j];
         where = min(c0 + j * threads, chunks - 1);
+        kept = w[j];
       }
   }
   uint64_t rank = 0;
   if (where >= 0) {
-    const u32x4 w = body[where];
     int first = kN - 1;
 #pragma unroll
-    for (int i = kN - 2; i >= 0; --i) first = S::at(w, i) == best ? i : first;
+    for (int i = kN - 2; i >= 0; --i) first = S::at(kept, i) == best ? i : first;
     rank = score_rank(best, from + head + where * kN + first);
   }
   if (tid < head) {
@@ -444,7 +461,7 @@ __global__ __launch_bounds__(256) void row_max_kernel(const void* scores, int64_
   __shared__ uint64_t waves[4];
   const int from = blockIdx.x * piece, to = min(from + piece, V);
   const typename S::T* row = static_cast<const typename S::T*>(scores) + blockIdx.y * stride;
-  const uint64_t rank = wave_max_u64(row_rank<S>(row, from, to, threadIdx.x, 256));
+  const uint64_t rank = wave_max_rank(row_rank<S>(row, from, to, threadIdx.x, 256));
   if ((threadIdx.x & (kWave - 1)) == 0) waves[threadIdx.x / kWave] = rank;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -468,28 +485,28 @@ __global__ __launch_bounds__(kThreads) void accept_walk_kernel(AcceptArgs a) {
   const int my_parent = tid < S ? parents[tid] : -1, my_token = tid < S ? tokens[tid] : -1;
   if (tid < 3) child[tid] = S;
   __syncthreads();
-  int at = 0, k = 0;
+  int at = 0, k = 0, my_at = -1, my_choice = -1;
   while (at < S && k < a.P) {
     int choice;
     if constexpr (kKind != 0) {
       typedef Score<kKind ? kKind : 1> R;
       const typename R::T* row = static_cast<const typename R::T*>(a.scores) + (start + at) * a.stride;
-      const uint64_t rank = wave_max_u64(row_rank<R>(row, 0, a.V, tid, kThreads));
+      const uint64_t rank = wave_max_rank(row_rank<R>(row, 0, a.V, tid, kThreads));
       if ((tid & (kWave - 1)) == 0) ranks[tid / kWave] = rank;
       __syncthreads();
-      uint64_t m = ranks[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) m = ranks[w] > m ? ranks[w] : m;
-      choice = score_place(m);
+      choice = score_place(wave_max_rank(ranks[tid % kWaves]));
     } else if (a.pieces) {
       uint64_t m = 0;
       const uint64_t* row = a.pieces + (int64_t)(start + at) * a.num_pieces;
       for (int i = tid & (kWave - 1); i < a.num_pieces; i += kWave) m = row[i] > m ? row[i] : m;
-      choice = score_place(wave_max_u64(m));
+      choice = score_place(wave_max_rank(m));
     } else {
       choice = static_cast<const int32_t*>(a.scores)[start + at];
     }
-    if (tid == 0) {
+    // Kept until the end by the first threads, one a step: a barrier behind a store would wait for it.
+    if (k < kThreads) {
+      if (tid == k) my_at = at, my_choice = choice;
+    } else if (tid == 0) {
       path[k] = at;
       chosen[k] = choice;
     }
@@ -504,13 +521,18 @@ __global__ __launch_bounds__(kThreads) void accept_walk_kernel(AcceptArgs a) {
     at = child[k % 3];
     ++k;
   }
+  if (tid < min(k, kThreads)) path[tid] = my_at, chosen[tid] = my_choice;
   for (int i = k + tid; i < a.P; i += kThreads) path[i] = chosen[i] = -1;
   if (tid == 0) a.accepted[b] = k;
 }
 
-// Bytes of all rows up to which a first launch reads them all.
-constexpr int64_t kAcceptFewBytes = 32 << 20;
-constexpr int kAcceptPiece = 16384;  // bytes of a workgroup's piece of a row
+// Bytes of all rows up to which a first launch reads them all, and of a workgroup's piece of a row.  131072 bf16 scores, the
+// first launch against the walk alone: 61 rows of one sequence with four on the path 8.5 us against 21.3, one on it 6.7 against
+// 8.1; 64 sequences of 3 rows (50 MB), one on the path 13.2 against 9.1; of 8 (134 MB), four on it 26.2 against 24.8, one 24.6
+// against 9.0; 32003 scores, 64 of 8 (33 MB): four 11.3 against 15.8, one 9.7 against 7.3.  Pieces of 8 or 16 KB: 11.1 and 9.3 us
+// where 32 KB take 8.5.
+constexpr int64_t kAcceptFewBytes = 48 << 20;
+constexpr int kAcceptPiece = 32768;
 
 struct AcceptPlan {
   bool all;       // every row in a first launch
