@@ -297,7 +297,7 @@ def some_path(rng, S, n):
     return sorted(rng.sample(range(S), min(n, S)))
 
 
-@pytest.mark.parametrize("shape,dtype", [((4, 128), torch.bfloat16), ((1, 576), torch.float16), ((2, 64), torch.float32),
+@pytest.mark.parametrize("shape,dtype", [((), torch.float32), ((4, 128), torch.bfloat16), ((1, 576), torch.float16), ((2, 64), torch.float32),
                                          ((1, 128), torch.float8_e4m3fn), ((1,), torch.float32), ((3, 6), torch.int16),
                                          ((5000,), torch.uint8), ((1, 4), torch.uint8)])
 @pytest.mark.parametrize("bs", [1, 16, 64])
@@ -322,11 +322,11 @@ def test_commit(dsa, dev, shape, dtype, bs):
     caches = [torch.randint(0, 256, (nb, bs) + shape, generator=g).to(torch.uint8).to(dtype) if dtype != torch.float8_e4m3fn
               else torch.randn((nb, bs) + shape, generator=g).to(dtype) for _ in range(3)]
     got = [c.to(dev) for c in caches]
-    raw = [c.view(torch.uint8) for c in caches]
+    raw = [c.view(nb, bs, -1).view(torch.uint8) for c in caches]
     R.commit(raw, table, ctx, path, accepted)
     dsa.paged_commit(got, ints(dev, table), ints(dev, ctx), ints(dev, path), ints(dev, accepted))
     for a, b in zip(got, raw):
-        assert torch.equal(a.view(torch.uint8).cpu(), b)
+        assert torch.equal(a.view(nb, bs, -1).view(torch.uint8).cpu(), b)
 
 
 @pytest.mark.parametrize("n", [1, 7, 128, 129, 300])

@@ -821,7 +821,7 @@ PyObject* paged_commit(PyObject*, PyObject* const* v, Py_ssize_t n) {
     PyObject* o = PyTuple_GET_ITEM(v[0], c);
     DSA_PLAIN(THPVariable_CheckExact(o));
     const at::Tensor& t = THPVariable_Unpack(o);
-    DSA_PLAIN(t.device() == dev && t.dim() >= 3 && t.is_contiguous() && t.numel() > 0);
+    DSA_PLAIN(t.device() == dev && t.dim() >= 2 && t.is_contiguous() && t.numel() > 0);
     if (c == 0) blocks = t.size(0), bs = t.size(1);
     DSA_PLAIN(t.size(0) == blocks && t.size(1) == bs);
     at_cache[c] = t.data_ptr();

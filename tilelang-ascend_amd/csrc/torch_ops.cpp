@@ -762,7 +762,7 @@ void paged_commit(at::TensorList caches, const at::Tensor& block_table, const at
   for (const at::Tensor& c : caches) {
     require(c, "caches");
     require_on(c, first, "caches");
-    TORCH_CHECK(c.dim() >= 3 && c.numel() > 0 && c.size(0) == first.size(0) && c.size(1) == first.size(1),
+    TORCH_CHECK(c.dim() >= 2 && c.numel() > 0 && c.size(0) == first.size(0) && c.size(1) == first.size(1),
                 "dsa.paged_commit: caches must be [blocks, block_size, ...] alike (got ", c.sizes(), ")");
     at_cache.push_back(ptr(c));
     bytes.push_back(c.numel() / (c.size(0) * c.size(1)) * (int64_t)c.element_size());

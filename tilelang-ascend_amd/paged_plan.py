@@ -59,7 +59,7 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
     where new tokens need one it comes off the end of ``free_blocks`` (the first ``free_count`` entries are free), in the
     order of sequences and blocks.  ``block_table`` and ``free_count`` (int32) change in place.  ``missing`` of the result
     counts the pages that a sequence did not get, since the list ran out or its table ended: slots there are -1 (nothing
-    is written), and the step is not whole for that sequence.
+    is written), and the step is not whole for that sequence.  Calls that share a list follow one another on one stream.
 
     ``parents`` [T] makes each sequence's new tokens a tree of drafted ones: the place of a token's parent in its
     sequence, less than its own; any other number (-1) marks a root.  Positions are then the context's length and the

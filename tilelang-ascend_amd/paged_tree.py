@@ -201,7 +201,7 @@ def paged_commit(caches: Union[torch.Tensor, Sequence[torch.Tensor]], block_tabl
     """Puts the accepted tokens' cache rows in order, in place.
 
     In each of ``caches`` ([blocks, block_size, ...], rows of any shape and type; keys and values of all layers, latents,
-    index keys), for k = 0, 1, .. below ``accepted[b]``, the row of key ``context_lens[b] + path[b, k]`` is copied to that
+    index keys and, [blocks, block_size], their scales), for k = 0, 1, .. below ``accepted[b]``, the row of key ``context_lens[b] + path[b, k]`` is copied to that
     of key ``context_lens[b] + k``, where path[b, k] > k (``path`` [B, max_path], as ``tree_accept`` leaves it).  Rows whose
     page is negative or outside the pool are left.  The context then holds ``context_lens + accepted`` tokens.  Rows must
     be multiples of 4 bytes; the caches must not overlap, and a sequence's new tokens lie in pages of its own.  One launch
@@ -217,7 +217,7 @@ def paged_commit(caches: Union[torch.Tensor, Sequence[torch.Tensor]], block_tabl
     dev = _lib.require_device(*caches, block_table, path, accepted)
     blocks = tuple(caches[0].shape[:2])
     for c in caches:
-        if c.dim() < 3 or tuple(c.shape[:2]) != blocks or c.numel() == 0:
+        if c.dim() < 2 or tuple(c.shape[:2]) != blocks or c.numel() == 0:
             raise ValueError(f"caches must be [blocks, block_size, ...] alike, got {tuple(c.shape)} beside {blocks}")
         _lib.require_contiguous("caches", c)
     if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1 or not _lib.is_integer(block_table):
