@@ -69,6 +69,35 @@ def test_plan_masks_past_their_words_and_windows(dsa, dev, win, max_nodes):
     check_plan(dsa, dev, new, ctx, table, free, [len(free)], 16, sum(new), parents, max_nodes, win)
 
 
+@pytest.mark.parametrize("win", [-1, 0, 63, 64, 500])
+@pytest.mark.parametrize("new,max_nodes", [([0, 3, 60, 66, 1, 130, 500], 64), ([900, 70], 4096), ([7, 1017], 128),
+                                           ([7, 1018], 0), ([200, 4500, 3, 700], 4096), ([77, 1500, 300], 200)])
+def test_plan_long_runs(dsa, dev, new, max_nodes, win):
+    """Rows whose parents are the rows before them, for whole sequences and parts, up to those that pass a workgroup's rows
+    and the parents that it holds at once, beside branches and rows without parents."""
+    rng = random.Random(sum(new) + win)
+    parents = []
+    for b, s in enumerate(new):
+        for i in range(s):
+            jump = b % 3 and rng.random() < 0.02
+            parents.append(rng.randint(-1, i) if jump else i - 1)
+    ctx = [rng.randint(0, 90) for _ in new]
+    mb = (max(new) + 90) // 16 + 2
+    table, free = make_lists(rng, ctx, 16, mb, sum(new) // 16 + 2 * len(new))
+    check_plan(dsa, dev, new, ctx, table, free, [len(free)], 16, sum(new) + 2, parents + [0, 1], max_nodes, win)
+
+
+@pytest.mark.parametrize("T", [1023, 1024, 1025, 2047, 2048, 2049])
+@pytest.mark.parametrize("tree", [False, True])
+def test_plan_on_both_sides_of_its_row_counts(dsa, dev, T, tree):
+    rng = random.Random(T)
+    new = [40] * (T // 40) + [T % 40]
+    ctx = [rng.randint(0, 60) for _ in new]
+    table, free = make_lists(rng, ctx, 16, 8, sum(new) // 16 + 2 * len(new))
+    parents = [p for s in new for p in R.tree(rng, s, 0.05)] if tree else None
+    check_plan(dsa, dev, new, ctx, table, free, [len(free)], 16, T, parents, 64)
+
+
 @pytest.mark.parametrize("count", [0, 1, 5, -3, 10**9])
 def test_plan_runs_out_of_pages_and_tables(dsa, dev, count):
     """Too few pages, contexts at and past the table's end, negative and huge lengths, holes in the context."""

@@ -25,6 +25,7 @@ def test_plan_c_checks(dsa):
     for kw, msg in [(dict(B=0), b"B must"), (dict(B=16385), b"B must"), (dict(bs=0), b"page"), (dict(mb=0), b"page"),
                     (dict(mb=2**30), b"page"), (dict(room=-1), b"page"), (dict(room=2**31), b"page"),
                     (dict(T=-1), b"T must"), (dict(T=2**30), b"T must"), (dict(par=16, W=-1), b"mask_words"),
+                    (dict(par=16, T=2**22 + 1), b"2^22 with parents"),
                     (dict(par=16, W=65), b"mask_words"), (dict(win=-2), b"win_left"), (dict(new=None), b"null"),
                     (dict(table=None), b"null"), (dict(free=None), b"null"), (dict(count=None), b"null"),
                     (dict(cu=None), b"null"), (dict(pos=None), b"null"), (dict(par=16, mask=None), b"null")]:

@@ -731,6 +731,8 @@ int dsa_paged_tree_fwd(int kind, const void* q, const void* k_cache, const void*
 
 // The limits of the page lists: the sums of a call's sequences lie in one workgroup's LDS, lengths in 30 bits.
 constexpr int64_t kPlanSeqs = 16384, kPlanRows = ((int64_t)1 << 30) - 1;
+// Of trees fewer rows: one that is 2^22 rows deep is followed to its root within 0.1 s.
+constexpr int64_t kPlanNodes = (int64_t)1 << 22;
 
 static int check_lists(const char* who, int64_t B, int64_t max_blocks, int64_t block_size, int64_t room) {
   char text[96];
@@ -750,6 +752,7 @@ int dsa_paged_plan(const int32_t* new_lens, const int32_t* context_lens, int32_t
                    uint64_t* tree_mask, void* stream) {
   if (const int rc = check_lists("paged_plan", B, max_blocks, block_size, free_room)) return rc;
   if (T < 0 || T > kPlanRows) return reject("paged_plan: T must be in [0, 2^30)");
+  if (parents && T > kPlanNodes) return reject("paged_plan: T must be at most 2^22 with parents");
   if (parents && (mask_words < 0 || mask_words > 64)) return reject("paged_plan: mask_words must be in [0, 64]");
   if (win_left < -1 || win_left > kMaxInt) return reject("paged_plan: win_left must be -1 (none) or a count");
   if (!new_lens || !context_lens || !block_table || !free_count || (free_room > 0 && !free_blocks) || !cu_seqlens ||

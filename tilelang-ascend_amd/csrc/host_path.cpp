@@ -708,7 +708,7 @@ PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   DSA_PLAIN(lists_ok(bt, list, count, dev));
   const int64_t B = bt.size(0);
   DSA_PLAIN(lens_ok(nl, dev, B) && lens_ok(ctx, dev, B) && lens_ok(parents, dev, T) && (win < 0 || parents) &&
-            (!parents || (nodes >= 0 && nodes <= 4096)));
+            (!parents || (nodes >= 0 && nodes <= 4096 && T <= 1 << 22)));
   const int64_t words = parents ? (nodes + 63) / 64 : 0;
   at::Tensor out[6];
   int rc;

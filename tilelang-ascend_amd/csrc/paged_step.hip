@@ -20,7 +20,8 @@ constexpr int kStepWaves = kStepThreads / kWave;
 //
 // Which page an entry gets depends on the entries before it in all sequences, and the table changes in place: one
 // workgroup counts and hands out (plan_pages_kernel), with the sums in LDS.  Its time is a chain of latencies (lengths,
-// sums, entries, list).  Few rows are written by the same workgroup, many by a second launch over the card.
+// sums, entries, list): 4.7 us for one tree of 64 nodes, 5.1 for 1024 rows of 16 sequences.  Few rows are written by the same
+// workgroup, many by a second launch over the card: 16384 rows of 256 trees in 9.8 us.
 
 struct PlanArgs {
   const int32_t* new_lens;   // [B]
@@ -75,56 +76,97 @@ __device__ __forceinline__ int plan_seq(const int* cu, int B, int t) {
   return b0;
 }
 
+struct PlanRow {
+  int t, start, i, position, slot;  // start: its sequence's first row, or t behind the last sequence
+  bool live;
+};
+
 // Row t: `cu` is a.cu or a copy.
-__device__ __forceinline__ void plan_row(const PlanArgs& a, const int* cu, int t) {
+__device__ __forceinline__ PlanRow plan_find(const PlanArgs& a, const int* cu, int t) {
   const int b = plan_seq(cu, a.B, t);
-  int position = -1, slot = -1, i = 0, start = 0;
-  if (b < a.B) {
-    start = b > 0 ? cu[b - 1] : 0;
-    i = t - start;
-    const int ctx = plan_len(a.ctx[b]), key = ctx + i, blk = key / a.block_size;
-    position = key;
-    if (blk < a.max_blocks) {
-      const int page = a.table[(int64_t)b * a.max_blocks + blk];
-      const int64_t at = (int64_t)page * a.block_size + (key - blk * a.block_size);
-      if (page >= 0 && at <= 0x7fffffff) slot = (int)at;
-    }
-    if (a.parents) position = ctx;
+  PlanRow r = {t, t, 0, -1, -1, b < a.B};
+  if (!r.live) return r;
+  r.start = b > 0 ? cu[b - 1] : 0;
+  r.i = t - r.start;
+  const int ctx = plan_len(a.ctx[b]), key = ctx + r.i, blk = key / a.block_size;
+  r.position = a.parents ? ctx : key;
+  if (blk < a.max_blocks) {
+    const int page = a.table[(int64_t)b * a.max_blocks + blk];
+    const int64_t at = (int64_t)page * a.block_size + (key - blk * a.block_size);
+    if (page >= 0 && at <= 0x7fffffff) r.slot = (int)at;
   }
-  if (a.parents) {
-    // Up to the root: parents lie before their children, so the words of the mask come from the last to the first.
-    uint64_t* row = a.mask + (int64_t)t * a.words;
-    int word = a.words - 1, depth = 0;
-    uint64_t bits = 0;
-    if (b < a.B) {
-      for (int n = i;; ++depth) {
-        if ((a.win < 0 || depth <= a.win) && (n >> 6) < a.words) {
-          for (; word > (n >> 6); --word) {
-            row[word] = bits;
-            bits = 0;
-          }
-          bits |= (uint64_t)1 << (n & 63);
-        }
-        const int up = a.parents[start + n];
-        if (up < 0 || up >= n) break;
-        n = up;
-      }
-      position += depth;
-    }
-    for (; word >= 0; --word) {
+  return r;
+}
+
+// A run of rows whose parent is the row before (drafts without branches, prompts) is taken at once on the way up, as far
+// as its part in the wave that reads its parents: `length` rows before row p are on it, `up` is the parent of the first.
+// One row a step took 0.2 us and more each, 106 us for a run of 512 rows and 2576 for 4096; now 6.6 and 25.
+struct PlanRun {
+  int length, up;
+};
+
+// Of the rows that the wave's lanes hold in order, with their places and parents.
+__device__ __forceinline__ PlanRun plan_run(int i, int parent) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const uint64_t before = __ballot(i <= 0 || parent != i - 1) & (~(uint64_t)0 >> (63 - lane));
+  const int top = before ? 63 - __clzll((long long)before) : 0;
+  return {lane - top, __shfl(parent, top, kWave)};
+}
+
+// A row's way up its tree, node n at a depth of `depth` below the row.
+struct PlanPath {
+  int n, depth = 0, word;
+  uint64_t bits = 0;
+  bool up;
+  uint64_t* row;
+  __device__ __forceinline__ PlanPath(const PlanArgs& a, const PlanRow& r)
+      : n(r.i), word(a.words - 1), up(r.live), row(a.mask + (int64_t)r.t * a.words) {}
+
+  // Parents lie before their children, so the words of the mask come from the last to the first.
+  __device__ __forceinline__ void down_to(int w) {
+    for (; word > w; --word) {
       row[word] = bits;
       bits = 0;
     }
   }
-  a.positions[t] = position;
-  a.slots[t] = slot;
-}
+  // Nodes from .. to, at most 64 of them.
+  __device__ __forceinline__ void add(int from, int to, int words) {
+    to = min(to, words * kWave - 1);
+    if (from > to) return;
+    const uint64_t all = ~(uint64_t)0, upper = all >> (63 - (to & 63)), lower = all << (from & 63);
+    down_to(to >> 6);
+    if (from >> 6 == to >> 6) {
+      bits |= upper & lower;
+    } else {
+      bits |= upper;
+      down_to(from >> 6);
+      bits |= lower;
+    }
+  }
+  __device__ __forceinline__ void take(const PlanArgs& a, PlanRun run) {
+    const int top = n - run.length;
+    if (a.win < 0 || depth <= a.win) add(a.win < 0 ? top : max(top, n - (a.win - depth)), n, a.words);
+    up = run.up >= 0 && run.up < top;
+    depth += run.length + (up ? 1 : 0);
+    n = run.up;
+  }
+  // As far as the window goes, `runs` from row lo on.
+  __device__ __forceinline__ void climb(const PlanArgs& a, const PlanRow& r, const PlanRun* runs, int lo) {
+    while (up && r.start + n >= lo) take(a, runs[r.start + n - lo]);
+  }
+  __device__ __forceinline__ void end(const PlanArgs& a, const PlanRow& r) {
+    down_to(-1);
+    a.positions[r.t] = r.live ? r.position + depth : -1;
+    a.slots[r.t] = r.slot;
+  }
+};
 
 // `rows`: this workgroup writes the rows too.
 __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, int rows) {
   extern __shared__ __align__(16) int plan_lds[];
   __shared__ int sums[kStepWaves];
   __shared__ int next[kStepThreads];  // the pages handed out first
+  __shared__ PlanRun runs[kStepThreads];
   int* cu = plan_lds;                 // [B] sums of the lengths
   int* touched = plan_lds + a.B;      // [B] sums of the touched blocks
   const int tid = threadIdx.x, bs = a.block_size;
@@ -133,6 +175,7 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
   const auto add = [](int x, int y) { return x + y; };
   int rows_before = 0, blocks_before = 0;
   const int count = min(max(a.free_count[0], 0), a.room);
+  const int parent = rows && a.parents && tid < a.T ? a.parents[tid] : -1;
   for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
     const int b = b0 + tid;
     const bool live = b < a.B;
@@ -183,27 +226,87 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
   }
   __syncthreads();
   if (tid == 0) a.free_count[0] = max(count - taken, 0);
-  if (rows)
-    for (int t = tid; t < a.T; t += kStepThreads) plan_row(a, cu, t);
+  if (!rows) return;
+  if (!a.parents) {
+    for (int t = tid; t < a.T; t += kStepThreads) {
+      const PlanRow r = plan_find(a, cu, t);
+      a.positions[t] = r.position;
+      a.slots[t] = r.slot;
+    }
+    return;
+  }
+  // Of trees a row a thread.
+  const bool in = tid < a.T;
+  const PlanRow r = in ? plan_find(a, cu, tid) : PlanRow{tid, tid, 0, -1, -1, false};
+  const PlanRun run = plan_run(r.i, parent);
+  runs[tid] = run;
+  __syncthreads();
+  if (!in) return;
+  PlanPath path(a, r);
+  if (path.up) path.take(a, run);
+  path.climb(a, r, runs, 0);
+  path.end(a, r);
 }
 
 constexpr int kPlanRowThreads = 256;
 constexpr int kPlanRowCu = 2048;
+constexpr int kPlanWindow = 2048;  // rows whose runs a workgroup holds at once
 __global__ __launch_bounds__(kPlanRowThreads) void plan_rows_kernel(PlanArgs a) {
   __shared__ int copy[kPlanRowCu];
+  const int t0 = blockIdx.x * kPlanRowThreads, t = t0 + threadIdx.x;
+  const bool in = t < a.T;
+  // Asked for first: the row's parent, and that of the row one workgroup before.
+  const int parent = a.parents && in ? a.parents[t] : -1;
+  const int before = a.parents && t0 > 0 ? a.parents[t - kPlanRowThreads] : -1;
   const bool copied = a.B <= kPlanRowCu;
   if (copied) {
     for (int b = threadIdx.x; b < a.B; b += kPlanRowThreads) copy[b] = a.cu[b];
     __syncthreads();
   }
-  const int t = blockIdx.x * kPlanRowThreads + threadIdx.x;
-  if (t < a.T) plan_row(a, copied ? copy : a.cu, t);
+  const PlanRow r = in ? plan_find(a, copied ? copy : a.cu, t) : PlanRow{t, t, 0, -1, -1, false};
+  if (!a.parents) {
+    if (in) {
+      a.positions[t] = r.position;
+      a.slots[t] = r.slot;
+    }
+    return;
+  }
+  // Three windows: the workgroup's own rows, as many before them, and, while any row's way goes on there, further ones of
+  // the sequence that the first row is in.
+  __shared__ PlanRun runs[2 * kPlanRowThreads];
+  __shared__ PlanRun more[kPlanWindow];
+  __shared__ int first;
+  if (threadIdx.x == 0) first = r.start;
+  __syncthreads();
+  const int s0 = first;
+  const PlanRun run = plan_run(r.i, parent);
+  runs[kPlanRowThreads + threadIdx.x] = run;
+  if (s0 < t0) runs[threadIdx.x] = plan_run(t - kPlanRowThreads - s0, before);
+  __syncthreads();
+  PlanPath path(a, r);
+  if (path.up) {
+    path.take(a, run);
+    path.climb(a, r, runs, t0 - kPlanRowThreads);
+  }
+  for (int lo = t0 - kPlanRowThreads; lo > s0;) {
+    if (!__syncthreads_or(path.up)) break;
+    const int end = lo;
+    lo = max(end - (end - s0 + kWave - 1) / kWave * kWave, end - kPlanWindow);
+#pragma unroll 4
+    for (int p = lo + (int)threadIdx.x; p < end; p += kPlanRowThreads)
+      more[p - lo] = plan_run(p - s0, p >= s0 ? a.parents[p] : -1);
+    __syncthreads();
+    path.climb(a, r, more, lo);
+  }
+  if (in) path.end(a, r);
 }
 
-// Rows that the workgroup of the plan writes by itself.
-constexpr int kPlanFewRows = 4096;
+// Rows that the workgroup of the plan writes by itself: without trees two a thread, with them one.  2048 rows without trees
+// 6.3 us, in a second launch 6.8; 4096 rows 8.3 and 7.1.  1024 rows of trees 7.0 and 8.0; a
+// second row a thread would cost them 2.4 more, the second launch 0.3.
+constexpr int kPlanFewRows = 2 * kStepThreads, kPlanFewNodes = kStepThreads;
 
-// Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, sizes and pointers; words 0 for no masks.
+// Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, with parents up to 2^22, sizes and pointers; words 0 for no masks.
 hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_t* table, const int32_t* free_list,
                              int32_t* free_count, const int32_t* parents, int64_t B, int64_t T, int64_t max_blocks,
                              int64_t block_size, int64_t room, int64_t words, int64_t win, int32_t* cu, int32_t* kv,
@@ -214,7 +317,7 @@ hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_
   const int lds = 2 * (int)B * (int)sizeof(int);
   hipError_t e = set_dynamic_lds_once<plan_pages_kernel>(2 * 16384 * (int)sizeof(int));
   if (e != hipSuccess) return e;
-  const bool few = T <= kPlanFewRows;
+  const bool few = T <= (parents ? kPlanFewNodes : kPlanFewRows);
   hipLaunchKernelGGL(plan_pages_kernel, dim3(1), dim3(kStepThreads), lds, stream, a, few ? 1 : 0);
   if (!few)
     hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((T + kPlanRowThreads - 1) / kPlanRowThreads)),
@@ -227,7 +330,8 @@ hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_
 // The pages behind the blocks of keep_b keys, up to the first negative entry, go back to the list: of n pages in the
 // order (sequence, block) the i-th to place count + n - 1 - i, so that giving back what a plan took leaves the list as it
 // was.  Pages that would lie past the list's room stay in the table.  One workgroup: a lane group a sequence counts, the
-// counts are summed, and the groups move the entries.
+// counts are summed, and the groups move the entries.  Bound by latencies: 3.0 us for a sequence's 128 pages, 3.4 for 64
+// sequences of up to 8 pages, 12.4 for 1024.
 
 struct FreeArgs {
   const int32_t* keep;  // [B]
@@ -307,7 +411,10 @@ hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_
     return hipGetLastError();
   };
   constexpr int kLds = 16384 * (int)sizeof(int);
-  // A pass of the workgroup over the sequences is a round trip: lanes enough for one pass, eight at least.
+  // A pass of the workgroup over the sequences is a round trip, and so is a step of a group along its row: lanes enough for
+  // one pass, eight at least.  64 lanes a sequence against 16: 16 sequences 3.6 us and 3.0 where they give back few pages, 5.9
+  // and 17.2 with 512 each; 64 sequences 7.4 and 3.4, 17.4 and 20.5.  16 against 8: 64 sequences 3.4 and 3.3, 7.4 and 10.9 with
+  // 128 pages; 256 sequences 7.2 and 4.8, 23.7 and 22.9.
   if (B <= kStepThreads / 64) return run(free_pages_kernel<64>, set_dynamic_lds_once<free_pages_kernel<64>>(kLds));
   if (B <= kStepThreads / 16) return run(free_pages_kernel<16>, set_dynamic_lds_once<free_pages_kernel<16>>(kLds));
   return run(free_pages_kernel<8>, set_dynamic_lds_once<free_pages_kernel<8>>(kLds));
@@ -585,7 +692,9 @@ hipError_t launch_tree_accept(int kind, const void* scores, int64_t stride, int6
 // In every cache, for k = 0, 1, ..: row(ctx_b + k) = row(ctx_b + path[b, k]), where path[b, k] > k.  A wave takes up to
 // 1 KB of the columns of a cache's rows of one sequence, a lane 16 bytes of each, so that no lane reads what another one
 // writes.  Eight rows are read before the eight are written: a source lies behind its own place and so behind all places
-// written before, which makes this the same as one row after the other.  Bound by latencies: lengths, path, table, rows.
+// written before, which makes this the same as one row after the other.  Bound by latencies (lengths, path, table, rows)
+// where there is little to move: 3.8 us for one sequence; 122 caches of 64 sequences, four rows of 1152 bytes each, take 16.0 us,
+// 4.5 TB/s.  Where rows or a cache do not start on 16 bytes a lane takes 4: 3.7 and 23.9 us at these sizes.
 
 constexpr int kCommitCaches = 128;  // of a launch: their descriptions are kernel arguments
 constexpr int kCommitWaves = 4;

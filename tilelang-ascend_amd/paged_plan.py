@@ -65,7 +65,9 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
     sequence, less than its own; any other number (-1) marks a root.  Positions are then the context's length and the
     depth, and ``tree_mask`` [T, W], W = ceil(max_nodes / 64), has the bits of a node and its ancestors, with ``win_left``
     those at most so many steps up.  ``max_nodes`` (at most 4096) bounds a sequence's nodes; nodes past 64 W are seen by
-    none.  With 0, the default, no masks are made: those of trees that keep their shape need not be made again.  At most 16384 sequences, fewer than 2^30 rows; lengths count up to 2^30.
+    none.  With 0, the default, no masks are made: those of trees that keep their shape need not be made again.
+
+    At most 16384 sequences; fewer than 2^30 rows, with ``parents`` at most 2^22; lengths count up to 2^30.
     """
     win = -1 if win_left is None else -2 if win_left == -1 else win_left  # -1: none, in the calls below
     res = _lib.host_path().paged_plan(new_lens, context_lens, block_table, free_blocks, free_count, block_size,
@@ -80,6 +82,8 @@ def paged_plan(new_lens, context_lens, block_table: torch.Tensor, free_blocks: t
         raise ValueError(f"at most 16384 sequences, got {B}")
     T, words = num_tokens, 0
     if parents is not None:
+        if T > 2**22:
+            raise ValueError(f"num_tokens must be at most 2^22 with parents, got {T}")
         if not isinstance(max_nodes, int) or not 0 <= max_nodes <= 4096:
             raise ValueError(f"max_nodes must be in [0, 4096], got {max_nodes}")
         words = -(-max_nodes // 64)
