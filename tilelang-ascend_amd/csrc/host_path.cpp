@@ -684,11 +684,13 @@ struct Ints {
   at::Tensor all;
   int64_t used = 0;
   Ints(int64_t n, int parts, c10::Device dev) : all(make({n + 4 * parts}, at::kInt, dev)) {}
-  at::Tensor part(at::IntArrayRef sizes) {
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-    t.unsafeGetTensorImpl()->set_storage_offset(used);
+  at::Tensor part(at::IntArrayRef sizes, at::ScalarType type = at::kInt) {
+    const int64_t ints = type == at::kLong ? 2 : 1;  // of an element
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                            at::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(used / ints);
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-    used += (t.numel() + 3) / 4 * 4;
+    used += (t.numel() * ints + 3) / 4 * 4;
     return t;
   }
 };
@@ -715,9 +717,9 @@ PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   {
     const NoGil unlocked;
     const c10::OptionalDeviceGuard guard(dev);
-    Ints ints(3 * B + 2 * T, 5, dev);
+    Ints ints(3 * B + 2 * T + 2 * T * words, 6, dev);
     for (int i = 0; i < 5; ++i) out[i] = ints.part({i == 2 || i == 3 ? T : B});
-    if (words) out[5] = make({T, words}, at::kLong, dev);
+    if (words) out[5] = ints.part({T, words}, at::kLong);
     int32_t* p[5];
     for (int i = 0; i < 5; ++i) p[i] = out[i].data_ptr<int32_t>();
     rc = E.plan(nl.ptr<int32_t>(), ctx.ptr<int32_t>(), bt.data_ptr<int32_t>(), list.data_ptr<int32_t>(),

@@ -20,8 +20,8 @@ constexpr int kStepWaves = kStepThreads / kWave;
 //
 // Which page an entry gets depends on the entries before it in all sequences, and the table changes in place: one
 // workgroup counts and hands out (plan_pages_kernel), with the sums in LDS.  Its time is a chain of latencies (lengths,
-// sums, entries, list): 4.7 us for one tree of 64 nodes, 5.1 for 1024 rows of 16 sequences.  Few rows are written by the same
-// workgroup, many by a second launch over the card: 16384 rows of 256 trees in 9.8 us.
+// sums, entries, list): 3.6 us for one tree of 64 nodes, 4.2 for 1024 rows of 16 sequences.  Few rows are written by the same
+// workgroup, many by a second launch over the card: 16384 rows of 256 trees in 8.2 us.
 
 struct PlanArgs {
   const int32_t* new_lens;   // [B]
@@ -43,26 +43,39 @@ constexpr int kPlanMost = 1 << 30;  // lengths past it count as this many, so th
 
 __device__ __forceinline__ int plan_len(int x) { return min(max(x, 0), kPlanMost); }
 
-// Inclusive scan of op over the workgroup's threads (kStepThreads of them); `sums` holds kStepWaves values.  Every thread
-// gets its own result and the total.
+// v of the lane that `kCtrl` names, 0 where there is none or outside the rows of lanes in `kRows`: a move within the registers.
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ int lane_move(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, false);
+}
+// Inclusive scan over each 16 lanes: neighbours 1, 2, 4 and 8 lanes below.  0 changes nothing under op.
 template <class Op>
-__device__ __forceinline__ int step_scan(int v, int* sums, int& total, Op op) {
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int u = __shfl_up(v, o, kWave);
-    if (lane >= o) v = op(u, v);
-  }
+__device__ __forceinline__ int scan16(int v, Op op) {
+  v = op(lane_move<0x111>(v), v);
+  v = op(lane_move<0x112>(v), v);
+  v = op(lane_move<0x114>(v), v);
+  return op(lane_move<0x118>(v), v);
+}
+
+// Scan of op over the workgroup's threads (kStepThreads of them); `sums` holds kStepWaves values.  Every thread gets its
+// own result, that of the threads before it and the total.  Lanes pass values within the registers: a step through LDS costs
+// a wave 60 cycles or more, and a plan makes three scans one behind the other.
+struct StepScan {
+  int upto, before, total;
+};
+template <class Op>
+__device__ __forceinline__ StepScan step_scan(int v, int* sums, Op op) {
+  static_assert(kStepWaves == 16, "a wave's 16 lanes scan the waves' sums");
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  v = scan16(v, op);
+  v = op(lane_move<0x142, 0xa>(v), v);  // rows of 16 lanes: the last lane of the row before, then of the half before
+  v = op(lane_move<0x143, 0xc>(v), v);
   if (lane == kWave - 1) sums[wave] = v;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kStepWaves; ++w) {
-    if (w == wave) before = total;
-    total = op(total, sums[w]);
-  }
+  const int all = scan16(sums[lane & 15], op);
+  const int before = wave > 0 ? __builtin_amdgcn_readlane(all, wave - 1) : 0;
   __syncthreads();  // sums may be written again
-  return wave > 0 ? op(before, v) : v;
+  return {op(before, v), op(before, lane_move<0x138>(v)), __builtin_amdgcn_readlane(all, 15)};
 }
 
 // The sequence of packed row t: the first whose sum is past it, B where there is none.
@@ -100,7 +113,7 @@ __device__ __forceinline__ PlanRow plan_find(const PlanArgs& a, const int* cu, i
 
 // A run of rows whose parent is the row before (drafts without branches, prompts) is taken at once on the way up, as far
 // as its part in the wave that reads its parents: `length` rows before row p are on it, `up` is the parent of the first.
-// One row a step took 0.2 us and more each, 106 us for a run of 512 rows and 2576 for 4096; now 6.6 and 25.
+// One row a step took 0.2 us and more each, 106 us for a run of 512 rows and 2576 for 4096; now 5.4 and 24.
 struct PlanRun {
   int length, up;
 };
@@ -161,12 +174,18 @@ struct PlanPath {
   }
 };
 
-// `rows`: this workgroup writes the rows too.
+// Rows that the workgroup of the plan writes by itself, in turns of kStepThreads.  One launch against two: 1024 rows 4.2 us
+// and 5.5 (of trees 6.0 and 7.3), 2048 rows 5.1 and 5.9 (8.7 and 7.5); 4096 rows take one workgroup 8 us and more (14 of
+// trees), two launches 6.2 (7.6).  The second launch costs the host 2 us or more as well: a plan of 1952 rows of 32 trees with
+// the pages' way back, call after call, 10.4 us with one and 12.7 with two.
+constexpr int kPlanRowsEach = 2, kPlanFewRows = kPlanRowsEach * kStepThreads;
+
+// `rows`: this workgroup writes the rows too, kPlanFewRows of them at most.
 __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, int rows) {
   extern __shared__ __align__(16) int plan_lds[];
   __shared__ int sums[kStepWaves];
   __shared__ int next[kStepThreads];  // the pages handed out first
-  __shared__ PlanRun runs[kStepThreads];
+  __shared__ PlanRun runs[kPlanFewRows];
   int* cu = plan_lds;                 // [B] sums of the lengths
   int* touched = plan_lds + a.B;      // [B] sums of the touched blocks
   const int tid = threadIdx.x, bs = a.block_size;
@@ -175,29 +194,30 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
   const auto add = [](int x, int y) { return x + y; };
   int rows_before = 0, blocks_before = 0;
   const int count = min(max(a.free_count[0], 0), a.room);
-  const int parent = rows && a.parents && tid < a.T ? a.parents[tid] : -1;
+  int parent[kPlanRowsEach];
+#pragma unroll
+  for (int u = 0; u < kPlanRowsEach; ++u)
+    parent[u] = rows && a.parents && u * kStepThreads + tid < a.T ? a.parents[u * kStepThreads + tid] : -1;
   for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
     const int b = b0 + tid;
     const bool live = b < a.B;
     const int ctx = live ? plan_len(a.ctx[b]) : 0, want = live ? min(plan_len(a.new_lens[b]), most) : 0;
     // Asked for while the sums are made.
     if (b0 == 0) next[tid] = tid < count ? a.free_list[count - 1 - tid] : -1;
-    int total;
-    const int sum = add_rows(rows_before, step_scan(want, sums, total, add_rows));
-    // The sum before this one is the neighbour's: through LDS.
-    if (live) cu[b] = sum;
-    __syncthreads();
-    const int len = live ? sum - (b > 0 ? cu[b - 1] : 0) : 0;
-    rows_before = add_rows(rows_before, total);
+    const StepScan rows_scan = step_scan(want, sums, add_rows);
+    const int sum = add_rows(rows_before, rows_scan.upto), len = live ? sum - add_rows(rows_before, rows_scan.before) : 0;
+    rows_before = add_rows(rows_before, rows_scan.total);
     int blocks = 0, past = 0;
     if (len > 0) {
       const int first = ctx / bs, last = (ctx + len - 1) / bs;
       blocks = max(min(last, a.max_blocks - 1) - first + 1, 0);
       past = last - first + 1 - blocks;
     }
-    const int upto = blocks_before + step_scan(blocks, sums, total, add);
-    blocks_before += total;
+    const StepScan blocks_scan = step_scan(blocks, sums, add);
+    const int upto = blocks_before + blocks_scan.upto;
+    blocks_before += blocks_scan.total;
     if (live) {
+      cu[b] = sum;
       touched[b] = upto;
       a.cu[b] = sum;
       a.kv[b] = ctx + len;
@@ -216,9 +236,9 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
       entry = a.table + (int64_t)b * a.max_blocks + blk;
     }
     const bool lacks = entry && *entry < 0;
-    int total;
-    const int rank = taken + step_scan(lacks ? 1 : 0, sums, total, add) - 1;
-    taken += total;
+    const StepScan scan = step_scan(lacks ? 1 : 0, sums, add);
+    const int rank = taken + scan.before;
+    taken += scan.total;
     if (lacks) {
       if (rank < count) *entry = rank < kStepThreads ? next[rank] : a.free_list[count - 1 - rank];
       else atomicAdd(a.missing + b, 1);
@@ -235,17 +255,24 @@ __global__ __launch_bounds__(kStepThreads) void plan_pages_kernel(PlanArgs a, in
     }
     return;
   }
-  // Of trees a row a thread.
-  const bool in = tid < a.T;
-  const PlanRow r = in ? plan_find(a, cu, tid) : PlanRow{tid, tid, 0, -1, -1, false};
-  const PlanRun run = plan_run(r.i, parent);
-  runs[tid] = run;
+  PlanRow r[kPlanRowsEach];
+  PlanRun run[kPlanRowsEach];
+#pragma unroll
+  for (int u = 0; u < kPlanRowsEach; ++u) {
+    const int t = u * kStepThreads + tid;
+    r[u] = t < a.T ? plan_find(a, cu, t) : PlanRow{t, t, 0, -1, -1, false};
+    run[u] = plan_run(r[u].i, parent[u]);
+    runs[t] = run[u];
+  }
   __syncthreads();
-  if (!in) return;
-  PlanPath path(a, r);
-  if (path.up) path.take(a, run);
-  path.climb(a, r, runs, 0);
-  path.end(a, r);
+#pragma unroll
+  for (int u = 0; u < kPlanRowsEach; ++u) {
+    if (r[u].t >= a.T) return;
+    PlanPath path(a, r[u]);
+    if (path.up) path.take(a, run[u]);
+    path.climb(a, r[u], runs, 0);
+    path.end(a, r[u]);
+  }
 }
 
 constexpr int kPlanRowThreads = 256;
@@ -301,11 +328,6 @@ __global__ __launch_bounds__(kPlanRowThreads) void plan_rows_kernel(PlanArgs a) 
   if (in) path.end(a, r);
 }
 
-// Rows that the workgroup of the plan writes by itself: without trees two a thread, with them one.  2048 rows without trees
-// 6.3 us, in a second launch 6.8; 4096 rows 8.3 and 7.1.  1024 rows of trees 7.0 and 8.0; a
-// second row a thread would cost them 2.4 more, the second launch 0.3.
-constexpr int kPlanFewRows = 2 * kStepThreads, kPlanFewNodes = kStepThreads;
-
 // Caller validated: 1 <= B <= 16384, 0 <= T < 2^30, with parents up to 2^22, sizes and pointers; words 0 for no masks.
 hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_t* table, const int32_t* free_list,
                              int32_t* free_count, const int32_t* parents, int64_t B, int64_t T, int64_t max_blocks,
@@ -317,7 +339,7 @@ hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_
   const int lds = 2 * (int)B * (int)sizeof(int);
   hipError_t e = set_dynamic_lds_once<plan_pages_kernel>(2 * 16384 * (int)sizeof(int));
   if (e != hipSuccess) return e;
-  const bool few = T <= (parents ? kPlanFewNodes : kPlanFewRows);
+  const bool few = T <= kPlanFewRows;
   hipLaunchKernelGGL(plan_pages_kernel, dim3(1), dim3(kStepThreads), lds, stream, a, few ? 1 : 0);
   if (!few)
     hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((T + kPlanRowThreads - 1) / kPlanRowThreads)),
@@ -330,8 +352,8 @@ hipError_t launch_paged_plan(const int32_t* new_lens, const int32_t* ctx, int32_
 // The pages behind the blocks of keep_b keys, up to the first negative entry, go back to the list: of n pages in the
 // order (sequence, block) the i-th to place count + n - 1 - i, so that giving back what a plan took leaves the list as it
 // was.  Pages that would lie past the list's room stay in the table.  One workgroup: a lane group a sequence counts, the
-// counts are summed, and the groups move the entries.  Bound by latencies: 3.0 us for a sequence's 128 pages, 3.4 for 64
-// sequences of up to 8 pages, 12.4 for 1024.
+// counts are summed, and the groups move the entries.  Bound by latencies: 2.4 us for a sequence's 128 pages, 2.7 for 64
+// sequences of up to 8 pages, 14.7 for 1024.
 
 struct FreeArgs {
   const int32_t* keep;  // [B]
@@ -353,6 +375,8 @@ __global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
     const int keep = plan_len(a.keep[b]);
     return keep / a.block_size + (keep % a.block_size ? 1 : 0);
   };
+  const int count = min(max(a.free_count[0], 0), a.room);
+  int kept[kAhead];  // the first entries of the group's first row
   for (int b = tid / kGroup; b < a.B; b += kSeqs) {
     const int32_t* row = a.table + (int64_t)b * a.max_blocks;
     const int from = first_block(b);
@@ -361,6 +385,9 @@ __global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
       int page[kAhead];  // negative: none
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) page[u] = row[min(j + u * kGroup + in, (int64_t)a.max_blocks - 1)];
+      if (b == tid / kGroup && j == from)
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) kept[u] = page[u];
       bool ended = false;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
@@ -378,24 +405,26 @@ __global__ __launch_bounds__(kStepThreads) void free_pages_kernel(FreeArgs a) {
   int all = 0;
   for (int b0 = 0; b0 < a.B; b0 += kStepThreads) {
     const int b = b0 + tid;
-    int total;
-    const int sum = all + step_scan(b < a.B ? upto[b] : 0, sums, total, [](int x, int y) { return x + y; });
-    all += total;
-    if (b < a.B) upto[b] = sum;
+    const StepScan scan = step_scan(b < a.B ? upto[b] : 0, sums, [](int x, int y) { return x + y; });
+    if (b < a.B) upto[b] = all + scan.upto;
+    all += scan.total;
   }
-  __syncthreads();
-  const int count = min(max(a.free_count[0], 0), a.room);
   __syncthreads();
   for (int b = tid / kGroup; b < a.B; b += kSeqs) {
     const int before = b > 0 ? upto[b - 1] : 0, n = upto[b] - before;
     int32_t* row = a.table + (int64_t)b * a.max_blocks + first_block(b);
-    for (int j = in; j < n; j += kGroup) {
+    const auto give = [&](int j, int page) {
       const int64_t to = (int64_t)count + all - 1 - (before + j);
       if (to < a.room) {
-        a.free_list[to] = row[j];
+        a.free_list[to] = page;
         row[j] = -1;
       }
-    }
+    };
+    const int held = b == tid / kGroup ? kAhead * kGroup : 0;  // of the row's entries in registers
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (u * kGroup + in < min(n, held)) give(u * kGroup + in, kept[u]);
+    for (int j = held + in; j < n; j += kGroup) give(j, row[j]);
   }
   if (tid == 0) a.free_count[0] = (int)min((int64_t)count + all, (int64_t)a.room);
 }
@@ -412,9 +441,9 @@ hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_
   };
   constexpr int kLds = 16384 * (int)sizeof(int);
   // A pass of the workgroup over the sequences is a round trip, and so is a step of a group along its row: lanes enough for
-  // one pass, eight at least.  64 lanes a sequence against 16: 16 sequences 3.6 us and 3.0 where they give back few pages, 5.9
-  // and 17.2 with 512 each; 64 sequences 7.4 and 3.4, 17.4 and 20.5.  16 against 8: 64 sequences 3.4 and 3.3, 7.4 and 10.9 with
-  // 128 pages; 256 sequences 7.2 and 4.8, 23.7 and 22.9.
+  // one pass, eight at least.  64 lanes a sequence against 16, before the scan lay in the registers (0.7 us less for all): 16
+  // sequences 3.6 us and 3.0 where they give back few pages, 5.9 and 17.2 with 512 each; 64 sequences 7.4 and 3.4, 17.4 and
+  // 20.5.  16 against 8: 64 sequences 3.4 and 3.3, 7.4 and 10.9 with 128 pages; 256 sequences 7.2 and 4.8, 23.7 and 22.9.
   if (B <= kStepThreads / 64) return run(free_pages_kernel<64>, set_dynamic_lds_once<free_pages_kernel<64>>(kLds));
   if (B <= kStepThreads / 16) return run(free_pages_kernel<16>, set_dynamic_lds_once<free_pages_kernel<16>>(kLds));
   return run(free_pages_kernel<8>, set_dynamic_lds_once<free_pages_kernel<8>>(kLds));
