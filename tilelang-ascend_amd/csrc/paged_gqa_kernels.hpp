@@ -49,6 +49,7 @@ constexpr int kPgWaves = 4;
 constexpr int kPgThreads = kPgWaves * kWave;
 constexpr int kPgUnit = kPgWaves * kPgTile;  // 128 keys
 constexpr int kPgMaxSlots = 4096;            // of a call whose tiles share the line of units
+constexpr int kPgTreeSlots = 1200;           // of trees in tiles of kPrRows
 constexpr int kPgFewSlots = 256;             // of all groups: the join takes a pass a workgroup
 constexpr float kPgInf = __builtin_huge_valf();
 
@@ -82,24 +83,32 @@ struct PgSeq {
 
 // b = B is the padding behind the last packed sequence: no keys.  span: tokens whose rows are written (a padded
 // batch's sequences hold S rows, of which len are real).  Lengths and prefix sums are clamped before any use.
-__device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, int b) {
+__device__ __forceinline__ void pg_keys(const PgArgs& a, PgSeq& s);
+// `cu`, `q_len` and `kv_len` are the arguments' or copies of them.
+template <class Cu, class Len>
+__device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, Cu cu, Len q_len, Len kv_len, int b) {
   PgSeq s;
   if (a.cu_q) {
-    const int from = b > 0 ? min(max(a.cu_q[b - 1], 0), a.T) : 0;
-    const int to = b < a.B ? min(max(a.cu_q[b], from), a.T) : a.T;
+    const int from = b > 0 ? min(max(cu[b - 1], 0), a.T) : 0;
+    const int to = b < a.B ? min(max(cu[b], from), a.T) : a.T;
     s.start = from;
     s.span = s.len = to - from;
   } else {
     s.start = b < a.B ? b * a.S : a.T;
     s.span = b < a.B ? a.S : 0;
-    s.len = b < a.B && a.q_len ? min(max(a.q_len[b], 0), a.S) : s.span;
+    s.len = b < a.B && a.q_len ? min(max(q_len[b], 0), a.S) : s.span;
   }
-  s.n = b < a.B ? min(max(a.kv_len[b], 0), a.max_blocks * a.block_size) : 0;
+  s.n = b < a.B ? min(max(kv_len[b], 0), a.max_blocks * a.block_size) : 0;
+  pg_keys(a, s);
+  return s;
+}
+__device__ __forceinline__ PgSeq pg_seq(const PgArgs& a, int b) { return pg_seq(a, a.cu_q, a.q_len, a.kv_len, b); }
+// The keys that its tokens see, at most.
+__device__ __forceinline__ void pg_keys(const PgArgs& a, PgSeq& s) {
   s.hi = s.len > 0 ? s.n : 0;
   const int first = s.n - s.len;  // position of the first token
   s.lo = a.win >= 0 && first > a.win ? (first - a.win) & ~(kPgTile - 1) : 0;
   if (s.lo > s.hi) s.lo = s.hi;
-  return s;
 }
 
 template <int kD>
@@ -568,10 +577,13 @@ __device__ __forceinline__ void pg_rows(const PgArgs& a, const PgSeq& s, int b, 
   const int lim = tok < s.len ? (kTree ? first_node - 1 : a.causal ? min(pos, s.n - 1) : s.n - 1) : -1;
   const int low = a.win >= 0 ? max(pos, 0) - a.win : 0;
   int lim_min = lim, low_max = low;  // tiles in which every row sees every key skip the comparisons
+  // Trees without a window nor padding: alike in all rows.
+  if (!kTree || a.win >= 0 || s.len != s.span) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    lim_min = min(lim_min, __shfl_xor(lim_min, o, kWave));
-    low_max = max(low_max, __shfl_xor(low_max, o, kWave));
+    for (int o = 1; o < 32; o <<= 1) {
+      lim_min = min(lim_min, __shfl_xor(lim_min, o, kWave));
+      low_max = max(low_max, __shfl_xor(low_max, o, kWave));
+    }
   }
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
   low_max = __builtin_amdgcn_readfirstlane(low_max);
@@ -1140,28 +1152,80 @@ __global__ __launch_bounds__(W::kThreads) void pg_direct_kernel(PgArgs a) {
 // LDS; the first writes it out for the join.
 constexpr int kPgExtra = 3;
 constexpr int kPgLineCu = 1024;
+template <bool kKept>
 struct PgLine {
   int at[kPgMaxSlots + 1];
   uint16_t seq[kPgMaxSlots];
   int32_t cu[kPgLineCu];
 };
+// Trees in tiles of kPrRows: what the slot's sequence was found to be stays beside it, so that a workgroup asks memory for
+// the lengths once, all of them together (8 nodes over 4097 keys: 16.0 -> 15.2 us).
+template <>
+struct PgLine<true> {
+  int at[kPgTreeSlots + 1];
+  uint16_t seq[kPgTreeSlots];
+  int32_t cu[kPgLineCu];
+  int start[kPgTreeSlots], len[kPgTreeSlots], n[kPgTreeSlots];
+  // The span: len in packed rows, S in a padded batch.
+  __device__ __forceinline__ PgSeq of(const PgArgs& a, int x) const {
+    PgSeq s;
+    s.start = __builtin_amdgcn_readfirstlane(start[x]);
+    s.len = __builtin_amdgcn_readfirstlane(len[x]);
+    s.n = __builtin_amdgcn_readfirstlane(n[x]);
+    s.span = a.cu_q || seq[x] >= a.B ? s.len : a.S;
+    pg_keys(a, s);
+    return s;
+  }
+};
 
 template <class W>
-__device__ __forceinline__ void pg_line(const PgArgs& a, PgLine& line, int threads) {
+constexpr bool kPgTreeRows = W::kTree && W::kR == kPrRows;
+
+// `room`: kPgLineCu lengths of queries and keys for the time of the call.
+template <class W>
+__device__ __forceinline__ void pg_line(const PgArgs& a, PgLine<kPgTreeRows<W>>& line, int threads, int32_t* room) {
   const int tid = threadIdx.x;
-  const bool copy = a.cu_q && a.B <= kPgLineCu;
-  if (copy)
-    for (int b = tid; b < a.B; b += threads) line.cu[b] = a.cu_q[b];
-  __syncthreads();
-  for (int x = tid; x < a.slots; x += threads) {
-    const int b = pg_find(a, copy ? line.cu : a.cu_q, x, W::kR);
-    const PgSeq s = pg_seq(a, b);
-    int lo, hi, units = 0;
-    // A tile without keys takes a unit too: it writes its zeros.
-    if (pg_range<W::kTree>(a, s, x - pg_slot(s.start, a.Hg, b, W::kR), W::kR, lo, hi))
-      units = kPgExtra + max(1, (hi - lo + W::kUnitKeys - 1) / W::kUnitKeys);
-    line.seq[x] = (uint16_t)b;
-    line.at[x + 1] = units;
+  if constexpr (kPgTreeRows<W>) {
+    const auto fill = [&](auto cu, auto q_len, auto kv_len) {
+      for (int x = tid; x < a.slots; x += threads) {
+        const int b = pg_find(a, cu, x, W::kR);
+        const PgSeq s = pg_seq(a, cu, q_len, kv_len, b);
+        int lo, hi, units = 0;
+        if (pg_range<true>(a, s, x - pg_slot(s.start, a.Hg, b, W::kR), W::kR, lo, hi))
+          units = kPgExtra + max(1, (hi - lo + W::kUnitKeys - 1) / W::kUnitKeys);
+        line.seq[x] = (uint16_t)b;
+        line.start[x] = s.start;
+        line.len[x] = s.len;
+        line.n[x] = s.n;
+        line.at[x + 1] = units;
+      }
+    };
+    if (a.B <= kPgLineCu) {
+      for (int b = tid; b < a.B; b += threads) {
+        const int kv = a.kv_len[b], q = a.cu_q ? a.cu_q[b] : a.q_len ? a.q_len[b] : 0;
+        line.cu[b] = q;
+        room[b] = kv;
+      }
+      __syncthreads();
+      fill(&line.cu[0], &line.cu[0], &room[0]);
+    } else {
+      fill(a.cu_q, a.q_len, a.kv_len);
+    }
+  } else {
+    const bool copy = a.cu_q && a.B <= kPgLineCu;
+    if (copy)
+      for (int b = tid; b < a.B; b += threads) line.cu[b] = a.cu_q[b];
+    __syncthreads();
+    for (int x = tid; x < a.slots; x += threads) {
+      const int b = pg_find(a, copy ? line.cu : a.cu_q, x, W::kR);
+      const PgSeq s = pg_seq(a, b);
+      int lo, hi, units = 0;
+      // A tile without keys takes a unit too: it writes its zeros.
+      if (pg_range<W::kTree>(a, s, x - pg_slot(s.start, a.Hg, b, W::kR), W::kR, lo, hi))
+        units = kPgExtra + max(1, (hi - lo + W::kUnitKeys - 1) / W::kUnitKeys);
+      line.seq[x] = (uint16_t)b;
+      line.at[x + 1] = units;
+    }
   }
   if (tid == 0) line.at[0] = 0;
   __syncthreads();
@@ -1202,8 +1266,8 @@ __device__ __forceinline__ int pg_mine(const PgArgs& a) {
 template <class W>
 __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
   extern __shared__ __align__(16) uint8_t lds[];
-  PgLine& line = *reinterpret_cast<PgLine*>(lds + W::kLds);
-  pg_line<W>(a, line, W::kThreads);
+  PgLine<kPgTreeRows<W>>& line = *reinterpret_cast<PgLine<kPgTreeRows<W>>*>(lds + W::kLds);
+  pg_line<W>(a, line, W::kThreads, reinterpret_cast<int32_t*>(lds));
   if (blockIdx.x == 0) {
     for (int x = threadIdx.x; x <= a.slots; x += W::kThreads) {
       a.line[x] = line.at[x];
@@ -1230,7 +1294,10 @@ __global__ __launch_bounds__(W::kThreads) void pg_split_kernel(PgArgs a) {
     const int length = __builtin_amdgcn_readfirstlane(line.at[x + 1] - line.at[x]);
     if (length == 0) continue;
     const int b = __builtin_amdgcn_readfirstlane((int)line.seq[x]);
-    const PgSeq s = pg_seq(a, b);
+    const PgSeq s = [&] {
+      if constexpr (kPgTreeRows<W>) return line.of(a, x);
+      else return pg_seq(a, b);
+    }();
     const int tile = x - pg_slot(s.start, a.Hg, b, W::kR);
     int lo, hi;
     if (!pg_range<W::kTree>(a, s, tile, W::kR, lo, hi)) break;  // not reached: the slot has units
@@ -1287,6 +1354,24 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
     const int rho = tile * kR + hh;
     if (rho - in / J::kPerRow >= s.span * a.Hg) break;  // no row of the pass
     const bool live = rho < s.span * a.Hg;
+    constexpr int kAhead = J::kGroups == 1 ? 4 : 8;  // parts whose loads are in flight together
+    f32x4 x0[kAhead], x1[kAhead];
+    float m[kAhead], l[kAhead];
+    const auto load = [&](int p0) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (W::kTree && p0 + J::kGroups * j >= np) break;  // alike in the group's wave
+        const float* pp = part(min(p0 + J::kGroups * j, np - 1));
+        const f32x4* row = reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
+        x0[j] = row[0];
+        x1[j] = row[1];
+        m[j] = pp[kR * kD + 2 * hh];
+        l[j] = pp[kR * kD + 2 * hh + 1];
+      }
+    };
+    // Trees: while the largest of all parts is looked for, and no part twice (8 nodes over 4097 keys: 6.0 -> 5.3 us; 100 trees of
+    // 8 over 500, the call: 59.0 -> 54.2, where one of 61 over 500 went from 28.5 to 29.1).
+    if (W::kTree) load(group);
     float M = -kPgInf;
     for (int p = t; p < np; p += J::kPerRow) M = fmaxf(M, part(p)[kR * kD + 2 * hh]);
 #pragma unroll
@@ -1294,20 +1379,11 @@ __global__ __launch_bounds__(kPgThreads) void pg_join_kernel(PgArgs a) {
     const int i = rho / a.Hg, h = kvg * a.Hg + rho - i * a.Hg;
     const float M_use = M == -kPgInf ? 0.f : M, sink = live ? pg_sink(a, h) : -kPgInf;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-    constexpr int kAhead = J::kGroups == 1 ? 4 : 8;  // parts whose loads are in flight together
     for (int p0 = group; p0 < np; p0 += J::kGroups * kAhead) {
-      f32x4 x0[kAhead], x1[kAhead];
-      float m[kAhead], l[kAhead];
+      if (!W::kTree || p0 != group) load(p0);
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const float* pp = part(min(p0 + J::kGroups * j, np - 1));
-        x0[j] = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0);
-        x1[j] = *reinterpret_cast<const f32x4*>(pp + hh * kD + c0 + 4);
-        m[j] = pp[kR * kD + 2 * hh];
-        l[j] = pp[kR * kD + 2 * hh + 1];
-      }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
+        if (W::kTree && p0 + J::kGroups * j >= np) break;
         const float f = p0 + J::kGroups * j < np ? fast_exp2(m[j] - M_use) : 0.f;
         sum += f * l[j];
 #pragma unroll
@@ -1351,8 +1427,8 @@ struct PgPlan {
   int wgs;        // workgroups that share the line of units; 0: a tile each
 };
 
-// `tree`, tiles of 256 rows: sequences bring alike numbers of rows, of which the last tile is seldom full, so that a workgroup a tile leaves
-// CUs idle in the last round: the line up to 1199 slots of all groups (32 trees of 61 nodes, 64 heads over 4, 620 slots:
+// `tree`, tiles of 256 rows: sequences bring alike numbers of rows, of which the last tile is seldom full, so that a workgroup
+// a tile leaves CUs idle in the last round: the line up to 1199 slots of all groups (32 trees of 61 nodes, 64 heads over 4, 620 slots:
 // 8192 keys 660 -> 562 us; 128 trees of 8 over 2000 keys, 772 slots: 158 -> 129; 200 trees of 8 over 500 keys, 1204 slots:
 // 80 -> 89; 24 nodes each, 2004 slots: 176 -> 197).
 inline PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most, bool tree) {
@@ -1366,7 +1442,8 @@ inline PgPlan pg_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t most, 
   // instead of 199).
   const int64_t unit = p.rows == kPrRows ? kPrTile : kPgUnit;
   const int64_t units = p.slots * G * ((most + unit - 1) / unit + 1 + kPgExtra);
-  if (p.slots <= kPgMaxSlots && units < ((int64_t)1 << 30) && (tree && p.rows == kPrRows ? p.slots * G < 1200 : p.slots * G < 512 || 4 * (B + 1) > p.slots))
+  const bool shared = tree && p.rows == kPrRows ? p.slots * G < kPgTreeSlots : p.slots * G < 512 || 4 * (B + 1) > p.slots;
+  if (p.slots <= kPgMaxSlots && units < ((int64_t)1 << 30) && shared)
     p.wgs = (int)(units < 256 ? units : 256);
   return p;
 }
@@ -1386,7 +1463,7 @@ inline size_t pg_workspace_bytes(const PgPlan& p, int64_t D) {
 
 template <class W>
 hipError_t pg_launch(const PgArgs& a, hipStream_t stream) {
-  constexpr int split_lds = W::kLds + (int)sizeof(PgLine);
+  constexpr int split_lds = W::kLds + (int)sizeof(PgLine<kPgTreeRows<W>>);
   static_assert(W::kLds % 16 == 0 && split_lds <= 160 * 1024, "LDS");
   const dim3 tiles((unsigned)((int64_t)a.slots * a.G));
   hipError_t e;
