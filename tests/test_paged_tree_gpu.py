@@ -236,3 +236,30 @@ def test_large_batch_of_tiles(dsa, dev):
     run(dsa, dev, c)
     c = build(dev, [(1 + i % 3, 100 + i) for i in range(300)], 8, 8, 128, 16, torch.float16, 18)
     run(dsa, dev, c, 60, what="windows")
+
+
+@pytest.mark.parametrize("B", [1024, 1025, 1100])
+@pytest.mark.parametrize("padded", [False, True])
+def test_many_sequences_in_tiles_of_256_rows(dsa, dev, B, padded):
+    """Both sides of the lengths that a workgroup keeps a copy of, in the shared line's tiles of 256 rows; padded: some of
+    the two rows of a sequence are padding."""
+    rng = random.Random(B)
+    H = 17 if padded else 16
+    lens = [(rng.choice((0, 1, 2, 2)) if padded else rng.choice((2, 2, 2, 3)), rng.randint(0, 90)) for _ in range(B)]
+    c = build(dev, lens, H, 1, 64, 16, torch.bfloat16, B)
+    if not padded:
+        run(dsa, dev, c)
+        return
+    cu = torch.tensor([0] + c["lens"]).cumsum(0).tolist()
+    q, mask = torch.zeros(B, 2, H, 64, dtype=torch.bfloat16), torch.zeros(B, 2, 1, dtype=torch.int64)
+    for b, (s, _) in enumerate(lens):
+        q[b, :s], mask[b, :s] = c["q"][cu[b]:cu[b + 1]], c["mask"][cu[b]:cu[b + 1]]
+    out, lse = dsa.paged_tree_fwd(q.to(dev), c["kc"].to(dev), c["vc"].to(dev), c["table"].int().to(dev), mask.to(dev),
+                                  c["scale"], actual_seq_lengths_query=ints(dev, c["lens"]),
+                                  actual_seq_lengths_kv=ints(dev, c["kv"]))
+    o, ot, l, lt = R.attention(c["q"], c["kc"], c["vc"], c["table"], c["mask"], cu[:-1], c["lens"], c["lens"], c["kv"],
+                               c["scale"])
+    live = torch.tensor([i < s for s, _ in lens for i in range(2)])
+    assert_within(out.cpu().reshape(2 * B, H, 64)[live], o, ot, "out")
+    assert_within(lse.cpu().reshape(2 * B, H)[live], l, lt, "lse")
+    assert not out.cpu().reshape(2 * B, H, 64)[~live].any() and bool(torch.isneginf(lse.cpu().reshape(2 * B, H)[~live]).all())
