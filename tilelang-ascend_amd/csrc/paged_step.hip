@@ -176,7 +176,7 @@ struct PlanPath {
 
 // Rows that the workgroup of the plan writes by itself, in turns of kStepThreads.  One launch against two: 1024 rows 4.2 us
 // and 5.5 (of trees 6.0 and 7.3), 2048 rows 5.1 and 5.9 (8.7 and 7.5); 4096 rows take one workgroup 8 us and more (14 of
-// trees), two launches 6.2 (7.6).  The second launch costs the host 2 us or more as well: a plan of 1952 rows of 32 trees with
+// trees), two launches 6.2 (7.6).  The second launch costs the host 2 us or more as well: a plan of 1421 rows of 61 trees with
 // the pages' way back, call after call, 10.4 us with one and 12.7 with two.
 constexpr int kPlanRowsEach = 2, kPlanFewRows = kPlanRowsEach * kStepThreads;
 
@@ -458,8 +458,9 @@ hipError_t launch_paged_free(const int32_t* keep, int32_t* table, int32_t* free_
 // Scores are read where the walk comes by: of 61 rows of a sequence some four.  A workgroup a sequence (accept_walk_kernel)
 // reads a row with all its threads, then looks for the child; each step is one row's bytes through one CU (108 GB/s) and
 // 2.5 us of latencies (the first loads, the reductions, the child): 64 sequences of 61 rows, 131072 bf16 scores, four nodes
-// on the path 24.6 us, where reading those rows at the card's rate would take 14 and all 3904 rows 215.  Where all rows together are few, a first launch takes the largest of every row in pieces over the card
-// (row_max_kernel), and the walk only joins pieces.
+// on the path 23.4 us, where reading those rows at the card's rate would take 14 and all 3904 rows 215.  Where all rows
+// together are few, a first launch takes the largest of every row in pieces over the card (row_max_kernel), and the walk only
+// joins pieces: 15 rows of 50021 fp32 scores 3.4 and 3.6 us.
 
 struct AcceptArgs {
   const void* scores;      // [T, V], or choices [T]
@@ -722,8 +723,8 @@ hipError_t launch_tree_accept(int kind, const void* scores, int64_t stride, int6
 // 1 KB of the columns of a cache's rows of one sequence, a lane 16 bytes of each, so that no lane reads what another one
 // writes.  Eight rows are read before the eight are written: a source lies behind its own place and so behind all places
 // written before, which makes this the same as one row after the other.  Bound by latencies (lengths, path, table, rows)
-// where there is little to move: 3.8 us for one sequence; 122 caches of 64 sequences, four rows of 1152 bytes each, take 16.0 us,
-// 4.5 TB/s.  Where rows or a cache do not start on 16 bytes a lane takes 4: 3.7 and 23.9 us at these sizes.
+// where there is little to move: 3.8 us for one sequence; 122 caches of 64 sequences, four rows of 1152 bytes each, take
+// 16.0 us, 4.5 TB/s.  Where rows or a cache do not start on 16 bytes a lane takes 4: 3.7 and 23.9 us at these sizes.
 
 constexpr int kCommitCaches = 128;  // of a launch: their descriptions are kernel arguments
 constexpr int kCommitWaves = 4;
