@@ -402,3 +402,17 @@ def test_commit_caches_off_16_bytes_and_refusals(dsa, dev):
     dsa.paged_commit(c, t.long(), [3], p.long(), a.long())  # moved again: the rows now there
     R.commit(want, *args)
     assert torch.equal(c.cpu(), want[0])
+
+
+@pytest.mark.parametrize("ops", [False, True])
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
+def test_accept_numbers_past_31_bits_match_nothing(dsa, dev, dtype, ops):
+    """Two of them are not alike, nor is either the largest of 31 bits."""
+    top, far = 2**31 - 1, 2**32 - 5
+    wide = lambda x: torch.tensor(x, dtype=torch.int64, device=dev).to(dtype)
+    args = (wide([top, far, far, 7, 2**31 + 1]), wide([0, far, top, 2**31, 7]), ints(dev, [-1, 0, 0, 2, 3]))
+    if ops:
+        accepted, path, chosen = dsa.load_torch_ops().tree_accept(*args, ints(dev, [5]), 4)
+    else:
+        accepted, path, chosen = dsa.tree_accept(*args, actual_seq_lengths_query=ints(dev, [5]), max_path=4)
+    assert accepted.tolist() == [2] and path.tolist() == [[0, 2, -1, -1]] and chosen.tolist() == [[top, -1, -1, -1]]

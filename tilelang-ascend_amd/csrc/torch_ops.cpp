@@ -717,8 +717,10 @@ Accepted accept_outputs(const at::Tensor& cu, int64_t max_path, const at::Tensor
 
 // Numbers past 31 bits become -1, which matches nothing.
 at::Tensor token_ids(const at::Tensor& t) {
-  if (t.scalar_type() != at::kLong) return saturated_i32(t);
-  return t.masked_fill(t.lt(0).logical_or(t.gt((int64_t)0x7fffffff)), -1).to(at::kInt);
+  const at::ScalarType st = t.scalar_type();
+  if (st != at::kLong && st != at::kUInt32 && st != at::kUInt64) return t;
+  const at::Tensor wide = t.to(at::kLong);  // numbers past 63 bits come out negative
+  return wide.masked_fill(wide.lt(0).logical_or(wide.gt((int64_t)0x7fffffff)), -1).to(at::kInt);
 }
 
 // scores [T, V] whose rows may lie apart, or [T] integer choices.
