@@ -416,3 +416,13 @@ def test_accept_numbers_past_31_bits_match_nothing(dsa, dev, dtype, ops):
     else:
         accepted, path, chosen = dsa.tree_accept(*args, actual_seq_lengths_query=ints(dev, [5]), max_path=4)
     assert accepted.tolist() == [2] and path.tolist() == [[0, 2, -1, -1]] and chosen.tolist() == [[top, -1, -1, -1]]
+
+
+@pytest.mark.parametrize("T", [2048, 2049])
+def test_plan_keeps_no_large_masks_beside_its_other_parts(dsa, dev, T):
+    """64 words a row: masks of 1 MB, and of more, which are an allocation of their own."""
+    table, free = [[-1] * (T // 64 + 1)], list(range(T // 64 + 1))
+    got, *_ = check_plan(dsa, dev, [T], [0], table, free, [len(free)], 64, T, [(i - 1) // 2 if i else -1 for i in range(T)], 4096)
+    parts = [x.untyped_storage().data_ptr() for x in got]
+    assert len(set(parts[:5])) == 1 and (parts[5] == parts[0]) == (T == 2048)
+    assert all(x.data_ptr() % 16 == 0 and x.is_contiguous() for x in got)

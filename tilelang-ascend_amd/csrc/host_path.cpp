@@ -717,9 +717,11 @@ PyObject* paged_plan(PyObject*, PyObject* const* v, Py_ssize_t n) {
   {
     const NoGil unlocked;
     const c10::OptionalDeviceGuard guard(dev);
-    Ints ints(3 * B + 2 * T + 2 * T * words, 6, dev);
+    // Masks of more than 1 MB are apart: who keeps another part would keep them.
+    const bool beside = 2 * T * words <= 1 << 18;
+    Ints ints(3 * B + 2 * T + (beside ? 2 * T * words : 0), 6, dev);
     for (int i = 0; i < 5; ++i) out[i] = ints.part({i == 2 || i == 3 ? T : B});
-    if (words) out[5] = ints.part({T, words}, at::kLong);
+    if (words) out[5] = beside ? ints.part({T, words}, at::kLong) : make({T, words}, at::kLong, dev);
     int32_t* p[5];
     for (int i = 0; i < 5; ++i) p[i] = out[i].data_ptr<int32_t>();
     rc = E.plan(nl.ptr<int32_t>(), ctx.ptr<int32_t>(), bt.data_ptr<int32_t>(), list.data_ptr<int32_t>(),
